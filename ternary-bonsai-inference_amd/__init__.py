@@ -22,6 +22,7 @@ PKG_DIR = Path(__file__).resolve().parent
 REPO_DIR = PKG_DIR.parent
 LIB_PATH = PKG_DIR / "lib" / "libbonsai_hip.so"
 HEADER_PATH = REPO_DIR / "include" / "bonsai_hip.h"
+SERVE_HEADER_PATH = REPO_DIR / "include" / "bonsai_hip_serve.h"
 
 BH_OK = 0
 BH_ERR_SHAPE = -1
@@ -149,12 +150,65 @@ _SIGNATURES = {
                                       _c_size, _c_size, _vp, _c_size]),
 }
 
+class PagedCache(ctypes.Structure):
+    """bh_paged_cache (include/bonsai_hip_serve.h)."""
+
+    _fields_ = [
+        ("k", _vp), ("v", _vp), ("kv_dtype", _c_int),
+        ("n_pages", _c_size), ("page_size", _c_size), ("n_kv", _c_size), ("hd", _c_size),
+        ("page_stride", _c_size), ("pos_stride", _c_size), ("head_stride", _c_size),
+    ]
+
+
+class PagedPlanArgs(ctypes.Structure):
+    """bh_paged_plan_args (include/bonsai_hip_serve.h)."""
+
+    _fields_ = [
+        ("cached", _vp), ("n_new", _vp), ("block_table", _vp), ("free_pages", _vp),
+        ("n_free", _vp), ("kv_len", _vp), ("q_start", _vp), ("slots", _vp), ("pos", _vp),
+        ("n_free_out", _vp), ("n_refused", _vp),
+        ("n_req", _c_size), ("n_tok", _c_size), ("table_width", _c_size), ("page_size", _c_size),
+        ("n_pages", _c_size),
+    ]
+
+
+class AttentionPagedArgs(ctypes.Structure):
+    """bh_attention_paged_args (include/bonsai_hip_serve.h)."""
+
+    _fields_ = [
+        ("cache", PagedCache), ("q", _vp), ("out", _vp), ("q_start", _vp), ("kv_len", _vp),
+        ("block_table", _vp), ("bad_page", _vp),
+        ("n_tok", _c_size), ("n_req", _c_size), ("n_head", _c_size), ("table_width", _c_size),
+        ("max_new", _c_size), ("workspace", _vp), ("workspace_bytes", _c_size),
+    ]
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    """bh_token_logprobs_args (include/bonsai_hip_serve.h)."""
+
+    _fields_ = [
+        ("x", _vp), ("tokens", _vp), ("logprob", _vp), ("entropy", _vp), ("top_ids", _vp),
+        ("top_logprobs", _vp), ("bad_id", _vp),
+        ("n_rows", _c_size), ("vocab", _c_size), ("row_stride", _c_size), ("n_top", _c_size),
+        ("inv_temp", _c_float), ("workspace", _vp), ("workspace_bytes", _c_size),
+    ]
+
+
+_SERVE_SIGNATURES = {
+    "bh_paged_plan": (_c_int, [ctypes.POINTER(PagedPlanArgs), _vp]),
+    "bh_kv_store_paged": (_c_int, [ctypes.POINTER(PagedCache), _vp, _vp, _vp, _c_size, _vp]),
+    "bh_attention_paged": (_c_int, [ctypes.POINTER(AttentionPagedArgs), _vp]),
+    "bh_attention_paged_workspace": (_c_size, [ctypes.POINTER(AttentionPagedArgs)]),
+    "bh_token_logprobs": (_c_int, [ctypes.POINTER(TokenLogprobsArgs), _vp]),
+    "bh_token_logprobs_workspace": (_c_size, [ctypes.POINTER(TokenLogprobsArgs)]),
+}
+
 _LIB = None
 
 
-def header_symbols() -> list[str]:
-    """Every function name declared in include/bonsai_hip.h."""
-    text = HEADER_PATH.read_text()
+def header_symbols(path: Path = HEADER_PATH) -> list[str]:
+    """Every function name declared in a header (include/bonsai_hip.h)."""
+    text = path.read_text()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     return sorted(set(re.findall(r"\b(bh_[a-z0-9_]+)\s*\(", text)))
 
@@ -172,7 +226,7 @@ def lib() -> ctypes.CDLL:
     except ImportError:
         pass
     handle = ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_LOCAL)
-    for name, (res, args) in _SIGNATURES.items():
+    for name, (res, args) in {**_SIGNATURES, **_SERVE_SIGNATURES}.items():
         fn = getattr(handle, name)
         fn.restype = res
         fn.argtypes = args
@@ -444,6 +498,226 @@ def pq2_matmul_n(payload, ne0: int, n_rows: int, x, base_row: int = 0, out=None,
                                 x.data_ptr(), x.numel(), n_tok, y.data_ptr(), y.numel(),
                                 _stream(stream)))
     return y
+
+
+# ---------------------------------------------------------------------------
+# a serving step over a paged cache (include/bonsai_hip_serve.h): argument
+# blocks over device tensors, made once for buffers that stay, and the calls
+# ---------------------------------------------------------------------------
+
+BH_PAGED_MAX_REQ = 4096
+BH_MAX_TOP = 32
+
+
+def _dev_tensor(t, name: str, dtypes, device, shape=None):
+    """t, checked: a contiguous tensor of one of dtypes on `device`."""
+    if t.dtype not in dtypes or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of {dtypes[0]}, got {t.dtype}")
+    if t.device != device or not t.is_cuda:
+        raise ValueError(f"{name} is on {t.device}, the call's tensors on {device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _ids_dtypes():
+    import torch
+    return (torch.int32, torch.uint32)
+
+
+def _hold(args, device, *tensors):
+    """args with the tensors whose addresses it holds, and their device."""
+    args.tensors, args.device = tensors, device
+    return args
+
+
+def _call(fn, args, stream):
+    """fn(args, stream) on the device of args' tensors, whichever is current."""
+    import torch
+    if torch.cuda.current_device() == args.device.index:
+        check(fn(ctypes.byref(args), _stream(stream)))
+        return
+    with torch.cuda.device(args.device):
+        check(fn(ctypes.byref(args), _stream(stream)))
+
+
+def make_paged_cache(k, v) -> PagedCache:
+    """The pool k, v [n_pages, page_size, n_kv, hd] of f32 or f16 (or 16-bit
+    integers holding f16 bits); any equal strides of the first three, so a
+    transposed [n_pages, n_kv, page_size, hd] or one of two halves of an
+    allocation will do."""
+    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+        raise ValueError("k and v must be [n_pages, page_size, n_kv, hd], alike in shape, "
+                         "strides and type")
+    if not k.is_cuda or k.device != v.device:
+        raise ValueError("k and v must be on one GPU")
+    if k.stride(3) != 1 and k.shape[3] != 1:
+        raise ValueError("a head's elements must lie side by side")
+    n_pages, page_size, n_kv, hd = k.shape
+    return _hold(PagedCache(k.data_ptr(), v.data_ptr(), _kv_dtype(k), n_pages, page_size, n_kv,
+                            hd, k.stride(0), k.stride(1), k.stride(2)), k.device, k, v)
+
+
+def make_paged_plan_args(cached, n_new, block_table, free_pages, n_free, page_size: int, *,
+                         kv_len, q_start, slots, pos=None, n_free_out=None,
+                         n_refused=None) -> PagedPlanArgs:
+    """int32 tensors: cached, n_new, kv_len [n_req], block_table [n_req, width],
+    free_pages [n_pages], n_free [1], q_start [n_req + 1], slots [n_tok],
+    pos [n_tok, 4]; n_free_out [1] (None: n_free moves on in place),
+    n_refused [1]."""
+    import torch
+    i32, dev = (torch.int32,), cached.device
+    n_req, n_tok = cached.numel(), slots.numel()
+    n_free_out = n_free if n_free_out is None else n_free_out
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [n_req, width]")
+    _dev_tensor(cached, "cached", i32, dev, (n_req,))
+    _dev_tensor(n_new, "n_new", i32, dev, (n_req,))
+    _dev_tensor(block_table, "block_table", i32, dev, (n_req, block_table.shape[1]))
+    _dev_tensor(free_pages, "free_pages", i32, dev, (free_pages.numel(),))
+    _dev_tensor(kv_len, "kv_len", i32, dev, (n_req,))
+    _dev_tensor(q_start, "q_start", i32, dev, (n_req + 1,))
+    _dev_tensor(slots, "slots", i32, dev, (n_tok,))
+    for name, word in (("n_free", n_free), ("n_free_out", n_free_out), ("n_refused", n_refused)):
+        if word is not None:
+            _dev_tensor(word, name, i32, dev)
+            if word.numel() != 1:
+                raise ValueError(f"{name} must be one word")
+    if pos is not None:
+        _dev_tensor(pos, "pos", i32, dev, (n_tok, 4))
+    return _hold(
+        PagedPlanArgs(_ptr(cached), _ptr(n_new), _ptr(block_table), _ptr(free_pages),
+                      _ptr(n_free), _ptr(kv_len), _ptr(q_start), _ptr(slots), _ptr(pos),
+                      _ptr(n_free_out), _ptr(n_refused), n_req, n_tok, block_table.shape[1],
+                      page_size, free_pages.numel()),
+        dev, cached, n_new, block_table, free_pages, n_free, kv_len, q_start, slots, pos,
+        n_free_out, n_refused)
+
+
+def paged_plan(args: PagedPlanArgs, stream=None) -> None:
+    """A step's pages, offsets, slots and positions from the requests' lengths."""
+    _call(lib().bh_paged_plan, args, stream)
+
+
+def kv_store_paged(cache: PagedCache, k, v, slots, stream=None) -> None:
+    """kv_store into pages: rows k, v [n_tok, n_kv * hd] f32 to the positions
+    slots int32 [n_tok] of the cache (page * page_size + offset; below 0: none)."""
+    import torch
+    dev, shape = cache.device, (slots.numel(), cache.n_kv * cache.hd)
+    _dev_tensor(slots, "slots", (torch.int32,), dev)
+    _dev_tensor(k, "k", (torch.float32,), dev, shape)
+    _dev_tensor(v, "v", (torch.float32,), dev, shape)
+
+    def store(ref, s):
+        return lib().bh_kv_store_paged(ref, k.data_ptr(), v.data_ptr(), slots.data_ptr(),
+                                       shape[0], s)
+    _call(store, cache, stream)
+
+
+def make_attention_paged_args(cache: PagedCache, q, q_start, kv_len, block_table, out=None,
+                              max_new: int = 0, bad_page=None,
+                              workspace=None) -> AttentionPagedArgs:
+    """Queries q [n_tok, n_head, hd] f32 of the requests whose tokens begin at
+    q_start int32 [n_req + 1], over kv_len int32 [n_req] positions in the pages
+    block_table int32 [n_req, width].  The result is args.out (new if out is
+    None; rows of no request are left as they were).  workspace: a uint8 tensor
+    of attention_paged_workspace(args) bytes for calls that may overlap; None:
+    the library's scratch."""
+    import torch
+    i32, dev = (torch.int32,), cache.device
+    if q.dim() != 3 or q.shape[2] != cache.hd:
+        raise ValueError(f"q must be [n_tok, n_head, {cache.hd}], got {tuple(q.shape)}")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [n_req, width]")
+    n_req = kv_len.numel()
+    _dev_tensor(q, "q", (torch.float32,), dev)
+    out = torch.zeros_like(q) if out is None else out
+    _dev_tensor(out, "out", (torch.float32,), dev, q.shape)
+    _dev_tensor(q_start, "q_start", i32, dev, (n_req + 1,))
+    _dev_tensor(kv_len, "kv_len", i32, dev, (n_req,))
+    _dev_tensor(block_table, "block_table", i32, dev, (n_req, block_table.shape[1]))
+    if bad_page is not None:
+        _dev_tensor(bad_page, "bad_page", i32, dev)
+    args = AttentionPagedArgs(cache, _ptr(q), _ptr(out), _ptr(q_start), _ptr(kv_len),
+                              _ptr(block_table), _ptr(bad_page), q.shape[0], n_req, q.shape[1],
+                              block_table.shape[1], max_new, None, 0)
+    if workspace is not None:
+        _dev_tensor(workspace, "workspace", (torch.uint8,), dev)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    args.out_tensor = out
+    return _hold(args, dev, cache.tensors, q, out, q_start, kv_len, block_table, bad_page,
+                 workspace)
+
+
+def attention_paged_workspace(args: AttentionPagedArgs) -> int:
+    """Bytes of workspace of attention_paged(args) on the args' device."""
+    import torch
+    with torch.cuda.device(args.device):
+        return int(lib().bh_attention_paged_workspace(ctypes.byref(args)))
+
+
+def attention_paged(args: AttentionPagedArgs, stream=None):
+    """attention for many requests at once over a paged cache; returns the
+    output tensor of the arguments."""
+    _call(lib().bh_attention_paged, args, stream)
+    return args.out_tensor
+
+
+def make_token_logprobs_args(x, tokens=None, n_top: int = 0, inv_temp: float = 1.0, *,
+                             logprob=None, entropy=None, top_ids=None, top_logprobs=None,
+                             bad_id=None, workspace=None) -> TokenLogprobsArgs:
+    """Logits x [n_rows, vocab] f32 (rows any stride apart), tokens int32 or
+    uint32 [n_rows].  Outputs that are None are made (logprob with tokens,
+    top_ids / top_logprobs with n_top); args.results holds (logprob, entropy,
+    top_ids, top_logprobs)."""
+    import torch
+    dev, f32, ids = x.device, (torch.float32,), _ids_dtypes()
+    if x.dim() != 2 or x.dtype != torch.float32 or not x.is_cuda:
+        raise ValueError("x must be a float32 CUDA tensor [n_rows, vocab]")
+    n_rows, vocab = x.shape
+    if vocab > 1 and x.stride(1) != 1:
+        raise ValueError("a row's logits must lie side by side")
+    if n_rows > 1 and x.stride(0) < vocab:
+        raise ValueError("rows of x must not overlap")
+    if tokens is not None:
+        _dev_tensor(tokens, "tokens", ids, dev, (n_rows,))
+        logprob = torch.empty(n_rows, dtype=torch.float32, device=dev) if logprob is None \
+            else _dev_tensor(logprob, "logprob", f32, dev, (n_rows,))
+    elif logprob is not None:
+        raise ValueError("logprob needs tokens")
+    entropy = torch.empty(n_rows, dtype=torch.float32, device=dev) if entropy is None \
+        else _dev_tensor(entropy, "entropy", f32, dev, (n_rows,))
+    if n_top:
+        shape = (n_rows, n_top)
+        top_ids = torch.empty(shape, dtype=torch.int32, device=dev) if top_ids is None \
+            else _dev_tensor(top_ids, "top_ids", ids, dev, shape)
+        top_logprobs = torch.empty(shape, dtype=torch.float32, device=dev) \
+            if top_logprobs is None else _dev_tensor(top_logprobs, "top_logprobs", f32, dev, shape)
+    else:
+        top_ids = top_logprobs = None
+    if bad_id is not None:
+        _dev_tensor(bad_id, "bad_id", ids, dev)
+    args = TokenLogprobsArgs(_ptr(x), _ptr(tokens), _ptr(logprob), _ptr(entropy), _ptr(top_ids),
+                             _ptr(top_logprobs), _ptr(bad_id), n_rows, vocab,
+                             x.stride(0) if n_rows > 1 else vocab, n_top, inv_temp, None, 0)
+    if workspace is not None:
+        _dev_tensor(workspace, "workspace", (torch.uint8,), dev)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    args.results = (logprob, entropy, top_ids, top_logprobs)
+    return _hold(args, dev, x, tokens, logprob, entropy, top_ids, top_logprobs, bad_id, workspace)
+
+
+def token_logprobs_workspace(args: TokenLogprobsArgs) -> int:
+    """Bytes of workspace of token_logprobs(args) on the args' device."""
+    import torch
+    with torch.cuda.device(args.device):
+        return int(lib().bh_token_logprobs_workspace(ctypes.byref(args)))
+
+
+def token_logprobs(args: TokenLogprobsArgs, stream=None):
+    """(logprob, entropy, top_ids, top_logprobs) of each row of logits."""
+    _call(lib().bh_token_logprobs, args, stream)
+    return args.results
 
 
 def env_info() -> dict:

@@ -59,7 +59,9 @@ constexpr int kScratchAttention = 2;  // attention: chunk partials or probabilit
 constexpr int kScratchGather = 3;     // gather + RMSNorm: the row scales
 constexpr int kScratchGdn = 4;        // gated delta-net chunks: prepared matrices
 constexpr int kScratchKvSplit = 5;    // attention: f32 cache split into f16 hi / lo
-constexpr int kScratchSlots = 6;
+constexpr int kScratchPaged = 6;      // paged attention: partial results of split requests
+constexpr int kScratchLogprobs = 7;   // log probabilities: chunk sums and candidates
+constexpr int kScratchSlots = 8;
 void *device_scratch(size_t bytes, int slot, hipStream_t stream, size_t least = 0);
 // Current size of this device's buffer for `slot` (0 before the first use).
 size_t scratch_bytes(int slot);
