@@ -25,7 +25,7 @@ struct PagedArgs {
   size_t page_stride, pos_stride, head_stride;
   int n_tok, n_req, n_head, n_kv, group, hd, width, n_pages, max_len;
   float scale;
-  FastDiv page;
+  FastDiv page, grp;
 };
 
 __device__ __forceinline__ float cache_at(const float *p) { return *p; }
@@ -116,6 +116,770 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedArgs a) {
   }
 }
 
+// ---- matrix-core path (hd 64, 128, 256) ---------------------------------------
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr float kPUnit = 16384.0f;  // probabilities in f16 stand in units of 2^-14
+constexpr float kNoScore = -3.402823466e38f;  // the maximum of scores that are all -inf
+constexpr int kJoinRows = 8;        // rows of a tile that the waves join at a time
+
+// Where a call's work lies.  A request with n tokens has ceil(n group / R) row
+// tiles a kv head and ceil(len / U) units of U positions; the list of all
+// (request, kv head, row tile, unit) is cut into equal runs, one a worker.
+struct Split {
+  int64_t *prefix;  // [n_req + 1] units before a request, written by worker 0
+  float *pm, *pl;   // [workers][2][R] running maximum (base 2) and sum
+  float *pacc;      // [workers][2][R][hd]
+  int workers;
+};
+
+__host__ __device__ __forceinline__ int64_t run_begin(int64_t total, int workers, int w) {
+  const int64_t base = total / workers, rest = total - base * workers;
+  return w * base + (w < rest ? w : rest);
+}
+
+template <int R, int U>
+__device__ __forceinline__ void tiles_units(const PagedArgs &a, int n, int len, int *tiles,
+                                            int *units) {
+  *tiles = static_cast<int>((static_cast<int64_t>(n) * a.group + R - 1) / R);
+  *units = max((len + U - 1) / U, 1);
+}
+
+// f16 cache: 32 positions a step on v_mfma_f32_16x16x32_f16.
+//
+// S^T = K Q^T: a lane (g = lane / 16, c = lane % 16) loads 16 bytes of position c's
+// row (dims 32 kk + 8 g ..) as its A operand, straight from memory; q stands in LDS
+// as B operands, split into f16 hi + lo (22 bits) after an exact power of two
+// that brings the row's largest to 2^14 .. 2^15.  Lane (g, c) gets the scores of
+// row c at positions 16 s + 4 g + i.
+// O^T = V^T P^T: with the k index of a lane's eight slots taken as those same
+// positions, its scores are its B operand as they stand (hi + lo), and the A
+// operand is what the lane has loaded: 8 positions by 8 dims, transposed by one
+// v_perm a pair.  Row c's output and running state stay with the lanes of c.
+template <int HD, int RT>
+struct EngineF16 {
+  using Elem = _Float16;
+  static constexpr int kHd = HD, kRt = RT, kStep = 32;
+  static constexpr int KK = HD / 32, DV = HD >= 128 ? 8 : 4, NB = HD / (16 * DV);
+  static constexpr int kQBytes = RT * KK * 2 * 64 * 16;
+  typedef _Float16 VVec __attribute__((ext_vector_type(DV)));
+
+  h8 k[2][KK];
+  VVec v[8][NB];
+  f32x4 acc[RT][NB][DV];
+  float sc[RT][8];
+  h8 phi[RT], plo[RT];
+
+  // Index of a lane's slot j among the positions of a step.
+  static __device__ __forceinline__ int pos_of(int g, int j) { return (j & 4) * 4 + 4 * g + (j & 3); }
+
+  static __device__ __forceinline__ void store_q(char *lds, int row, int d, float4 x, float up) {
+    const int kk = d / 32, g = d % 32 / 8, e = d % 8;
+    const f32x4 y = {x.x * up, x.y * up, x.z * up, x.w * up};
+    const h4 hi = __builtin_convertvector(y, h4);
+    const h4 lo = __builtin_convertvector(y - __builtin_convertvector(hi, f32x4), h4);
+    h8 *base = reinterpret_cast<h8 *>(lds) + ((row / 16) * KK + kk) * 128 + g * 16 + row % 16;
+    *reinterpret_cast<h4 *>(reinterpret_cast<_Float16 *>(base) + e) = hi;
+    *reinterpret_cast<h4 *>(reinterpret_cast<_Float16 *>(base + 64) + e) = lo;
+  }
+  static constexpr bool kScaleQ = true;
+
+  __device__ __forceinline__ void load_k(const Elem *kc, const int64_t *off, int lane) {
+    const int g = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const Elem *row = kc + off[16 * s + c] + 8 * g;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) k[s][kk] = *reinterpret_cast<const h8 *>(row + 32 * kk);
+    }
+  }
+  __device__ __forceinline__ void load_v(const Elem *vc, const int64_t *off, int lane) {
+    const int g = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const Elem *row = vc + off[pos_of(g, j)] + DV * c;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) v[j][b] = *reinterpret_cast<const VVec *>(row + 16 * DV * b);
+    }
+  }
+  __device__ __forceinline__ void scores(const char *lds, int lane) {
+    const h8 *q = reinterpret_cast<const h8 *>(lds) + lane;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+      h8 hi_next = q[t * KK * 128], lo_next = q[t * KK * 128 + 64];
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        // the next operands are read here and not earlier: registers are short
+        __builtin_amdgcn_sched_barrier(0);
+        const h8 hi = hi_next, lo = lo_next;
+        if (kk + 1 < KK) {
+          hi_next = q[(t * KK + kk + 1) * 128];
+          lo_next = q[(t * KK + kk + 1) * 128 + 64];
+        }
+        s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][kk], hi, s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][kk], hi, s1, 0, 0, 0);
+        s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][kk], lo, s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][kk], lo, s1, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[t][i] = s0[i], sc[t][4 + i] = s1[i];
+    }
+  }
+  // sc holds the probabilities: their halves.
+  __device__ __forceinline__ void split_p(int t) {
+    const f32x4 a = f32x4{sc[t][0], sc[t][1], sc[t][2], sc[t][3]} * kPUnit;
+    const f32x4 b = f32x4{sc[t][4], sc[t][5], sc[t][6], sc[t][7]} * kPUnit;
+    const h4 ah = __builtin_convertvector(a, h4), bh = __builtin_convertvector(b, h4);
+    const h4 al = __builtin_convertvector(a - __builtin_convertvector(ah, f32x4), h4);
+    const h4 bl = __builtin_convertvector(b - __builtin_convertvector(bh, f32x4), h4);
+    phi[t] = __builtin_shufflevector(ah, bh, 0, 1, 2, 3, 4, 5, 6, 7);
+    plo[t] = __builtin_shufflevector(al, bl, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  __device__ __forceinline__ void values() {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < DV; ++e) {
+        __builtin_amdgcn_sched_barrier(0);
+        const h8 x = {v[0][b][e], v[1][b][e], v[2][b][e], v[3][b][e],
+                      v[4][b][e], v[5][b][e], v[6][b][e], v[7][b][e]};
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          acc[t][b][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, phi[t], acc[t][b][e], 0, 0, 0);
+          acc[t][b][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, plo[t], acc[t][b][e], 0, 0, 0);
+        }
+      }
+  }
+  __device__ __forceinline__ bool finite(int j) const {
+    bool bad = false;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < DV; ++e)
+        bad |= (__builtin_bit_cast(uint16_t, v[j][b][e]) & 0x7c00u) == 0x7c00u;
+    return !bad;
+  }
+  // One position's values, from memory, with weight p in row c.
+  __device__ __forceinline__ void add_value(int t, const Elem *row, float p, int lane) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const VVec x = *reinterpret_cast<const VVec *>(row + 16 * DV * b + DV * (4 * (lane >> 4) + i));
+#pragma unroll
+        for (int e = 0; e < DV; ++e) acc[t][b][e][i] += p * kPUnit * static_cast<float>(x[e]);
+      }
+  }
+  // Lane (g, c) holds dims 16 DV b + DV (4 g + i) + e of row c.
+  template <class F>
+  __device__ __forceinline__ void each_piece(int t, int lane, F f) const {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < DV; e += 4)
+          f(16 * DV * b + DV * (4 * g + i) + e,
+            f32x4{acc[t][b][e][i], acc[t][b][e + 1][i], acc[t][b][e + 2][i], acc[t][b][e + 3][i]});
+  }
+  __device__ __forceinline__ void scale_acc(int t, float by) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < DV; ++e) acc[t][b][e] *= by;
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < DV; ++e) acc[t][b][e] = f32x4{0, 0, 0, 0};
+  }
+  static constexpr int kSlots = 8;            // positions of a lane
+  static constexpr float kAccUnit = 1.0f / kPUnit;
+  __device__ __forceinline__ void drop_value(int j) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) v[j][b] = VVec{};
+  }
+};
+
+// f32 cache: 16 positions a step on v_mfma_f32_16x16x4_f32, products and sums in
+// f32, nothing split.  The same scheme: lane (g, c) loads 16 bytes of position
+// c's row (dims 16 kk + 4 g ..), gets row c's scores at positions 4 g + i, and
+// multiplies them by 4 dims of those positions' values.
+template <int HD, int RT>
+struct EngineF32 {
+  using Elem = float;
+  static constexpr int kHd = HD, kRt = RT, kStep = 16;
+  static constexpr int KK = HD / 16, NB = HD / 64;
+  static constexpr int kQBytes = RT * KK * 64 * 16;
+
+  f32x4 k[KK], v[4][NB];
+  f32x4 acc[RT][NB][4];
+  float sc[RT][4];
+
+  static __device__ __forceinline__ int pos_of(int g, int j) { return 4 * g + j; }
+  static __device__ __forceinline__ void store_q(char *lds, int row, int d, float4 x, float) {
+    reinterpret_cast<float4 *>(lds)[((row / 16) * KK + d / 16) * 64 + d % 16 / 4 * 16 + row % 16] = x;
+  }
+  static constexpr bool kScaleQ = false;
+
+  __device__ __forceinline__ void load_k(const Elem *kc, const int64_t *off, int lane) {
+    const Elem *row = kc + off[lane & 15] + 4 * (lane >> 4);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) k[kk] = *reinterpret_cast<const f32x4 *>(row + 16 * kk);
+  }
+  __device__ __forceinline__ void load_v(const Elem *vc, const int64_t *off, int lane) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Elem *row = vc + off[pos_of(lane >> 4, j)] + 4 * (lane & 15);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) v[j][b] = *reinterpret_cast<const f32x4 *>(row + 64 * b);
+    }
+  }
+  __device__ __forceinline__ void scores(const char *lds, int lane) {
+    const f32x4 *q = reinterpret_cast<const f32x4 *>(lds) + lane;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};  // two chains
+      f32x4 an = q[t * KK * 64], bn = q[(t * KK + 1) * 64];
+#pragma unroll
+      for (int kk = 0; kk < KK; kk += 2) {
+        __builtin_amdgcn_sched_barrier(0);
+        const f32x4 a = an, b = bn;
+        if (kk + 2 < KK) an = q[(t * KK + kk + 2) * 64], bn = q[(t * KK + kk + 3) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(k[kk][e], a[e], s0, 0, 0, 0);
+          s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(k[kk + 1][e], b[e], s1, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[t][i] = s0[i] + s1[i];
+    }
+  }
+  __device__ __forceinline__ void split_p(int) {}
+  __device__ __forceinline__ void values() {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+            acc[t][b][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j][b][e], sc[t][j], acc[t][b][e],
+                                                               0, 0, 0);
+  }
+  __device__ __forceinline__ bool finite(int j) const {
+    bool bad = false;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        bad |= (__float_as_uint(v[j][b][e]) & 0x7f800000u) == 0x7f800000u;
+    return !bad;
+  }
+  __device__ __forceinline__ void add_value(int t, const Elem *row, float p, int lane) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(row + 64 * b + 4 * (4 * (lane >> 4) + i));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][b][e][i] += p * x[e];
+      }
+  }
+  // Lane (g, c) holds dims 64 b + 4 (4 g + i) + e of row c.
+  template <class F>
+  __device__ __forceinline__ void each_piece(int t, int lane, F f) const {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        f(64 * b + 4 * (4 * (lane >> 4) + i),
+          f32x4{acc[t][b][0][i], acc[t][b][1][i], acc[t][b][2][i], acc[t][b][3][i]});
+  }
+  __device__ __forceinline__ void scale_acc(int t, float by) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][b][e] *= by;
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][b][e] = f32x4{0, 0, 0, 0};
+  }
+  static constexpr int kSlots = 4;
+  static constexpr float kAccUnit = 1.0f;
+  __device__ __forceinline__ void drop_value(int j) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) v[j][b] = f32x4{0, 0, 0, 0};
+  }
+};
+
+// Over the four lanes of a row (lanes c, c + 16, c + 32, c + 48).
+template <class Op>
+__device__ __forceinline__ float row_lanes(float x, Op op) {
+  float lo, hi;
+  lane_swap<16>(x, lo, hi);
+  x = op(lo, hi);
+  lane_swap<32>(x, lo, hi);
+  return op(lo, hi);
+}
+
+// The cache rows of a step's positions, a lane each: element offsets, and which
+// of them the request has.
+template <int STEP>
+struct Rows {
+  int page;  // table entry of the lane's position, -1 past the end
+  __device__ __forceinline__ void fetch(const PagedArgs &a, const int32_t *table, int p, int end) {
+    page = p < end ? table[a.page.div(p)] : -1;
+  }
+  // Writes the offsets, returns the mask of valid positions.
+  __device__ __forceinline__ uint32_t place(const PagedArgs &a, int64_t *off, int p, int end,
+                                            int lane) const {
+    const bool in = page >= 0 && page < a.n_pages;
+    if (p < end && !in && a.bad_page) *a.bad_page = page;
+    const int64_t o = in ? static_cast<int64_t>(page) * static_cast<int64_t>(a.page_stride) +
+                               static_cast<int64_t>(a.page.mod(p)) *
+                                   static_cast<int64_t>(a.pos_stride)
+                         : 0;
+    if (lane < STEP) off[lane] = o;
+    return static_cast<uint32_t>(__ballot(in)) & (STEP == 32 ? ~0u : (1u << STEP) - 1);
+  }
+};
+
+template <class E>
+__global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kernel(PagedArgs a, Split sp) {
+  using Elem = typename E::Elem;
+  constexpr int HD = E::kHd, RT = E::kRt, R = 16 * RT, STEP = E::kStep, U = STEP * kWaves;
+  constexpr int kJoinStride = HD + 4;
+  constexpr int kJoin = kWaves * kJoinRows * kJoinStride * 4;
+  constexpr int kLds = kJoin > E::kQBytes ? kJoin : E::kQBytes;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+  __shared__ int64_t off_s[kWaves][2][STEP];
+  __shared__ float fac_s[R], m_s[kWaves][R], l_s[kWaves][R];
+  __shared__ int64_t scan_s[kWaves];
+  __shared__ int64_t first_s[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int g = lane >> 4, c = lane & 15;
+
+  // the run of this worker in the list of all units
+  const int per = (a.n_req + kThreads - 1) / kThreads;
+  int64_t mine = 0;
+  for (int r = tid * per; r < min((tid + 1) * per, a.n_req); ++r) {
+    int q0, n, len, tiles, units;
+    request(a, r, &q0, &n, &len);
+    tiles_units<R, U>(a, n, len, &tiles, &units);
+    mine += static_cast<int64_t>(tiles) * a.n_kv * units;
+  }
+  int64_t run = mine;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(run, d);
+    if (lane >= d) run += o;
+  }
+  if (lane == 63) scan_s[wave] = run;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) run += scan_s[w];
+    total += scan_s[w];
+  }
+  const int worker = blockIdx.x;
+  const int64_t begin = run_begin(total, sp.workers, worker);
+  const int64_t end = run_begin(total, sp.workers, worker + 1);
+  int64_t before = run - mine;
+  if ((worker == 0 && sp.prefix) || (before <= begin && begin < run)) {
+    for (int r = tid * per; r < min((tid + 1) * per, a.n_req); ++r) {
+      int q0, n, len, tiles, units;
+      request(a, r, &q0, &n, &len);
+      tiles_units<R, U>(a, n, len, &tiles, &units);
+      const int64_t cost = static_cast<int64_t>(tiles) * a.n_kv * units;
+      if (worker == 0 && sp.prefix) sp.prefix[r] = before;
+      if (before <= begin && begin < before + cost) first_s[0] = r, first_s[1] = before;
+      before += cost;
+    }
+  }
+  if (worker == 0 && sp.prefix && tid == 0) sp.prefix[a.n_req] = total;
+  if (begin >= end) return;
+  __syncthreads();
+  int r = static_cast<int>(first_s[0]);
+  int64_t base = first_s[1];
+
+  E eng;
+  for (int64_t at = begin; at < end;) {
+    int q0, n, len, tiles, units;
+    request(a, r, &q0, &n, &len);
+    tiles_units<R, U>(a, n, len, &tiles, &units);
+    const int64_t cost = static_cast<int64_t>(tiles) * a.n_kv * units;
+    if (at - base >= cost) {  // on to the next request
+      base += cost;
+      ++r;
+      continue;
+    }
+    const int64_t x = at - base;
+    const int task = static_cast<int>(x / units), unit = static_cast<int>(x - static_cast<int64_t>(task) * units);
+    const int head = task / tiles, tile = task - head * tiles;
+    const int unit_end = static_cast<int>(min<int64_t>(units, unit + (end - at)));
+    const int rows = min(R, n * a.group - tile * R);
+    const int first_tok = a.grp.div(tile * R), last_tok = a.grp.div(tile * R + rows - 1);
+    const int min_vis = max(len - n + first_tok + 1, 0);
+    const int max_vis = max(len - n + last_tok + 1, 0);
+    const int p_end = min(min(unit_end * U, len), max_vis);
+    const int32_t *table = a.table + static_cast<size_t>(r) * a.width;
+    const Elem *kc = static_cast<const Elem *>(a.kc) + head * a.head_stride;
+    const Elem *vc = static_cast<const Elem *>(a.vc) + head * a.head_stride;
+
+    // this wave's first rows on their way
+    int p0 = unit * U + wave * STEP;
+    Rows<STEP> rows_of;
+    rows_of.fetch(a, table, p0 + lane % STEP, p_end);
+
+    // q into LDS as matrix operands
+    __syncthreads();
+    {
+      constexpr int kLanes = HD / 4, kAt = kThreads / kLanes;  // lanes of a row, rows at once
+      for (int i = tid / kLanes; i < R; i += kAt) {
+        const int d = tid % kLanes * 4;
+        const int row = tile * R + i, tok = a.grp.div(row);
+        float4 qv = make_float4(0, 0, 0, 0);
+        if (i < rows)
+          qv = *reinterpret_cast<const float4 *>(
+              a.q + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                     (row - tok * a.group)) * HD + d);
+        float up = 1.0f, down = a.scale;
+        if constexpr (E::kScaleQ) {
+          float mx = fmaxf(fmaxf(fabsf(qv.x), fabsf(qv.y)), fmaxf(fabsf(qv.z), fabsf(qv.w)));
+          mx = lane_group_reduce<kLanes>(mx, MaxOp{});
+          int ex = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+          if (ex > -127 && ex < 128) {
+            ex = max(ex, -100);
+            up = ldexpf(1.0f, 14 - ex);
+            down = ldexpf(a.scale, ex - 14);
+          }
+        }
+        E::store_q(lds, i, d, qv, up);
+        if (d == 0) fac_s[i] = down * kExpL2E;
+      }
+    }
+    __syncthreads();
+
+    float m[RT], l[RT], fac[RT];
+    bool some[RT];  // of this lane's positions the row sees one
+    int vis[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int i = 16 * t + c;
+      m[t] = -INFINITY;
+      l[t] = 0.0f;
+      some[t] = false;
+      fac[t] = fac_s[i];
+      vis[t] = i < rows ? len - n + a.grp.div(tile * R + i) + 1 : 0;
+    }
+    eng.clear();
+    if (p0 < p_end) {
+      uint32_t mask = rows_of.place(a, off_s[wave][0], p0 + lane % STEP, p_end, lane);
+      eng.load_k(kc, off_s[wave][0], lane);
+      eng.load_v(vc, off_s[wave][0], lane);
+      rows_of.fetch(a, table, p0 + U + lane % STEP, p_end);
+      for (int s = 1;; s ^= 1) {
+        const int next = p0 + U;
+        eng.scores(lds, lane);
+        uint32_t next_mask = 0;
+        if (next < p_end) {
+          next_mask = rows_of.place(a, off_s[wave][s], next + lane % STEP, p_end, lane);
+          eng.load_k(kc, off_s[wave][s], lane);
+          rows_of.fetch(a, table, next + U + lane % STEP, p_end);
+        }
+        constexpr uint32_t kAll = STEP == 32 ? ~0u : (1u << STEP) - 1;
+        const bool edge = mask != kAll || p0 + STEP > min_vis;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+#pragma unroll
+          for (int j = 0; j < E::kSlots; ++j) eng.sc[t][j] *= fac[t];
+          if (edge) {
+#pragma unroll
+            for (int j = 0; j < E::kSlots; ++j) {
+              const int o = E::pos_of(g, j);
+              const bool sees = p0 + o < vis[t] && (mask >> o & 1);
+              if (!sees) eng.sc[t][j] = -INFINITY;
+              some[t] |= sees;
+            }
+          } else {
+            some[t] = true;
+          }
+          if constexpr (E::kScaleQ) {
+            // an infinite key times the two halves of q may be inf - inf or 0 inf
+            // where the whole product is infinite: such a score is formed again
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < E::kSlots; ++j) odd |= eng.sc[t][j] != eng.sc[t][j];
+            if (__builtin_expect(__any(odd), false)) {
+              const int row = tile * R + 16 * t + c, tok = a.grp.div(row);
+              const float *q = a.q + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                                      (row - tok * a.group)) * HD;
+#pragma unroll
+              for (int j = 0; j < E::kSlots; ++j) {
+                if (eng.sc[t][j] == eng.sc[t][j]) continue;
+                const Elem *key = kc + off_s[wave][s ^ 1][E::pos_of(g, j)];
+                float dot = 0.0f;
+                for (int d = 0; d < HD; ++d) dot += q[d] * static_cast<float>(key[d]);
+                eng.sc[t][j] = dot * (a.scale * kExpL2E);
+              }
+            }
+          }
+          float top = eng.sc[t][0];
+#pragma unroll
+          for (int j = 1; j < E::kSlots; ++j) top = fmaxf(top, eng.sc[t][j]);
+          top = row_lanes(top, MaxOp{});
+          const float now = fmaxf(m[t], top);
+          // a row that has seen nothing above -inf is measured from 0
+          const float ref = now == -INFINITY ? 0.0f : now;
+          if (__any(now > m[t])) {
+            const float keep = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - ref);
+            l[t] *= keep;
+            eng.scale_acc(t, keep);
+          }
+          m[t] = now;
+#pragma unroll
+          for (int j = 0; j < E::kSlots; ++j) {
+            eng.sc[t][j] = __builtin_amdgcn_exp2f(eng.sc[t][j] - ref);
+            l[t] += eng.sc[t][j];
+          }
+          eng.split_p(t);
+        }
+        // A value that is not finite must not meet the zero weights of the rows that
+        // do not see it: its position is left out of the product and added to the
+        // rows that do.
+        uint32_t apart = 0;
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < E::kSlots; ++j) {
+            const int o = E::pos_of(g, j);
+            if (!(mask >> o & 1)) eng.drop_value(j);
+            if (p0 + STEP > min_vis) {
+              const uint64_t bad = __ballot(!eng.finite(j) && p0 + o >= min_vis);
+              if (bad >> (16 * g) & 0xffff) eng.drop_value(j);
+#pragma unroll
+              for (int w = 0; w < 4; ++w)
+                if (bad >> (16 * w) & 0xffff) apart |= 1u << E::pos_of(w, j);
+            }
+          }
+        }
+        eng.values();
+        while (__builtin_expect(apart != 0, false)) {
+          const int o = __ffs(apart) - 1;
+          apart &= apart - 1;
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            float p = 0.0f;
+#pragma unroll
+            for (int j = 0; j < E::kSlots; ++j)
+              if (E::pos_of(o % 16 / 4, j) == o) p = eng.sc[t][j];
+            p = __shfl(p, o % 16 / 4 * 16 + c);
+            if (p0 + o < vis[t]) eng.add_value(t, vc + off_s[wave][s ^ 1][o], p, lane);
+          }
+        }
+        if (next >= p_end) break;
+        eng.load_v(vc, off_s[wave][s], lane);
+        p0 = next;
+        mask = next_mask;
+      }
+    }
+
+    // the waves' states joined, kJoinRows rows at a time
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      l[t] = row_lanes(l[t], SumOp{});
+      // a row whose every score is -inf is 0 / 0; one that sees nothing keeps -inf
+      // as its maximum and is 0
+      const float seen = row_lanes(some[t] ? 1.0f : 0.0f, MaxOp{});
+      if (m[t] == -INFINITY && seen != 0.0f) m[t] = kNoScore;
+      if (g == 0) m_s[wave][16 * t + c] = m[t], l_s[wave][16 * t + c] = l[t];
+    }
+    const bool whole = unit == 0 && unit_end == units;
+    const size_t slot = static_cast<size_t>(worker) * 2 + (at == begin ? 0 : 1);
+    float *join = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int half = 0; half < 16; half += kJoinRows) {
+        const int r0 = 16 * t + half;
+        if (r0 >= rows) continue;
+        __syncthreads();
+        if (c >= half && c < half + kJoinRows && 16 * t + c < rows)
+          eng.each_piece(t, lane, [&](int d, f32x4 o) {
+            *reinterpret_cast<f32x4 *>(join + (wave * kJoinRows + c - half) * kJoinStride + d) = o;
+          });
+        __syncthreads();
+        const int here = min(kJoinRows, rows - r0);
+        for (int i = tid; i < here * (HD / 4); i += kThreads) {
+          const int rr = i / (HD / 4), d = i % (HD / 4) * 4, row = r0 + rr;
+          float top = m_s[0][row];
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_s[w][row]);
+          const float ref = top == -INFINITY ? 0.0f : top;
+          float sum = 0.0f;
+          f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) {
+            const float keep = __builtin_amdgcn_exp2f(m_s[w][row] - ref);
+            sum += keep * l_s[w][row];
+            o += keep * *reinterpret_cast<const f32x4 *>(join + (w * kJoinRows + rr) * kJoinStride + d);
+          }
+          if (whole) {
+            const int tok = a.grp.div(tile * R + row);
+            const float inv = top == -INFINITY ? 0.0f : E::kAccUnit / sum;
+            float *dst = a.out + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                                  (tile * R + row - tok * a.group)) * HD + d;
+            *reinterpret_cast<f32x4 *>(dst) = o * inv;
+          } else {
+            *reinterpret_cast<f32x4 *>(sp.pacc + (slot * R + row) * HD + d) = o * E::kAccUnit;
+            if (d == 0) sp.pm[slot * R + row] = top, sp.pl[slot * R + row] = sum;
+          }
+        }
+      }
+    at += unit_end - unit;
+  }
+}
+
+// Joins the parts of the rows that more than one worker has: a block per
+// (token, head).
+template <int HD, int R, int U>
+__global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, Split sp) {
+  constexpr int kLanes = HD / 4, kAt = kThreads / kLanes;
+  __shared__ int owner;
+  __shared__ float part[kAt][HD], red[kWaves];
+  const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+  if (tid == 0) owner = a.n_req;
+  __syncthreads();
+  for (int r = tid; r < a.n_req; r += kThreads) {
+    int q0, n, len;
+    request(a, r, &q0, &n, &len);
+    if (t >= q0 && t < q0 + n) atomicMin(&owner, r);
+  }
+  __syncthreads();
+  const int r = owner;
+  if (r == a.n_req) return;
+  int q0, n, len, tiles, units;
+  request(a, r, &q0, &n, &len);
+  tiles_units<R, U>(a, n, len, &tiles, &units);
+  const int head = a.grp.div(h), at_row = (t - q0) * a.group + (h - head * a.group);
+  const int tile = at_row / R, row = at_row - tile * R;
+  const int64_t total = sp.prefix[a.n_req];
+  const int64_t u0 = sp.prefix[r] + (static_cast<int64_t>(head) * tiles + tile) * units, u1 = u0 + units;
+  const int64_t base = total / sp.workers, rest = total - base * sp.workers;
+  // the worker of a unit
+  const int64_t big = rest * (base + 1);
+  const int w0 = static_cast<int>(u0 < big ? u0 / (base + 1) : rest + (u0 - big) / base);
+  const int64_t ul = u1 - 1;
+  const int w1 = static_cast<int>(ul < big ? ul / (base + 1) : rest + (ul - big) / base);
+  if (w0 == w1) return;
+  float *dst = a.out + (static_cast<size_t>(t) * a.n_head + h) * HD;
+
+  // only the first worker may have the task as its second piece
+  const auto slot = [&](int w) {
+    return static_cast<size_t>(w) * 2 + (w == w0 && run_begin(total, sp.workers, w) < u0 ? 1 : 0);
+  };
+  float top = -INFINITY;
+  for (int w = w0 + tid; w <= w1; w += kThreads) top = fmaxf(top, sp.pm[slot(w) * R + row]);
+  top = group_reduce<kThreads>(top, MaxOp{}, red);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  __syncthreads();
+  const int d = tid % kLanes * 4;
+  f32x4 o = {0, 0, 0, 0};
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int w = w0 + tid / kLanes; w <= w1; w += kAt) {
+    const size_t i = slot(w) * R + row;
+    const float keep = __builtin_amdgcn_exp2f(sp.pm[i] - ref);
+    sum += keep * sp.pl[i];
+    o += keep * *reinterpret_cast<const f32x4 *>(sp.pacc + i * HD + d);
+  }
+  *reinterpret_cast<f32x4 *>(&part[tid / kLanes][d]) = o;
+  if (tid % kLanes != 0) sum = 0.0f;
+  sum = group_reduce<kThreads>(sum, SumOp{}, red);  // and the parts are written
+  __syncthreads();
+  if (tid < kLanes) {
+#pragma unroll
+    for (int w = 1; w < kAt; ++w) o += *reinterpret_cast<const f32x4 *>(&part[w][d]);
+    *reinterpret_cast<f32x4 *>(dst + d) = o * (top == -INFINITY ? 0.0f : 1.0f / sum);
+  }
+}
+
+// Workers of a launch: two blocks a compute unit with one row tile, one with two.
+int workers_of(int rt) { return static_cast<int>(device_cu_count()) * (rt == 1 ? 2 : 1); }
+
+size_t align256(size_t n) { return (n + 255) & ~size_t{255}; }
+
+// Workspace: prefix, maxima, sums, accumulators.
+size_t workspace_of(size_t n_req, size_t hd, int rt) {
+  const size_t parts = static_cast<size_t>(workers_of(rt)) * 2 * 16 * rt;
+  return align256((n_req + 1) * 8) + 2 * align256(parts * 4) + parts * hd * 4;
+}
+
+template <class E>
+int launch(const PagedArgs &a, char *ws, hipStream_t st) {
+  constexpr int R = 16 * E::kRt, U = E::kStep * kWaves;
+  Split sp{};
+  sp.workers = workers_of(E::kRt);
+  const size_t parts = static_cast<size_t>(sp.workers) * 2 * R;
+  sp.prefix = reinterpret_cast<int64_t *>(ws);
+  ws += align256((static_cast<size_t>(a.n_req) + 1) * 8);
+  sp.pm = reinterpret_cast<float *>(ws);
+  ws += align256(parts * 4);
+  sp.pl = reinterpret_cast<float *>(ws);
+  ws += align256(parts * 4);
+  sp.pacc = reinterpret_cast<float *>(ws);
+  BH_LAUNCH(attn_paged_kernel<E>, static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
+  if (a.max_len > U) {  // with one unit a task nothing is split
+    const dim3 grid(static_cast<unsigned>(a.n_tok), static_cast<unsigned>(a.n_head));
+    BH_LAUNCH((attn_paged_join_kernel<E::kHd, R, U>), grid, kThreads, 0, st, a, sp);
+  }
+  return BH_OK;
+}
+
+template <int RT>
+int launch_rt(const PagedArgs &a, bool f16, char *ws, hipStream_t st) {
+  if (f16) {
+    if (a.hd == 64) return launch<EngineF16<64, RT>>(a, ws, st);
+    if (a.hd == 128) return launch<EngineF16<128, RT>>(a, ws, st);
+    return launch<EngineF16<256, RT>>(a, ws, st);
+  }
+  if (a.hd == 64) return launch<EngineF32<64, RT>>(a, ws, st);
+  if (a.hd == 128) return launch<EngineF32<128, RT>>(a, ws, st);
+  return launch<EngineF32<256, RT>>(a, ws, st);
+}
+
+// Whether a call runs on the matrix cores: rows of whole 16-byte pieces.
+bool on_matrix_cores(const bh_attention_paged_args &p) {
+  const bh_paged_cache &c = p.cache;
+  const size_t piece = c.kv_dtype == BH_KV_F16 ? 8 : 4;
+  return (c.hd == 64 || c.hd == 128 || c.hd == 256) && c.page_stride % piece == 0 &&
+         c.pos_stride % piece == 0 && c.head_stride % piece == 0 && aligned16(c.k) &&
+         aligned16(c.v) && aligned16(p.q) && aligned16(p.out);
+}
+
+// Row tiles a block: two where a request may have more than 16 rows a kv head.
+int row_tiles(const bh_attention_paged_args &p) {
+  const size_t most = p.max_new == 0 || p.max_new > p.n_tok ? p.n_tok : p.max_new;
+  return most * (p.n_head / p.cache.n_kv) <= 16 ? 1 : 2;
+}
+
 // Checks the arguments and fills `a`.
 int prepare(const bh_attention_paged_args &p, PagedArgs *a) {
   const bh_paged_cache &c = p.cache;
@@ -148,6 +912,7 @@ int prepare(const bh_attention_paged_args &p, PagedArgs *a) {
   a->max_len = static_cast<int>(p.table_width * c.page_size);
   a->scale = 1.0f / sqrtf(static_cast<float>(c.hd));
   a->page = FastDiv(static_cast<uint32_t>(c.page_size));
+  a->grp = FastDiv(static_cast<uint32_t>(a->group));
   return BH_OK;
 }
 
@@ -157,18 +922,40 @@ int prepare(const bh_attention_paged_args &p, PagedArgs *a) {
 using namespace bh;
 
 extern "C" size_t bh_attention_paged_workspace(const bh_attention_paged_args *args) {
-  return 0;
+  PagedArgs a{};
+  if (!args || prepare(*args, &a) != BH_OK || !on_matrix_cores(*args)) return 0;
+  if (a.n_tok == 0 || a.n_req == 0) return 0;
+  return workspace_of(args->n_req, args->cache.hd, row_tiles(*args));
 }
 
 extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream stream) {
   if (!args) return fail(BH_ERR_ARG, "attention_paged: null args");
+  const bh_attention_paged_args &p = *args;
   PagedArgs a{};
-  if (int e = prepare(*args, &a)) return e;
+  if (int e = prepare(p, &a)) return e;
   if (a.n_tok == 0 || a.n_req == 0) return ok();
+  const bool f16 = p.cache.kv_dtype == BH_KV_F16;
+  hipStream_t st = as_stream(stream);
+  if (on_matrix_cores(p)) {
+    const int rt = row_tiles(p);
+    const size_t need = workspace_of(p.n_req, p.cache.hd, rt);
+    char *ws = static_cast<char *>(p.workspace);
+    if (ws) {
+      if (!aligned16(ws) || p.workspace_bytes < need)
+        return fail(BH_ERR_SHAPE, "attention_paged: workspace of " +
+                                      std::to_string(p.workspace_bytes) + " bytes, " +
+                                      std::to_string(need) + " needed on a 16-byte boundary");
+    } else {
+      ws = static_cast<char *>(device_scratch(need, kScratchPaged, st));
+      if (!ws) return BH_ERR_HIP;
+    }
+    if (int e = rt == 1 ? launch_rt<1>(a, f16, ws, st) : launch_rt<2>(a, f16, ws, st)) return e;
+    return ok();
+  }
   const dim3 grid(static_cast<unsigned>(a.n_tok), static_cast<unsigned>(a.n_head));
-  if (args->cache.kv_dtype == BH_KV_F16)
-    BH_LAUNCH(attn_paged_any_kernel<_Float16>, grid, 256, 0, as_stream(stream), a);
+  if (f16)
+    BH_LAUNCH(attn_paged_any_kernel<_Float16>, grid, 256, 0, st, a);
   else
-    BH_LAUNCH(attn_paged_any_kernel<float>, grid, 256, 0, as_stream(stream), a);
+    BH_LAUNCH(attn_paged_any_kernel<float>, grid, 256, 0, st, a);
   return ok();
 }
