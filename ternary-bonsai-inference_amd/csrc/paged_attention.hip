@@ -131,17 +131,39 @@ constexpr int kJoinRows = 8;        // rows of a tile that the waves join at a t
 
 // Where a call's work lies.  A request with n tokens has ceil(n group / R) row
 // tiles a kv head and ceil(len / U) units of U positions; the list of all
-// (request, kv head, row tile, unit) is cut into equal runs, one a worker.
+// (request, kv head, row tile, unit) is cut into equal runs, one a worker.  Of the
+// tiles in a run only the first and the last can be cut: their parts go to the
+// worker's slots 0 and 1.
+struct Cut {  // a tile, written by the worker of its first part
+  int rows;         // 0: it has one part, and its rows are done
+  int first, last;  // workers of its parts
+  int slot;         // of the first part; the others are in their workers' slots 0
+  int row0;         // its first row: (token, head of the group) pairs of the request
+  int q0, head;
+};
 struct Split {
-  int64_t *prefix;  // [n_req + 1] units before a request, written by worker 0
-  float *pm, *pl;   // [workers][2][R] running maximum (base 2) and sum
-  float *pacc;      // [workers][2][R][hd]
+  int *n_tiles;    // one word
+  Cut *cut;        // [n_tiles]
+  float *pm, *pl;  // [workers][2][R] running maximum (base 2) and sum
+  float *pacc;     // [workers][2][R][hd]
   int workers;
 };
 
-__host__ __device__ __forceinline__ int64_t run_begin(int64_t total, int workers, int w) {
-  const int64_t base = total / workers, rest = total - base * workers;
+// x / d; by the 32-bit divide, a tenth of the 64-bit one, where that does.
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t d) {
+  if ((x | d) >> 32 == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(d);
+  return x / d;
+}
+__device__ __forceinline__ int64_t run_begin(int64_t total, int workers, int w) {
+  const int64_t base = divide(total, workers), rest = total - base * workers;
   return w * base + (w < rest ? w : rest);
+}
+
+// The worker whose run holds unit u.
+__device__ __forceinline__ int worker_of(int64_t total, int workers, int64_t u) {
+  const int64_t base = divide(total, workers), rest = total - base * workers;
+  const int64_t big = rest * (base + 1);
+  return static_cast<int>(u < big ? divide(u, base + 1) : rest + divide(u - big, base));
 }
 
 template <int R, int U>
@@ -151,33 +173,44 @@ __device__ __forceinline__ void tiles_units(const PagedArgs &a, int n, int len, 
   *units = max((len + U - 1) / U, 1);
 }
 
-// f16 cache: 32 positions a step on v_mfma_f32_16x16x32_f16.
+// f16 cache: SUB times 16 positions a step on v_mfma_f32_16x16x32_f16.
 //
 // S^T = K Q^T: a lane (g = lane / 16, c = lane % 16) loads 16 bytes of position c's
 // row (dims 32 kk + 8 g ..) as its A operand, straight from memory; q stands in LDS
 // as B operands, split into f16 hi + lo (22 bits) after an exact power of two
 // that brings the row's largest to 2^14 .. 2^15.  Lane (g, c) gets the scores of
 // row c at positions 16 s + 4 g + i.
-// O^T = V^T P^T: with the k index of a lane's eight slots taken as those same
+// O^T = V^T P^T: with the k index of a lane's 4 SUB slots taken as those same
 // positions, its scores are its B operand as they stand (hi + lo), and the A
-// operand is what the lane has loaded: 8 positions by 8 dims, transposed by one
+// operand is what the lane has loaded: its positions by 8 dims, transposed by one
 // v_perm a pair.  Row c's output and running state stay with the lanes of c.
+// With hd 256 a step is 16 positions: at 32 the accumulators and both tiles take
+// 192 of the 256 registers of two waves a SIMD and the rest spills (64 requests
+// at 16384 positions: 1222 us, ____ with 16).
 template <int HD, int RT>
 struct EngineF16 {
   using Elem = _Float16;
-  static constexpr int kHd = HD, kRt = RT, kStep = 32;
+  static constexpr int SUB = HD >= 256 ? 1 : 2;
+  static constexpr int kHd = HD, kRt = RT, kStep = 16 * SUB;
   static constexpr int KK = HD / 32, DV = HD >= 128 ? 8 : 4, NB = HD / (16 * DV);
   static constexpr int kQBytes = RT * KK * 2 * 64 * 16;
+  static constexpr int kSlots = 4 * SUB;  // positions of a lane
+  static constexpr float kAccUnit = 1.0f / kPUnit;
   typedef _Float16 VVec __attribute__((ext_vector_type(DV)));
+  typedef _Float16 PVec __attribute__((ext_vector_type(kSlots)));
 
-  h8 k[2][KK];
-  VVec v[8][NB];
+  h8 k[SUB][KK];
+  VVec v[kSlots][NB];
   f32x4 acc[RT][NB][DV];
-  float sc[RT][8];
-  h8 phi[RT], plo[RT];
+  float sc[RT][kSlots];
+  PVec phi[RT], plo[RT];
 
   // Index of a lane's slot j among the positions of a step.
   static __device__ __forceinline__ int pos_of(int g, int j) { return (j & 4) * 4 + 4 * g + (j & 3); }
+  static __device__ __forceinline__ f32x4 mma(PVec a, PVec b, f32x4 c) {
+    if constexpr (SUB == 2) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+  }
 
   static __device__ __forceinline__ void store_q(char *lds, int row, int d, float4 x, float up) {
     const int kk = d / 32, g = d % 32 / 8, e = d % 8;
@@ -193,7 +226,7 @@ struct EngineF16 {
   __device__ __forceinline__ void load_k(const Elem *kc, const int64_t *off, int lane) {
     const int g = lane >> 4, c = lane & 15;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < SUB; ++s) {
       const Elem *row = kc + off[16 * s + c] + 8 * g;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) k[s][kk] = *reinterpret_cast<const h8 *>(row + 32 * kk);
@@ -202,7 +235,7 @@ struct EngineF16 {
   __device__ __forceinline__ void load_v(const Elem *vc, const int64_t *off, int lane) {
     const int g = lane >> 4, c = lane & 15;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kSlots; ++j) {
       const Elem *row = vc + off[pos_of(g, j)] + DV * c;
 #pragma unroll
       for (int b = 0; b < NB; ++b) v[j][b] = *reinterpret_cast<const VVec *>(row + 16 * DV * b);
@@ -212,7 +245,10 @@ struct EngineF16 {
     const h8 *q = reinterpret_cast<const h8 *>(lds) + lane;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+      // one chain for each half of q, summed at the end: the small ones first
+      f32x4 sh[SUB], sl[SUB];
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) sh[s] = sl[s] = f32x4{0, 0, 0, 0};
       h8 hi_next = q[t * KK * 128], lo_next = q[t * KK * 128 + 64];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
@@ -223,37 +259,40 @@ struct EngineF16 {
           hi_next = q[(t * KK + kk + 1) * 128];
           lo_next = q[(t * KK + kk + 1) * 128 + 64];
         }
-        s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][kk], hi, s0, 0, 0, 0);
-        s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][kk], hi, s1, 0, 0, 0);
-        s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][kk], lo, s0, 0, 0, 0);
-        s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][kk], lo, s1, 0, 0, 0);
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          sh[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], hi, sh[s], 0, 0, 0);
+          sl[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], lo, sl[s], 0, 0, 0);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[t][i] = s0[i], sc[t][4 + i] = s1[i];
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[t][4 * s + i] = sl[s][i] + sh[s][i];
     }
   }
   // sc holds the probabilities: their halves.
   __device__ __forceinline__ void split_p(int t) {
-    const f32x4 a = f32x4{sc[t][0], sc[t][1], sc[t][2], sc[t][3]} * kPUnit;
-    const f32x4 b = f32x4{sc[t][4], sc[t][5], sc[t][6], sc[t][7]} * kPUnit;
-    const h4 ah = __builtin_convertvector(a, h4), bh = __builtin_convertvector(b, h4);
-    const h4 al = __builtin_convertvector(a - __builtin_convertvector(ah, f32x4), h4);
-    const h4 bl = __builtin_convertvector(b - __builtin_convertvector(bh, f32x4), h4);
-    phi[t] = __builtin_shufflevector(ah, bh, 0, 1, 2, 3, 4, 5, 6, 7);
-    plo[t] = __builtin_shufflevector(al, bl, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      const float x = sc[t][j] * kPUnit;
+      phi[t][j] = static_cast<_Float16>(x);
+      plo[t][j] = static_cast<_Float16>(x - static_cast<float>(phi[t][j]));
+    }
   }
   __device__ __forceinline__ void values() {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < DV; ++e) {
-        __builtin_amdgcn_sched_barrier(0);
-        const h8 x = {v[0][b][e], v[1][b][e], v[2][b][e], v[3][b][e],
-                      v[4][b][e], v[5][b][e], v[6][b][e], v[7][b][e]};
+        if (e % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        PVec x;
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) x[j] = v[j][b][e];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          acc[t][b][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, phi[t], acc[t][b][e], 0, 0, 0);
-          acc[t][b][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, plo[t], acc[t][b][e], 0, 0, 0);
+          acc[t][b][e] = mma(x, phi[t], acc[t][b][e]);
+          acc[t][b][e] = mma(x, plo[t], acc[t][b][e]);
         }
       }
   }
@@ -304,8 +343,6 @@ struct EngineF16 {
 #pragma unroll
         for (int e = 0; e < DV; ++e) acc[t][b][e] = f32x4{0, 0, 0, 0};
   }
-  static constexpr int kSlots = 8;            // positions of a lane
-  static constexpr float kAccUnit = 1.0f / kPUnit;
   __device__ __forceinline__ void drop_value(int j) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) v[j][b] = VVec{};
@@ -459,9 +496,24 @@ struct Rows {
                                    static_cast<int64_t>(a.pos_stride)
                          : 0;
     if (lane < STEP) off[lane] = o;
-    return static_cast<uint32_t>(__ballot(in)) & (STEP == 32 ? ~0u : (1u << STEP) - 1);
+    return static_cast<uint32_t>(__ballot(in)) & (~0u >> (32 - STEP));
   }
 };
+
+// Running totals over the wave's lanes, this lane's included.
+__device__ __forceinline__ void wave_scan(int64_t *x, int *y, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t ox = __shfl_up(*x, d);
+    const int oy = __shfl_up(*y, d);
+    if (lane >= d) *x += ox, *y += oy;
+  }
+}
+__device__ __forceinline__ int64_t wave_uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
 
 template <class E>
 __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kernel(PagedArgs a, Split sp) {
@@ -473,66 +525,81 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
   __shared__ __attribute__((aligned(16))) char lds[kLds];
   __shared__ int64_t off_s[kWaves][2][STEP];
   __shared__ float fac_s[R], m_s[kWaves][R], l_s[kWaves][R];
-  __shared__ int64_t scan_s[kWaves];
-  __shared__ int64_t first_s[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int g = lane >> 4, c = lane & 15;
 
-  // the run of this worker in the list of all units
-  const int per = (a.n_req + kThreads - 1) / kThreads;
+  // The run of this worker in the list of all units.  Every wave finds it by
+  // itself: lane i adds up requests i per .. (i + 1) per - 1, a scan over the
+  // lanes gives the total, and the lanes then go through the one lane's requests
+  // that hold the run's beginning.
+  const int worker = blockIdx.x;
+  const int per = (a.n_req + 63) / 64;
+  int q0 = 0, n = 0, len = 0, tiles = 0, units = 1;
   int64_t mine = 0;
-  for (int r = tid * per; r < min((tid + 1) * per, a.n_req); ++r) {
-    int q0, n, len, tiles, units;
-    request(a, r, &q0, &n, &len);
+  int mine_tiles = 0;
+  for (int i = lane * per; i < min((lane + 1) * per, a.n_req); ++i) {
+    request(a, i, &q0, &n, &len);
     tiles_units<R, U>(a, n, len, &tiles, &units);
     mine += static_cast<int64_t>(tiles) * a.n_kv * units;
+    mine_tiles += tiles * a.n_kv;
   }
-  int64_t run = mine;
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(run, d);
-    if (lane >= d) run += o;
-  }
-  if (lane == 63) scan_s[wave] = run;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) run += scan_s[w];
-    total += scan_s[w];
-  }
-  const int worker = blockIdx.x;
+  int64_t upto = mine;
+  int upto_tiles = mine_tiles;
+  wave_scan(&upto, &upto_tiles, lane);
+  const int64_t total = wave_uniform(__shfl(upto, 63));
   const int64_t begin = run_begin(total, sp.workers, worker);
   const int64_t end = run_begin(total, sp.workers, worker + 1);
-  int64_t before = run - mine;
-  if ((worker == 0 && sp.prefix) || (before <= begin && begin < run)) {
-    for (int r = tid * per; r < min((tid + 1) * per, a.n_req); ++r) {
-      int q0, n, len, tiles, units;
-      request(a, r, &q0, &n, &len);
-      tiles_units<R, U>(a, n, len, &tiles, &units);
-      const int64_t cost = static_cast<int64_t>(tiles) * a.n_kv * units;
-      if (worker == 0 && sp.prefix) sp.prefix[r] = before;
-      if (before <= begin && begin < before + cost) first_s[0] = r, first_s[1] = before;
-      before += cost;
+  if (worker == 0 && tid == 63) *sp.n_tiles = upto_tiles;
+  if (begin >= end) return;
+  int owner = __builtin_ffsll(__ballot(begin < upto)) - 1;
+  int64_t base = wave_uniform(__shfl(upto - mine, owner));
+  int tile_base = __builtin_amdgcn_readlane(upto_tiles - mine_tiles, owner);
+  int r = __builtin_amdgcn_readfirstlane(owner);
+  if (per > 1) {
+    for (int i = owner * per;; i += 64) {
+      mine = 0;
+      mine_tiles = 0;
+      if (i + lane < min((owner + 1) * per, a.n_req)) {
+        request(a, i + lane, &q0, &n, &len);
+        tiles_units<R, U>(a, n, len, &tiles, &units);
+        mine = static_cast<int64_t>(tiles) * a.n_kv * units;
+        mine_tiles = tiles * a.n_kv;
+      }
+      upto = mine;
+      upto_tiles = mine_tiles;
+      wave_scan(&upto, &upto_tiles, lane);
+      upto += base;
+      upto_tiles += tile_base;
+      const uint64_t past = __ballot(begin < upto);
+      if (past) {
+        const int at_lane = __builtin_ffsll(past) - 1;
+        r = i + at_lane;
+        base = wave_uniform(__shfl(upto - mine, at_lane));
+        tile_base = __builtin_amdgcn_readlane(upto_tiles - mine_tiles, at_lane);
+        owner = at_lane;
+        break;
+      }
+      base = wave_uniform(__shfl(upto, 63));
+      tile_base = __builtin_amdgcn_readlane(upto_tiles, 63);
     }
   }
-  if (worker == 0 && sp.prefix && tid == 0) sp.prefix[a.n_req] = total;
-  if (begin >= end) return;
-  __syncthreads();
-  int r = static_cast<int>(first_s[0]);
-  int64_t base = first_s[1];
+  r = __builtin_amdgcn_readfirstlane(r);
+  q0 = __builtin_amdgcn_readlane(q0, owner), n = __builtin_amdgcn_readlane(n, owner);
+  len = __builtin_amdgcn_readlane(len, owner), tiles = __builtin_amdgcn_readlane(tiles, owner);
+  units = __builtin_amdgcn_readlane(units, owner);
 
-  E eng;
   for (int64_t at = begin; at < end;) {
-    int q0, n, len, tiles, units;
-    request(a, r, &q0, &n, &len);
-    tiles_units<R, U>(a, n, len, &tiles, &units);
     const int64_t cost = static_cast<int64_t>(tiles) * a.n_kv * units;
     if (at - base >= cost) {  // on to the next request
       base += cost;
+      tile_base += tiles * a.n_kv;
       ++r;
+      request(a, r, &q0, &n, &len);
+      tiles_units<R, U>(a, n, len, &tiles, &units);
       continue;
     }
     const int64_t x = at - base;
-    const int task = static_cast<int>(x / units), unit = static_cast<int>(x - static_cast<int64_t>(task) * units);
+    const int task = static_cast<int>(divide(x, units)), unit = static_cast<int>(x - static_cast<int64_t>(task) * units);
     const int head = task / tiles, tile = task - head * tiles;
     const int unit_end = static_cast<int>(min<int64_t>(units, unit + (end - at)));
     const int rows = min(R, n * a.group - tile * R);
@@ -544,36 +611,51 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
     const Elem *kc = static_cast<const Elem *>(a.kc) + head * a.head_stride;
     const Elem *vc = static_cast<const Elem *>(a.vc) + head * a.head_stride;
 
-    // this wave's first rows on their way
+    // the table entries of this wave's first rows and the block's q rows on their
+    // way together, then the cache rows, then q into LDS as matrix operands
     int p0 = unit * U + wave * STEP;
     Rows<STEP> rows_of;
     rows_of.fetch(a, table, p0 + lane % STEP, p_end);
-
-    // q into LDS as matrix operands
-    __syncthreads();
-    {
-      constexpr int kLanes = HD / 4, kAt = kThreads / kLanes;  // lanes of a row, rows at once
-      for (int i = tid / kLanes; i < R; i += kAt) {
-        const int d = tid % kLanes * 4;
-        const int row = tile * R + i, tok = a.grp.div(row);
-        float4 qv = make_float4(0, 0, 0, 0);
-        if (i < rows)
-          qv = *reinterpret_cast<const float4 *>(
-              a.q + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
-                     (row - tok * a.group)) * HD + d);
-        float up = 1.0f, down = a.scale;
-        if constexpr (E::kScaleQ) {
-          float mx = fmaxf(fmaxf(fabsf(qv.x), fabsf(qv.y)), fmaxf(fabsf(qv.z), fabsf(qv.w)));
-          mx = lane_group_reduce<kLanes>(mx, MaxOp{});
-          int ex = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
-          if (ex > -127 && ex < 128) {
-            ex = max(ex, -100);
-            up = ldexpf(1.0f, 14 - ex);
-            down = ldexpf(a.scale, ex - 14);
-          }
+    constexpr int kLanes = HD / 4, kAt = kThreads / kLanes;  // lanes of a row, rows at once
+    constexpr int kQ = (R + kAt - 1) / kAt;
+    float4 qv[kQ];
+    const int qd = tid % kLanes * 4;
+#pragma unroll
+    for (int x = 0; x < kQ; ++x) {
+      const int i = tid / kLanes + x * kAt, row = tile * R + i, tok = a.grp.div(row);
+      qv[x] = make_float4(0, 0, 0, 0);
+      if (i < rows)
+        qv[x] = *reinterpret_cast<const float4 *>(
+            a.q + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                   (row - tok * a.group)) * HD + qd);
+    }
+    E eng;
+    uint32_t mask = 0;
+    if (p0 < p_end) {
+      mask = rows_of.place(a, off_s[wave][0], p0 + lane % STEP, p_end, lane);
+      eng.load_k(kc, off_s[wave][0], lane);
+      eng.load_v(vc, off_s[wave][0], lane);
+      rows_of.fetch(a, table, p0 + U + lane % STEP, p_end);
+    }
+    __syncthreads();  // the piece before has been read
+#pragma unroll
+    for (int x = 0; x < kQ; ++x) {
+      const int i = tid / kLanes + x * kAt;
+      float up = 1.0f, down = a.scale;
+      if constexpr (E::kScaleQ) {
+        float mx = fmaxf(fmaxf(fabsf(qv[x].x), fabsf(qv[x].y)),
+                         fmaxf(fabsf(qv[x].z), fabsf(qv[x].w)));
+        mx = lane_group_reduce<kLanes>(mx, MaxOp{});
+        int ex = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+        if (ex > -127 && ex < 128) {
+          ex = max(ex, -100);
+          up = ldexpf(1.0f, 14 - ex);
+          down = ldexpf(a.scale, ex - 14);
         }
-        E::store_q(lds, i, d, qv, up);
-        if (d == 0) fac_s[i] = down * kExpL2E;
+      }
+      if (kQ * kAt == R || i < R) {
+        E::store_q(lds, i, qd, qv[x], up);
+        if (qd == 0) fac_s[i] = down * kExpL2E;
       }
     }
     __syncthreads();
@@ -592,10 +674,6 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
     }
     eng.clear();
     if (p0 < p_end) {
-      uint32_t mask = rows_of.place(a, off_s[wave][0], p0 + lane % STEP, p_end, lane);
-      eng.load_k(kc, off_s[wave][0], lane);
-      eng.load_v(vc, off_s[wave][0], lane);
-      rows_of.fetch(a, table, p0 + U + lane % STEP, p_end);
       for (int s = 1;; s ^= 1) {
         const int next = p0 + U;
         eng.scores(lds, lane);
@@ -605,7 +683,7 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
           eng.load_k(kc, off_s[wave][s], lane);
           rows_of.fetch(a, table, next + U + lane % STEP, p_end);
         }
-        constexpr uint32_t kAll = STEP == 32 ? ~0u : (1u << STEP) - 1;
+        constexpr uint32_t kAll = ~0u >> (32 - STEP);
         const bool edge = mask != kAll || p0 + STEP > min_vis;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -753,71 +831,86 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
           }
         }
       }
+    if (unit == 0 && tid == 0) {
+      Cut cut{whole ? 0 : rows, worker, worker, at == begin ? 0 : 1, tile * R, q0, head};
+      if (!whole) cut.last = worker_of(total, sp.workers, at + units - 1);
+      sp.cut[tile_base + task] = cut;
+    }
     at += unit_end - unit;
   }
 }
 
-// Joins the parts of the rows that more than one worker has: a block per
-// (token, head).
-template <int HD, int R, int U>
-__global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, Split sp) {
-  constexpr int kLanes = HD / 4, kAt = kThreads / kLanes;
-  __shared__ int owner;
-  __shared__ float part[kAt][HD], red[kWaves];
-  const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  if (tid == 0) owner = a.n_req;
-  __syncthreads();
-  for (int r = tid; r < a.n_req; r += kThreads) {
-    int q0, n, len;
-    request(a, r, &q0, &n, &len);
-    if (t >= q0 && t < q0 + n) atomicMin(&owner, r);
-  }
-  __syncthreads();
-  const int r = owner;
-  if (r == a.n_req) return;
-  int q0, n, len, tiles, units;
-  request(a, r, &q0, &n, &len);
-  tiles_units<R, U>(a, n, len, &tiles, &units);
-  const int head = a.grp.div(h), at_row = (t - q0) * a.group + (h - head * a.group);
-  const int tile = at_row / R, row = at_row - tile * R;
-  const int64_t total = sp.prefix[a.n_req];
-  const int64_t u0 = sp.prefix[r] + (static_cast<int64_t>(head) * tiles + tile) * units, u1 = u0 + units;
-  const int64_t base = total / sp.workers, rest = total - base * sp.workers;
-  // the worker of a unit
-  const int64_t big = rest * (base + 1);
-  const int w0 = static_cast<int>(u0 < big ? u0 / (base + 1) : rest + (u0 - big) / base);
-  const int64_t ul = u1 - 1;
-  const int w1 = static_cast<int>(ul < big ? ul / (base + 1) : rest + (ul - big) / base);
-  if (w0 == w1) return;
-  float *dst = a.out + (static_cast<size_t>(t) * a.n_head + h) * HD;
-
-  // only the first worker may have the task as its second piece
-  const auto slot = [&](int w) {
-    return static_cast<size_t>(w) * 2 + (w == w0 && run_begin(total, sp.workers, w) < u0 ? 1 : 0);
-  };
-  float top = -INFINITY;
-  for (int w = w0 + tid; w <= w1; w += kThreads) top = fmaxf(top, sp.pm[slot(w) * R + row]);
-  top = group_reduce<kThreads>(top, MaxOp{}, red);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  __syncthreads();
-  const int d = tid % kLanes * 4;
-  f32x4 o = {0, 0, 0, 0};
-  float sum = 0.0f;
-#pragma unroll 4
-  for (int w = w0 + tid / kLanes; w <= w1; w += kAt) {
-    const size_t i = slot(w) * R + row;
-    const float keep = __builtin_amdgcn_exp2f(sp.pm[i] - ref);
-    sum += keep * sp.pl[i];
-    o += keep * *reinterpret_cast<const f32x4 *>(sp.pacc + i * HD + d);
-  }
-  *reinterpret_cast<f32x4 *>(&part[tid / kLanes][d]) = o;
-  if (tid % kLanes != 0) sum = 0.0f;
-  sum = group_reduce<kThreads>(sum, SumOp{}, red);  // and the parts are written
-  __syncthreads();
-  if (tid < kLanes) {
+// Joins the parts of the tiles that more than one worker has: `share` blocks a
+// tile, each over every share-th (row, 64 dims) of it.  16 lanes take the dims, 16
+// threads each every sixteenth part, whose loads are all issued before the first
+// is needed: one round trip for up to 16 kAhead parts.
+template <int HD, int R>
+__global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, Split sp, int share) {
+  constexpr int kAt = kThreads / 16, kSlices = HD / 64, kAhead = 8;
+  __shared__ float part[kAt][64], sums[kAt], red[kWaves];
+  const int tile = blockIdx.x / share, tid = threadIdx.x;
+  const Cut cut = sp.cut[tile];
+  if (tile >= *sp.n_tiles) return;  // cut holds nothing then
+  const int lane_part = tid >> 4, d = (tid & 15) * 4;
+  for (int i = blockIdx.x - tile * share; i < cut.rows * kSlices; i += share) {
+    const int row = i / kSlices, dim = i % kSlices * 64 + d;
+    const auto at = [&](int w) {
+      return (static_cast<size_t>(w) * 2 + (w == cut.first ? cut.slot : 0)) * R + row;
+    };
+    f32x4 ahead[kAhead];
+    float pm[kAhead], pl[kAhead];
 #pragma unroll
-    for (int w = 1; w < kAt; ++w) o += *reinterpret_cast<const f32x4 *>(&part[w][d]);
-    *reinterpret_cast<f32x4 *>(dst + d) = o * (top == -INFINITY ? 0.0f : 1.0f / sum);
+    for (int x = 0; x < kAhead; ++x) {
+      // past the last part: the last again, at no weight
+      const int w = cut.first + lane_part + x * kAt;
+      if (cut.first + x * kAt > cut.last) break;
+      const size_t o = at(min(w, cut.last));
+      ahead[x] = *reinterpret_cast<const f32x4 *>(sp.pacc + o * HD + dim);
+      pm[x] = sp.pm[o];
+      pl[x] = sp.pl[o];
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      if (cut.first + x * kAt > cut.last) break;
+      top = fmaxf(top, pm[x]);
+    }
+    for (int w = cut.first + lane_part + kAhead * kAt; w <= cut.last; w += kAt)
+      top = fmaxf(top, sp.pm[at(w)]);
+    top = group_reduce<kThreads>(top, MaxOp{}, red);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    f32x4 o = {0, 0, 0, 0};
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      if (cut.first + x * kAt > cut.last) break;
+      if (cut.first + lane_part + x * kAt > cut.last) continue;
+      const float keep = __builtin_amdgcn_exp2f(pm[x] - ref);
+      sum += keep * pl[x];
+      o += keep * ahead[x];
+    }
+#pragma unroll 4
+    for (int w = cut.first + lane_part + kAhead * kAt; w <= cut.last; w += kAt) {
+      const size_t p = at(w);
+      const float keep = __builtin_amdgcn_exp2f(sp.pm[p] - ref);
+      sum += keep * sp.pl[p];
+      o += keep * *reinterpret_cast<const f32x4 *>(sp.pacc + p * HD + dim);
+    }
+    *reinterpret_cast<f32x4 *>(&part[lane_part][d]) = o;
+    if (d == 0) sums[lane_part] = sum;
+    __syncthreads();
+    if (tid < 16) {
+#pragma unroll
+      for (int w = 1; w < kAt; ++w) {
+        o += *reinterpret_cast<const f32x4 *>(&part[w][d]);
+        sum += sums[w];
+      }
+      const int q_row = cut.row0 + row, tok = a.grp.div(q_row);
+      *reinterpret_cast<f32x4 *>(
+          a.out + (static_cast<size_t>(cut.q0 + tok) * a.n_head + cut.head * a.group +
+                   (q_row - tok * a.group)) * HD + dim) = o * (top == -INFINITY ? 0.0f : 1.0f / sum);
+    }
+    __syncthreads();  // for the next row
   }
 }
 
@@ -826,10 +919,17 @@ int workers_of(int rt) { return static_cast<int>(device_cu_count()) * (rt == 1 ?
 
 size_t align256(size_t n) { return (n + 255) & ~size_t{255}; }
 
-// Workspace: prefix, maxima, sums, accumulators.
-size_t workspace_of(size_t n_req, size_t hd, int rt) {
+// Tiles that a call can have at most.
+size_t most_tiles(const PagedArgs &a, int R) {
+  const size_t rows = static_cast<size_t>(a.n_tok) * a.group;
+  return static_cast<size_t>(a.n_kv) * (rows / R + (static_cast<size_t>(a.n_req) < static_cast<size_t>(a.n_tok) ? a.n_req : a.n_tok));
+}
+
+// Workspace: tile count, tiles, maxima, sums, accumulators.
+size_t workspace_of(const PagedArgs &a, int rt) {
   const size_t parts = static_cast<size_t>(workers_of(rt)) * 2 * 16 * rt;
-  return align256((n_req + 1) * 8) + 2 * align256(parts * 4) + parts * hd * 4;
+  return 256 + align256(most_tiles(a, 16 * rt) * sizeof(Cut)) + 2 * align256(parts * 4) +
+         parts * a.hd * 4;
 }
 
 template <class E>
@@ -837,18 +937,24 @@ int launch(const PagedArgs &a, char *ws, hipStream_t st) {
   constexpr int R = 16 * E::kRt, U = E::kStep * kWaves;
   Split sp{};
   sp.workers = workers_of(E::kRt);
-  const size_t parts = static_cast<size_t>(sp.workers) * 2 * R;
-  sp.prefix = reinterpret_cast<int64_t *>(ws);
-  ws += align256((static_cast<size_t>(a.n_req) + 1) * 8);
+  const size_t parts = static_cast<size_t>(sp.workers) * 2 * R, tiles = most_tiles(a, R);
+  sp.n_tiles = reinterpret_cast<int *>(ws);
+  ws += 256;
+  sp.cut = reinterpret_cast<Cut *>(ws);
+  ws += align256(tiles * sizeof(Cut));
   sp.pm = reinterpret_cast<float *>(ws);
   ws += align256(parts * 4);
   sp.pl = reinterpret_cast<float *>(ws);
   ws += align256(parts * 4);
   sp.pacc = reinterpret_cast<float *>(ws);
   BH_LAUNCH(attn_paged_kernel<E>, static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
-  if (a.max_len > U) {  // with one unit a task nothing is split
-    const dim3 grid(static_cast<unsigned>(a.n_tok), static_cast<unsigned>(a.n_head));
-    BH_LAUNCH((attn_paged_join_kernel<E::kHd, R, U>), grid, kThreads, 0, st, a, sp);
+  if (a.max_len > U) {  // with one unit a tile nothing is cut
+    // a block a (row, 64 dims) while they are not many times what fits the card
+    const size_t most = static_cast<size_t>(a.n_tok > 1 ? R : a.group < R ? a.group : R) * (E::kHd / 64);
+    size_t share = 16 * device_cu_count() / tiles;
+    share = share < 1 ? 1 : share > most ? most : share;
+    BH_LAUNCH((attn_paged_join_kernel<E::kHd, R>), static_cast<unsigned>(tiles * share), kThreads,
+              0, st, a, sp, static_cast<int>(share));
   }
   return BH_OK;
 }
@@ -892,7 +998,8 @@ int prepare(const bh_attention_paged_args &p, PagedArgs *a) {
                                   std::to_string(kAnyMaxHd));
   size_t n;
   if (p.n_head > 65535 || p.n_tok > 0x7fffffffu || p.n_req > 0x7ffffffeu ||
-      !mul_size(p.n_tok, p.n_head * c.hd, sizeof(float), &n) || n > SIZE_MAX / 2)
+      p.n_tok * p.n_head > 0x7fffffffu || !mul_size(p.n_tok, p.n_head * c.hd, sizeof(float), &n) ||
+      n > SIZE_MAX / 2)
     return fail(BH_ERR_SHAPE, "attention_paged: size overflow");
   if (p.table_width == 0 || !mul_size(p.table_width, c.page_size, &n) || n > 0x7fffffffu)
     return fail(BH_ERR_SHAPE, "attention_paged: table_width * page_size must be 1 .. 2^31 - 1");
@@ -925,7 +1032,7 @@ extern "C" size_t bh_attention_paged_workspace(const bh_attention_paged_args *ar
   PagedArgs a{};
   if (!args || prepare(*args, &a) != BH_OK || !on_matrix_cores(*args)) return 0;
   if (a.n_tok == 0 || a.n_req == 0) return 0;
-  return workspace_of(args->n_req, args->cache.hd, row_tiles(*args));
+  return workspace_of(a, row_tiles(*args));
 }
 
 extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream stream) {
@@ -938,7 +1045,7 @@ extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream
   hipStream_t st = as_stream(stream);
   if (on_matrix_cores(p)) {
     const int rt = row_tiles(p);
-    const size_t need = workspace_of(p.n_req, p.cache.hd, rt);
+    const size_t need = workspace_of(a, rt);
     char *ws = static_cast<char *>(p.workspace);
     if (ws) {
       if (!aligned16(ws) || p.workspace_bytes < need)
