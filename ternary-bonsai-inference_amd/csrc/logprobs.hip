@@ -1,5 +1,24 @@
 // Log probabilities of given tokens, entropy and top alternatives of rows of
-// logits.
+// logits, each logit read once.
+//
+// With m a running maximum and z = (x - m) inv_temp log2(e), a thread keeps
+//   S = sum 2^z and T = sum 2^z z
+// over what it has read; a larger maximum m' moves them by d = (m - m') inv_temp
+// log2(e) to 2^d S and 2^d (T + d S).  Then log Z = m inv_temp + ln S and the
+// entropy is ln S - ln 2 T / S: two terms of one sign, so that nothing cancels for
+// a row that is sure of its token.
+//
+// Alternatives: a logit and its id make one 64-bit key in the order asked for
+// (larger first, of equal ones the lower id), so all keys differ.  Each wave
+// keeps its best n in LDS.  In a tile of 64 x 16 logits the n-th largest of the
+// lanes' own maxima is a bound that the wave's n best all reach, and at most
+// 16 n keys do; those join the kept ones, and each key's rank, counted by
+// comparing it with all of them, is its place.  Later tiles are only looked at
+// where a lane's maximum passes the n-th key kept.
+//
+// Rows are split over as many blocks as fill the card; a second launch then joins
+// a row's parts.  Bound by reading the logits where there are many, by the chain
+// load - exponentials - selection - second launch where there are few.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -11,6 +30,18 @@
 namespace bh {
 namespace {
 
+constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
+constexpr int kPer = 16;                     // logits of a thread and tile
+constexpr int kLpTile = kPer * kLpThreads;   // 4096
+constexpr int kMaxParts = 128;               // blocks of a row
+// keys of a wave: those kept (fewer than 64 between two cuts), and a tile's
+constexpr int kKeep = 64 + kPer * BH_MAX_TOP;
+
+struct Part {
+  double s, t;
+  float m;
+};
+
 struct LogprobArgs {
   const float *x;
   const uint32_t *tokens;
@@ -19,72 +50,289 @@ struct LogprobArgs {
   float *top_logprobs;
   uint32_t *bad_id;
   size_t row_stride;
-  int vocab, n_top;
-  float inv_temp;
+  int vocab, n_top, n_parts;
+  float inv_temp, k2;  // k2 = inv_temp log2(e)
+  Part *parts;         // [n_rows][n_parts]
+  uint64_t *keys;      // [n_rows][n_parts][n_top]
 };
 
-// A logit and its id as one number that grows with the order of the
-// alternatives: larger logits first, of equal ones the lower id; NaN below all.
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
   uint32_t b = __float_as_uint(x + 0.0f);  // -0 becomes 0
   b = b & 0x80000000u ? ~b : b | 0x80000000u;
-  if (x != x) b = 0;
+  if (x != x) b = 0;  // NaN below every number
   return static_cast<uint64_t>(b) << 32 | (~id);
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t b = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
 struct Max64 {
   __device__ uint64_t operator()(uint64_t a, uint64_t b) const { return a > b ? a : b; }
 };
 
-__global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
-  __shared__ double lds[4];
-  __shared__ float fl[4];
-  __shared__ uint64_t kl[4];
-  const float *x = a.x + blockIdx.x * a.row_stride;
-  float m = -INFINITY;
-  bool nan = false;
-  for (int i = threadIdx.x; i < a.vocab; i += 256) {
-    m = x[i] > m ? x[i] : m;
-    nan |= x[i] != x[i];
+__device__ __forceinline__ uint64_t lane_value(uint64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(x), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(x >> 32), lane);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// Orders the wave's LDS writes before its reads (the wave runs in step).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The n-th largest of the lanes' keys (equal ones, which are 0s, count as one).
+__device__ __forceinline__ uint64_t nth_of_lanes(uint64_t key, int n, int lane) {
+  int rank = 0;
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) rank += lane_value(key, i) > key;
+  const uint64_t at = __ballot(rank == n - 1);
+  return at ? lane_value(key, __builtin_ffsll(at) - 1) : 0;
+}
+
+// The n largest of buf[0 .. count), in order, into out and to the front of buf;
+// returns how many there are.
+__device__ __forceinline__ int keep_best(uint64_t *buf, uint64_t *out, int count, int n, int lane) {
+  wave_sync();
+  for (int k = 0; k < count; k += 64) {
+    const uint64_t mine = k + lane < count ? buf[k + lane] : 0;
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) rank += buf[j] > mine;
+    if (mine != 0 && rank < n) out[rank] = mine;
   }
-  m = group_reduce<256>(m, MaxOp{}, fl);
-  double s = 0.0, t = 0.0;
-  for (int i = threadIdx.x; i < a.vocab; i += 256) {
-    const float z = (x[i] - m) * a.inv_temp;
-    const float e = expf(z);
-    s += e;
-    if (e > 0.0f) t += static_cast<double>(e) * z;
+  count = min(count, n);
+  wave_sync();
+  if (lane < count) buf[lane] = out[lane];
+  wave_sync();
+  return count;
+}
+
+// The waves' lists of n keys (0: none) into the n largest of them all, in order;
+// 0 behind the last.  put(place, key) takes one.
+template <class F>
+__device__ __forceinline__ void merge_waves(const uint64_t (*lists)[BH_MAX_TOP], int n, F put) {
+  const int tid = threadIdx.x;
+  if (tid < kLpWaves * n) {
+    const uint64_t mine = lists[tid / n][tid % n];
+    int rank = 0, there = 0;
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w)
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        rank += lists[w][j] > mine;
+        there += lists[w][j] != 0;
+      }
+    if (mine != 0 && rank < n) put(rank, mine);
+    if (tid < n && tid >= there) put(tid, 0);
   }
-  s = group_reduce<256>(s, SumOp{}, lds);
+}
+
+// Joins the block's (m, s, t) into one; every thread gets it.
+__device__ __forceinline__ Part join_block(float m, double s, double t, float k2, float *fl,
+                                           double *dl) {
+  Part p;
+  p.m = group_reduce<kLpThreads>(m, MaxOp{}, fl);
+  if (m == -INFINITY) {  // s, t: 0, or NaN from a NaN logit
+    t = s;
+  } else {
+    const float d = (m - p.m) * k2;
+    const double by = __builtin_amdgcn_exp2f(d);
+    t = by == 0.0 ? 0.0 : by * (t + d * s);
+    s *= by;
+  }
+  p.s = group_reduce<kLpThreads>(s, SumOp{}, dl);
   __syncthreads();
-  t = group_reduce<256>(t, SumOp{}, lds);
-  const bool bad = __syncthreads_or(nan) || !(m > -INFINITY && m < INFINITY);
-  const float log_s = bad ? NAN : static_cast<float>(log(s));
+  p.t = group_reduce<kLpThreads>(t, SumOp{}, dl);
+  return p;
+}
+
+// The row's logprob and entropy from its joined sums; ln S for the alternatives.
+__device__ __forceinline__ float finish_row(const LogprobArgs &a, size_t row, const Part &p) {
+  const bool bad = !(p.m > -INFINITY && p.m < INFINITY);
+  const float log_s = bad ? NAN : static_cast<float>(log(p.s));
   if (threadIdx.x == 0) {
     if (a.logprob) {
-      const uint32_t id = a.tokens[blockIdx.x];
+      const uint32_t id = a.tokens[row];
       const bool in = id < static_cast<uint32_t>(a.vocab);
       if (!in && a.bad_id) *a.bad_id = id;
-      a.logprob[blockIdx.x] = in ? (x[id] - m) * a.inv_temp - log_s : NAN;
+      a.logprob[row] = in ? (a.x[row * a.row_stride + id] - p.m) * a.inv_temp - log_s : NAN;
     }
-    if (a.entropy) a.entropy[blockIdx.x] = bad ? NAN : static_cast<float>(log(s) - t / s);
+    if (a.entropy)
+      a.entropy[row] = bad ? NAN : static_cast<float>(log(p.s) - 0.693147180559945309 * (p.t / p.s));
   }
-  uint64_t below = ~uint64_t{0};
-  for (int j = 0; j < a.n_top; ++j) {
-    uint64_t best = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += 256) {
-      const uint64_t k = key_of(x[i], i);
-      if (k < below && k > best) best = k;
+  return log_s;
+}
+
+__device__ __forceinline__ void put_top(const LogprobArgs &a, size_t row, int place, uint64_t key,
+                                        float m, float log_s) {
+  const size_t o = row * a.n_top + place;
+  a.top_ids[o] = ~static_cast<uint32_t>(key);
+  a.top_logprobs[o] = (value_of(key) - m) * a.inv_temp - log_s;
+}
+
+// Block (row, part): the tiles of a part of a row.  Tiles begin at the row's last
+// 16-byte boundary before it, so that whole pieces load at once for any row.
+template <bool TOP>
+__global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs a) {
+  __shared__ uint64_t keep[TOP ? kLpWaves : 1][TOP ? kKeep : 1];
+  __shared__ uint64_t lists[TOP ? kLpWaves : 1][BH_MAX_TOP];
+  __shared__ float fl[kLpWaves];
+  __shared__ double dl[kLpWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const size_t row = blockIdx.x / a.n_parts;
+  const int part = blockIdx.x - row * a.n_parts;
+  const float *x = a.x + row * a.row_stride;
+  const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(x) >> 2 & 3);
+  const int64_t n = static_cast<int64_t>(a.vocab) + skew;  // places, of which `skew` before the row
+  const int64_t tiles = (n + kLpTile - 1) / kLpTile;
+  const int64_t tile0 = tiles * part / a.n_parts, tile1 = tiles * (part + 1) / a.n_parts;
+
+  float m = -INFINITY;
+  double s = 0.0, t = 0.0;
+  int count = 0;
+  uint64_t bound = 0;  // keys above this may be among the best
+  bool first = true;
+  for (int64_t tile = tile0; tile < tile1; ++tile) {
+    // id of the thread's first logit; those before the row wrap round to no id
+    const uint32_t at = static_cast<uint32_t>(tile) * kLpTile + 4 * tid - skew, vocab = a.vocab;
+    float v[kPer];
+    if (tile * kLpTile >= skew && (tile + 1) * kLpTile <= n) {
+#pragma unroll
+      for (int k = 0; k < kPer; k += 4) {
+        const float4 p = *reinterpret_cast<const float4 *>(x + at + k * kLpThreads);
+        v[k] = p.x, v[k + 1] = p.y, v[k + 2] = p.z, v[k + 3] = p.w;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
+        v[k] = id < vocab ? x[id] : -INFINITY;
+      }
     }
+    float top = v[0];
+#pragma unroll
+    for (int k = 1; k < kPer; ++k) top = fmaxf(top, v[k]);
+    if (top > m) {
+      if (m > -INFINITY) {
+        const float d = (m - top) * a.k2;
+        const double by = __builtin_amdgcn_exp2f(d);
+        t = by == 0.0 ? 0.0 : by * (t + d * s);
+        s *= by;
+      }
+      m = top;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float es = 0.0f, et = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const float z = (v[k] - ref) * a.k2;
+      const float e = __builtin_amdgcn_exp2f(z);
+      es += e;
+      et = __builtin_fmaf(e, fmaxf(z, -1000.0f), et);  // -inf has weight 0, and 0 times it
+    }
+    s += es;
+    t += et;
+
+    if constexpr (TOP) {
+      // a lane's largest; NaN logits only count while there are too few others
+      const bool look = first || __any(top > value_of(bound)) || (bound >> 32) == 0;
+      if (look) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
+          const uint64_t key = id < vocab ? key_of(v[k], id) : 0;
+          best = key > best ? key : best;
+        }
+        uint64_t from = bound + 1;
+        if (__popcll(__ballot(best > bound)) > a.n_top) {
+          const uint64_t nth = nth_of_lanes(best, a.n_top, lane);
+          from = nth > from ? nth : from;
+        }
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
+          const uint64_t key = id < vocab ? key_of(v[k], id) : 0;
+          const uint64_t pass = __ballot(key >= from);
+          if (pass == 0) continue;
+          if (key >= from)
+            keep[wave][count + __popcll(pass & ((uint64_t{1} << lane) - 1))] = key;
+          count += __popcll(pass);
+        }
+        if (first || count >= 64) {
+          count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
+          if (count == a.n_top) bound = keep[wave][a.n_top - 1];
+        }
+        first = false;
+      }
+    }
+  }
+
+  const Part p = join_block(m, s, t, a.k2, fl, dl);
+  const bool whole = a.n_parts == 1;
+  float log_s = 0.0f;
+  if (whole) log_s = finish_row(a, row, p);
+  else if (tid == 0) a.parts[blockIdx.x] = p;
+  if constexpr (TOP) {
+    count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
+    if (lane >= count && lane < a.n_top) lists[wave][lane] = 0;
     __syncthreads();
-    best = group_reduce<256>(best, Max64{}, kl);
-    below = best;
-    if (threadIdx.x == 0) {
-      const uint32_t id = ~static_cast<uint32_t>(best);
-      const size_t o = static_cast<size_t>(blockIdx.x) * a.n_top + j;
-      a.top_ids[o] = id;
-      a.top_logprobs[o] = (x[id] - m) * a.inv_temp - log_s;
+    uint64_t *out = a.keys + static_cast<size_t>(blockIdx.x) * a.n_top;
+    merge_waves(lists, a.n_top, [&](int place, uint64_t key) {
+      if (whole) put_top(a, row, place, key, p.m, log_s);
+      else out[place] = key;
+    });
+  }
+}
+
+// A row's parts: their sums joined, their lists' best keys.
+template <bool TOP>
+__global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(LogprobArgs a) {
+  constexpr int kKeys = kMaxParts * BH_MAX_TOP / kLpThreads;  // keys of a thread at most
+  __shared__ uint64_t keep[TOP ? kLpWaves : 1][TOP ? kKeep : 1];
+  __shared__ uint64_t lists[TOP ? kLpWaves : 1][BH_MAX_TOP];
+  __shared__ float fl[kLpWaves];
+  __shared__ double dl[kLpWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const size_t row = blockIdx.x;
+  uint64_t key[kKeys];
+  const int n = a.n_parts * a.n_top;
+  if constexpr (TOP) {
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k)
+      key[k] = tid + k * kLpThreads < n ? a.keys[row * n + tid + k * kLpThreads] : 0;
+  }
+  Part mine{0.0, 0.0, -INFINITY};
+  if (tid < a.n_parts) mine = a.parts[row * a.n_parts + tid];
+  const Part p = join_block(mine.m, mine.s, mine.t, a.k2, fl, dl);
+  const float log_s = finish_row(a, row, p);
+  if constexpr (TOP) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k) best = key[k] > best ? key[k] : best;
+    uint64_t from = 1;
+    if (n > 64 * kLpWaves) {  // more than a key a lane
+      const uint64_t nth = nth_of_lanes(best, a.n_top, lane);
+      from = nth > from ? nth : from;
     }
+    int count = 0;
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k) {
+      const uint64_t pass = __ballot(key[k] >= from);
+      if (pass == 0) continue;
+      if (key[k] >= from) keep[wave][count + __popcll(pass & ((uint64_t{1} << lane) - 1))] = key[k];
+      count += __popcll(pass);
+    }
+    count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
+    if (lane >= count && lane < a.n_top) lists[wave][lane] = 0;
+    __syncthreads();
+    merge_waves(lists, a.n_top, [&](int place, uint64_t k) {
+      put_top(a, row, place, k, p.m, log_s);
+    });
   }
 }
 
@@ -95,12 +343,12 @@ int check(const bh_token_logprobs_args &p) {
     return fail(BH_ERR_SHAPE, "token_logprobs: row_stride " + std::to_string(p.row_stride) +
                                   " below vocab " + std::to_string(p.vocab));
   size_t n;
-  if (p.n_rows > 0x7fffffffu || !mul_size(p.n_rows, p.row_stride, sizeof(float), &n))
+  if (p.n_rows > 0x7fffffffu / kMaxParts || !mul_size(p.n_rows, p.row_stride, sizeof(float), &n))
     return fail(BH_ERR_SHAPE, "token_logprobs: size overflow");
   if (p.n_top > BH_MAX_TOP || p.n_top > p.vocab)
     return fail(BH_ERR_SHAPE, "token_logprobs: n_top " + std::to_string(p.n_top) + " above " +
                                   std::to_string(BH_MAX_TOP) + " or vocab");
-  if (!(p.inv_temp > 0.0f) || std::isinf(p.inv_temp))
+  if (!(p.inv_temp > 0.0f) || std::isinf(p.inv_temp * kExpL2E))
     return fail(BH_ERR_ARG, "token_logprobs: inv_temp must be finite and above 0");
   if (p.n_rows != 0) {
     if (!p.x || (p.logprob && !p.tokens) || (p.n_top != 0 && (!p.top_ids || !p.top_logprobs)))
@@ -109,20 +357,68 @@ int check(const bh_token_logprobs_args &p) {
   return BH_OK;
 }
 
+bool nothing(const bh_token_logprobs_args &p) {
+  return p.n_rows == 0 || (!p.logprob && !p.entropy && p.n_top == 0);
+}
+
+// Blocks of a row: about eight blocks a compute unit in all, a tile each at least.
+size_t parts_of(const bh_token_logprobs_args &p) {
+  const size_t tiles = (p.vocab + kLpTile - 1) / kLpTile;
+  size_t parts = 8 * device_cu_count() / p.n_rows;
+  if (parts > tiles) parts = tiles;
+  if (parts > static_cast<size_t>(kMaxParts)) parts = kMaxParts;
+  return parts < 1 ? 1 : parts;
+}
+
+size_t workspace_of(const bh_token_logprobs_args &p) {
+  const size_t parts = parts_of(p);
+  return parts == 1 ? 0 : p.n_rows * parts * (sizeof(Part) + 8 * p.n_top);
+}
+
 }  // namespace
 }  // namespace bh
 
 using namespace bh;
 
-extern "C" size_t bh_token_logprobs_workspace(const bh_token_logprobs_args *args) { return 0; }
+extern "C" size_t bh_token_logprobs_workspace(const bh_token_logprobs_args *args) {
+  if (!args || check(*args) != BH_OK || nothing(*args)) return 0;
+  return workspace_of(*args);
+}
 
 extern "C" int bh_token_logprobs(const bh_token_logprobs_args *args, bh_stream stream) {
   if (!args) return fail(BH_ERR_ARG, "token_logprobs: null args");
   const bh_token_logprobs_args &p = *args;
   if (int e = check(p)) return e;
-  if (p.n_rows == 0 || (!p.logprob && !p.entropy && p.n_top == 0)) return ok();
-  LogprobArgs a{p.x, p.tokens, p.logprob, p.entropy, p.top_ids, p.top_logprobs, p.bad_id,
-                p.row_stride, static_cast<int>(p.vocab), static_cast<int>(p.n_top), p.inv_temp};
-  BH_LAUNCH(token_logprobs_kernel, static_cast<unsigned>(p.n_rows), 256, 0, as_stream(stream), a);
+  if (nothing(p)) return ok();
+  hipStream_t st = as_stream(stream);
+  const size_t need = workspace_of(p), parts = parts_of(p);
+  char *ws = static_cast<char *>(p.workspace);
+  if (need != 0) {
+    if (ws) {
+      if (!aligned16(ws) || p.workspace_bytes < need)
+        return fail(BH_ERR_SHAPE, "token_logprobs: workspace of " +
+                                      std::to_string(p.workspace_bytes) + " bytes, " +
+                                      std::to_string(need) + " needed on a 16-byte boundary");
+    } else {
+      ws = static_cast<char *>(device_scratch(need, kScratchLogprobs, st));
+      if (!ws) return BH_ERR_HIP;
+    }
+  }
+  LogprobArgs a{};
+  a.x = p.x, a.tokens = p.tokens, a.logprob = p.logprob, a.entropy = p.entropy;
+  a.top_ids = p.top_ids, a.top_logprobs = p.top_logprobs, a.bad_id = p.bad_id;
+  a.row_stride = p.row_stride, a.vocab = static_cast<int>(p.vocab);
+  a.n_top = static_cast<int>(p.n_top), a.n_parts = static_cast<int>(parts);
+  a.inv_temp = p.inv_temp, a.k2 = p.inv_temp * kExpL2E;
+  a.parts = reinterpret_cast<Part *>(ws);
+  a.keys = reinterpret_cast<uint64_t *>(ws + p.n_rows * parts * sizeof(Part));
+  const unsigned blocks = static_cast<unsigned>(p.n_rows * parts);
+  if (p.n_top) BH_LAUNCH(token_logprobs_kernel<true>, blocks, kLpThreads, 0, st, a);
+  else BH_LAUNCH(token_logprobs_kernel<false>, blocks, kLpThreads, 0, st, a);
+  if (parts > 1) {
+    const unsigned rows = static_cast<unsigned>(p.n_rows);
+    if (p.n_top) BH_LAUNCH(token_logprobs_join_kernel<true>, rows, kLpThreads, 0, st, a);
+    else BH_LAUNCH(token_logprobs_join_kernel<false>, rows, kLpThreads, 0, st, a);
+  }
   return ok();
 }
