@@ -34,8 +34,8 @@ constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
 constexpr int kPer = 16;                     // logits of a thread and tile
 constexpr int kLpTile = kPer * kLpThreads;   // 4096
 constexpr int kMaxParts = 128;               // blocks of a row
-// keys of a wave: those kept (fewer than 64 between two cuts), and a tile's
-constexpr int kKeep = 64 + kPer * BH_MAX_TOP;
+// keys of a wave: those kept, and a tile's
+constexpr int kKeep = (1 + kPer) * BH_MAX_TOP;
 
 struct Part {
   double s, t;
@@ -56,15 +56,20 @@ struct LogprobArgs {
   uint64_t *keys;      // [n_rows][n_parts][n_top]
 };
 
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
-  uint32_t b = __float_as_uint(x + 0.0f);  // -0 becomes 0
+// Bits that grow with the value; -0 as 0, NaN below every number.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  uint32_t b = __float_as_uint(x + 0.0f);
   b = b & 0x80000000u ? ~b : b | 0x80000000u;
-  if (x != x) b = 0;  // NaN below every number
-  return static_cast<uint64_t>(b) << 32 | (~id);
+  return x != x ? 0 : b;
+}
+__device__ __forceinline__ float value_of_order(uint32_t b) {
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
+  return static_cast<uint64_t>(order_of(x)) << 32 | (~id);
 }
 __device__ __forceinline__ float value_of(uint64_t key) {
-  const uint32_t b = static_cast<uint32_t>(key >> 32);
-  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+  return value_of_order(static_cast<uint32_t>(key >> 32));
 }
 
 struct Max64 {
@@ -93,6 +98,19 @@ __device__ __forceinline__ uint64_t nth_of_lanes(uint64_t key, int n, int lane) 
   return at ? lane_value(key, __builtin_ffsll(at) - 1) : 0;
 }
 
+// The largest b of 16 significant bits that at least n lanes reach: sixteen
+// ballots, where the exact n-th takes 64 compares of keys.  It may let a few more
+// than n lanes pass, and any number of equal ones.
+__device__ __forceinline__ uint32_t bound_of_lanes(uint32_t order, int n) {
+  uint32_t b = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t up = b | 1u << bit;
+    if (__popcll(__ballot(order >= up)) >= n) b = up;
+  }
+  return b;
+}
+
 // The n largest of buf[0 .. count), in order, into out and to the front of buf;
 // returns how many there are.
 __device__ __forceinline__ int keep_best(uint64_t *buf, uint64_t *out, int count, int n, int lane) {
@@ -111,23 +129,32 @@ __device__ __forceinline__ int keep_best(uint64_t *buf, uint64_t *out, int count
   return count;
 }
 
-// The waves' lists of n keys (0: none) into the n largest of them all, in order;
-// 0 behind the last.  put(place, key) takes one.
+// The waves' ordered lists of n keys (0: none) into the n largest of them all, in
+// order; 0 behind the last.  put(place, key) takes one.  A key's place is its own
+// in its list and, by halving, that in the three others.
 template <class F>
 __device__ __forceinline__ void merge_waves(const uint64_t (*lists)[BH_MAX_TOP], int n, F put) {
   const int tid = threadIdx.x;
-  if (tid < kLpWaves * n) {
-    const uint64_t mine = lists[tid / n][tid % n];
-    int rank = 0, there = 0;
+  if (tid >= kLpWaves * n) return;
+  const int own = tid / n;
+  const uint64_t mine = lists[own][tid - own * n];
+  int above[kLpWaves];
 #pragma unroll
-    for (int w = 0; w < kLpWaves; ++w)
-#pragma unroll 8
-      for (int j = 0; j < n; ++j) {
-        rank += lists[w][j] > mine;
-        there += lists[w][j] != 0;
-      }
-    if (mine != 0 && rank < n) put(rank, mine);
-    if (tid < n && tid >= there) put(tid, 0);
+  for (int w = 0; w < kLpWaves; ++w) above[w] = 0;
+#pragma unroll
+  for (int step = BH_MAX_TOP; step > 0; step >>= 1)
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) {
+      const int at = above[w] + step;
+      if (at <= n && lists[w][at - 1] > mine) above[w] = at;
+    }
+  int rank = 0;
+#pragma unroll
+  for (int w = 0; w < kLpWaves; ++w) rank += above[w];
+  if (mine != 0) {
+    if (rank < n) put(rank, mine);
+  } else {  // the keys are `rank` in all: 0s behind them
+    for (int i = rank; i < n; ++i) put(i, 0);
   }
 }
 
@@ -150,19 +177,35 @@ __device__ __forceinline__ Part join_block(float m, double s, double t, float k2
   return p;
 }
 
+// The chosen token's logit, loaded by thread 0 ahead of its use.
+struct Chosen {
+  uint32_t id;
+  float x;
+  bool in;
+};
+__device__ __forceinline__ Chosen load_chosen(const LogprobArgs &a, size_t row) {
+  Chosen c{0, 0.0f, false};
+  if (threadIdx.x == 0 && a.logprob) {
+    c.id = a.tokens[row];
+    c.in = c.id < static_cast<uint32_t>(a.vocab);
+    if (c.in) c.x = a.x[row * a.row_stride + c.id];
+  }
+  return c;
+}
+
 // The row's logprob and entropy from its joined sums; ln S for the alternatives.
-__device__ __forceinline__ float finish_row(const LogprobArgs &a, size_t row, const Part &p) {
+__device__ __forceinline__ float finish_row(const LogprobArgs &a, size_t row, const Part &p,
+                                            const Chosen &c) {
   const bool bad = !(p.m > -INFINITY && p.m < INFINITY);
-  const float log_s = bad ? NAN : static_cast<float>(log(p.s));
+  const double ln = log(p.s);
+  const float log_s = bad ? NAN : static_cast<float>(ln);
   if (threadIdx.x == 0) {
     if (a.logprob) {
-      const uint32_t id = a.tokens[row];
-      const bool in = id < static_cast<uint32_t>(a.vocab);
-      if (!in && a.bad_id) *a.bad_id = id;
-      a.logprob[row] = in ? (a.x[row * a.row_stride + id] - p.m) * a.inv_temp - log_s : NAN;
+      if (!c.in && a.bad_id) *a.bad_id = c.id;
+      a.logprob[row] = c.in ? (c.x - p.m) * a.inv_temp - log_s : NAN;
     }
     if (a.entropy)
-      a.entropy[row] = bad ? NAN : static_cast<float>(log(p.s) - 0.693147180559945309 * (p.t / p.s));
+      a.entropy[row] = bad ? NAN : static_cast<float>(ln - 0.693147180559945309 * (p.t / p.s));
   }
   return log_s;
 }
@@ -191,11 +234,14 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
   const int64_t tiles = (n + kLpTile - 1) / kLpTile;
   const int64_t tile0 = tiles * part / a.n_parts, tile1 = tiles * (part + 1) / a.n_parts;
 
+  const bool whole = a.n_parts == 1;
+  Chosen chosen{};
+  if (whole) chosen = load_chosen(a, row);
   float m = -INFINITY;
   double s = 0.0, t = 0.0;
   int count = 0;
-  uint64_t bound = 0;  // keys above this may be among the best
-  bool first = true;
+  uint64_t bound = 0;  // the last of the kept keys, once they are n
+  bool full = false;
   for (int64_t tile = tile0; tile < tile1; ++tile) {
     // id of the thread's first logit; those before the row wrap round to no id
     const uint32_t at = static_cast<uint32_t>(tile) * kLpTile + 4 * tid - skew, vocab = a.vocab;
@@ -238,48 +284,62 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
     t += et;
 
     if constexpr (TOP) {
-      // a lane's largest; NaN logits only count while there are too few others
-      const bool look = first || __any(top > value_of(bound)) || (bound >> 32) == 0;
-      if (look) {
-        uint64_t best = 0;
+      // full: n keys are kept, and a later logit has to pass the last one's value
+      if (!full || __any(top > value_of(bound))) {
+        // logits from `least` on join the kept ones
+        float least = full ? value_of(bound) : -INFINITY;
+        const bool many = __popcll(__ballot(top > least)) > a.n_top;
+        if (many) {
+          const float of_lanes = value_of_order(bound_of_lanes(order_of(top), a.n_top));
+          least = of_lanes > least ? of_lanes : least;
+        }
+        uint64_t pass[kPer];
+        int more = 0;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-          const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
-          const uint64_t key = id < vocab ? key_of(v[k], id) : 0;
-          best = key > best ? key : best;
+          pass[k] = __ballot(many || !full ? v[k] >= least : v[k] > least);
+          more += __popcll(pass[k]);
         }
-        uint64_t from = bound + 1;
-        if (__popcll(__ballot(best > bound)) > a.n_top) {
-          const uint64_t nth = nth_of_lanes(best, a.n_top, lane);
-          from = nth > from ? nth : from;
+        uint64_t from = full ? bound + 1 : 1;
+        // Too few for the list, or too many equal ones: by keys.  Then NaN logits
+        // count too, and the lanes' n-th best is a bound that at most n lanes reach.
+        const bool by_key = (!full && (!many || more < a.n_top)) || more > kPer * a.n_top;
+        if (by_key) {
+          uint64_t best = 0;
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) {
+            const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
+            const uint64_t key = id < vocab ? key_of(v[k], id) : 0;
+            best = key > best ? key : best;
+          }
+          if (__popcll(__ballot(best >= from)) > a.n_top) {
+            const uint64_t nth = nth_of_lanes(best, a.n_top, lane);
+            from = nth > from ? nth : from;
+          }
         }
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
+          if (!by_key && pass[k] == 0) continue;
           const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
-          const uint64_t key = id < vocab ? key_of(v[k], id) : 0;
-          const uint64_t pass = __ballot(key >= from);
-          if (pass == 0) continue;
+          const uint64_t key = id < vocab && (by_key || (pass[k] >> lane & 1)) ? key_of(v[k], id) : 0;
+          const uint64_t in = __ballot(key >= from);
           if (key >= from)
-            keep[wave][count + __popcll(pass & ((uint64_t{1} << lane) - 1))] = key;
-          count += __popcll(pass);
+            keep[wave][count + __popcll(in & ((uint64_t{1} << lane) - 1))] = key;
+          count += __popcll(in);
         }
-        if (first || count >= 64) {
-          count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
-          if (count == a.n_top) bound = keep[wave][a.n_top - 1];
-        }
-        first = false;
+        count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
+        if (count == a.n_top) bound = keep[wave][a.n_top - 1];
+        full = count == a.n_top && bound >> 32 != 0;  // a NaN at the end gives way to any number
       }
     }
   }
 
   const Part p = join_block(m, s, t, a.k2, fl, dl);
-  const bool whole = a.n_parts == 1;
   float log_s = 0.0f;
-  if (whole) log_s = finish_row(a, row, p);
+  if (whole) log_s = finish_row(a, row, p, chosen);
   else if (tid == 0) a.parts[blockIdx.x] = p;
   if constexpr (TOP) {
-    count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
-    if (lane >= count && lane < a.n_top) lists[wave][lane] = 0;
+    if (lane < a.n_top) lists[wave][lane] = lane < count ? keep[wave][lane] : 0;
     __syncthreads();
     uint64_t *out = a.keys + static_cast<size_t>(blockIdx.x) * a.n_top;
     merge_waves(lists, a.n_top, [&](int place, uint64_t key) {
@@ -306,18 +366,23 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(Logprob
     for (int k = 0; k < kKeys; ++k)
       key[k] = tid + k * kLpThreads < n ? a.keys[row * n + tid + k * kLpThreads] : 0;
   }
+  const Chosen chosen = load_chosen(a, row);
   Part mine{0.0, 0.0, -INFINITY};
   if (tid < a.n_parts) mine = a.parts[row * a.n_parts + tid];
   const Part p = join_block(mine.m, mine.s, mine.t, a.k2, fl, dl);
-  const float log_s = finish_row(a, row, p);
+  const float log_s = finish_row(a, row, p, chosen);
   if constexpr (TOP) {
     uint64_t best = 0;
 #pragma unroll
     for (int k = 0; k < kKeys; ++k) best = key[k] > best ? key[k] : best;
     uint64_t from = 1;
     if (n > 64 * kLpWaves) {  // more than a key a lane
-      const uint64_t nth = nth_of_lanes(best, a.n_top, lane);
-      from = nth > from ? nth : from;
+      from = static_cast<uint64_t>(bound_of_lanes(static_cast<uint32_t>(best >> 32), a.n_top)) << 32;
+      int more = 0;
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k) more += __popcll(__ballot(key[k] >= from));
+      if (more > kKeep) from = nth_of_lanes(best, a.n_top, lane);
+      from = from > 1 ? from : 1;
     }
     int count = 0;
 #pragma unroll
