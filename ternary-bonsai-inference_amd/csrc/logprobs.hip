@@ -217,6 +217,25 @@ __device__ __forceinline__ void put_top(const LogprobArgs &a, size_t row, int pl
   a.top_logprobs[o] = (value_of(key) - m) * a.inv_temp - log_s;
 }
 
+// A thread's logits of a tile: four pieces of four; -inf outside the row.
+__device__ __forceinline__ void load_tile(const LogprobArgs &a, const float *x, int64_t tile,
+                                          int64_t n, int skew, float *v) {
+  const uint32_t at = static_cast<uint32_t>(tile) * kLpTile + 4 * threadIdx.x - skew;
+  if (tile * kLpTile >= skew && (tile + 1) * kLpTile <= n) {
+#pragma unroll
+    for (int k = 0; k < kPer; k += 4) {
+      const float4 p = *reinterpret_cast<const float4 *>(x + at + k * kLpThreads);
+      v[k] = p.x, v[k + 1] = p.y, v[k + 2] = p.z, v[k + 3] = p.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
+      v[k] = id < static_cast<uint32_t>(a.vocab) ? x[id] : -INFINITY;
+    }
+  }
+}
+
 // Block (row, part): the tiles of a part of a row.  Tiles begin at the row's last
 // 16-byte boundary before it, so that whole pieces load at once for any row.
 template <bool TOP>
@@ -225,6 +244,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
   __shared__ uint64_t lists[TOP ? kLpWaves : 1][BH_MAX_TOP];
   __shared__ float fl[kLpWaves];
   __shared__ double dl[kLpWaves];
+  __shared__ uint64_t shown[kLpWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t row = blockIdx.x / a.n_parts;
   const int part = blockIdx.x - row * a.n_parts;
@@ -241,24 +261,20 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
   double s = 0.0, t = 0.0;
   int count = 0;
   uint64_t bound = 0;  // the last of the kept keys, once they are n
-  bool full = false;
+  bool full = false, strict = true;  // strict: the bound is a key of this wave
+  if constexpr (TOP) {
+    if (tid < kLpWaves) shown[tid] = 0;
+    __syncthreads();
+  }
+  float ahead[kPer];
+  load_tile(a, x, tile0, n, skew, ahead);
   for (int64_t tile = tile0; tile < tile1; ++tile) {
     // id of the thread's first logit; those before the row wrap round to no id
     const uint32_t at = static_cast<uint32_t>(tile) * kLpTile + 4 * tid - skew, vocab = a.vocab;
     float v[kPer];
-    if (tile * kLpTile >= skew && (tile + 1) * kLpTile <= n) {
 #pragma unroll
-      for (int k = 0; k < kPer; k += 4) {
-        const float4 p = *reinterpret_cast<const float4 *>(x + at + k * kLpThreads);
-        v[k] = p.x, v[k + 1] = p.y, v[k + 2] = p.z, v[k + 3] = p.w;
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
-        v[k] = id < vocab ? x[id] : -INFINITY;
-      }
-    }
+    for (int k = 0; k < kPer; ++k) v[k] = ahead[k];
+    if (tile + 1 < tile1) load_tile(a, x, tile + 1, n, skew, ahead);
     float top = v[0];
 #pragma unroll
     for (int k = 1; k < kPer; ++k) top = fmaxf(top, v[k]);
@@ -284,11 +300,26 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
     t += et;
 
     if constexpr (TOP) {
-      // full: n keys are kept, and a later logit has to pass the last one's value
-      if (!full || __any(top > value_of(bound))) {
+      // full: n keys are kept, and a later logit has to pass the last one's value.
+      // Each wave also shows its ceil(n / 4)-th best: n keys of the block reach the
+      // least of the four, which soon lies far above a wave's own n-th.  (A wave
+      // may read an older one, which bounds less.)  Another wave's key may stand
+      // behind an equal logit of this one, so that bound lets equal ones pass.
+      if (full) {
+        uint64_t all = ~uint64_t{0};
+#pragma unroll
+        for (int w = 0; w < kLpWaves; ++w) {
+          const uint64_t of =
+              __hip_atomic_load(&shown[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          all = of < all ? of : all;
+        }
+        if (all > bound) bound = all, strict = false;
+      }
+      const float last = value_of(bound);
+      if (!full || __any(strict ? top > last : top >= last)) {
         // logits from `least` on join the kept ones
-        float least = full ? value_of(bound) : -INFINITY;
-        const bool many = __popcll(__ballot(top > least)) > a.n_top;
+        float least = full ? last : -INFINITY;
+        const bool many = __popcll(__ballot(strict ? top > least : top >= least)) > a.n_top;
         if (many) {
           const float of_lanes = value_of_order(bound_of_lanes(order_of(top), a.n_top));
           least = of_lanes > least ? of_lanes : least;
@@ -297,7 +328,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
         int more = 0;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-          pass[k] = __ballot(many || !full ? v[k] >= least : v[k] > least);
+          pass[k] = __ballot(many || !full || !strict ? v[k] >= least : v[k] > least);
           more += __popcll(pass[k]);
         }
         uint64_t from = full ? bound + 1 : 1;
@@ -328,7 +359,13 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
           count += __popcll(in);
         }
         count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
-        if (count == a.n_top) bound = keep[wave][a.n_top - 1];
+        if (count == a.n_top) {
+          const uint64_t own = keep[wave][a.n_top - 1];
+          if (own > bound) bound = own, strict = true;
+          if (lane == 0)
+            __hip_atomic_store(&shown[wave], keep[wave][(a.n_top - 1) / kLpWaves],
+                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
         full = count == a.n_top && bound >> 32 != 0;  // a NaN at the end gives way to any number
       }
     }
@@ -426,10 +463,12 @@ bool nothing(const bh_token_logprobs_args &p) {
   return p.n_rows == 0 || (!p.logprob && !p.entropy && p.n_top == 0);
 }
 
-// Blocks of a row: about eight blocks a compute unit in all, a tile each at least.
+// Blocks of a row: about four blocks a compute unit in all, a tile each at least.
+// 512 rows of 248320 with 5 alternatives, 1 / 2 / 4 / 8 a unit: 121 / 117 / 111 / 123
+// us; 64 rows with 20: 58 / 41 / 35 / 36.
 size_t parts_of(const bh_token_logprobs_args &p) {
   const size_t tiles = (p.vocab + kLpTile - 1) / kLpTile;
-  size_t parts = 8 * device_cu_count() / p.n_rows;
+  size_t parts = 4 * device_cu_count() / p.n_rows;
   if (parts > tiles) parts = tiles;
   if (parts > static_cast<size_t>(kMaxParts)) parts = kMaxParts;
   return parts < 1 ? 1 : parts;
