@@ -14,7 +14,8 @@
 // lanes' own maxima is a bound that the wave's n best all reach, and at most
 // 16 n keys do; those join the kept ones, and each key's rank, counted by
 // comparing it with all of them, is its place.  Later tiles are only looked at
-// where a lane's maximum passes the n-th key kept.
+// where a lane's maximum passes the n-th key kept, and their few keys move into
+// the list one by one.
 //
 // Rows are split over as many blocks as fill the card; a second launch then joins
 // a row's parts.  Bound by reading the logits where there are many, by the chain
@@ -36,6 +37,7 @@ constexpr int kLpTile = kPer * kLpThreads;   // 4096
 constexpr int kMaxParts = 128;               // blocks of a row
 // keys of a wave: those kept, and a tile's
 constexpr int kKeep = (1 + kPer) * BH_MAX_TOP;
+constexpr int kFew = 8;  // up to so many keys of a tile go into the list one by one
 
 struct Part {
   double s, t;
@@ -111,23 +113,37 @@ __device__ __forceinline__ uint32_t bound_of_lanes(uint32_t order, int n) {
   return b;
 }
 
-// The n largest of buf[0 .. count), in order, into out and to the front of buf;
-// returns how many there are.
-__device__ __forceinline__ int keep_best(uint64_t *buf, uint64_t *out, int count, int n, int lane) {
-  wave_sync();
-  for (int k = 0; k < count; k += 64) {
-    const uint64_t mine = k + lane < count ? buf[k + lane] : 0;
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < count; ++j) rank += buf[j] > mine;
-    if (mine != 0 && rank < n) out[rank] = mine;
+// A wave's best keys in order, lane i holding the i-th; 0 behind the last.
+struct Kept {
+  uint64_t key = 0;
+  int count = 0;
+
+  // Takes in one key: the lanes from its place on move up by one.
+  __device__ __forceinline__ void insert(uint64_t x, int n, int lane) {
+    const int place = __popcll(__ballot(key > x));
+    const uint64_t below = dpp_move<0x138>(key);  // of the lane before
+    key = lane < place ? key : lane == place ? x : below;
+    if (lane >= n) key = 0;
+    count = min(count + 1, n);
   }
-  count = min(count, n);
-  wave_sync();
-  if (lane < count) buf[lane] = out[lane];
-  wave_sync();
-  return count;
-}
+  // Takes in buf[0 .. total): each key's place is the number of larger ones.
+  __device__ __forceinline__ void replace(const uint64_t *buf, uint64_t *out, int total, int n,
+                                          int lane) {
+    wave_sync();
+    if (lane < n) out[lane] = 0;
+    wave_sync();
+    for (int k = 0; k < total; k += 64) {
+      const uint64_t mine = k + lane < total ? buf[k + lane] : 0;
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < total; ++j) rank += buf[j] > mine;
+      if (mine != 0 && rank < n) out[rank] = mine;
+    }
+    wave_sync();
+    key = lane < n ? out[lane] : 0;
+    count = __popcll(__ballot(key != 0));
+  }
+};
 
 // The waves' ordered lists of n keys (0: none) into the n largest of them all, in
 // order; 0 behind the last.  put(place, key) takes one.  A key's place is its own
@@ -259,7 +275,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
   if (whole) chosen = load_chosen(a, row);
   float m = -INFINITY;
   double s = 0.0, t = 0.0;
-  int count = 0;
+  Kept kept;
   uint64_t bound = 0;  // the last of the kept keys, once they are n
   bool full = false, strict = true;  // strict: the bound is a key of this wave
   if constexpr (TOP) {
@@ -347,26 +363,49 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
             const uint64_t nth = nth_of_lanes(best, a.n_top, lane);
             from = nth > from ? nth : from;
           }
-        }
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-          if (!by_key && pass[k] == 0) continue;
-          const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
-          const uint64_t key = id < vocab && (by_key || (pass[k] >> lane & 1)) ? key_of(v[k], id) : 0;
-          const uint64_t in = __ballot(key >= from);
-          if (key >= from)
-            keep[wave][count + __popcll(in & ((uint64_t{1} << lane) - 1))] = key;
-          count += __popcll(in);
+          for (int k = 0; k < kPer; ++k) {
+            const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
+            pass[k] = __ballot((id < vocab ? key_of(v[k], id) : 0) >= from);
+          }
         }
-        count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
-        if (count == a.n_top) {
-          const uint64_t own = keep[wave][a.n_top - 1];
+        if (!by_key && more <= kFew) {
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) {
+            if (pass[k] == 0) continue;
+            const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
+            const uint64_t key = id < vocab ? key_of(v[k], id) : 0;
+            for (uint64_t left = pass[k]; left != 0; left &= left - 1) {
+              const uint64_t x = lane_value(key, __builtin_ffsll(left) - 1);
+              if (x >= from) kept.insert(x, a.n_top, lane);
+            }
+          }
+        } else {
+          uint64_t *buf = keep[wave];
+          int total = kept.count;
+          if (lane < total) buf[lane] = kept.key;
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) {
+            if (pass[k] == 0) continue;
+            const uint32_t id = at + (k & ~3) * kLpThreads + (k & 3);
+            if (pass[k] >> lane & 1) {
+              const uint64_t key = key_of(v[k], id);
+              buf[total + __popcll(pass[k] & ((uint64_t{1} << lane) - 1))] =
+                  id < vocab && key >= from ? key : 0;
+            }
+            total += __popcll(pass[k]);
+          }
+          kept.replace(buf, lists[wave], total, a.n_top, lane);
+        }
+        if (kept.count == a.n_top) {
+          const uint64_t own = lane_value(kept.key, a.n_top - 1);
           if (own > bound) bound = own, strict = true;
-          if (lane == 0)
-            __hip_atomic_store(&shown[wave], keep[wave][(a.n_top - 1) / kLpWaves],
-                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          if (lane == (a.n_top - 1) / kLpWaves)
+            __hip_atomic_store(&shown[wave], kept.key, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_WORKGROUP);
         }
-        full = count == a.n_top && bound >> 32 != 0;  // a NaN at the end gives way to any number
+        // a NaN at the end gives way to any number
+        full = kept.count == a.n_top && bound >> 32 != 0;
       }
     }
   }
@@ -376,7 +415,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
   if (whole) log_s = finish_row(a, row, p, chosen);
   else if (tid == 0) a.parts[blockIdx.x] = p;
   if constexpr (TOP) {
-    if (lane < a.n_top) lists[wave][lane] = lane < count ? keep[wave][lane] : 0;
+    if (lane < a.n_top) lists[wave][lane] = kept.key;
     __syncthreads();
     uint64_t *out = a.keys + static_cast<size_t>(blockIdx.x) * a.n_top;
     merge_waves(lists, a.n_top, [&](int place, uint64_t key) {
@@ -429,8 +468,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(Logprob
       if (key[k] >= from) keep[wave][count + __popcll(pass & ((uint64_t{1} << lane) - 1))] = key[k];
       count += __popcll(pass);
     }
-    count = keep_best(keep[wave], lists[wave], count, a.n_top, lane);
-    if (lane >= count && lane < a.n_top) lists[wave][lane] = 0;
+    Kept kept;
+    kept.replace(keep[wave], lists[wave], count, a.n_top, lane);  // and into lists
     __syncthreads();
     merge_waves(lists, a.n_top, [&](int place, uint64_t k) {
       put_top(a, row, place, k, p.m, log_s);
