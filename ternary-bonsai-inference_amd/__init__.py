@@ -513,9 +513,9 @@ def _dev_tensor(t, name: str, dtypes, device, shape=None):
     """t, checked: a contiguous tensor of one of dtypes on `device`."""
     if t.dtype not in dtypes or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of {dtypes[0]}, got {t.dtype}")
-    if t.device != device or not t.is_cuda:
+    if not t.is_cuda or t.get_device() != device.index:
         raise ValueError(f"{name} is on {t.device}, the call's tensors on {device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     return t
 
@@ -535,10 +535,14 @@ def _call(fn, args, stream):
     """fn(args, stream) on the device of args' tensors, whichever is current."""
     import torch
     if torch.cuda.current_device() == args.device.index:
-        check(fn(ctypes.byref(args), _stream(stream)))
-        return
-    with torch.cuda.device(args.device):
-        check(fn(ctypes.byref(args), _stream(stream)))
+        s = torch._C._cuda_getCurrentRawStream(args.device.index) if stream is None \
+            else stream.cuda_stream  # a stream object a call would cost as much as its launch
+        status = fn(ctypes.byref(args), s)
+    else:
+        with torch.cuda.device(args.device):
+            status = fn(ctypes.byref(args), _stream(stream))
+    if status != BH_OK:
+        raise BonsaiError(status, last_error())
 
 
 def make_paged_cache(k, v) -> PagedCache:
@@ -603,15 +607,14 @@ def kv_store_paged(cache: PagedCache, k, v, slots, stream=None) -> None:
     """kv_store into pages: rows k, v [n_tok, n_kv * hd] f32 to the positions
     slots int32 [n_tok] of the cache (page * page_size + offset; below 0: none)."""
     import torch
-    dev, shape = cache.device, (slots.numel(), cache.n_kv * cache.hd)
+    dev, n_tok = cache.device, slots.numel()
+    shape, f32 = (n_tok, cache.n_kv * cache.hd), (torch.float32,)
     _dev_tensor(slots, "slots", (torch.int32,), dev)
-    _dev_tensor(k, "k", (torch.float32,), dev, shape)
-    _dev_tensor(v, "v", (torch.float32,), dev, shape)
-
-    def store(ref, s):
-        return lib().bh_kv_store_paged(ref, k.data_ptr(), v.data_ptr(), slots.data_ptr(),
-                                       shape[0], s)
-    _call(store, cache, stream)
+    _dev_tensor(k, "k", f32, dev, shape)
+    _dev_tensor(v, "v", f32, dev, shape)
+    fn = lib().bh_kv_store_paged
+    _call(lambda ref, s: fn(ref, k.data_ptr(), v.data_ptr(), slots.data_ptr(), n_tok, s), cache,
+          stream)
 
 
 def make_attention_paged_args(cache: PagedCache, q, q_start, kv_len, block_table, out=None,

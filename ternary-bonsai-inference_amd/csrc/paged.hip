@@ -12,8 +12,10 @@
 //   second one, over the admitted requests.
 //
 // One workgroup does it: every step needs the totals of all requests, and the
-// data is a few hundred KB at most.  It is bound by the chain of dependent
-// steps (load, scan, scan, pages, tokens), not by bytes.
+// data is a few hundred KB at most.  It is bound by the chain of dependent steps
+// (load, scan, scan, pages, tokens), not by bytes; so few requests take one wave,
+// whose barriers cost nothing (16 requests: ____ us, with 16 waves ____), and a
+// thread works on four pages or tokens at once, whose searches overlap.
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -25,8 +27,7 @@
 namespace bh {
 namespace {
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanPer = BH_PAGED_MAX_REQ / kPlanThreads;  // requests of a thread
+constexpr int kMost = 0x7fffffff;  // where running totals stop: past every limit
 
 struct PlanArgs {
   const int32_t *cached, *n_new, *n_free;
@@ -35,49 +36,88 @@ struct PlanArgs {
   FastDiv page;
 };
 
-// Exclusive running total over the block in thread order; *total gets the sum.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *lds, int64_t *total) {
-  int64_t run = v;
+__device__ __forceinline__ int add_most(int a, int b) {
+  const uint32_t s = static_cast<uint32_t>(a) + static_cast<uint32_t>(b);
+  return s > static_cast<uint32_t>(kMost) ? kMost : static_cast<int>(s);
+}
+
+// Inclusive running totals over the lanes of a wave.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int x) {
+  return add_most(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x = scan_step<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+  x = scan_step<0x112, 0xF>(x);
+  x = scan_step<0x114, 0xF>(x);
+  x = scan_step<0x118, 0xF>(x);
+  x = scan_step<0x142, 0xA>(x);  // lane 15 of a row into the next
+  return scan_step<0x143, 0xC>(x);  // lane 31 into the upper half
+}
+
+struct Three {
+  int a, b, c;
+};
+
+// Exclusive running totals of three numbers over the block in thread order;
+// *total gets the sums.
+template <int WAVES>
+__device__ __forceinline__ Three block_scan(Three v, Three *lds, Three *total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(run, d);
-    if (lane >= d) run += o;
+  const Three run{wave_scan(v.a), wave_scan(v.b), wave_scan(v.c)};
+  // the lane before's, 0 for lane 0
+  Three out{dpp_move<0x138>(run.a), dpp_move<0x138>(run.b), dpp_move<0x138>(run.c)};
+  if constexpr (WAVES == 1) {
+    *total = Three{__builtin_amdgcn_readlane(run.a, 63), __builtin_amdgcn_readlane(run.b, 63),
+                   __builtin_amdgcn_readlane(run.c, 63)};
+    return out;
   }
   __syncthreads();
   if (lane == 63) lds[wave] = run;
   __syncthreads();
-  int64_t before = 0, all = 0;
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
-    if (w < wave) before += lds[w];
-    all += lds[w];
+  Three w = lane < WAVES ? lds[lane] : Three{0, 0, 0};
+  w = Three{wave_scan(w.a), wave_scan(w.b), wave_scan(w.c)};
+  *total = Three{__builtin_amdgcn_readlane(w.a, 63), __builtin_amdgcn_readlane(w.b, 63),
+                 __builtin_amdgcn_readlane(w.c, 63)};
+  if (wave > 0) {
+    out.a = add_most(out.a, __builtin_amdgcn_readlane(w.a, wave - 1));
+    out.b = add_most(out.b, __builtin_amdgcn_readlane(w.b, wave - 1));
+    out.c = add_most(out.c, __builtin_amdgcn_readlane(w.c, wave - 1));
   }
-  *total = all;
-  return before + run - v;
+  return out;
 }
 
-// The request r with start[r] <= x < start[r + 1], for 0 <= x < start[n].
-__device__ __forceinline__ int find(const int *start, int n, int x) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+// For each x[k] >= 0 the last r < n with start[r] <= x[k] (start[0] = 0); `top`: the
+// power of two from which to halve, at least n.
+template <int N>
+__device__ __forceinline__ void find(const int *start, int n, int top, const int *x, int *r) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) r[k] = 0;
+  for (int step = top; step > 0; step >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int at = r[k] + step;
+      if (at < n && start[at] <= x[k]) r[k] = at;
+    }
 }
 
-__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
-  __shared__ int64_t part[kPlanThreads / 64];
-  __shared__ int start[BH_PAGED_MAX_REQ + 1];
-  __shared__ int lens[BH_PAGED_MAX_REQ];
+constexpr int kAtOnce = 4;
+
+template <int THREADS, int PER>
+__global__ __launch_bounds__(THREADS) void paged_plan_kernel(PlanArgs a) {
+  constexpr int kReq = THREADS * PER;
+  __shared__ Three part[THREADS / 64];
+  __shared__ int start[kReq + 1], lens[kReq];
   const int tid = threadIdx.x;
   const int64_t page = a.page.d;
 
-  int cached[kPlanPer], grow[kPlanPer], have[kPlanPer], need[kPlanPer];
-  bool gone[kPlanPer], refused[kPlanPer];
-  int64_t sn = 0, sg = 0, sb = 0;
-  for (int k = 0; k < kPlanPer; ++k) {
-    const int i = tid * kPlanPer + k;
+  int cached[PER], grow[PER], have[PER], need[PER];
+  bool gone[PER], refused[PER];
+  Three own{0, 0, 0};  // new pages, new tokens, released pages
+  int n_free = *a.n_free;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = tid * PER + k;
     cached[k] = grow[k] = have[k] = need[k] = 0;
     gone[k] = refused[k] = false;
     if (i >= a.n_req) continue;
@@ -96,94 +136,130 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       }
     }
     have[k] = min(have[k], a.width);
-    sn += need[k];
-    sg += grow[k];
-    sb += gone[k] ? have[k] : 0;
+    own.a = add_most(own.a, need[k]);
+    own.b = add_most(own.b, grow[k]);
+    own.c = add_most(own.c, gone[k] ? have[k] : 0);
   }
-  const int n_free = min(max(*a.n_free, 0), a.n_pages);
-  int64_t tn, tg, tb;
-  int64_t on = block_scan(sn, part, &tn), og = block_scan(sg, part, &tg);
-  int64_t ob = block_scan(sb, part, &tb);
+  n_free = min(max(n_free, 0), a.n_pages);
+  Three all;
+  Three run = block_scan<THREADS / 64>(own, part, &all);
+  int top = 1;
+  while (top < a.n_req) top <<= 1;
 
   // the released pages go on the stack
-  for (int k = 0; k < kPlanPer; ++k) {
-    const int i = tid * kPlanPer + k;
-    if (i <= a.n_req) start[i] = static_cast<int>(min<int64_t>(ob, a.n_pages));
-    if (i < a.n_req && gone[k]) ob += have[k];
+  const int n_back = min(all.c, a.n_pages - n_free), avail = n_free + n_back;
+  if (n_back > 0) {
+    int at = run.c;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if (tid * PER + k < a.n_req) start[tid * PER + k] = at;
+      if (gone[k]) at = add_most(at, have[k]);
+    }
+    __syncthreads();
+    for (int p0 = tid; p0 < n_back; p0 += kAtOnce * THREADS) {
+      int p[kAtOnce], r[kAtOnce], entry[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) p[k] = min(p0 + k * THREADS, n_back - 1);
+      find<kAtOnce>(start, a.n_req, top, p, r);
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        entry[k] = a.table[static_cast<size_t>(r[k]) * a.width + (p[k] - start[r[k]])];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) a.free_pages[n_free + p[k]] = entry[k];
+    }
+    __syncthreads();
   }
-  if (tid == 0 && a.n_req == BH_PAGED_MAX_REQ)
-    start[a.n_req] = static_cast<int>(min<int64_t>(tb, a.n_pages));
-  __syncthreads();
-  const int n_back = static_cast<int>(min<int64_t>(tb, a.n_pages - n_free));
-  for (int p = tid; p < n_back; p += kPlanThreads) {
-    const int r = find(start, a.n_req, p);
-    a.free_pages[n_free + p] = a.table[static_cast<size_t>(r) * a.width + (p - start[r])];
-  }
-  const int avail = n_free + n_back;
 
   // who fits
-  int64_t taken = 0, admitted = 0, out = 0;
-  const int64_t first = on;
-  for (int k = 0; k < kPlanPer; ++k) {
-    on += need[k];
-    og += grow[k];
-    if ((need[k] > 0 && on > avail) || (grow[k] > 0 && og > a.n_tok)) refused[k] = true;
+  const int first = run.a;
+  Three fit{0, 0, 0};  // pages taken, tokens admitted, requests refused
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    run.a = add_most(run.a, need[k]);
+    run.b = add_most(run.b, grow[k]);
+    if ((need[k] > 0 && run.a > avail) || (grow[k] > 0 && run.b > a.n_tok)) refused[k] = true;
     if (refused[k]) {
       need[k] = grow[k] = 0;
-      ++out;
+      ++fit.c;
     }
-    taken += need[k];
-    admitted += grow[k];
+    fit.a += need[k];
+    fit.b += grow[k];
   }
-  int64_t all_taken, n_out, n_admitted;
-  block_scan(taken, part, &all_taken);
-  block_scan(out, part, &n_out);
-  int64_t at = block_scan(admitted, part, &n_admitted);
+  Three sums;
+  const Three before = block_scan<THREADS / 64>(fit, part, &sums);
 
-  // the pages taken, from the top of the stack; start: where a request's begin
-  int64_t base = first;
-  for (int k = 0; k < kPlanPer; ++k) {
-    const int i = tid * kPlanPer + k;
-    // a refused request's range is empty: it begins where the taken ones end
-    if (i <= a.n_req) start[i] = static_cast<int>(min(base, all_taken));
-    if (i < a.n_req) lens[i] = have[k];
-    base += need[k];
+  // the pages taken, from the top of the stack
+  if (sums.a > 0) {
+    int at = first;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = tid * PER + k;
+      // a refused request's range is empty: it begins where the taken ones end
+      if (i < a.n_req) start[i] = min(at, sums.a), lens[i] = have[k];
+      at = add_most(at, need[k]);
+    }
+    __syncthreads();
+    for (int p0 = tid; p0 < sums.a; p0 += kAtOnce * THREADS) {
+      int p[kAtOnce], r[kAtOnce], entry[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        p[k] = min(p0 + k * THREADS, sums.a - 1);
+        entry[k] = a.free_pages[avail - 1 - p[k]];
+      }
+      find<kAtOnce>(start, a.n_req, top, p, r);
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        a.table[static_cast<size_t>(r[k]) * a.width + lens[r[k]] + (p[k] - start[r[k]])] = entry[k];
+    }
+    __syncthreads();
   }
-  if (tid == 0 && a.n_req == BH_PAGED_MAX_REQ) start[a.n_req] = static_cast<int>(all_taken);
-  __syncthreads();
-  for (int p = tid; p < static_cast<int>(all_taken); p += kPlanThreads) {
-    const int r = find(start, a.n_req, p);
-    a.table[static_cast<size_t>(r) * a.width + lens[r] + (p - start[r])] =
-        a.free_pages[avail - 1 - p];
-  }
-  __syncthreads();
 
-  // offsets, lengths, tokens
-  for (int k = 0; k < kPlanPer; ++k) {
-    const int i = tid * kPlanPer + k;
-    if (i <= a.n_req) a.q_start[i] = start[i] = static_cast<int>(at);
-    if (i < a.n_req) a.kv_len[i] = lens[i] = gone[k] || refused[k] ? 0 : cached[k] + grow[k];
-    at += grow[k];
+  // offsets and lengths
+  {
+    int at = before.b;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = tid * PER + k;
+      if (i < a.n_req) {
+        const int len = gone[k] || refused[k] ? 0 : cached[k] + grow[k];
+        a.q_start[i] = start[i] = at;
+        a.kv_len[i] = len;
+        lens[i] = len;
+      }
+      at += grow[k];
+    }
   }
+  const int live = sums.b;
   if (tid == 0) {
-    *a.n_free_out = avail - static_cast<int>(all_taken);
-    if (a.n_refused) *a.n_refused = static_cast<int>(n_out);
-    if (a.n_req == BH_PAGED_MAX_REQ)
-      a.q_start[a.n_req] = start[a.n_req] = static_cast<int>(n_admitted);
+    start[a.n_req] = a.q_start[a.n_req] = live;
+    *a.n_free_out = avail - sums.a;
+    if (a.n_refused) *a.n_refused = sums.c;
   }
   __syncthreads();
-  const int live = static_cast<int>(n_admitted);
-  for (int t = tid; t < a.n_tok; t += kPlanThreads) {
-    int p = 0, slot = -1;
-    if (t < live) {
-      const int r = find(start, a.n_req, t);
-      p = lens[r] - start[r + 1] + t;
-      const int b = a.page.div(p);
-      const int at_page = a.table[static_cast<size_t>(r) * a.width + b];
-      if (at_page >= 0 && at_page < a.n_pages) slot = at_page * a.page.d + (p - b * a.page.d);
+
+  // tokens
+  for (int t0 = tid; t0 < a.n_tok; t0 += kAtOnce * THREADS) {
+    int t[kAtOnce], r[kAtOnce], p[kAtOnce], entry[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) t[k] = t0 + k * THREADS;
+    if (t0 < live) find<kAtOnce>(start, a.n_req, top, t, r);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      p[k] = 0, entry[k] = -1;
+      if (t[k] < live) {
+        p[k] = lens[r[k]] - start[r[k] + 1] + t[k];
+        entry[k] = a.table[static_cast<size_t>(r[k]) * a.width + a.page.div(p[k])];
+      }
     }
-    a.slots[t] = slot;
-    if (a.pos) *reinterpret_cast<int4 *>(a.pos + static_cast<size_t>(t) * 4) = make_int4(p, p, p, p);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (t[k] >= a.n_tok) continue;
+      const bool in = entry[k] >= 0 && entry[k] < a.n_pages;
+      a.slots[t[k]] = in ? entry[k] * a.page.d + a.page.mod(p[k]) : -1;
+      if (a.pos)
+        *reinterpret_cast<int4 *>(a.pos + static_cast<size_t>(t[k]) * 4) =
+            make_int4(p[k], p[k], p[k], p[k]);
+    }
   }
 }
 
@@ -202,9 +278,37 @@ struct StoreArgs {
   const int32_t *slots;
   void *kc, *vc;
   size_t page_stride, pos_stride, head_stride;
-  int n_tok, n_slots, elems, hd;
-  FastDiv page;
+  int n_tok, n_slots, elems, hd, pieces;
+  FastDiv page, row, head;  // row, head: pieces of four elements
 };
+
+// Four elements a thread, for heads, strides and pointers of whole pieces: as many
+// bytes in flight a wave as a copy has.
+template <class T>
+__global__ __launch_bounds__(256) void kv_store_paged_pieces_kernel(StoreArgs a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.pieces) return;
+  const int t = a.row.div(i), e = i - t * a.row.d, h = a.head.div(e);
+  const float4 k = reinterpret_cast<const float4 *>(a.k)[i];  // fresh from the call before: cached
+  const float4 v = reinterpret_cast<const float4 *>(a.v)[i];
+  const int slot = a.slots[t];
+  if (slot < 0 || slot >= a.n_slots) return;
+  const int b = a.page.div(slot);
+  const size_t at = b * a.page_stride + static_cast<size_t>(slot - b * a.page.d) * a.pos_stride +
+                    h * a.head_stride + 4 * (e - h * a.head.d);
+  if constexpr (sizeof(T) == 2) {
+    typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<u16x4 *>(static_cast<T *>(a.kc) + at) =
+        u16x4{store_half(k.x), store_half(k.y), store_half(k.z), store_half(k.w)};
+    *reinterpret_cast<u16x4 *>(static_cast<T *>(a.vc) + at) =
+        u16x4{store_half(v.x), store_half(v.y), store_half(v.z), store_half(v.w)};
+  } else {
+    *reinterpret_cast<float4 *>(static_cast<T *>(a.kc) + at) = k;
+    *reinterpret_cast<float4 *>(static_cast<T *>(a.vc) + at) = v;
+  }
+}
+
+// Any layout: a block a token.
 
 template <class T>
 __global__ __launch_bounds__(256) void kv_store_paged_kernel(StoreArgs a) {
@@ -274,7 +378,7 @@ extern "C" int bh_paged_plan(const bh_paged_plan_args *args, bh_stream stream) {
     return fail(BH_ERR_SHAPE, "paged_plan: n_pages * page_size passes 2^31");
   if (!mul_size(p.table_width, p.page_size, &n) || n > 0x7fffffffu)
     return fail(BH_ERR_SHAPE, "paged_plan: table_width * page_size passes 2^31");
-  if (p.n_tok > 0x7fffffffu - kPlanThreads)
+  if (p.n_tok > 0x7fffffffu - 4096)
     return fail(BH_ERR_SHAPE, "paged_plan: n_tok passes 2^31");
   if (!p.q_start || !p.n_free || !p.n_free_out || !p.free_pages || (p.n_tok != 0 && !p.slots) ||
       (p.n_req != 0 && (!p.cached || !p.n_new || !p.block_table || !p.kv_len)))
@@ -290,7 +394,10 @@ extern "C" int bh_paged_plan(const bh_paged_plan_args *args, bh_stream stream) {
   a.n_req = static_cast<int>(p.n_req), a.n_tok = static_cast<int>(p.n_tok);
   a.width = static_cast<int>(p.table_width), a.n_pages = static_cast<int>(p.n_pages);
   a.page = FastDiv(static_cast<uint32_t>(p.page_size));
-  BH_LAUNCH(paged_plan_kernel, 1, kPlanThreads, 0, as_stream(stream), a);
+  hipStream_t st = as_stream(stream);
+  if (p.n_req <= 64 && p.n_tok <= 512) BH_LAUNCH((paged_plan_kernel<64, 1>), 1, 64, 0, st, a);
+  else if (p.n_req <= 1024) BH_LAUNCH((paged_plan_kernel<1024, 1>), 1, 1024, 0, st, a);
+  else BH_LAUNCH((paged_plan_kernel<1024, 4>), 1, 1024, 0, st, a);
   return ok();
 }
 
@@ -311,6 +418,22 @@ extern "C" int bh_kv_store_paged(const bh_paged_cache *cache, const float *k, co
   a.n_slots = static_cast<int>(cache->n_pages * cache->page_size);
   a.elems = static_cast<int>(cache->n_kv * cache->hd), a.hd = static_cast<int>(cache->hd);
   a.page = FastDiv(static_cast<uint32_t>(cache->page_size));
+  const size_t pieces = n_tok * (cache->n_kv * cache->hd / 4);
+  const size_t piece = cache->kv_dtype == BH_KV_F16 ? 8 : 16;
+  const auto whole = [](const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  if (cache->hd % 4 == 0 && pieces <= 0x7fffff00u && (cache->page_stride | cache->pos_stride |
+      cache->head_stride) % 4 == 0 && whole(cache->k, piece) && whole(cache->v, piece) &&
+      whole(k, 16) && whole(v, 16)) {
+    a.pieces = static_cast<int>(pieces);
+    a.row = FastDiv(static_cast<uint32_t>(cache->n_kv * cache->hd / 4));
+    a.head = FastDiv(static_cast<uint32_t>(cache->hd / 4));
+    const unsigned blocks = static_cast<unsigned>((pieces + 255) / 256);
+    if (cache->kv_dtype == BH_KV_F16)
+      BH_LAUNCH(kv_store_paged_pieces_kernel<uint16_t>, blocks, 256, 0, as_stream(stream), a);
+    else
+      BH_LAUNCH(kv_store_paged_pieces_kernel<float>, blocks, 256, 0, as_stream(stream), a);
+    return ok();
+  }
   if (cache->kv_dtype == BH_KV_F16)
     BH_LAUNCH(kv_store_paged_kernel<uint16_t>, static_cast<unsigned>(n_tok), 256, 0,
               as_stream(stream), a);
