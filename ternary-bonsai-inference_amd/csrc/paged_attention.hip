@@ -129,10 +129,13 @@ constexpr float kPUnit = 16384.0f;  // probabilities in f16 stand in units of 2^
 constexpr float kNoScore = -3.402823466e38f;  // the maximum of scores that are all -inf
 constexpr int kJoinRows = 8;        // rows of a tile that the waves join at a time
 
-// Where a call's work lies.  A request with n tokens has ceil(n group / R) row
-// tiles a kv head and ceil(len / U) units of U positions; the list of all
-// (request, kv head, row tile, unit) is cut into equal runs, one a worker.  Of the
-// tiles in a run only the first and the last can be cut: their parts go to the
+// Where a call's work lies.  A request with n tokens has T = ceil(n group / R) row
+// tiles a kv head, and a tile as many units of U positions as its last row sees.
+// Tiles t and T - 1 - t together have about the same number for every t (what a
+// tile sees grows evenly with t), so they stand side by side in a space of as many
+// units as any such pair has, and where a unit lies is found by dividing.  The list
+// of all (request, kv head, pair, unit) is cut into equal runs, one a worker.  Of
+// the tiles in a run only the first and the last can be cut: their parts go to the
 // worker's slots 0 and 1.
 struct Cut {  // a tile, written by the worker of its first part
   int rows;         // 0: it has one part, and its rows are done
@@ -147,6 +150,7 @@ struct Split {
   float *pm, *pl;  // [workers][2][R] running maximum (base 2) and sum
   float *pacc;     // [workers][2][R][hd]
   int workers;
+  int over, most;  // requests of more than `over` and up to `most` rows a kv head
 };
 
 // x / d; by the 32-bit divide, a tenth of the 64-bit one, where that does.
@@ -166,12 +170,42 @@ __device__ __forceinline__ int worker_of(int64_t total, int workers, int64_t u) 
   return static_cast<int>(u < big ? divide(u, base + 1) : rest + divide(u - big, base));
 }
 
+// A request's tiles and units.
 template <int R, int U>
-__device__ __forceinline__ void tiles_units(const PagedArgs &a, int n, int len, int *tiles,
-                                            int *units) {
-  *tiles = static_cast<int>((static_cast<int64_t>(n) * a.group + R - 1) / R);
-  *units = max((len + U - 1) / U, 1);
-}
+struct Work {
+  int q0, n, len;  // first token, tokens (0: not this launch's), positions
+  int tiles, pair, mid;  // units of a pair of tiles; of the one in the middle, or 0
+  int64_t head;          // units of a kv head
+
+  // Units of tile t; of a last tile that is not full also as if it were.
+  __device__ __forceinline__ int units(const PagedArgs &a, int t, bool full = false) const {
+    const int64_t last = (static_cast<int64_t>(t) + 1) * R - 1;
+    const int tok = last > 0x7fffffff ? 0x7fffffff : a.grp.div(static_cast<int>(last));
+    const int64_t sees = static_cast<int64_t>(len) - n + tok + 1;
+    const int64_t seen = full || sees < len ? sees : len;
+    return seen <= U ? 1 : static_cast<int>((seen + U - 1) / U);
+  }
+  __device__ __forceinline__ void load(const PagedArgs &a, const Split &sp, int r) {
+    request(a, r, &q0, &n, &len);
+    const int64_t rows = static_cast<int64_t>(n) * a.group;
+    if (rows <= sp.over || rows > sp.most) n = 0;
+    tiles = n == 0 ? 0 : static_cast<int>((rows + R - 1) / R);
+    pair = 1, mid = 0;
+    // two tiles with as many positions in all, but for a token of rounding, have as
+    // many units but for one
+    if (tiles > 1) pair = units(a, 0) + units(a, tiles - 1, true) + 1;
+    if (tiles & 1) mid = units(a, tiles / 2);
+    head = static_cast<int64_t>(tiles / 2) * pair + mid;
+  }
+  __device__ __forceinline__ int64_t cost(const PagedArgs &a) const { return head * a.n_kv; }
+  // From lane `l`.
+  __device__ __forceinline__ void take(int l) {
+    q0 = __builtin_amdgcn_readlane(q0, l), n = __builtin_amdgcn_readlane(n, l);
+    len = __builtin_amdgcn_readlane(len, l), tiles = __builtin_amdgcn_readlane(tiles, l);
+    pair = __builtin_amdgcn_readlane(pair, l), mid = __builtin_amdgcn_readlane(mid, l);
+    head = static_cast<int64_t>(tiles / 2) * pair + mid;
+  }
+};
 
 // f16 cache: SUB times 16 positions a step on v_mfma_f32_16x16x32_f16.
 //
@@ -190,7 +224,8 @@ __device__ __forceinline__ void tiles_units(const PagedArgs &a, int n, int len, 
 template <int HD, int RT>
 struct EngineF16 {
   using Elem = _Float16;
-  static constexpr int SUB = HD >= 256 ? 1 : 2;
+  static constexpr int SUB = HD >= 256 && RT == 1 ? 1 : 2;
+  static constexpr int kAhead = RT == 1 ? 1 : 3;  // steps of 32 dims whose q is read ahead
   static constexpr int kHd = HD, kRt = RT, kStep = 16 * SUB;
   static constexpr int KK = HD / 32, DV = HD >= 128 ? 8 : 4, NB = HD / (16 * DV);
   static constexpr int kQBytes = RT * KK * 2 * 64 * 16;
@@ -243,33 +278,44 @@ struct EngineF16 {
   }
   __device__ __forceinline__ void scores(const char *lds, int lane) {
     const h8 *q = reinterpret_cast<const h8 *>(lds) + lane;
+    // one chain for each half of q, summed at the end: the small ones first
+    f32x4 sh[RT][SUB], sl[RT][SUB];
+    h8 hi[kAhead][RT], lo[kAhead][RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      // one chain for each half of q, summed at the end: the small ones first
-      f32x4 sh[SUB], sl[SUB];
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) sh[s] = sl[s] = f32x4{0, 0, 0, 0};
-      h8 hi_next = q[t * KK * 128], lo_next = q[t * KK * 128 + 64];
+      for (int s = 0; s < SUB; ++s) sh[t][s] = sl[t][s] = f32x4{0, 0, 0, 0};
+    const auto read = [&](int kk) {
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        // the next operands are read here and not earlier: registers are short
-        __builtin_amdgcn_sched_barrier(0);
-        const h8 hi = hi_next, lo = lo_next;
-        if (kk + 1 < KK) {
-          hi_next = q[(t * KK + kk + 1) * 128];
-          lo_next = q[(t * KK + kk + 1) * 128 + 64];
-        }
+      for (int t = 0; t < RT; ++t) {
+        hi[kk % kAhead][t] = q[(t * KK + kk) * 128];
+        lo[kk % kAhead][t] = q[(t * KK + kk) * 128 + 64];
+      }
+    };
+#pragma unroll
+    for (int kk = 0; kk < kAhead && kk < KK; ++kk) read(kk);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      // operands are read kAhead steps ahead and not earlier: registers are short
+      __builtin_amdgcn_sched_barrier(0);
+      h8 h[RT], l[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) h[t] = hi[kk % kAhead][t], l[t] = lo[kk % kAhead][t];
+      if (kk + kAhead < KK) read(kk + kAhead);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-          sh[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], hi, sh[s], 0, 0, 0);
-          sl[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], lo, sl[s], 0, 0, 0);
+          sh[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], h[t], sh[t][s], 0, 0, 0);
+          sl[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], l[t], sl[t][s], 0, 0, 0);
         }
-      }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int s = 0; s < SUB; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[t][4 * s + i] = sl[s][i] + sh[s][i];
-    }
+        for (int i = 0; i < 4; ++i) sc[t][4 * s + i] = sl[t][s][i] + sh[t][s][i];
   }
   // sc holds the probabilities: their halves.
   __device__ __forceinline__ void split_p(int t) {
@@ -515,17 +561,38 @@ __device__ __forceinline__ int64_t wave_uniform(int64_t x) {
   return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-template <class E>
+// WIDE: the waves of a block take rows of their own, 16 RT each, and go through all
+// positions of a piece side by side, so that K and V come to the CU once for 64
+// RT rows; for many rows.  Otherwise they share the rows and take every fourth
+// step of positions each, and join what they have at the piece's end.
+// (within a wave LDS operations are in order; this keeps the compiler to it)
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <class E, bool WIDE>
+struct Shape {
+  static constexpr int kWaveRows = 16 * E::kRt, R = kWaveRows * (WIDE ? kWaves : 1);
+  static constexpr int kStride = E::kStep * (WIDE ? 1 : kWaves);  // from a wave's step to its next
+  static constexpr int U = WIDE ? 128 : kStride;
+};
+
+template <class E, bool WIDE>
 __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kernel(PagedArgs a, Split sp) {
   using Elem = typename E::Elem;
-  constexpr int HD = E::kHd, RT = E::kRt, R = 16 * RT, STEP = E::kStep, U = STEP * kWaves;
-  constexpr int kJoinStride = HD + 4;
-  constexpr int kJoin = kWaves * kJoinRows * kJoinStride * 4;
-  constexpr int kLds = kJoin > E::kQBytes ? kJoin : E::kQBytes;
+  using S = Shape<E, WIDE>;
+  constexpr int HD = E::kHd, RT = E::kRt, R = S::R, STEP = E::kStep, U = S::U;
+  constexpr int kJoinStride = HD + 4, kJoinWave = kJoinRows * kJoinStride * 4;
+  constexpr int kJoin = kWaves * kJoinWave, kQ = E::kQBytes * (WIDE ? kWaves : 1);
+  constexpr int kLds = kJoin > kQ ? kJoin : kQ;
+  static_assert(!WIDE || kJoinWave <= E::kQBytes, "a wave's rows leave through its own part");
   __shared__ __attribute__((aligned(16))) char lds[kLds];
   __shared__ int64_t off_s[kWaves][2][STEP];
-  __shared__ float fac_s[R], m_s[kWaves][R], l_s[kWaves][R];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ float fac_s[R], m_s[kWaves][WIDE ? 1 : R], l_s[kWaves][WIDE ? 1 : R];
+  // (read from a lane, so that what follows from the wave branches by scalars)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
 
   // The run of this worker in the list of all units.  Every wave finds it by
@@ -534,14 +601,13 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
   // that hold the run's beginning.
   const int worker = blockIdx.x;
   const int per = (a.n_req + 63) / 64;
-  int q0 = 0, n = 0, len = 0, tiles = 0, units = 1;
+  Work<R, U> work;
   int64_t mine = 0;
   int mine_tiles = 0;
   for (int i = lane * per; i < min((lane + 1) * per, a.n_req); ++i) {
-    request(a, i, &q0, &n, &len);
-    tiles_units<R, U>(a, n, len, &tiles, &units);
-    mine += static_cast<int64_t>(tiles) * a.n_kv * units;
-    mine_tiles += tiles * a.n_kv;
+    work.load(a, sp, i);
+    mine += work.cost(a);
+    mine_tiles += work.tiles * a.n_kv;
   }
   int64_t upto = mine;
   int upto_tiles = mine_tiles;
@@ -560,10 +626,9 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
       mine = 0;
       mine_tiles = 0;
       if (i + lane < min((owner + 1) * per, a.n_req)) {
-        request(a, i + lane, &q0, &n, &len);
-        tiles_units<R, U>(a, n, len, &tiles, &units);
-        mine = static_cast<int64_t>(tiles) * a.n_kv * units;
-        mine_tiles = tiles * a.n_kv;
+        work.load(a, sp, i + lane);
+        mine = work.cost(a);
+        mine_tiles = work.tiles * a.n_kv;
       }
       upto = mine;
       upto_tiles = mine_tiles;
@@ -584,28 +649,45 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
     }
   }
   r = __builtin_amdgcn_readfirstlane(r);
-  q0 = __builtin_amdgcn_readlane(q0, owner), n = __builtin_amdgcn_readlane(n, owner);
-  len = __builtin_amdgcn_readlane(len, owner), tiles = __builtin_amdgcn_readlane(tiles, owner);
-  units = __builtin_amdgcn_readlane(units, owner);
+  work.take(owner);
 
   for (int64_t at = begin; at < end;) {
-    const int64_t cost = static_cast<int64_t>(tiles) * a.n_kv * units;
-    if (at - base >= cost) {  // on to the next request
-      base += cost;
-      tile_base += tiles * a.n_kv;
-      ++r;
-      request(a, r, &q0, &n, &len);
-      tiles_units<R, U>(a, n, len, &tiles, &units);
+    if (at - base >= work.cost(a)) {  // on to the next request
+      base += work.cost(a);
+      tile_base += work.tiles * a.n_kv;
+      work.load(a, sp, ++r);
       continue;
     }
-    const int64_t x = at - base;
-    const int task = static_cast<int>(divide(x, units)), unit = static_cast<int>(x - static_cast<int64_t>(task) * units);
-    const int head = task / tiles, tile = task - head * tiles;
+    const int head = static_cast<int>(divide(at - base, work.head));
+    const int64_t in_head = at - base - head * work.head;
+    const int pair = static_cast<int>(min<int64_t>(divide(in_head, work.pair), work.tiles / 2));
+    int unit = static_cast<int>(in_head - static_cast<int64_t>(pair) * work.pair);
+    int tile = work.tiles / 2, units = work.mid;
+    if (pair < work.tiles / 2) {  // the longer tile first, then its partner
+      tile = work.tiles - 1 - pair;
+      units = work.units(a, tile);
+      if (unit >= units) {
+        unit -= units;
+        tile = pair;
+        const int before = units;
+        units = work.units(a, tile);
+        if (unit >= units) {  // the rest of the pair's space is empty
+          at += work.pair - before - unit;
+          continue;
+        }
+      }
+    }
+    const int q0 = work.q0, n = work.n, len = work.len;
     const int unit_end = static_cast<int>(min<int64_t>(units, unit + (end - at)));
     const int rows = min(R, n * a.group - tile * R);
-    const int first_tok = a.grp.div(tile * R), last_tok = a.grp.div(tile * R + rows - 1);
-    const int min_vis = max(len - n + first_tok + 1, 0);
-    const int max_vis = max(len - n + last_tok + 1, 0);
+    // this wave's rows
+    const int row0 = WIDE ? wave * S::kWaveRows : 0;
+    const int my_rows = WIDE ? min(S::kWaveRows, rows - row0) : rows;
+    int min_vis = 0, max_vis = 0;
+    if (my_rows > 0) {
+      min_vis = max(len - n + a.grp.div(tile * R + row0) + 1, 0);
+      max_vis = max(len - n + a.grp.div(tile * R + row0 + my_rows - 1) + 1, 0);
+    }
     const int p_end = min(min(unit_end * U, len), max_vis);
     const int32_t *table = a.table + static_cast<size_t>(r) * a.width;
     const Elem *kc = static_cast<const Elem *>(a.kc) + head * a.head_stride;
@@ -613,15 +695,15 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
 
     // the table entries of this wave's first rows and the block's q rows on their
     // way together, then the cache rows, then q into LDS as matrix operands
-    int p0 = unit * U + wave * STEP;
+    int p0 = unit * U + (WIDE ? 0 : wave * STEP);
     Rows<STEP> rows_of;
     rows_of.fetch(a, table, p0 + lane % STEP, p_end);
     constexpr int kLanes = HD / 4, kAt = kThreads / kLanes;  // lanes of a row, rows at once
-    constexpr int kQ = (R + kAt - 1) / kAt;
-    float4 qv[kQ];
+    constexpr int kRows = (R + kAt - 1) / kAt;
+    float4 qv[kRows];
     const int qd = tid % kLanes * 4;
 #pragma unroll
-    for (int x = 0; x < kQ; ++x) {
+    for (int x = 0; x < kRows; ++x) {
       const int i = tid / kLanes + x * kAt, row = tile * R + i, tok = a.grp.div(row);
       qv[x] = make_float4(0, 0, 0, 0);
       if (i < rows)
@@ -635,11 +717,11 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
       mask = rows_of.place(a, off_s[wave][0], p0 + lane % STEP, p_end, lane);
       eng.load_k(kc, off_s[wave][0], lane);
       eng.load_v(vc, off_s[wave][0], lane);
-      rows_of.fetch(a, table, p0 + U + lane % STEP, p_end);
+      rows_of.fetch(a, table, p0 + S::kStride + lane % STEP, p_end);
     }
     __syncthreads();  // the piece before has been read
 #pragma unroll
-    for (int x = 0; x < kQ; ++x) {
+    for (int x = 0; x < kRows; ++x) {
       const int i = tid / kLanes + x * kAt;
       float up = 1.0f, down = a.scale;
       if constexpr (E::kScaleQ) {
@@ -653,8 +735,8 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
           down = ldexpf(a.scale, ex - 14);
         }
       }
-      if (kQ * kAt == R || i < R) {
-        E::store_q(lds, i, qd, qv[x], up);
+      if (kRows * kAt == R || i < R) {
+        E::store_q(lds + i / S::kWaveRows * E::kQBytes, i % S::kWaveRows, qd, qv[x], up);
         if (qd == 0) fac_s[i] = down * kExpL2E;
       }
     }
@@ -665,7 +747,7 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
     int vis[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int i = 16 * t + c;
+      const int i = row0 + 16 * t + c;
       m[t] = -INFINITY;
       l[t] = 0.0f;
       some[t] = false;
@@ -675,13 +757,13 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
     eng.clear();
     if (p0 < p_end) {
       for (int s = 1;; s ^= 1) {
-        const int next = p0 + U;
-        eng.scores(lds, lane);
+        const int next = p0 + S::kStride;
+        eng.scores(lds + (WIDE ? wave * E::kQBytes : 0), lane);
         uint32_t next_mask = 0;
         if (next < p_end) {
           next_mask = rows_of.place(a, off_s[wave][s], next + lane % STEP, p_end, lane);
           eng.load_k(kc, off_s[wave][s], lane);
-          rows_of.fetch(a, table, next + U + lane % STEP, p_end);
+          rows_of.fetch(a, table, next + S::kStride + lane % STEP, p_end);
         }
         constexpr uint32_t kAll = ~0u >> (32 - STEP);
         const bool edge = mask != kAll || p0 + STEP > min_vis;
@@ -707,7 +789,7 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
 #pragma unroll
             for (int j = 0; j < E::kSlots; ++j) odd |= eng.sc[t][j] != eng.sc[t][j];
             if (__builtin_expect(__any(odd), false)) {
-              const int row = tile * R + 16 * t + c, tok = a.grp.div(row);
+              const int row = tile * R + row0 + 16 * t + c, tok = a.grp.div(row);
               const float *q = a.q + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
                                       (row - tok * a.group)) * HD;
 #pragma unroll
@@ -779,7 +861,6 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
       }
     }
 
-    // the waves' states joined, kJoinRows rows at a time
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       l[t] = row_lanes(l[t], SumOp{});
@@ -787,10 +868,45 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
       // as its maximum and is 0
       const float seen = row_lanes(some[t] ? 1.0f : 0.0f, MaxOp{});
       if (m[t] == -INFINITY && seen != 0.0f) m[t] = kNoScore;
-      if (g == 0) m_s[wave][16 * t + c] = m[t], l_s[wave][16 * t + c] = l[t];
     }
     const bool whole = unit == 0 && unit_end == units;
     const size_t slot = static_cast<size_t>(worker) * 2 + (at == begin ? 0 : 1);
+    if constexpr (WIDE) {
+      // through the wave's part of LDS, so that rows leave in whole lines
+      float *mine_s = reinterpret_cast<float *>(lds + wave * E::kQBytes);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const float by = !whole ? E::kAccUnit : m[t] == -INFINITY ? 0.0f : E::kAccUnit / l[t];
+        if (!whole && g == 0 && 16 * t + c < my_rows) {
+          sp.pm[slot * R + row0 + 16 * t + c] = m[t];
+          sp.pl[slot * R + row0 + 16 * t + c] = l[t];
+        }
+#pragma unroll
+        for (int half = 0; half < 16; half += kJoinRows) {
+          const int here = min(kJoinRows, my_rows - 16 * t - half);
+          if (here <= 0) continue;
+          wave_sync();
+          if (c >= half && c < half + kJoinRows)
+            eng.each_piece(t, lane, [&](int d, f32x4 o) {
+              *reinterpret_cast<f32x4 *>(mine_s + (c - half) * kJoinStride + d) = o * by;
+            });
+          wave_sync();
+          for (int i = lane; i < here * (HD / 4); i += 64) {
+            const int rr = i / (HD / 4), d = i % (HD / 4) * 4, row = row0 + 16 * t + half + rr;
+            const int tok = a.grp.div(tile * R + row);
+            float *dst = whole ? a.out + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                                          (tile * R + row - tok * a.group)) * HD
+                               : sp.pacc + (slot * R + row) * HD;
+            *reinterpret_cast<f32x4 *>(dst + d) =
+                *reinterpret_cast<const f32x4 *>(mine_s + rr * kJoinStride + d);
+          }
+        }
+      }
+    } else {
+      // the waves' states joined, kJoinRows rows at a time
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        if (g == 0) m_s[wave][16 * t + c] = m[t], l_s[wave][16 * t + c] = l[t];
     float *join = reinterpret_cast<float *>(lds);
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -831,29 +947,36 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
           }
         }
       }
+    }
     if (unit == 0 && tid == 0) {
       Cut cut{whole ? 0 : rows, worker, worker, at == begin ? 0 : 1, tile * R, q0, head};
       if (!whole) cut.last = worker_of(total, sp.workers, at + units - 1);
-      sp.cut[tile_base + task] = cut;
+      sp.cut[tile_base + head * work.tiles + tile] = cut;
     }
     at += unit_end - unit;
   }
 }
 
 // Joins the parts of the tiles that more than one worker has: `share` blocks a
-// tile, each over every share-th (row, 64 dims) of it.  16 lanes take the dims, 16
-// threads each every sixteenth part, whose loads are all issued before the first
-// is needed: one round trip for up to 16 kAhead parts.
+// tile.  16 lanes take 64 dims of a row; of the block's 16 such groups as many
+// share a row as it has parts, each with every sixteenth part, whose loads are all
+// issued before the first is needed: one round trip for up to 16 kAhead parts.
 template <int HD, int R>
 __global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, Split sp, int share) {
   constexpr int kAt = kThreads / 16, kSlices = HD / 64, kAhead = 8;
-  __shared__ float part[kAt][64], sums[kAt], red[kWaves];
+  __shared__ float part[kAt][64], sums[kAt], tops[kAt];
   const int tile = blockIdx.x / share, tid = threadIdx.x;
   const Cut cut = sp.cut[tile];
-  if (tile >= *sp.n_tiles) return;  // cut holds nothing then
-  const int lane_part = tid >> 4, d = (tid & 15) * 4;
-  for (int i = blockIdx.x - tile * share; i < cut.rows * kSlices; i += share) {
-    const int row = i / kSlices, dim = i % kSlices * 64 + d;
+  if (tile >= *sp.n_tiles || cut.rows == 0) return;  // (past n_tiles cut holds nothing)
+  const int parts = cut.last - cut.first + 1;
+  int p = 2;  // groups of a row
+  while (p < parts && p < kAt) p <<= 1;
+  const int group = tid >> 4, mine = group & (p - 1), d = (tid & 15) * 4;
+  const int items = cut.rows * kSlices, at_once = kAt / p;
+  for (int i0 = (blockIdx.x - tile * share) * at_once; i0 < items; i0 += share * at_once) {
+    const int item = i0 + group / p;
+    const bool live = item < items;
+    const int row = live ? item / kSlices : 0, dim = item % kSlices * 64 + d;
     const auto at = [&](int w) {
       return (static_cast<size_t>(w) * 2 + (w == cut.first ? cut.slot : 0)) * R + row;
     };
@@ -862,9 +985,8 @@ __global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, 
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) {
       // past the last part: the last again, at no weight
-      const int w = cut.first + lane_part + x * kAt;
-      if (cut.first + x * kAt > cut.last) break;
-      const size_t o = at(min(w, cut.last));
+      if (x * p >= parts) break;
+      const size_t o = at(min(cut.first + mine + x * p, cut.last));
       ahead[x] = *reinterpret_cast<const f32x4 *>(sp.pacc + o * HD + dim);
       pm[x] = sp.pm[o];
       pl[x] = sp.pl[o];
@@ -872,72 +994,81 @@ __global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, 
     float top = -INFINITY;
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) {
-      if (cut.first + x * kAt > cut.last) break;
+      if (x * p >= parts) break;
       top = fmaxf(top, pm[x]);
     }
-    for (int w = cut.first + lane_part + kAhead * kAt; w <= cut.last; w += kAt)
+    for (int w = cut.first + mine + kAhead * p; w <= cut.last; w += p)
       top = fmaxf(top, sp.pm[at(w)]);
-    top = group_reduce<kThreads>(top, MaxOp{}, red);
+    if (d == 0) tops[group] = top;
+    __syncthreads();
+    for (int k = 0; k < p; ++k) top = fmaxf(top, tops[(group - mine) + k]);
     const float ref = top == -INFINITY ? 0.0f : top;
     f32x4 o = {0, 0, 0, 0};
     float sum = 0.0f;
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) {
-      if (cut.first + x * kAt > cut.last) break;
-      if (cut.first + lane_part + x * kAt > cut.last) continue;
+      if (x * p >= parts) break;
+      if (mine + x * p >= parts) continue;
       const float keep = __builtin_amdgcn_exp2f(pm[x] - ref);
       sum += keep * pl[x];
       o += keep * ahead[x];
     }
 #pragma unroll 4
-    for (int w = cut.first + lane_part + kAhead * kAt; w <= cut.last; w += kAt) {
-      const size_t p = at(w);
-      const float keep = __builtin_amdgcn_exp2f(sp.pm[p] - ref);
-      sum += keep * sp.pl[p];
-      o += keep * *reinterpret_cast<const f32x4 *>(sp.pacc + p * HD + dim);
+    for (int w = cut.first + mine + kAhead * p; w <= cut.last; w += p) {
+      const size_t x = at(w);
+      const float keep = __builtin_amdgcn_exp2f(sp.pm[x] - ref);
+      sum += keep * sp.pl[x];
+      o += keep * *reinterpret_cast<const f32x4 *>(sp.pacc + x * HD + dim);
     }
-    *reinterpret_cast<f32x4 *>(&part[lane_part][d]) = o;
-    if (d == 0) sums[lane_part] = sum;
+    *reinterpret_cast<f32x4 *>(&part[group][d]) = o;
+    if (d == 0) sums[group] = sum;
     __syncthreads();
-    if (tid < 16) {
-#pragma unroll
-      for (int w = 1; w < kAt; ++w) {
-        o += *reinterpret_cast<const f32x4 *>(&part[w][d]);
-        sum += sums[w];
+    if (mine == 0 && live) {
+      for (int k = 1; k < p; ++k) {
+        o += *reinterpret_cast<const f32x4 *>(&part[group + k][d]);
+        sum += sums[group + k];
       }
       const int q_row = cut.row0 + row, tok = a.grp.div(q_row);
       *reinterpret_cast<f32x4 *>(
           a.out + (static_cast<size_t>(cut.q0 + tok) * a.n_head + cut.head * a.group +
                    (q_row - tok * a.group)) * HD + dim) = o * (top == -INFINITY ? 0.0f : 1.0f / sum);
     }
-    __syncthreads();  // for the next row
+    __syncthreads();  // for the next rows
   }
 }
 
-// Workers of a launch: two blocks a compute unit with one row tile, one with two.
-int workers_of(int rt) { return static_cast<int>(device_cu_count()) * (rt == 1 ? 2 : 1); }
+// One launch of the kernel with RT row tiles a wave.
+struct Form {
+  int rt;
+  bool wide;
+  int over, most;  // the requests it takes, by rows a kv head
+
+  int rows() const { return 16 * rt * (wide ? kWaves : 1); }
+  // two blocks a compute unit with one row tile, one with two
+  int workers() const { return static_cast<int>(device_cu_count()) * (rt == 1 ? 2 : 1); }
+};
 
 size_t align256(size_t n) { return (n + 255) & ~size_t{255}; }
 
-// Tiles that a call can have at most.
-size_t most_tiles(const PagedArgs &a, int R) {
+// Tiles that a launch can have at most.
+size_t most_tiles(const PagedArgs &a, const Form &f) {
   const size_t rows = static_cast<size_t>(a.n_tok) * a.group;
-  return static_cast<size_t>(a.n_kv) * (rows / R + (static_cast<size_t>(a.n_req) < static_cast<size_t>(a.n_tok) ? a.n_req : a.n_tok));
+  return static_cast<size_t>(a.n_kv) * (rows / f.rows() + (a.n_req < a.n_tok ? a.n_req : a.n_tok));
 }
 
 // Workspace: tile count, tiles, maxima, sums, accumulators.
-size_t workspace_of(const PagedArgs &a, int rt) {
-  const size_t parts = static_cast<size_t>(workers_of(rt)) * 2 * 16 * rt;
-  return 256 + align256(most_tiles(a, 16 * rt) * sizeof(Cut)) + 2 * align256(parts * 4) +
-         parts * a.hd * 4;
+size_t workspace_of(const PagedArgs &a, const Form &f) {
+  const size_t parts = static_cast<size_t>(f.workers()) * 2 * f.rows();
+  return 256 + align256(most_tiles(a, f) * sizeof(Cut)) + 2 * align256(parts * 4) +
+         align256(parts * a.hd * 4);
 }
 
-template <class E>
-int launch(const PagedArgs &a, char *ws, hipStream_t st) {
-  constexpr int R = 16 * E::kRt, U = E::kStep * kWaves;
+template <class E, bool WIDE>
+int launch(const PagedArgs &a, const Form &f, char *ws, hipStream_t st) {
+  constexpr int R = Shape<E, WIDE>::R;
   Split sp{};
-  sp.workers = workers_of(E::kRt);
-  const size_t parts = static_cast<size_t>(sp.workers) * 2 * R, tiles = most_tiles(a, R);
+  sp.workers = f.workers(), sp.over = f.over, sp.most = f.most;
+  const size_t parts = static_cast<size_t>(sp.workers) * 2 * R, tiles = most_tiles(a, f);
   sp.n_tiles = reinterpret_cast<int *>(ws);
   ws += 256;
   sp.cut = reinterpret_cast<Cut *>(ws);
@@ -947,8 +1078,8 @@ int launch(const PagedArgs &a, char *ws, hipStream_t st) {
   sp.pl = reinterpret_cast<float *>(ws);
   ws += align256(parts * 4);
   sp.pacc = reinterpret_cast<float *>(ws);
-  BH_LAUNCH(attn_paged_kernel<E>, static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
-  if (a.max_len > U) {  // with one unit a tile nothing is cut
+  BH_LAUNCH((attn_paged_kernel<E, WIDE>), static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
+  if (a.max_len > Shape<E, WIDE>::U) {  // with one unit a tile nothing is cut
     // a block a (row, 64 dims) while they are not many times what fits the card
     const size_t most = static_cast<size_t>(a.n_tok > 1 ? R : a.group < R ? a.group : R) * (E::kHd / 64);
     size_t share = 16 * device_cu_count() / tiles;
@@ -959,16 +1090,22 @@ int launch(const PagedArgs &a, char *ws, hipStream_t st) {
   return BH_OK;
 }
 
-template <int RT>
-int launch_rt(const PagedArgs &a, bool f16, char *ws, hipStream_t st) {
+template <int RT, bool WIDE>
+int launch_rt(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st) {
   if (f16) {
-    if (a.hd == 64) return launch<EngineF16<64, RT>>(a, ws, st);
-    if (a.hd == 128) return launch<EngineF16<128, RT>>(a, ws, st);
-    return launch<EngineF16<256, RT>>(a, ws, st);
+    if (a.hd == 64) return launch<EngineF16<64, RT>, WIDE>(a, f, ws, st);
+    if (a.hd == 128) return launch<EngineF16<128, RT>, WIDE>(a, f, ws, st);
+    return launch<EngineF16<256, RT>, WIDE>(a, f, ws, st);
   }
-  if (a.hd == 64) return launch<EngineF32<64, RT>>(a, ws, st);
-  if (a.hd == 128) return launch<EngineF32<128, RT>>(a, ws, st);
-  return launch<EngineF32<256, RT>>(a, ws, st);
+  if (a.hd == 64) return launch<EngineF32<64, RT>, WIDE>(a, f, ws, st);
+  if (a.hd == 128) return launch<EngineF32<128, RT>, WIDE>(a, f, ws, st);
+  return launch<EngineF32<256, RT>, WIDE>(a, f, ws, st);
+}
+
+int launch_form(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st) {
+  if (f.wide) return launch_rt<2, true>(a, f16, f, ws, st);
+  if (f.rt == 1) return launch_rt<1, false>(a, f16, f, ws, st);
+  return launch_rt<2, false>(a, f16, f, ws, st);
 }
 
 // Whether a call runs on the matrix cores: rows of whole 16-byte pieces.
@@ -980,10 +1117,23 @@ bool on_matrix_cores(const bh_attention_paged_args &p) {
          aligned16(c.v) && aligned16(p.q) && aligned16(p.out);
 }
 
-// Row tiles a block: two where a request may have more than 16 rows a kv head.
-int row_tiles(const bh_attention_paged_args &p) {
-  const size_t most = p.max_new == 0 || p.max_new > p.n_tok ? p.n_tok : p.max_new;
-  return most * (p.n_head / p.cache.n_kv) <= 16 ? 1 : 2;
+// The launches of a call, by the most rows a kv head that a request may have.
+constexpr int kWideOver = 32;  // rows from which a request goes to the wide form where there is one
+int forms_of(const bh_attention_paged_args &p, Form *f) {
+  const size_t tokens = p.max_new == 0 || p.max_new > p.n_tok ? p.n_tok : p.max_new;
+  const size_t rows = tokens * (p.n_head / p.cache.n_kv);
+  constexpr int kAll = 0x7fffffff;
+  if (rows <= 64) {
+    f[0] = Form{rows <= 16 ? 1 : 2, false, 0, kAll};
+    return 1;
+  }
+  if (p.n_req == 1) {
+    f[0] = Form{2, true, 0, kAll};
+    return 1;
+  }
+  f[0] = Form{2, true, kWideOver, kAll};
+  f[1] = Form{1, false, 0, kWideOver};
+  return 2;
 }
 
 // Checks the arguments and fills `a`.
@@ -1001,8 +1151,8 @@ int prepare(const bh_attention_paged_args &p, PagedArgs *a) {
       p.n_tok * p.n_head > 0x7fffffffu || !mul_size(p.n_tok, p.n_head * c.hd, sizeof(float), &n) ||
       n > SIZE_MAX / 2)
     return fail(BH_ERR_SHAPE, "attention_paged: size overflow");
-  if (p.table_width == 0 || !mul_size(p.table_width, c.page_size, &n) || n > 0x7fffffffu)
-    return fail(BH_ERR_SHAPE, "attention_paged: table_width * page_size must be 1 .. 2^31 - 1");
+  if (p.table_width == 0 || !mul_size(p.table_width, c.page_size, &n) || n > 0x7fff0000u)
+    return fail(BH_ERR_SHAPE, "attention_paged: table_width * page_size must be 1 .. 2^31 - 65536");
   if (p.n_tok != 0 && p.n_req != 0) {
     if (!p.q || !p.out || !p.q_start || !p.kv_len || !p.block_table)
       return fail(BH_ERR_ARG, "attention_paged: null pointer");
@@ -1032,7 +1182,10 @@ extern "C" size_t bh_attention_paged_workspace(const bh_attention_paged_args *ar
   PagedArgs a{};
   if (!args || prepare(*args, &a) != BH_OK || !on_matrix_cores(*args)) return 0;
   if (a.n_tok == 0 || a.n_req == 0) return 0;
-  return workspace_of(a, row_tiles(*args));
+  Form f[2];
+  size_t need = 0;
+  for (int i = 0, n = forms_of(*args, f); i < n; ++i) need += workspace_of(a, f[i]);
+  return need;
 }
 
 extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream stream) {
@@ -1044,8 +1197,10 @@ extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream
   const bool f16 = p.cache.kv_dtype == BH_KV_F16;
   hipStream_t st = as_stream(stream);
   if (on_matrix_cores(p)) {
-    const int rt = row_tiles(p);
-    const size_t need = workspace_of(a, rt);
+    Form f[2];
+    const int n = forms_of(p, f);
+    size_t need = 0;
+    for (int i = 0; i < n; ++i) need += workspace_of(a, f[i]);
     char *ws = static_cast<char *>(p.workspace);
     if (ws) {
       if (!aligned16(ws) || p.workspace_bytes < need)
@@ -1056,7 +1211,10 @@ extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream
       ws = static_cast<char *>(device_scratch(need, kScratchPaged, st));
       if (!ws) return BH_ERR_HIP;
     }
-    if (int e = rt == 1 ? launch_rt<1>(a, f16, ws, st) : launch_rt<2>(a, f16, ws, st)) return e;
+    for (int i = 0; i < n; ++i) {
+      if (int e = launch_form(a, f16, f[i], ws, st)) return e;
+      ws += workspace_of(a, f[i]);
+    }
     return ok();
   }
   const dim3 grid(static_cast<unsigned>(a.n_tok), static_cast<unsigned>(a.n_head));
