@@ -118,10 +118,9 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedArgs a) {
 
 // ---- matrix-core path (hd 64, 128, 256) ---------------------------------------
 
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
@@ -285,30 +284,30 @@ struct EngineF16 {
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int s = 0; s < SUB; ++s) sh[t][s] = sl[t][s] = f32x4{0, 0, 0, 0};
-    const auto read = [&](int kk) {
+#pragma unroll
+    for (int kk = 0; kk < kAhead && kk < KK; ++kk)
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        hi[kk % kAhead][t] = q[(t * KK + kk) * 128];
-        lo[kk % kAhead][t] = q[(t * KK + kk) * 128 + 64];
+        hi[kk][t] = q[(t * KK + kk) * 128];
+        lo[kk][t] = q[(t * KK + kk) * 128 + 64];
       }
-    };
-#pragma unroll
-    for (int kk = 0; kk < kAhead && kk < KK; ++kk) read(kk);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       // operands are read kAhead steps ahead and not earlier: registers are short
       __builtin_amdgcn_sched_barrier(0);
-      h8 h[RT], l[RT];
 #pragma unroll
-      for (int t = 0; t < RT; ++t) h[t] = hi[kk % kAhead][t], l[t] = lo[kk % kAhead][t];
-      if (kk + kAhead < KK) read(kk + kAhead);
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
+      for (int t = 0; t < RT; ++t) {
+        const h8 h = hi[kk % kAhead][t], l = lo[kk % kAhead][t];
+        if (kk + kAhead < KK) {
+          hi[kk % kAhead][t] = q[(t * KK + kk + kAhead) * 128];
+          lo[kk % kAhead][t] = q[(t * KK + kk + kAhead) * 128 + 64];
+        }
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-          sh[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], h[t], sh[t][s], 0, 0, 0);
-          sl[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], l[t], sl[t][s], 0, 0, 0);
+          sh[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], h, sh[t][s], 0, 0, 0);
+          sl[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s][kk], l, sl[t][s], 0, 0, 0);
         }
+      }
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -561,6 +560,136 @@ __device__ __forceinline__ int64_t wave_uniform(int64_t x) {
   return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
+// A worker's run, piece by piece.
+struct Piece {
+  int r, q0, n, len;             // request
+  int head, tile, units;         // kv head, row tile and its units
+  int unit, unit_end;            // those of this piece
+  int rows;                      // rows of the tile
+  int slot;                      // where a part of a tile goes: [workers][2]
+  bool whole;                    // the piece is all of the tile
+};
+
+template <int R, int U>
+struct Walk {
+  int64_t total, end, at, base, begin;
+  int tile_base, r, worker;
+  Work<R, U> work;
+
+  // Every wave finds the run by itself: lane i adds up requests i per .. (i + 1)
+  // per - 1, a scan over the lanes gives the total, and the lanes then go through
+  // the one lane's requests that hold the run's beginning.
+  __device__ __forceinline__ void start(const PagedArgs &a, const Split &sp, int lane) {
+    worker = blockIdx.x;
+    const int per = (a.n_req + 63) / 64;
+    int64_t mine = 0;
+    int mine_tiles = 0;
+    for (int i = lane * per; i < min((lane + 1) * per, a.n_req); ++i) {
+      work.load(a, sp, i);
+      mine += work.cost(a);
+      mine_tiles += work.tiles * a.n_kv;
+    }
+    int64_t upto = mine;
+    int upto_tiles = mine_tiles;
+    wave_scan(&upto, &upto_tiles, lane);
+    total = wave_uniform(__shfl(upto, 63));
+    at = begin = wave_uniform(run_begin(total, sp.workers, worker));
+    end = wave_uniform(run_begin(total, sp.workers, worker + 1));
+    if (worker == 0 && threadIdx.x == 63) *sp.n_tiles = upto_tiles;
+    base = 0, tile_base = 0, r = 0;
+    if (begin >= end) {
+      work.take(0);
+      return;
+    }
+    int owner = __builtin_ffsll(__ballot(begin < upto)) - 1;
+    base = wave_uniform(__shfl(upto - mine, owner));
+    tile_base = __builtin_amdgcn_readlane(upto_tiles - mine_tiles, owner);
+    r = owner;
+    if (per > 1) {
+      for (int i = owner * per;; i += 64) {
+        mine = 0;
+        mine_tiles = 0;
+        if (i + lane < min((owner + 1) * per, a.n_req)) {
+          work.load(a, sp, i + lane);
+          mine = work.cost(a);
+          mine_tiles = work.tiles * a.n_kv;
+        }
+        upto = mine;
+        upto_tiles = mine_tiles;
+        wave_scan(&upto, &upto_tiles, lane);
+        upto += base;
+        upto_tiles += tile_base;
+        const uint64_t past = __ballot(begin < upto);
+        if (past) {
+          const int at_lane = __builtin_ffsll(past) - 1;
+          r = i + at_lane;
+          base = wave_uniform(__shfl(upto - mine, at_lane));
+          tile_base = __builtin_amdgcn_readlane(upto_tiles - mine_tiles, at_lane);
+          owner = at_lane;
+          break;
+        }
+        base = wave_uniform(__shfl(upto, 63));
+        tile_base = __builtin_amdgcn_readlane(upto_tiles, 63);
+      }
+    }
+    r = __builtin_amdgcn_readfirstlane(r);
+    work.take(owner);
+  }
+
+  // The next piece, or false at the run's end.
+  __device__ __forceinline__ bool next(const PagedArgs &a, const Split &sp, Piece *p) {
+    while (at < end) {
+      if (at - base >= work.cost(a)) {  // on to the next request
+        base += work.cost(a);
+        tile_base += work.tiles * a.n_kv;
+        work.load(a, sp, ++r);
+        continue;
+      }
+      const int head = static_cast<int>(divide(at - base, work.head));
+      const int64_t in_head = at - base - head * work.head;
+      const int pair = static_cast<int>(min<int64_t>(divide(in_head, work.pair), work.tiles / 2));
+      int unit = static_cast<int>(in_head - static_cast<int64_t>(pair) * work.pair);
+      int tile = work.tiles / 2, units = work.mid;
+      if (pair < work.tiles / 2) {  // the longer tile first, then its partner
+        tile = work.tiles - 1 - pair;
+        units = work.units(a, tile);
+        if (unit >= units) {
+          unit -= units;
+          tile = pair;
+          const int before = units;
+          units = work.units(a, tile);
+          if (unit >= units) {  // the rest of the pair's space is empty
+            at += work.pair - before - unit;
+            continue;
+          }
+        }
+      }
+      const int unit_end = static_cast<int>(min<int64_t>(units, unit + (end - at)));
+      // all of it is the wave's, and stays in scalars
+      *p = Piece{uni(r), uni(work.q0), uni(work.n), uni(work.len), uni(head), uni(tile), uni(units),
+                 uni(unit), uni(unit_end), uni(min(R, work.n * a.group - tile * R)),
+                 uni(worker * 2 + (at == begin ? 0 : 1)), uni(unit == 0 && unit_end == units) != 0};
+      at = wave_uniform(at), base = wave_uniform(base), tile_base = uni(tile_base), r = p->r;
+      work.q0 = p->q0, work.n = p->n, work.len = p->len, work.tiles = uni(work.tiles);
+      work.pair = uni(work.pair), work.mid = uni(work.mid);
+      work.head = static_cast<int64_t>(work.tiles / 2) * work.pair + work.mid;
+      return true;
+    }
+    return false;
+  }
+  static __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+  // After a piece: the worker of a tile's first part says where its parts are.
+  __device__ __forceinline__ void done(const Split &sp, const Piece &p) {
+    if (p.unit == 0 && threadIdx.x == 0) {
+      Cut cut{p.whole ? 0 : p.rows, worker, worker, at == begin ? 0 : 1, p.tile * R, p.q0, p.head};
+      if (!p.whole) cut.last = worker_of(total, sp.workers, at + p.units - 1);
+      sp.cut[tile_base + p.head * work.tiles + p.tile] = cut;
+    }
+    at += p.unit_end - p.unit;
+  }
+};
+
 // WIDE: the waves of a block take rows of their own, 16 RT each, and go through all
 // positions of a piece side by side, so that K and V come to the CU once for 64
 // RT rows; for many rows.  Otherwise they share the rows and take every fourth
@@ -595,91 +724,12 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
 
-  // The run of this worker in the list of all units.  Every wave finds it by
-  // itself: lane i adds up requests i per .. (i + 1) per - 1, a scan over the
-  // lanes gives the total, and the lanes then go through the one lane's requests
-  // that hold the run's beginning.
-  const int worker = blockIdx.x;
-  const int per = (a.n_req + 63) / 64;
-  Work<R, U> work;
-  int64_t mine = 0;
-  int mine_tiles = 0;
-  for (int i = lane * per; i < min((lane + 1) * per, a.n_req); ++i) {
-    work.load(a, sp, i);
-    mine += work.cost(a);
-    mine_tiles += work.tiles * a.n_kv;
-  }
-  int64_t upto = mine;
-  int upto_tiles = mine_tiles;
-  wave_scan(&upto, &upto_tiles, lane);
-  const int64_t total = wave_uniform(__shfl(upto, 63));
-  const int64_t begin = run_begin(total, sp.workers, worker);
-  const int64_t end = run_begin(total, sp.workers, worker + 1);
-  if (worker == 0 && tid == 63) *sp.n_tiles = upto_tiles;
-  if (begin >= end) return;
-  int owner = __builtin_ffsll(__ballot(begin < upto)) - 1;
-  int64_t base = wave_uniform(__shfl(upto - mine, owner));
-  int tile_base = __builtin_amdgcn_readlane(upto_tiles - mine_tiles, owner);
-  int r = __builtin_amdgcn_readfirstlane(owner);
-  if (per > 1) {
-    for (int i = owner * per;; i += 64) {
-      mine = 0;
-      mine_tiles = 0;
-      if (i + lane < min((owner + 1) * per, a.n_req)) {
-        work.load(a, sp, i + lane);
-        mine = work.cost(a);
-        mine_tiles = work.tiles * a.n_kv;
-      }
-      upto = mine;
-      upto_tiles = mine_tiles;
-      wave_scan(&upto, &upto_tiles, lane);
-      upto += base;
-      upto_tiles += tile_base;
-      const uint64_t past = __ballot(begin < upto);
-      if (past) {
-        const int at_lane = __builtin_ffsll(past) - 1;
-        r = i + at_lane;
-        base = wave_uniform(__shfl(upto - mine, at_lane));
-        tile_base = __builtin_amdgcn_readlane(upto_tiles - mine_tiles, at_lane);
-        owner = at_lane;
-        break;
-      }
-      base = wave_uniform(__shfl(upto, 63));
-      tile_base = __builtin_amdgcn_readlane(upto_tiles, 63);
-    }
-  }
-  r = __builtin_amdgcn_readfirstlane(r);
-  work.take(owner);
-
-  for (int64_t at = begin; at < end;) {
-    if (at - base >= work.cost(a)) {  // on to the next request
-      base += work.cost(a);
-      tile_base += work.tiles * a.n_kv;
-      work.load(a, sp, ++r);
-      continue;
-    }
-    const int head = static_cast<int>(divide(at - base, work.head));
-    const int64_t in_head = at - base - head * work.head;
-    const int pair = static_cast<int>(min<int64_t>(divide(in_head, work.pair), work.tiles / 2));
-    int unit = static_cast<int>(in_head - static_cast<int64_t>(pair) * work.pair);
-    int tile = work.tiles / 2, units = work.mid;
-    if (pair < work.tiles / 2) {  // the longer tile first, then its partner
-      tile = work.tiles - 1 - pair;
-      units = work.units(a, tile);
-      if (unit >= units) {
-        unit -= units;
-        tile = pair;
-        const int before = units;
-        units = work.units(a, tile);
-        if (unit >= units) {  // the rest of the pair's space is empty
-          at += work.pair - before - unit;
-          continue;
-        }
-      }
-    }
-    const int q0 = work.q0, n = work.n, len = work.len;
-    const int unit_end = static_cast<int>(min<int64_t>(units, unit + (end - at)));
-    const int rows = min(R, n * a.group - tile * R);
+  Walk<R, U> walk;
+  walk.start(a, sp, lane);
+  Piece piece;
+  while (walk.next(a, sp, &piece)) {
+    const int q0 = piece.q0, n = piece.n, len = piece.len, head = piece.head, tile = piece.tile;
+    const int rows = piece.rows, r = piece.r;
     // this wave's rows
     const int row0 = WIDE ? wave * S::kWaveRows : 0;
     const int my_rows = WIDE ? min(S::kWaveRows, rows - row0) : rows;
@@ -688,56 +738,63 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
       min_vis = max(len - n + a.grp.div(tile * R + row0) + 1, 0);
       max_vis = max(len - n + a.grp.div(tile * R + row0 + my_rows - 1) + 1, 0);
     }
-    const int p_end = min(min(unit_end * U, len), max_vis);
+    const int p_end = min(min(piece.unit_end * U, len), max_vis);
     const int32_t *table = a.table + static_cast<size_t>(r) * a.width;
     const Elem *kc = static_cast<const Elem *>(a.kc) + head * a.head_stride;
     const Elem *vc = static_cast<const Elem *>(a.vc) + head * a.head_stride;
 
     // the table entries of this wave's first rows and the block's q rows on their
     // way together, then the cache rows, then q into LDS as matrix operands
-    int p0 = unit * U + (WIDE ? 0 : wave * STEP);
+    int p0 = piece.unit * U + (WIDE ? 0 : wave * STEP);
     Rows<STEP> rows_of;
     rows_of.fetch(a, table, p0 + lane % STEP, p_end);
     constexpr int kLanes = HD / 4, kAt = kThreads / kLanes;  // lanes of a row, rows at once
     constexpr int kRows = (R + kAt - 1) / kAt;
-    float4 qv[kRows];
     const int qd = tid % kLanes * 4;
-#pragma unroll
-    for (int x = 0; x < kRows; ++x) {
-      const int i = tid / kLanes + x * kAt, row = tile * R + i, tok = a.grp.div(row);
-      qv[x] = make_float4(0, 0, 0, 0);
-      if (i < rows)
-        qv[x] = *reinterpret_cast<const float4 *>(
-            a.q + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
-                   (row - tok * a.group)) * HD + qd);
-    }
     E eng;
     uint32_t mask = 0;
-    if (p0 < p_end) {
-      mask = rows_of.place(a, off_s[wave][0], p0 + lane % STEP, p_end, lane);
-      eng.load_k(kc, off_s[wave][0], lane);
-      eng.load_v(vc, off_s[wave][0], lane);
-      rows_of.fetch(a, table, p0 + S::kStride + lane % STEP, p_end);
-    }
-    __syncthreads();  // the piece before has been read
+    // four rows of a thread at a time: the registers of the cache rows are taken
+    constexpr int kBatch = kRows < 4 ? kRows : 4;
 #pragma unroll
-    for (int x = 0; x < kRows; ++x) {
-      const int i = tid / kLanes + x * kAt;
-      float up = 1.0f, down = a.scale;
-      if constexpr (E::kScaleQ) {
-        float mx = fmaxf(fmaxf(fabsf(qv[x].x), fabsf(qv[x].y)),
-                         fmaxf(fabsf(qv[x].z), fabsf(qv[x].w)));
-        mx = lane_group_reduce<kLanes>(mx, MaxOp{});
-        int ex = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
-        if (ex > -127 && ex < 128) {
-          ex = max(ex, -100);
-          up = ldexpf(1.0f, 14 - ex);
-          down = ldexpf(a.scale, ex - 14);
-        }
+    for (int x0 = 0; x0 < kRows; x0 += kBatch) {
+      float4 qv[kBatch];
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x) {
+        const int i = tid / kLanes + (x0 + x) * kAt, row = tile * R + i, tok = a.grp.div(row);
+        qv[x] = make_float4(0, 0, 0, 0);
+        if (i < rows)
+          qv[x] = *reinterpret_cast<const float4 *>(
+              a.q + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                     (row - tok * a.group)) * HD + qd);
       }
-      if (kRows * kAt == R || i < R) {
-        E::store_q(lds + i / S::kWaveRows * E::kQBytes, i % S::kWaveRows, qd, qv[x], up);
-        if (qd == 0) fac_s[i] = down * kExpL2E;
+      if (x0 == 0) {
+        if (p0 < p_end) {
+          mask = rows_of.place(a, off_s[wave][0], p0 + lane % STEP, p_end, lane);
+          eng.load_k(kc, off_s[wave][0], lane);
+          eng.load_v(vc, off_s[wave][0], lane);
+          rows_of.fetch(a, table, p0 + S::kStride + lane % STEP, p_end);
+        }
+        __syncthreads();  // the piece before has been read
+      }
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x) {
+        const int i = tid / kLanes + (x0 + x) * kAt;
+        float up = 1.0f, down = a.scale;
+        if constexpr (E::kScaleQ) {
+          float mx = fmaxf(fmaxf(fabsf(qv[x].x), fabsf(qv[x].y)),
+                           fmaxf(fabsf(qv[x].z), fabsf(qv[x].w)));
+          mx = lane_group_reduce<kLanes>(mx, MaxOp{});
+          int ex = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+          if (ex > -127 && ex < 128) {
+            ex = max(ex, -100);
+            up = ldexpf(1.0f, 14 - ex);
+            down = ldexpf(a.scale, ex - 14);
+          }
+        }
+        if (kRows * kAt == R || i < R) {
+          E::store_q(lds + i / S::kWaveRows * E::kQBytes, i % S::kWaveRows, qd, qv[x], up);
+          if (qd == 0) fac_s[i] = down * kExpL2E;
+        }
       }
     }
     __syncthreads();
@@ -794,7 +851,7 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
                                       (row - tok * a.group)) * HD;
 #pragma unroll
               for (int j = 0; j < E::kSlots; ++j) {
-                if (eng.sc[t][j] == eng.sc[t][j]) continue;
+                if (eng.sc[t][j] == eng.sc[t][j] || 16 * t + c >= my_rows) continue;
                 const Elem *key = kc + off_s[wave][s ^ 1][E::pos_of(g, j)];
                 float dot = 0.0f;
                 for (int d = 0; d < HD; ++d) dot += q[d] * static_cast<float>(key[d]);
@@ -869,8 +926,8 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
       const float seen = row_lanes(some[t] ? 1.0f : 0.0f, MaxOp{});
       if (m[t] == -INFINITY && seen != 0.0f) m[t] = kNoScore;
     }
-    const bool whole = unit == 0 && unit_end == units;
-    const size_t slot = static_cast<size_t>(worker) * 2 + (at == begin ? 0 : 1);
+    const bool whole = piece.whole;
+    const size_t slot = piece.slot;
     if constexpr (WIDE) {
       // through the wave's part of LDS, so that rows leave in whole lines
       float *mine_s = reinterpret_cast<float *>(lds + wave * E::kQBytes);
@@ -948,12 +1005,315 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
         }
       }
     }
-    if (unit == 0 && tid == 0) {
-      Cut cut{whole ? 0 : rows, worker, worker, at == begin ? 0 : 1, tile * R, q0, head};
-      if (!whole) cut.last = worker_of(total, sp.workers, at + units - 1);
-      sp.cut[tile_base + head * work.tiles + tile] = cut;
+    walk.done(sp, piece);
+  }
+}
+
+// ---- f16 cache, requests of many rows --------------------------------------------
+//
+// A block of eight waves of 16 rows goes through the positions of a piece 32 at a
+// time.  The block loads a K and a V tile once, into the order in which the waves
+// read matrix operands (the same operands as EngineF16's), two buffers of each in
+// LDS; a tile is on its way from memory while the one before it is multiplied, and
+// is put into LDS beside the next.  q's operands stay in registers.
+//
+// An operand piece of 16 bytes lies at its lane's place within 1 KB, its place
+// among 16 exchanged by an XOR so that the stores of a row's pieces, which are 1 KB
+// or 256 bytes apart, fall into different banks.
+constexpr int kWideWaves = 8, kWideThreads = 64 * kWideWaves, kWideRows = 16 * kWideWaves;
+constexpr int kWideUnit = 128;
+
+template <int HD>
+__global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedArgs a, Split sp) {
+  constexpr int KK = HD / 32, DT = HD / 16, STEP = 32, R = kWideRows, U = kWideUnit;
+  constexpr int kTile = STEP * HD;                                   // halves
+  constexpr int kPieces = STEP * HD / 8;                             // of K, 16 bytes each
+  constexpr int kOwn = (kPieces + kWideThreads - 1) / kWideThreads;  // a thread's
+  constexpr int kJoinStride = HD + 4, kOutRows = 4;                  // rows a wave lets out at once
+  static_assert(kWideWaves * kOutRows * kJoinStride * 4 <= 4 * kTile * 2, "rows leave through the tiles");
+  __shared__ __attribute__((aligned(16))) _Float16 tiles_s[4 * kTile];  // K, K, V, V
+  __shared__ int64_t off_s[4][STEP];  // cache rows of a step's positions, four steps in turn
+  __shared__ uint32_t mask_s[4];      // which of them the request has
+  __shared__ uint32_t apart_s[4];     // those with values that are not finite
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c = lane & 15;
+
+  Walk<R, U> walk;
+  walk.start(a, sp, lane);
+  Piece piece;
+  while (walk.next(a, sp, &piece)) {
+    const int q0 = piece.q0, n = piece.n, len = piece.len, head = piece.head, tile = piece.tile;
+    const int rows = piece.rows, row0 = wave * 16, my_rows = min(16, rows - row0);
+    const int min_vis = max(len - n + a.grp.div(tile * R) + 1, 0);  // of the block's rows
+    const int max_vis = max(len - n + a.grp.div(tile * R + rows - 1) + 1, 0);
+    const int p_beg = piece.unit * U, p_end = min(min(piece.unit_end * U, len), max_vis);
+    const int steps = p_beg < p_end ? (p_end - p_beg + STEP - 1) / STEP : 0;
+    int my_end = 0;  // positions that a row of this wave sees
+    if (my_rows > 0) my_end = min(p_end, len - n + a.grp.div(tile * R + row0 + my_rows - 1) + 1);
+    const int32_t *table = a.table + static_cast<size_t>(piece.r) * a.width;
+    const _Float16 *kc = static_cast<const _Float16 *>(a.kc) + head * a.head_stride;
+    const _Float16 *vc = static_cast<const _Float16 *>(a.vc) + head * a.head_stride;
+
+    // the first three steps' rows; the table entry of the fourth's
+    Rows<STEP> entry{-1};
+    __syncthreads();  // the piece before is done with LDS
+    if (wave == 0) {
+      Rows<STEP> e0, e1, e2;
+      const int p = p_beg + (lane & 31);
+      e0.fetch(a, table, p, p_end);
+      e1.fetch(a, table, p + STEP, p_end);
+      e2.fetch(a, table, p + 2 * STEP, p_end);
+      entry.fetch(a, table, p + 3 * STEP, p_end);
+      const uint32_t m0 = e0.place(a, off_s[0], p, p_end, lane);
+      const uint32_t m1 = e1.place(a, off_s[1], p + STEP, p_end, lane);
+      const uint32_t m2 = e2.place(a, off_s[2], p + 2 * STEP, p_end, lane);
+      if (lane < 4) {
+        mask_s[lane] = lane == 0 ? m0 : lane == 1 ? m1 : m2;
+        apart_s[lane] = 0;
+      }
     }
-    at += unit_end - unit;
+    // q: row c's dims 32 kk + 8 g .. as B operands
+    h8 qh[KK], ql[KK];
+    float fac;
+    int vis;
+    {
+      const int row = tile * R + row0 + c, tok = a.grp.div(row);
+      const bool in = c < my_rows;
+      const float *q = a.q + (static_cast<size_t>(q0 + (in ? tok : 0)) * a.n_head + head * a.group +
+                              (in ? row - tok * a.group : 0)) * HD + 8 * g;
+      f32x4 x[2 * KK];
+      float mx = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2 * KK; ++k) {
+        x[k] = in ? *reinterpret_cast<const f32x4 *>(q + 32 * (k >> 1) + 4 * (k & 1))
+                  : f32x4{0, 0, 0, 0};
+        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
+      }
+      mx = row_lanes(mx, MaxOp{});
+      float up = 1.0f;
+      fac = a.scale * kExpL2E;
+      int ex = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+      if (ex > -127 && ex < 128) {
+        ex = max(ex, -100);
+        up = ldexpf(1.0f, 14 - ex);
+        fac = ldexpf(fac, ex - 14);
+      }
+#pragma unroll
+      for (int k = 0; k < KK; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = x[2 * k + (e >> 2)][e & 3] * up;
+          qh[k][e] = static_cast<_Float16>(y);
+          ql[k][e] = static_cast<_Float16>(y - static_cast<float>(qh[k][e]));
+        }
+      vis = in ? len - n + tok + 1 : 0;
+    }
+    f32x4 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    bool some = false;
+
+    // a thread's share of a step: K pieces tid + 512 i; V dims 4 dq .. of positions
+    // 4 pg .. 4 pg + 3
+    const int dq = tid % (HD / 4), pg = tid / (HD / 4);
+    h8 kr[kOwn];
+    h4 vr[4];
+    __syncthreads();
+    for (int t = -2; t < steps; ++t) {
+      // step t + 1 into LDS, beside step t's products
+      if (t >= -1 && t + 1 < steps) {
+        const int b = (t + 1) & 1, at = (t + 1) & 3;
+        _Float16 *ks = tiles_s + b * kTile, *vs = tiles_s + (2 + b) * kTile;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          const int x = tid + kWideThreads * i, pos = x / (HD / 8), pc = x % (HD / 8);
+          if (kPieces % kWideThreads == 0 || x < kPieces)
+            *reinterpret_cast<h8 *>(ks + ((pos / 16 * KK + pc / 4) * 64 + pc % 4 * 16 +
+                                          ((pos & 15) ^ (pc & 15))) * 8) = kr[i];
+        }
+        if (tid < 2 * HD) {
+          const uint32_t mask = mask_s[at];
+          const int p = p_beg + (t + 1) * STEP;
+          if (mask != ~0u || p + STEP > min_vis) {
+            // no weight of 0 may meet a value that is not finite: what lies past the
+            // end is 0, and where not every row sees a position such elements are
+            // left out, to be added to the rows that do
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int o = 4 * pg + k;
+              if (!(mask >> o & 1)) vr[k] = h4{0, 0, 0, 0};
+              if (p + o >= min_vis) {
+                // (on the bits: all ones in the exponent)
+                const u16x4 bits = __builtin_bit_cast(u16x4, vr[k]);
+                const u16x4 odd = __builtin_bit_cast(u16x4, (bits & uint16_t{0x7c00}) == uint16_t{0x7c00});
+                vr[k] = __builtin_bit_cast(h4, bits & ~odd);
+                if (odd[0] | odd[1] | odd[2] | odd[3]) atomicOr(&apart_s[at], 1u << o);
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = 4 * dq + e;
+            *reinterpret_cast<h4 *>(vs + (d / 16 * 64 + (pg & 3) * 16 + ((d & 15) ^ (d / 16 & 15))) * 8 +
+                                    (pg >> 2) * 4) = h4{vr[0][e], vr[1][e], vr[2][e], vr[3][e]};
+          }
+        }
+      }
+      // step t + 2 on its way
+      if (t + 2 < steps) {
+        const int64_t *off = off_s[(t + 2) & 3];
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          const int x = tid + kWideThreads * i, pos = x / (HD / 8), pc = x % (HD / 8);
+          if (kPieces % kWideThreads == 0 || x < kPieces)
+            kr[i] = *reinterpret_cast<const h8 *>(kc + off[pos] + 8 * pc);
+        }
+        if (tid < 2 * HD) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            vr[k] = *reinterpret_cast<const h4 *>(vc + off[4 * pg + k] + 4 * dq);
+        }
+      }
+      // the rows of step t + 3
+      if (t >= 0 && wave == 0 && t + 3 < steps) {
+        const int p = p_beg + (t + 3) * STEP + (lane & 31), at = (t + 3) & 3;
+        const uint32_t mk = entry.place(a, off_s[at], p, p_end, lane);
+        if (lane == 0) mask_s[at] = mk, apart_s[at] = 0;
+        entry.fetch(a, table, p + STEP, p_end);
+      }
+      const int p0 = p_beg + t * STEP;
+      if (t >= 0 && p0 < my_end) {
+        const _Float16 *ks = tiles_s + (t & 1) * kTile, *vs = tiles_s + (2 + (t & 1)) * kTile;
+        const uint32_t mask = mask_s[t & 3];
+        f32x4 sh[2], sl[2];
+        sh[0] = sh[1] = sl[0] = sl[1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          if (kk % 2 == 0) __builtin_amdgcn_sched_barrier(0);  // (operands are not read far ahead)
+          const int o = (kk * 64 + g * 16 + (c ^ ((4 * kk + g) & 15))) * 8;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const h8 k = *reinterpret_cast<const h8 *>(ks + s * KK * 512 + o);
+            sh[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[kk], sh[s], 0, 0, 0);
+            sl[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[kk], sl[s], 0, 0, 0);
+          }
+        }
+        float sc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j] = (sl[j >> 2][j & 3] + sh[j >> 2][j & 3]) * fac;
+        if (mask != ~0u || p0 + STEP > min_vis) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int o = (j >> 2) * 16 + 4 * g + (j & 3);
+            const bool sees = p0 + o < vis && (mask >> o & 1);
+            if (!sees) sc[j] = -INFINITY;
+            some |= sees;
+          }
+        } else {
+          some = true;
+        }
+        float sum = 0.0f, top = sc[0];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += sc[j], top = fmaxf(top, sc[j]);
+        if (__builtin_expect(__any(sum != sum), false)) {
+          // as in attn_paged_kernel: an infinite key against the halves of q (or
+          // infinities of both signs, which are formed again to no harm)
+          const int row = tile * R + row0 + c, tok = a.grp.div(row);
+          const float *q = a.q + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                                  (row - tok * a.group)) * HD;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (sc[j] == sc[j] || c >= my_rows) continue;
+            const _Float16 *key = kc + off_s[t & 3][(j >> 2) * 16 + 4 * g + (j & 3)];
+            float dot = 0.0f;
+            for (int d = 0; d < HD; ++d) dot += q[d] * static_cast<float>(key[d]);
+            sc[j] = dot * (a.scale * kExpL2E);
+            top = fmaxf(top, sc[j]);
+          }
+        }
+        top = row_lanes(top, MaxOp{});
+        const float now = fmaxf(m, top);
+        const float ref = now == -INFINITY ? 0.0f : now;
+        if (__any(now > m)) {
+          const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - ref);
+          l *= keep;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[d] *= keep;
+        }
+        m = now;
+        h8 ph, pl;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sc[j] = __builtin_amdgcn_exp2f(sc[j] - ref);
+          l += sc[j];
+          const float x = sc[j] * kPUnit;
+          ph[j] = static_cast<_Float16>(x);
+          pl[j] = static_cast<_Float16>(x - static_cast<float>(ph[j]));
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          if (d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+          const h8 v = *reinterpret_cast<const h8 *>(vs + (d * 64 + g * 16 + (c ^ (d & 15))) * 8);
+          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[d], 0, 0, 0);
+          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[d], 0, 0, 0);
+        }
+        uint32_t apart = __builtin_amdgcn_readfirstlane(apart_s[t & 3]);
+        while (__builtin_expect(apart != 0, false)) {
+          const int o = __ffs(apart) - 1;
+          apart &= apart - 1;
+          float p = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((j >> 2) * 16 + 4 * (o % 16 / 4) + (j & 3) == o) p = sc[j];
+          p = __shfl(p, o % 16 / 4 * 16 + c) * kPUnit;
+          const _Float16 *v = vc + off_s[t & 3][o] + 4 * g;
+          if (p0 + o < vis) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float x = static_cast<float>(v[16 * d + i]);
+                if (!(fabsf(x) < INFINITY)) acc[d][i] += p * x;
+              }
+          }
+        }
+      }
+      __syncthreads();
+    }
+
+    l = row_lanes(l, SumOp{});
+    const float seen = row_lanes(some ? 1.0f : 0.0f, MaxOp{});
+    if (m == -INFINITY && seen != 0.0f) m = kNoScore;
+    const float by = !piece.whole ? 1.0f / kPUnit : m == -INFINITY ? 0.0f : 1.0f / kPUnit / l;
+    const size_t slot = piece.slot;
+    if (!piece.whole && g == 0 && c < my_rows) {
+      sp.pm[slot * R + row0 + c] = m;
+      sp.pl[slot * R + row0 + c] = l;
+    }
+    // rows leave in whole lines through the wave's part of LDS
+    float *mine = reinterpret_cast<float *>(tiles_s) + wave * kOutRows * kJoinStride;
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += kOutRows) {
+      const int here = min(kOutRows, my_rows - r0);
+      if (here <= 0) continue;
+      wave_sync();
+      if (c >= r0 && c < r0 + kOutRows)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          *reinterpret_cast<f32x4 *>(mine + (c - r0) * kJoinStride + 16 * d + 4 * g) = acc[d] * by;
+      wave_sync();
+      for (int i = lane; i < here * (HD / 4); i += 64) {
+        const int rr = i / (HD / 4), d = i % (HD / 4) * 4, row = row0 + r0 + rr;
+        const int tok = a.grp.div(tile * R + row);
+        float *dst = piece.whole ? a.out + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                                            (tile * R + row - tok * a.group)) * HD
+                                 : sp.pacc + (slot * R + row) * HD;
+        *reinterpret_cast<f32x4 *>(dst + d) =
+            *reinterpret_cast<const f32x4 *>(mine + rr * kJoinStride + d);
+      }
+    }
+    walk.done(sp, piece);
   }
 }
 
@@ -1063,49 +1423,75 @@ size_t workspace_of(const PagedArgs &a, const Form &f) {
          align256(parts * a.hd * 4);
 }
 
-template <class E, bool WIDE>
-int launch(const PagedArgs &a, const Form &f, char *ws, hipStream_t st) {
-  constexpr int R = Shape<E, WIDE>::R;
+// Where a launch's parts lie in its workspace.
+Split split_of(const PagedArgs &a, const Form &f, char *ws) {
   Split sp{};
   sp.workers = f.workers(), sp.over = f.over, sp.most = f.most;
-  const size_t parts = static_cast<size_t>(sp.workers) * 2 * R, tiles = most_tiles(a, f);
+  const size_t parts = static_cast<size_t>(sp.workers) * 2 * f.rows();
   sp.n_tiles = reinterpret_cast<int *>(ws);
   ws += 256;
   sp.cut = reinterpret_cast<Cut *>(ws);
-  ws += align256(tiles * sizeof(Cut));
+  ws += align256(most_tiles(a, f) * sizeof(Cut));
   sp.pm = reinterpret_cast<float *>(ws);
   ws += align256(parts * 4);
   sp.pl = reinterpret_cast<float *>(ws);
   ws += align256(parts * 4);
   sp.pacc = reinterpret_cast<float *>(ws);
-  BH_LAUNCH((attn_paged_kernel<E, WIDE>), static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
-  if (a.max_len > Shape<E, WIDE>::U) {  // with one unit a tile nothing is cut
-    // a block a (row, 64 dims) while they are not many times what fits the card
-    const size_t most = static_cast<size_t>(a.n_tok > 1 ? R : a.group < R ? a.group : R) * (E::kHd / 64);
-    size_t share = 16 * device_cu_count() / tiles;
-    share = share < 1 ? 1 : share > most ? most : share;
-    BH_LAUNCH((attn_paged_join_kernel<E::kHd, R>), static_cast<unsigned>(tiles * share), kThreads,
-              0, st, a, sp, static_cast<int>(share));
-  }
+  return sp;
+}
+
+template <int HD, int R>
+int launch_join(const PagedArgs &a, const Form &f, const Split &sp, int unit, hipStream_t st) {
+  if (a.max_len <= unit) return BH_OK;  // with one unit a tile nothing is cut
+  // a block a (row, 64 dims) while they are not many times what fits the card
+  const size_t tiles = most_tiles(a, f);
+  const size_t most = static_cast<size_t>(a.n_tok > 1 ? R : a.group < R ? a.group : R) * (HD / 64);
+  size_t share = 16 * device_cu_count() / tiles;
+  share = share < 1 ? 1 : share > most ? most : share;
+  BH_LAUNCH((attn_paged_join_kernel<HD, R>), static_cast<unsigned>(tiles * share), kThreads, 0, st,
+            a, sp, static_cast<int>(share));
   return BH_OK;
 }
 
-template <int RT, bool WIDE>
+template <class E, bool WIDE>
+int launch(const PagedArgs &a, const Form &f, char *ws, hipStream_t st) {
+  const Split sp = split_of(a, f, ws);
+  BH_LAUNCH((attn_paged_kernel<E, WIDE>), static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
+  return launch_join<E::kHd, Shape<E, WIDE>::R>(a, f, sp, Shape<E, WIDE>::U, st);
+}
+
+template <int HD>
+int launch_wide(const PagedArgs &a, const Form &f, char *ws, hipStream_t st) {
+  const Split sp = split_of(a, f, ws);
+  BH_LAUNCH(attn_paged_wide_kernel<HD>, static_cast<unsigned>(sp.workers), kWideThreads, 0, st, a, sp);
+  return launch_join<HD, kWideRows>(a, f, sp, kWideUnit, st);
+}
+
+template <int RT>
 int launch_rt(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st) {
   if (f16) {
-    if (a.hd == 64) return launch<EngineF16<64, RT>, WIDE>(a, f, ws, st);
-    if (a.hd == 128) return launch<EngineF16<128, RT>, WIDE>(a, f, ws, st);
-    return launch<EngineF16<256, RT>, WIDE>(a, f, ws, st);
+    if (a.hd == 64) return launch<EngineF16<64, RT>, false>(a, f, ws, st);
+    if (a.hd == 128) return launch<EngineF16<128, RT>, false>(a, f, ws, st);
+    return launch<EngineF16<256, RT>, false>(a, f, ws, st);
   }
-  if (a.hd == 64) return launch<EngineF32<64, RT>, WIDE>(a, f, ws, st);
-  if (a.hd == 128) return launch<EngineF32<128, RT>, WIDE>(a, f, ws, st);
-  return launch<EngineF32<256, RT>, WIDE>(a, f, ws, st);
+  if (a.hd == 64) return launch<EngineF32<64, RT>, false>(a, f, ws, st);
+  if (a.hd == 128) return launch<EngineF32<128, RT>, false>(a, f, ws, st);
+  return launch<EngineF32<256, RT>, false>(a, f, ws, st);
 }
 
 int launch_form(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st) {
-  if (f.wide) return launch_rt<2, true>(a, f16, f, ws, st);
-  if (f.rt == 1) return launch_rt<1, false>(a, f16, f, ws, st);
-  return launch_rt<2, false>(a, f16, f, ws, st);
+  if (f.wide && f16) {
+    if (a.hd == 64) return launch_wide<64>(a, f, ws, st);
+    if (a.hd == 128) return launch_wide<128>(a, f, ws, st);
+    return launch_wide<256>(a, f, ws, st);
+  }
+  if (f.wide) {
+    if (a.hd == 64) return launch<EngineF32<64, 2>, true>(a, f, ws, st);
+    if (a.hd == 128) return launch<EngineF32<128, 2>, true>(a, f, ws, st);
+    return launch<EngineF32<256, 2>, true>(a, f, ws, st);
+  }
+  if (f.rt == 1) return launch_rt<1>(a, f16, f, ws, st);
+  return launch_rt<2>(a, f16, f, ws, st);
 }
 
 // Whether a call runs on the matrix cores: rows of whole 16-byte pieces.
