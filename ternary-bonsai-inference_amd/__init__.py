@@ -527,20 +527,27 @@ def _ids_dtypes():
 
 def _hold(args, device, *tensors):
     """args with the tensors whose addresses it holds, and their device."""
-    args.tensors, args.device = tensors, device
+    args.tensors, args.device, args.index = tensors, device, device.index
     return args
 
 
+_TORCH_STREAM = None  # torch's current device and raw current stream, looked up once
+
+
 def _call(fn, args, stream):
-    """fn(args, stream) on the device of args' tensors, whichever is current."""
+    """fn(args, stream) on the device of args' tensors, whichever is current.
+    (A stream object a call would cost as much as the launch.)"""
+    global _TORCH_STREAM
     import torch
-    if torch.cuda.current_device() == args.device.index:
-        s = torch._C._cuda_getCurrentRawStream(args.device.index) if stream is None \
-            else stream.cuda_stream  # a stream object a call would cost as much as its launch
-        status = fn(ctypes.byref(args), s)
+    if _TORCH_STREAM is None:
+        _TORCH_STREAM = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    device, raw = _TORCH_STREAM
+    index = args.index
+    if device() == index:
+        status = fn(ctypes.byref(args), raw(index) if stream is None else stream.cuda_stream)
     else:
-        with torch.cuda.device(args.device):
-            status = fn(ctypes.byref(args), _stream(stream))
+        with torch.cuda.device(index):
+            status = fn(ctypes.byref(args), raw(index) if stream is None else stream.cuda_stream)
     if status != BH_OK:
         raise BonsaiError(status, last_error())
 
@@ -607,11 +614,14 @@ def kv_store_paged(cache: PagedCache, k, v, slots, stream=None) -> None:
     """kv_store into pages: rows k, v [n_tok, n_kv * hd] f32 to the positions
     slots int32 [n_tok] of the cache (page * page_size + offset; below 0: none)."""
     import torch
-    dev, n_tok = cache.device, slots.numel()
-    shape, f32 = (n_tok, cache.n_kv * cache.hd), (torch.float32,)
-    _dev_tensor(slots, "slots", (torch.int32,), dev)
-    _dev_tensor(k, "k", f32, dev, shape)
-    _dev_tensor(v, "v", f32, dev, shape)
+    n_tok, index, f32 = slots.numel(), cache.index, torch.float32
+    shape = (n_tok, cache.n_kv * cache.hd)
+    if not (slots.dtype is torch.int32 and k.dtype is f32 and v.dtype is f32
+            and k.shape == shape and v.shape == shape
+            and slots.get_device() == k.get_device() == v.get_device() == index
+            and slots.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
+        raise ValueError(f"k and v must be contiguous float32 tensors {shape} and slots a "
+                         f"contiguous int32 tensor [{n_tok}] on {cache.device}")
     fn = lib().bh_kv_store_paged
     _call(lambda ref, s: fn(ref, k.data_ptr(), v.data_ptr(), slots.data_ptr(), n_tok, s), cache,
           stream)

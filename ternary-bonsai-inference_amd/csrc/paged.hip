@@ -14,8 +14,9 @@
 // One workgroup does it: every step needs the totals of all requests, and the
 // data is a few hundred KB at most.  It is bound by the chain of dependent steps
 // (load, scan, scan, pages, tokens), not by bytes; so few requests take one wave,
-// whose barriers cost nothing (16 requests: ____ us, with 16 waves ____), and a
-// thread works on four pages or tokens at once, whose searches overlap.
+// whose barriers cost nothing (16 requests: 3.6 us, with 16 waves 4.6 us).  509
+// requests of 8192 tokens: 14.5 us.  Two or four pages and tokens of a thread side
+// by side were slower (4.3, 6.0 and 15.9, 16.6 us): the searches are LDS reads.
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -41,19 +42,10 @@ __device__ __forceinline__ int add_most(int a, int b) {
   return s > static_cast<uint32_t>(kMost) ? kMost : static_cast<int>(s);
 }
 
-// Inclusive running totals over the lanes of a wave.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int scan_step(int x) {
-  return add_most(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false));
-}
-__device__ __forceinline__ int wave_scan(int x) {
-  x = scan_step<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
-  x = scan_step<0x112, 0xF>(x);
-  x = scan_step<0x114, 0xF>(x);
-  x = scan_step<0x118, 0xF>(x);
-  x = scan_step<0x142, 0xA>(x);  // lane 15 of a row into the next
-  return scan_step<0x143, 0xC>(x);  // lane 31 into the upper half
-}
+struct AddMost {
+  __device__ int operator()(int a, int b) const { return add_most(a, b); }
+};
+__device__ __forceinline__ int wave_scan(int x) { return lane_scan(x, AddMost{}); }
 
 struct Three {
   int a, b, c;
@@ -87,21 +79,16 @@ __device__ __forceinline__ Three block_scan(Three v, Three *lds, Three *total) {
   return out;
 }
 
-// For each x[k] >= 0 the last r < n with start[r] <= x[k] (start[0] = 0); `top`: the
-// power of two from which to halve, at least n.
-template <int N>
-__device__ __forceinline__ void find(const int *start, int n, int top, const int *x, int *r) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) r[k] = 0;
-  for (int step = top; step > 0; step >>= 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int at = r[k] + step;
-      if (at < n && start[at] <= x[k]) r[k] = at;
-    }
+// The last r < n with start[r] <= x (start[0] = 0, x >= 0); `top`: the power of two
+// from which to halve, at least n.
+__device__ __forceinline__ int find(const int *start, int n, int top, int x) {
+  int r = 0;
+  for (int step = top; step > 0; step >>= 1) {
+    const int at = r + step;
+    if (at < n && start[at] <= x) r = at;
+  }
+  return r;
 }
-
-constexpr int kAtOnce = 4;
 
 template <int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PlanArgs a) {
@@ -156,16 +143,9 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PlanArgs a) {
       if (gone[k]) at = add_most(at, have[k]);
     }
     __syncthreads();
-    for (int p0 = tid; p0 < n_back; p0 += kAtOnce * THREADS) {
-      int p[kAtOnce], r[kAtOnce], entry[kAtOnce];
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) p[k] = min(p0 + k * THREADS, n_back - 1);
-      find<kAtOnce>(start, a.n_req, top, p, r);
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
-        entry[k] = a.table[static_cast<size_t>(r[k]) * a.width + (p[k] - start[r[k]])];
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) a.free_pages[n_free + p[k]] = entry[k];
+    for (int p = tid; p < n_back; p += THREADS) {
+      const int r = find(start, a.n_req, top, p);
+      a.free_pages[n_free + p] = a.table[static_cast<size_t>(r) * a.width + (p - start[r])];
     }
     __syncthreads();
   }
@@ -199,17 +179,10 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PlanArgs a) {
       at = add_most(at, need[k]);
     }
     __syncthreads();
-    for (int p0 = tid; p0 < sums.a; p0 += kAtOnce * THREADS) {
-      int p[kAtOnce], r[kAtOnce], entry[kAtOnce];
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        p[k] = min(p0 + k * THREADS, sums.a - 1);
-        entry[k] = a.free_pages[avail - 1 - p[k]];
-      }
-      find<kAtOnce>(start, a.n_req, top, p, r);
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
-        a.table[static_cast<size_t>(r[k]) * a.width + lens[r[k]] + (p[k] - start[r[k]])] = entry[k];
+    for (int p = tid; p < sums.a; p += THREADS) {
+      const int entry = a.free_pages[avail - 1 - p];
+      const int r = find(start, a.n_req, top, p);
+      a.table[static_cast<size_t>(r) * a.width + lens[r] + (p - start[r])] = entry;
     }
     __syncthreads();
   }
@@ -238,28 +211,16 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PlanArgs a) {
   __syncthreads();
 
   // tokens
-  for (int t0 = tid; t0 < a.n_tok; t0 += kAtOnce * THREADS) {
-    int t[kAtOnce], r[kAtOnce], p[kAtOnce], entry[kAtOnce];
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) t[k] = t0 + k * THREADS;
-    if (t0 < live) find<kAtOnce>(start, a.n_req, top, t, r);
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      p[k] = 0, entry[k] = -1;
-      if (t[k] < live) {
-        p[k] = lens[r[k]] - start[r[k] + 1] + t[k];
-        entry[k] = a.table[static_cast<size_t>(r[k]) * a.width + a.page.div(p[k])];
-      }
+  for (int t = tid; t < a.n_tok; t += THREADS) {
+    int p = 0, slot = -1;
+    if (t < live) {
+      const int r = find(start, a.n_req, top, t);
+      p = lens[r] - start[r + 1] + t;
+      const int entry = a.table[static_cast<size_t>(r) * a.width + a.page.div(p)];
+      if (entry >= 0 && entry < a.n_pages) slot = entry * a.page.d + a.page.mod(p);
     }
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      if (t[k] >= a.n_tok) continue;
-      const bool in = entry[k] >= 0 && entry[k] < a.n_pages;
-      a.slots[t[k]] = in ? entry[k] * a.page.d + a.page.mod(p[k]) : -1;
-      if (a.pos)
-        *reinterpret_cast<int4 *>(a.pos + static_cast<size_t>(t[k]) * 4) =
-            make_int4(p[k], p[k], p[k], p[k]);
-    }
+    a.slots[t] = slot;
+    if (a.pos) *reinterpret_cast<int4 *>(a.pos + static_cast<size_t>(t) * 4) = make_int4(p, p, p, p);
   }
 }
 
@@ -395,7 +356,7 @@ extern "C" int bh_paged_plan(const bh_paged_plan_args *args, bh_stream stream) {
   a.width = static_cast<int>(p.table_width), a.n_pages = static_cast<int>(p.n_pages);
   a.page = FastDiv(static_cast<uint32_t>(p.page_size));
   hipStream_t st = as_stream(stream);
-  if (p.n_req <= 64 && p.n_tok <= 512) BH_LAUNCH((paged_plan_kernel<64, 1>), 1, 64, 0, st, a);
+  if (p.n_req <= 64 && p.n_tok <= 128) BH_LAUNCH((paged_plan_kernel<64, 1>), 1, 64, 0, st, a);
   else if (p.n_req <= 1024) BH_LAUNCH((paged_plan_kernel<1024, 1>), 1, 1024, 0, st, a);
   else BH_LAUNCH((paged_plan_kernel<1024, 4>), 1, 1024, 0, st, a);
   return ok();

@@ -223,8 +223,9 @@ struct Work {
 template <int HD, int RT>
 struct EngineF16 {
   using Elem = _Float16;
-  static constexpr int SUB = HD >= 256 && RT == 1 ? 1 : 2;
-  static constexpr int kAhead = RT == 1 ? 1 : 3;  // steps of 32 dims whose q is read ahead
+  static constexpr int SUB = HD >= 256 || (HD == 128 && RT == 2) ? 1 : 2;
+  static constexpr int kBlocks = RT == 1 || HD <= 128 ? 2 : 1;  // a compute unit
+  static constexpr int kAhead = kBlocks == 2 ? 1 : 3;  // steps of 32 dims whose q is read ahead
   static constexpr int kHd = HD, kRt = RT, kStep = 16 * SUB;
   static constexpr int KK = HD / 32, DV = HD >= 128 ? 8 : 4, NB = HD / (16 * DV);
   static constexpr int kQBytes = RT * KK * 2 * 64 * 16;
@@ -402,6 +403,7 @@ template <int HD, int RT>
 struct EngineF32 {
   using Elem = float;
   static constexpr int kHd = HD, kRt = RT, kStep = 16;
+  static constexpr int kBlocks = RT == 1 || HD <= 128 ? 2 : 1;  // a compute unit
   static constexpr int KK = HD / 16, NB = HD / 64;
   static constexpr int kQBytes = RT * KK * 64 * 16;
 
@@ -545,15 +547,6 @@ struct Rows {
   }
 };
 
-// Running totals over the wave's lanes, this lane's included.
-__device__ __forceinline__ void wave_scan(int64_t *x, int *y, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t ox = __shfl_up(*x, d);
-    const int oy = __shfl_up(*y, d);
-    if (lane >= d) *x += ox, *y += oy;
-  }
-}
 __device__ __forceinline__ int64_t wave_uniform(int64_t x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
@@ -591,7 +584,8 @@ struct Walk {
     }
     int64_t upto = mine;
     int upto_tiles = mine_tiles;
-    wave_scan(&upto, &upto_tiles, lane);
+    upto = lane_scan(upto, SumOp{});
+    upto_tiles = lane_scan(upto_tiles, SumOp{});
     total = wave_uniform(__shfl(upto, 63));
     at = begin = wave_uniform(run_begin(total, sp.workers, worker));
     end = wave_uniform(run_begin(total, sp.workers, worker + 1));
@@ -616,7 +610,8 @@ struct Walk {
         }
         upto = mine;
         upto_tiles = mine_tiles;
-        wave_scan(&upto, &upto_tiles, lane);
+        upto = lane_scan(upto, SumOp{});
+      upto_tiles = lane_scan(upto_tiles, SumOp{});
         upto += base;
         upto_tiles += tile_base;
         const uint64_t past = __ballot(begin < upto);
@@ -679,8 +674,8 @@ struct Walk {
   }
   static __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-  // After a piece: the worker of a tile's first part says where its parts are.
-  __device__ __forceinline__ void done(const Split &sp, const Piece &p) {
+  // The worker of a tile's first part says where its parts are; then past the piece.
+  __device__ __forceinline__ void pass(const Split &sp, const Piece &p) {
     if (p.unit == 0 && threadIdx.x == 0) {
       Cut cut{p.whole ? 0 : p.rows, worker, worker, at == begin ? 0 : 1, p.tile * R, p.q0, p.head};
       if (!p.whole) cut.last = worker_of(total, sp.workers, at + p.units - 1);
@@ -709,7 +704,7 @@ struct Shape {
 };
 
 template <class E, bool WIDE>
-__global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kernel(PagedArgs a, Split sp) {
+__global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedArgs a, Split sp) {
   using Elem = typename E::Elem;
   using S = Shape<E, WIDE>;
   constexpr int HD = E::kHd, RT = E::kRt, R = S::R, STEP = E::kStep, U = S::U;
@@ -728,6 +723,7 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
   walk.start(a, sp, lane);
   Piece piece;
   while (walk.next(a, sp, &piece)) {
+    walk.pass(sp, piece);
     const int q0 = piece.q0, n = piece.n, len = piece.len, head = piece.head, tile = piece.tile;
     const int rows = piece.rows, r = piece.r;
     // this wave's rows
@@ -1005,7 +1001,6 @@ __global__ __launch_bounds__(kThreads, E::kRt == 1 ? 2 : 1) void attn_paged_kern
         }
       }
     }
-    walk.done(sp, piece);
   }
 }
 
@@ -1042,6 +1037,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
   walk.start(a, sp, lane);
   Piece piece;
   while (walk.next(a, sp, &piece)) {
+    walk.pass(sp, piece);
     const int q0 = piece.q0, n = piece.n, len = piece.len, head = piece.head, tile = piece.tile;
     const int rows = piece.rows, row0 = wave * 16, my_rows = min(16, rows - row0);
     const int min_vis = max(len - n + a.grp.div(tile * R) + 1, 0);  // of the block's rows
@@ -1313,7 +1309,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
             *reinterpret_cast<const f32x4 *>(mine + rr * kJoinStride + d);
       }
     }
-    walk.done(sp, piece);
   }
 }
 
@@ -1402,10 +1397,10 @@ struct Form {
   int rt;
   bool wide;
   int over, most;  // the requests it takes, by rows a kv head
+  int blocks;      // a compute unit
 
   int rows() const { return 16 * rt * (wide ? kWaves : 1); }
-  // two blocks a compute unit with one row tile, one with two
-  int workers() const { return static_cast<int>(device_cu_count()) * (rt == 1 ? 2 : 1); }
+  int workers() const { return static_cast<int>(device_cu_count()) * blocks; }
 };
 
 size_t align256(size_t n) { return (n + 255) & ~size_t{255}; }
@@ -1509,16 +1504,19 @@ int forms_of(const bh_attention_paged_args &p, Form *f) {
   const size_t tokens = p.max_new == 0 || p.max_new > p.n_tok ? p.n_tok : p.max_new;
   const size_t rows = tokens * (p.n_head / p.cache.n_kv);
   constexpr int kAll = 0x7fffffff;
+  const int two = p.cache.hd <= 128 ? 2 : 1;  // E::kBlocks of two row tiles
+  const int wide = p.cache.kv_dtype == BH_KV_F16 ? 1 : two;
   if (rows <= 64) {
-    f[0] = Form{rows <= 16 ? 1 : 2, false, 0, kAll};
+    const int rt = rows <= 16 ? 1 : 2;
+    f[0] = Form{rt, false, 0, kAll, rt == 1 ? 2 : two};
     return 1;
   }
   if (p.n_req == 1) {
-    f[0] = Form{2, true, 0, kAll};
+    f[0] = Form{2, true, 0, kAll, wide};
     return 1;
   }
-  f[0] = Form{2, true, kWideOver, kAll};
-  f[1] = Form{1, false, 0, kWideOver};
+  f[0] = Form{2, true, kWideOver, kAll, wide};
+  f[1] = Form{1, false, 0, kWideOver, 2};
   return 2;
 }
 
