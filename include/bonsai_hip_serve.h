@@ -84,8 +84,10 @@ typedef struct bh_paged_cache {
  * n_free and n_free_out are separate words (they may be the same one, for a
  * stack that moves on by itself), and nothing below *n_free on the stack is
  * written.  kv_len must not be cached.  cached[i] < 0 counts as 0, *n_free is
- * clipped to 0 .. n_pages, pages pushed past n_pages are dropped.  Page numbers
- * are passed on as they are; a token on a page outside the pool has slot -1.
+ * clipped to 0 .. n_pages, pages pushed past n_pages are dropped, a released
+ * request has no more pages than its table row.  Page numbers are passed on as
+ * they are (a page that two requests share is to be released by one of them); a
+ * token on a page outside the pool has slot -1.
  * n_req <= BH_PAGED_MAX_REQ. */
 typedef struct bh_paged_plan_args {
   const int32_t *cached; /* [n_req]                                  */
@@ -129,9 +131,9 @@ int bh_kv_store_paged(const bh_paged_cache *cache, const float *k, const float *
  * rows of a page among it, may hold anything.  A query at p < 0 sees nothing
  * and gets zeros.  Tokens of no request are left as they were.
  *
- * q, out: [n_tok][n_head][hd] f32, out is not q.  Entries q_start are not
- * decreasing and are clipped to 0 .. n_tok, kv_len to 0 .. table_width *
- * page_size.  A table entry outside 0 .. n_pages - 1 among a request's
+ * q, out: [n_tok][n_head][hd] f32, out is not q.  Entries of q_start do not
+ * decrease (if they do, some tokens' results are unspecified) and are clipped to
+ * 0 .. n_tok, kv_len to 0 .. table_width * page_size (at most 2^31 - 65536).  A table entry outside 0 .. n_pages - 1 among a request's
  * ceil(kv_len / page_size) leaves its positions out, and is written to
  * *bad_page where that is not NULL (the caller presets it).
  *
@@ -140,7 +142,9 @@ int bh_kv_store_paged(const bh_paged_cache *cache, const float *k, const float *
  * n_head that n_kv divides; hd 64, 128 and 256 with strides and pointers of
  * whole 16 bytes run on the matrix cores.  Results agree with 64-bit arithmetic
  * to about 1e-6 of the output's magnitude and are the same bits from call to
- * call. */
+ * call on one device.  Scores q.k / sqrtf(hd) stay below the largest f32.  What
+ * is infinite or NaN among the values a query sees makes the dimensions it is in
+ * not finite. */
 typedef struct bh_attention_paged_args {
   bh_paged_cache cache;
   const float *q;

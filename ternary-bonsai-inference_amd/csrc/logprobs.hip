@@ -492,6 +492,8 @@ int check(const bh_token_logprobs_args &p) {
   if (!(p.inv_temp > 0.0f) || std::isinf(p.inv_temp * kExpL2E))
     return fail(BH_ERR_ARG, "token_logprobs: inv_temp must be finite and above 0");
   if (p.n_rows != 0) {
+    if (reinterpret_cast<uintptr_t>(p.x) % sizeof(float) != 0)
+      return fail(BH_ERR_ARG, "token_logprobs: misaligned x");
     if (!p.x || (p.logprob && !p.tokens) || (p.n_top != 0 && (!p.top_ids || !p.top_logprobs)))
       return fail(BH_ERR_ARG, "token_logprobs: null pointer");
   }

@@ -75,6 +75,7 @@ def _attn(bh, cache=None, **kw):
     (dict(n_req=1 << 31), "SHAPE", "overflow"),
     (dict(table_width=0), "SHAPE", "table_width"),
     (dict(table_width=1 << 27), "SHAPE", "table_width"),
+    (dict(table_width=(1 << 27) - 4095), "SHAPE", "table_width"),
     (dict(q=None), "ARG", "null pointer"),
     (dict(out=None), "ARG", "null pointer"),
     (dict(q_start=None), "ARG", "null pointer"),
@@ -147,6 +148,7 @@ def _lp(bh, **kw):
     (dict(inv_temp=float("nan")), "ARG", "inv_temp"),
     (dict(inv_temp=float("inf")), "ARG", "inv_temp"),
     (dict(x=None), "ARG", "null pointer"),
+    (dict(x=P + 2), "ARG", "misaligned x"),
     (dict(tokens=None), "ARG", "null pointer"),
     (dict(top_ids=None), "ARG", "null pointer"),
     (dict(top_logprobs=None), "ARG", "null pointer"),

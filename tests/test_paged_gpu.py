@@ -503,6 +503,42 @@ def test_strange_offsets_stay_in_bounds(bh, dev):
     assert (_attend(bh, dev, s)[0][0] == 0).all()
 
 
+def test_overlapping_offsets_stay_in_bounds(bh, dev):
+    """Offsets that go back and forth ask for far more row tiles than tokens that
+    do not overlap have: nothing is written past the workspace or the output."""
+    import torch
+    rng = np.random.default_rng(18)
+    for max_new in (1, 40):
+        s = _step(rng, dev, [600] * 64, [1] * 64, 16, 24, 4, 256, True, pad=2)
+        s["start"] = np.array([0, 60] * 32 + [0], np.int32)
+        d = [_t(s[n], dev) for n in ("q", "start", "lens", "table")]
+        out = torch.full((70, 24, 256), 5.25, device=dev)
+        args = bh.make_attention_paged_args(bh.make_paged_cache(s["k"], s["v"]), *d, out=out[2:68],
+                                            max_new=max_new)
+        need = bh.attention_paged_workspace(args)
+        ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device=dev)
+        args = bh.make_attention_paged_args(bh.make_paged_cache(s["k"], s["v"]), *d, out=out[2:68],
+                                            max_new=max_new, workspace=ws[:need])
+        bh.attention_paged(args)
+        torch.cuda.synchronize()
+        assert (ws[need:] == 0x5A).all()
+        assert (out[:2] == 5.25).all() and (out[62:] == 5.25).all()
+
+
+@pytest.mark.parametrize("hd", [256, 128, 64])
+@pytest.mark.parametrize("new", [[1], [3], [40]])
+def test_infinite_keys_and_padding_rows(bh, dev, hd, new):
+    """An infinite key that every row sees, in steps where nothing is masked; the
+    rows that fill up a tile of 16 belong to nobody."""
+    rng = np.random.default_rng(19)
+    s = _step(rng, dev, [700], new, 16, 5, 1, hd, True)
+    s["q"][:] = np.abs(s["q"]) + 0.1
+    for p in (3, 100, 333):
+        s["k"][int(s["table"][0, p // 16]), p % 16, 0, 2] = -float("inf")
+    got = _check(bh, dev, s)
+    assert np.isfinite(got).all()
+
+
 def test_offsets_past_32_bits(bh, dev):
     """A pool of over 2^32 bytes and 2^31 elements, a request in its last pages."""
     import torch
