@@ -1032,6 +1032,13 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
 // An operand piece of 16 bytes lies at its lane's place within 1 KB, its place
 // among 16 exchanged by an XOR so that the stores of a row's pieces, which are 1 KB
 // or 256 bytes apart, fall into different banks.
+//
+// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions 323-354
+// (280-309 TFLOP/s of useful products, twice that of issued ones), 128 there 130, 2048
+// from position 0 209.  Two waves a SIMD hide about half of the LDS reads and the
+// softmax; half of the waves half a step behind the others, to run one's
+// exponentials beside the other's products, took the registers past 256 and three
+// times as long (at hd 128, where nothing spills, 319 for 265).
 constexpr int kWideWaves = 8, kWideThreads = 64 * kWideWaves, kWideRows = 16 * kWideWaves;
 constexpr int kWideUnit = 128;
 
@@ -1283,12 +1290,15 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
           const _Float16 *v = vc + off_s[t & 3][o] + 4 * g;
           if (p0 + o < vis) {
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d) {
+              __builtin_amdgcn_sched_barrier(0);  // (rare: it is not to cost the rest registers)
+              const h4 x = *reinterpret_cast<const h4 *>(v + 16 * d);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float x = static_cast<float>(v[16 * d + i]);
-                if (!(fabsf(x) < INFINITY)) acc[d][i] += p * x;
+                const float y = static_cast<float>(x[i]);
+                if (!(fabsf(y) < INFINITY)) acc[d][i] += p * y;
               }
+            }
           }
         }
       }
@@ -1422,10 +1432,15 @@ struct Form {
 
 size_t align256(size_t n) { return (n + 255) & ~size_t{255}; }
 
-// Tiles that a launch can have at most.
+// Tiles that a launch can have at most: requests of over `over` and up to `most`
+// rows, n_tok group rows in all.
 size_t most_tiles(const PagedArgs &a, const Form &f) {
-  const size_t rows = static_cast<size_t>(a.n_tok) * a.group;
-  return static_cast<size_t>(a.n_kv) * (rows / f.rows() + (a.n_req < a.n_tok ? a.n_req : a.n_tok));
+  const size_t R = f.rows(), rows = static_cast<size_t>(a.n_tok) * a.group;
+  const size_t fit = f.over > a.group ? rows / f.over : static_cast<size_t>(a.n_tok);
+  const size_t req = static_cast<size_t>(a.n_req) < fit ? a.n_req : fit;
+  const size_t of_one = (static_cast<size_t>(f.most) + R - 1) / R;
+  const size_t all = rows / R + req;
+  return static_cast<size_t>(a.n_kv) * (req < all / of_one ? req * of_one : all);
 }
 
 // Workspace: tile count, tiles, maxima, sums, accumulators.
