@@ -131,14 +131,16 @@ int bh_kv_store_paged(const bh_paged_cache *cache, const float *k, const float *
  * rows of a page among it, may hold anything.  A query at p < 0 sees nothing
  * and gets zeros.  Tokens of no request are left as they were.
  *
- * q, out: [n_tok][n_head][hd] f32, out is not q.  Entries of q_start do not
+ * q, out: [n_tok][n_head][hd] f32, out is not q; n_tok < 2^24.  Entries of q_start do not
  * decrease (if they do, some tokens' results are unspecified) and are clipped to
- * 0 .. n_tok, kv_len to 0 .. table_width * page_size (at most 2^31 - 65536).  A table entry outside 0 .. n_pages - 1 among a request's
+ * 0 .. n_tok, kv_len to 0 .. table_width * page_size (at most 2^31 - 65536).
+ * A table entry outside 0 .. n_pages - 1 among a request's
  * ceil(kv_len / page_size) leaves its positions out, and is written to
  * *bad_page where that is not NULL (the caller presets it).
  *
- * max_new: no request has more new tokens than this; it steers how the work is
- * laid out and no result depends on it (0: n_tok).  Any hd up to 512 and any
+ * max_new: no request has more new tokens than this (0: n_tok); it steers how
+ * the work is laid out, and a wrong one costs time: results agree to rounding
+ * whatever it is.  Any hd up to 512 and any
  * n_head that n_kv divides; hd 64, 128 and 256 with strides and pointers of
  * whole 16 bytes run on the matrix cores.  Results agree with 64-bit arithmetic
  * to about 1e-6 of the output's magnitude and are the same bits from call to
@@ -198,8 +200,8 @@ typedef struct bh_token_logprobs_args {
 } bh_token_logprobs_args;
 
 int bh_token_logprobs(const bh_token_logprobs_args *args, bh_stream stream);
-/* Bytes of workspace that a call with these arguments needs (0: none, or bad
- * arguments). */
+/* Bytes of workspace that a call with these arguments needs on the current
+ * device (0: none, or bad arguments). */
 size_t bh_token_logprobs_workspace(const bh_token_logprobs_args *args);
 
 #ifdef __cplusplus

@@ -632,8 +632,9 @@ def make_attention_paged_args(cache: PagedCache, q, q_start, kv_len, block_table
                               workspace=None) -> AttentionPagedArgs:
     """Queries q [n_tok, n_head, hd] f32 of the requests whose tokens begin at
     q_start int32 [n_req + 1], over kv_len int32 [n_req] positions in the pages
-    block_table int32 [n_req, width].  The result is args.out (new if out is
-    None; rows of no request are left as they were).  workspace: a uint8 tensor
+    block_table int32 [n_req, width].  The result is args.out_tensor (if out is
+    None, zeros made on the current stream); rows of no request are left as they
+    were.  workspace: a uint8 tensor
     of attention_paged_workspace(args) bytes for calls that may overlap; None:
     the library's scratch."""
     import torch

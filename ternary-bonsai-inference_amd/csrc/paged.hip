@@ -269,26 +269,28 @@ __global__ __launch_bounds__(256) void kv_store_paged_pieces_kernel(StoreArgs a)
   }
 }
 
-// Any layout: a block a token.
+// Any layout: a block a token (and every kStoreBlocks-th after it).
+constexpr int kStoreBlocks = 1 << 20;
 
 template <class T>
 __global__ __launch_bounds__(256) void kv_store_paged_kernel(StoreArgs a) {
-  const int t = blockIdx.x;
-  const int slot = a.slots[t];
-  if (slot < 0 || slot >= a.n_slots) return;
-  const int b = a.page.div(slot);
-  const size_t at = b * a.page_stride + static_cast<size_t>(slot - b * a.page.d) * a.pos_stride;
-  T *kc = static_cast<T *>(a.kc) + at, *vc = static_cast<T *>(a.vc) + at;
-  for (int e = threadIdx.x; e < a.elems; e += 256) {
-    const int h = e / a.hd;
-    const size_t o = h * a.head_stride + (e - h * a.hd);
-    const size_t i = static_cast<size_t>(t) * a.elems + e;
-    if constexpr (sizeof(T) == 2) {
-      kc[o] = store_half(a.k[i]);
-      vc[o] = store_half(a.v[i]);
-    } else {
-      kc[o] = a.k[i];
-      vc[o] = a.v[i];
+  for (int64_t t = blockIdx.x; t < a.n_tok; t += kStoreBlocks) {
+    const int slot = a.slots[t];
+    if (slot < 0 || slot >= a.n_slots) continue;
+    const int b = a.page.div(slot);
+    const size_t at = b * a.page_stride + static_cast<size_t>(slot - b * a.page.d) * a.pos_stride;
+    T *kc = static_cast<T *>(a.kc) + at, *vc = static_cast<T *>(a.vc) + at;
+    for (int e = threadIdx.x; e < a.elems; e += 256) {
+      const int h = e / a.hd;
+      const size_t o = h * a.head_stride + (e - h * a.hd);
+      const size_t i = static_cast<size_t>(t) * a.elems + e;
+      if constexpr (sizeof(T) == 2) {
+        kc[o] = store_half(a.k[i]);
+        vc[o] = store_half(a.v[i]);
+      } else {
+        kc[o] = a.k[i];
+        vc[o] = a.v[i];
+      }
     }
   }
 }
@@ -395,11 +397,10 @@ extern "C" int bh_kv_store_paged(const bh_paged_cache *cache, const float *k, co
       BH_LAUNCH(kv_store_paged_pieces_kernel<float>, blocks, 256, 0, as_stream(stream), a);
     return ok();
   }
+  const unsigned blocks = static_cast<unsigned>(n_tok < kStoreBlocks ? n_tok : kStoreBlocks);
   if (cache->kv_dtype == BH_KV_F16)
-    BH_LAUNCH(kv_store_paged_kernel<uint16_t>, static_cast<unsigned>(n_tok), 256, 0,
-              as_stream(stream), a);
+    BH_LAUNCH(kv_store_paged_kernel<uint16_t>, blocks, 256, 0, as_stream(stream), a);
   else
-    BH_LAUNCH(kv_store_paged_kernel<float>, static_cast<unsigned>(n_tok), 256, 0,
-              as_stream(stream), a);
+    BH_LAUNCH(kv_store_paged_kernel<float>, blocks, 256, 0, as_stream(stream), a);
   return ok();
 }

@@ -4,8 +4,8 @@
 // a kv head, (token, head of its group) pairs, go through the matrix cores 16 at
 // a time; the work of a call, whatever its requests' lengths, is cut into equal
 // runs of positions, one a worker, and what was cut is joined by a second launch
-// (a counter and fences inside one launch cost more than the second on this
-// card).  Three forms:
+// (inside the first it would take counters that are zero at its start, and
+// fences across the L2s of eight dies).  Three forms:
 //   attn_paged_kernel       few rows a request: the waves of a block split the
 //                           positions; bound by reading the cache
 //   attn_paged_wide_kernel  many rows over f16: the waves share K and V in LDS;
@@ -1553,6 +1553,10 @@ int forms_of(const bh_attention_paged_args &p, Form *f) {
   return 2;
 }
 
+// Blocks of a launch: a grid has fewer than 2^32 threads a dimension.
+constexpr size_t kMostBlocks = 0xffffff;
+static_assert(kMostBlocks * kThreads < (size_t{1} << 32), "");
+
 // Checks the arguments and fills `a`.
 int prepare(const bh_attention_paged_args &p, PagedArgs *a) {
   const bh_paged_cache &c = p.cache;
@@ -1564,7 +1568,7 @@ int prepare(const bh_attention_paged_args &p, PagedArgs *a) {
     return fail(BH_ERR_SHAPE, "attention_paged: hd " + std::to_string(c.hd) + " above " +
                                   std::to_string(kAnyMaxHd));
   size_t n;
-  if (p.n_head > 65535 || p.n_tok > 0x7fffffffu || p.n_req > 0x7ffffffeu ||
+  if (p.n_head > 65535 || p.n_tok > kMostBlocks || p.n_req > 0x7ffffffeu ||
       p.n_tok * p.n_head > 0x7fffffffu || !mul_size(p.n_tok, p.n_head * c.hd, sizeof(float), &n) ||
       n > SIZE_MAX / 2)
     return fail(BH_ERR_SHAPE, "attention_paged: size overflow");
@@ -1617,7 +1621,11 @@ extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream
     Form f[2];
     const int n = forms_of(p, f);
     size_t need = 0;
-    for (int i = 0; i < n; ++i) need += workspace_of(a, f[i]);
+    for (int i = 0; i < n; ++i) {
+      need += workspace_of(a, f[i]);
+      if (most_tiles(a, f[i]) > kMostBlocks)
+        return fail(BH_ERR_SHAPE, "attention_paged: more row tiles than a launch has blocks");
+    }
     char *ws = static_cast<char *>(p.workspace);
     if (ws) {
       if (!aligned16(ws) || p.workspace_bytes < need)

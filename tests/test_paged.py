@@ -100,6 +100,19 @@ def test_attention_head_size_limit_and_empty(bh):
         assert bh.lib().bh_attention_paged(ctypes.byref(a), None) == bh.BH_OK
 
 
+def test_attention_refuses_more_than_a_grid_holds(bh):
+    # the generic layout: a block a (token, head)
+    odd = _cache(bh, hd=40, n_kv=1, head_stride=40, pos_stride=40, page_stride=640)
+    a = _attn(bh, cache=odd, n_head=1, n_tok=1 << 24)
+    assert bh.lib().bh_attention_paged(ctypes.byref(a), None) == bh.BH_ERR_SHAPE
+    assert "size overflow" in bh.last_error()
+    # a tile a (request, kv head) and more
+    c = _cache(bh, hd=64, n_kv=64, head_stride=64, pos_stride=4096, page_stride=65536)
+    a = _attn(bh, cache=c, n_head=64, n_tok=1 << 20, n_req=1 << 20)
+    assert bh.lib().bh_attention_paged(ctypes.byref(a), None) == bh.BH_ERR_SHAPE
+    assert "row tiles" in bh.last_error()
+
+
 def _plan(bh, **kw):
     f = dict(cached=P, n_new=P, block_table=P, free_pages=P, n_free=P, kv_len=2 * P, q_start=P,
              slots=P, pos=P, n_free_out=P, n_refused=None, n_req=4, n_tok=8, table_width=4,
