@@ -1339,23 +1339,36 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
   }
 }
 
-// Joins the parts of the tiles that more than one worker has: `share` blocks a
-// tile.  16 lanes take 64 dims of a row; of the block's 16 such groups as many
-// share a row as it has parts, each with every sixteenth part, whose loads are all
-// issued before the first is needed: one round trip for up to 16 kAhead parts.
-template <int HD, int R>
-__global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, Split sp, int share) {
+// The join of a launch: `share` blocks a tile of `rows` rows.
+struct Join {
+  Split sp;
+  int rows, share;
+  unsigned blocks;
+};
+
+// Joins the parts of the tiles that more than one worker has, of both launches of a
+// call.  16 lanes take 64 dims of a row; of the block's 16 such groups p share a
+// row of more than 8 parts, each with every p-th, and the loads of up to 8 a group
+// are all issued before the first is needed: one round trip for up to 128 parts,
+// and no barrier for up to 8.  (Groups that share from 2 parts on: 21 us for the
+// tiles of 128 rows of a chunk of 512 tokens, 12 so, 58 MB read and written.)
+template <int HD>
+__global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, Join one, Join two) {
   constexpr int kAt = kThreads / 16, kSlices = HD / 64, kAhead = 8;
   __shared__ float part[kAt][64], sums[kAt], tops[kAt];
-  const int tile = blockIdx.x / share, tid = threadIdx.x;
+  const bool of_two = blockIdx.x >= one.blocks;
+  const unsigned block = blockIdx.x - (of_two ? one.blocks : 0);
+  const Split sp = of_two ? two.sp : one.sp;
+  const int share = of_two ? two.share : one.share, R = of_two ? two.rows : one.rows;
+  const int tile = block / share, tid = threadIdx.x;
   const Cut cut = sp.cut[tile];
   if (tile >= *sp.n_tiles || cut.rows == 0) return;  // (past n_tiles cut holds nothing)
   const int parts = cut.last - cut.first + 1;
-  int p = 2;  // groups of a row
-  while (p < parts && p < kAt) p <<= 1;
+  int p = 1;  // groups of a row
+  while (kAhead * p < parts && p < kAt) p <<= 1;
   const int group = tid >> 4, mine = group & (p - 1), d = (tid & 15) * 4;
   const int items = cut.rows * kSlices, at_once = kAt / p;
-  for (int i0 = (blockIdx.x - tile * share) * at_once; i0 < items; i0 += share * at_once) {
+  for (int i0 = (block - tile * share) * at_once; i0 < items; i0 += share * at_once) {
     const int item = i0 + group / p;
     const bool live = item < items;
     const int row = live ? item / kSlices : 0, dim = item % kSlices * 64 + d;
@@ -1381,9 +1394,11 @@ __global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, 
     }
     for (int w = cut.first + mine + kAhead * p; w <= cut.last; w += p)
       top = fmaxf(top, sp.pm[at(w)]);
-    if (d == 0) tops[group] = top;
-    __syncthreads();
-    for (int k = 0; k < p; ++k) top = fmaxf(top, tops[(group - mine) + k]);
+    if (p > 1) {
+      if (d == 0) tops[group] = top;
+      __syncthreads();
+      for (int k = 0; k < p; ++k) top = fmaxf(top, tops[(group - mine) + k]);
+    }
     const float ref = top == -INFINITY ? 0.0f : top;
     f32x4 o = {0, 0, 0, 0};
     float sum = 0.0f;
@@ -1402,9 +1417,11 @@ __global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, 
       sum += keep * sp.pl[x];
       o += keep * *reinterpret_cast<const f32x4 *>(sp.pacc + x * HD + dim);
     }
-    *reinterpret_cast<f32x4 *>(&part[group][d]) = o;
-    if (d == 0) sums[group] = sum;
-    __syncthreads();
+    if (p > 1) {
+      *reinterpret_cast<f32x4 *>(&part[group][d]) = o;
+      if (d == 0) sums[group] = sum;
+      __syncthreads();
+    }
     if (mine == 0 && live) {
       for (int k = 1; k < p; ++k) {
         o += *reinterpret_cast<const f32x4 *>(&part[group + k][d]);
@@ -1415,7 +1432,7 @@ __global__ __launch_bounds__(kThreads) void attn_paged_join_kernel(PagedArgs a, 
           a.out + (static_cast<size_t>(cut.q0 + tok) * a.n_head + cut.head * a.group +
                    (q_row - tok * a.group)) * HD + dim) = o * (top == -INFINITY ? 0.0f : 1.0f / sum);
     }
-    __syncthreads();  // for the next rows
+    if (p > 1) __syncthreads();  // for the next rows
   }
 }
 
@@ -1468,58 +1485,70 @@ Split split_of(const PagedArgs &a, const Form &f, char *ws) {
   return sp;
 }
 
-template <int HD, int R>
-int launch_join(const PagedArgs &a, const Form &f, const Split &sp, int unit, hipStream_t st) {
-  if (a.max_len <= unit) return BH_OK;  // with one unit a tile nothing is cut
-  // a block a (row, 64 dims) while they are not many times what fits the card
-  const size_t tiles = most_tiles(a, f);
-  const size_t most = static_cast<size_t>(a.n_tok > 1 ? R : a.group < R ? a.group : R) * (HD / 64);
-  size_t share = 16 * device_cu_count() / tiles;
-  share = share < 1 ? 1 : share > most ? most : share;
-  BH_LAUNCH((attn_paged_join_kernel<HD, R>), static_cast<unsigned>(tiles * share), kThreads, 0, st,
-            a, sp, static_cast<int>(share));
+Join join_of(const PagedArgs &a, const Form &f, const Split &sp, int unit) {
+  Join j{sp, f.rows(), 1, 0};
+  if (a.max_len <= unit) return j;  // with one unit a tile nothing is cut
+  // a block a (row, 64 dims), as rows of many parts need, while they are not many
+  // times what fits the card (4 / 8 / 16 a compute unit: draft 7.4 / 5.6 / 4.9 us,
+  // batch 6.6 / 5.4 / 6.5, chunk 11.2 / 12.1 / 12.6)
+  const size_t tiles = most_tiles(a, f), R = f.rows(), group = a.group;
+  const size_t most = (a.n_tok > 1 ? R : group < R ? group : R) * (a.hd / 64);
+  const size_t share = 8 * device_cu_count() / tiles;
+  j.share = static_cast<int>(share < 1 ? 1 : share > most ? most : share);
+  j.blocks = static_cast<unsigned>(tiles * j.share);
+  return j;
+}
+
+int launch_join(const PagedArgs &a, const Join &one, const Join &two, hipStream_t st) {
+  const unsigned blocks = one.blocks + two.blocks;
+  if (blocks == 0) return BH_OK;
+  if (a.hd == 64) BH_LAUNCH(attn_paged_join_kernel<64>, blocks, kThreads, 0, st, a, one, two);
+  else if (a.hd == 128) BH_LAUNCH(attn_paged_join_kernel<128>, blocks, kThreads, 0, st, a, one, two);
+  else BH_LAUNCH(attn_paged_join_kernel<256>, blocks, kThreads, 0, st, a, one, two);
   return BH_OK;
 }
 
 template <class E, bool WIDE>
-int launch(const PagedArgs &a, const Form &f, char *ws, hipStream_t st) {
+int launch(const PagedArgs &a, const Form &f, char *ws, hipStream_t st, Join *join) {
   const Split sp = split_of(a, f, ws);
   BH_LAUNCH((attn_paged_kernel<E, WIDE>), static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
-  return launch_join<E::kHd, Shape<E, WIDE>::R>(a, f, sp, Shape<E, WIDE>::U, st);
+  *join = join_of(a, f, sp, Shape<E, WIDE>::U);
+  return BH_OK;
 }
 
 template <int HD>
-int launch_wide(const PagedArgs &a, const Form &f, char *ws, hipStream_t st) {
+int launch_wide(const PagedArgs &a, const Form &f, char *ws, hipStream_t st, Join *join) {
   const Split sp = split_of(a, f, ws);
   BH_LAUNCH(attn_paged_wide_kernel<HD>, static_cast<unsigned>(sp.workers), kWideThreads, 0, st, a, sp);
-  return launch_join<HD, kWideRows>(a, f, sp, kWideUnit, st);
+  *join = join_of(a, f, sp, kWideUnit);
+  return BH_OK;
 }
 
 template <int RT>
-int launch_rt(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st) {
+int launch_rt(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st, Join *join) {
   if (f16) {
-    if (a.hd == 64) return launch<EngineF16<64, RT>, false>(a, f, ws, st);
-    if (a.hd == 128) return launch<EngineF16<128, RT>, false>(a, f, ws, st);
-    return launch<EngineF16<256, RT>, false>(a, f, ws, st);
+    if (a.hd == 64) return launch<EngineF16<64, RT>, false>(a, f, ws, st, join);
+    if (a.hd == 128) return launch<EngineF16<128, RT>, false>(a, f, ws, st, join);
+    return launch<EngineF16<256, RT>, false>(a, f, ws, st, join);
   }
-  if (a.hd == 64) return launch<EngineF32<64, RT>, false>(a, f, ws, st);
-  if (a.hd == 128) return launch<EngineF32<128, RT>, false>(a, f, ws, st);
-  return launch<EngineF32<256, RT>, false>(a, f, ws, st);
+  if (a.hd == 64) return launch<EngineF32<64, RT>, false>(a, f, ws, st, join);
+  if (a.hd == 128) return launch<EngineF32<128, RT>, false>(a, f, ws, st, join);
+  return launch<EngineF32<256, RT>, false>(a, f, ws, st, join);
 }
 
-int launch_form(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st) {
+int launch_form(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st, Join *join) {
   if (f.wide && f16) {
-    if (a.hd == 64) return launch_wide<64>(a, f, ws, st);
-    if (a.hd == 128) return launch_wide<128>(a, f, ws, st);
-    return launch_wide<256>(a, f, ws, st);
+    if (a.hd == 64) return launch_wide<64>(a, f, ws, st, join);
+    if (a.hd == 128) return launch_wide<128>(a, f, ws, st, join);
+    return launch_wide<256>(a, f, ws, st, join);
   }
   if (f.wide) {
-    if (a.hd == 64) return launch<EngineF32<64, 2>, true>(a, f, ws, st);
-    if (a.hd == 128) return launch<EngineF32<128, 2>, true>(a, f, ws, st);
-    return launch<EngineF32<256, 2>, true>(a, f, ws, st);
+    if (a.hd == 64) return launch<EngineF32<64, 2>, true>(a, f, ws, st, join);
+    if (a.hd == 128) return launch<EngineF32<128, 2>, true>(a, f, ws, st, join);
+    return launch<EngineF32<256, 2>, true>(a, f, ws, st, join);
   }
-  if (f.rt == 1) return launch_rt<1>(a, f16, f, ws, st);
-  return launch_rt<2>(a, f16, f, ws, st);
+  if (f.rt == 1) return launch_rt<1>(a, f16, f, ws, st, join);
+  return launch_rt<2>(a, f16, f, ws, st, join);
 }
 
 // Whether a call runs on the matrix cores: rows of whole 16-byte pieces.
@@ -1620,12 +1649,13 @@ extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream
   if (on_matrix_cores(p)) {
     Form f[2];
     const int n = forms_of(p, f);
-    size_t need = 0;
+    size_t need = 0, tiles = 0;
     for (int i = 0; i < n; ++i) {
       need += workspace_of(a, f[i]);
-      if (most_tiles(a, f[i]) > kMostBlocks)
-        return fail(BH_ERR_SHAPE, "attention_paged: more row tiles than a launch has blocks");
+      tiles += most_tiles(a, f[i]);
     }
+    if (tiles > kMostBlocks)  // (the join has more than a block a tile only of few)
+      return fail(BH_ERR_SHAPE, "attention_paged: more row tiles than a launch has blocks");
     char *ws = static_cast<char *>(p.workspace);
     if (ws) {
       if (!aligned16(ws) || p.workspace_bytes < need)
@@ -1636,10 +1666,12 @@ extern "C" int bh_attention_paged(const bh_attention_paged_args *args, bh_stream
       ws = static_cast<char *>(device_scratch(need, kScratchPaged, st));
       if (!ws) return BH_ERR_HIP;
     }
+    Join join[2] = {};
     for (int i = 0; i < n; ++i) {
-      if (int e = launch_form(a, f16, f[i], ws, st)) return e;
+      if (int e = launch_form(a, f16, f[i], ws, st, &join[i])) return e;
       ws += workspace_of(a, f[i]);
     }
+    if (int e = launch_join(a, join[0], join[1], st)) return e;
     return ok();
   }
   const dim3 grid(static_cast<unsigned>(a.n_tok), static_cast<unsigned>(a.n_head));
