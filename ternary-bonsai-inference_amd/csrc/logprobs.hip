@@ -506,9 +506,14 @@ bool nothing(const bh_token_logprobs_args &p) {
 
 // Blocks of a row: about four blocks a compute unit in all, a tile each at least.
 // 512 rows of 248320 with 5 alternatives, 1 / 2 / 4 / 8 a unit: 121 / 117 / 111 / 123
-// us; 64 rows with 20: 58 / 41 / 35 / 36.
+// us; 64 rows with 20: 58 / 41 / 35 / 36.  A row of few tiles has one block, whose
+// time then is about that of the second launch: up to 8 tiles without alternatives
+// (256 rows of 32000: 8.4 us, split 12.7; 61 rows: 8.0 and 7.8, and half the
+// launches), up to 2 with them (one row of 8192 with 5: 8.6, 11.4 split; 16 rows of
+// 16384 with 20: 16.2, 13.9 split).
 size_t parts_of(const bh_token_logprobs_args &p) {
   const size_t tiles = (p.vocab + kLpTile - 1) / kLpTile;
+  if (tiles <= (p.n_top == 0 ? 8 : 2)) return 1;
   size_t parts = 4 * device_cu_count() / p.n_rows;
   if (parts > tiles) parts = tiles;
   if (parts > static_cast<size_t>(kMaxParts)) parts = kMaxParts;
