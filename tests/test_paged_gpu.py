@@ -489,6 +489,56 @@ def test_two_streams_with_their_own_workspaces(bh, dev):
         assert rel_err(c.out_tensor.cpu().numpy(), _want(s).astype(np.float32)) <= TOL
 
 
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(6, 1, 256), (24, 1, 128), (3, 1, 64)])
+def test_one_head_in_hundreds_of_parts(bh, dev, n_q, n_kv, hd, f16):
+    """A single row tile that every worker has a part of."""
+    rng = np.random.default_rng(31)
+    _check(bh, dev, _step(rng, dev, [40000], [1], 64, n_q, n_kv, hd, f16))
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(24, 4, 256), (32, 8, 128), (8, 8, 64)])
+def test_prompts_beside_decoders_replayed(bh, dev, n_q, n_kv, hd, f16):
+    """Both forms of a step in one graph, their tiles cut and joined, replayed over
+    other lengths: prompts alone, decoders alone, nothing at all."""
+    import torch
+    rng = np.random.default_rng(32)
+    s = _step(rng, dev, [1500, 900, 2600, 40], [130, 1, 61, 5], 32, n_q, n_kv, hd, f16, pad=3)
+    d = {n: _t(s[n], dev) for n in ("q", "start", "lens", "table")}
+    out = torch.empty(s["q"].shape, device=dev)
+
+    def make(workspace=None):
+        return bh.make_attention_paged_args(
+            bh.make_paged_cache(s["k"], s["v"]), d["q"], d["start"], d["lens"], d["table"],
+            out=out, max_new=200, workspace=workspace)
+    ws = torch.empty(max(16, bh.attention_paged_workspace(make())), dtype=torch.uint8, device=dev)
+    args, st = make(ws), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        bh.attention_paged(args, stream=st)
+    for start, lens in (([0, 130, 131, 192, 197], [1500, 900, 2600, 40]),
+                        ([0, 200, 200, 200, 200], [700, 0, 2600, 17]),
+                        ([0, 0, 0, 0, 0], [1500, 900, 2600, 40]),
+                        ([0, 1, 2, 3, 4], [1500, 900, 1, 40]),
+                        ([0, 90, 91, 197, 198], [1311, 1, 2600, 3])):
+        s["start"], s["lens"] = np.array(start, np.int32), np.array(lens, np.int32)
+        d["start"].copy_(_t(s["start"], dev))
+        d["lens"].copy_(_t(s["lens"], dev))
+        out.fill_(5.25)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.cpu().numpy()
+        assert rel_err(got, _want(s).astype(np.float32)) <= TOL
+        assert (got[start[-1]:] == 5.25).all()
+        out.fill_(5.25)
+        bh.attention_paged(make())
+        torch.cuda.synchronize()
+        assert np.array_equal(got.view(np.uint32), out.cpu().numpy().view(np.uint32))
+
+
 def test_strange_offsets_stay_in_bounds(bh, dev):
     """Offsets past the tokens and lengths past the table are clipped."""
     import torch
