@@ -15,9 +15,10 @@
 // A position that a query does not see has no effect on it, whatever it holds.
 //
 // Measured (24 / 4 heads of 256, us of the call, both launches): one token at 100 /
-// 5000 / 32768 f16 positions 12 / 15.7 / 30 (the last 4.4 TB/s), 64 requests at
-// 16384 720 (6.0 TB/s), 64 at 8192 f32 695 (6.2 TB/s); a copy reaches 5.1 TB/s
-// here.  Error against 64-bit arithmetic 2e-7 to 4e-7.
+// 5000 / 32768 f16 positions 12 / 15.9 / 30.6 (the last 4.4 TB/s), 64 requests at
+// 16384 715 (6.0 TB/s), 64 at 8192 f32 689 (6.2 TB/s); a copy reaches 5.1 TB/s
+// here.  Of one token's 12 us the wait for offsets, table, K and V one after the
+// other is most; K, V, q and the next table entry are asked for together.  Error against 64-bit arithmetic 2e-7 to 4e-7.
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -235,7 +236,7 @@ struct Work {
 // v_perm a pair.  Row c's output and running state stay with the lanes of c.
 // With hd 256 a step is 16 positions: at 32 the accumulators and both tiles take
 // 192 of the 256 registers of two waves a SIMD and the rest spills (64 requests
-// at 16384 positions: 1222 us, 720 with 16, of which 13 are the join).
+// at 16384 positions: 1222 us, 715 with 16).
 template <int HD, int RT>
 struct EngineF16 {
   using Elem = _Float16;
@@ -414,7 +415,9 @@ struct EngineF16 {
 // f32 cache: 16 positions a step on v_mfma_f32_16x16x4_f32, products and sums in
 // f32, nothing split.  The same scheme: lane (g, c) loads 16 bytes of position
 // c's row (dims 16 kk + 4 g ..), gets row c's scores at positions 4 g + i, and
-// multiplies them by 4 dims of those positions' values.
+// multiplies them by 4 dims of those positions' values.  Decoders are bound by the
+// reads (64 at 8192: 6.2 TB/s, the matrix unit a quarter busy), many rows by that
+// instruction: 512 tokens at 8192 512 us, 94 of the 154 TFLOP/s of a large product.
 template <int HD, int RT>
 struct EngineF32 {
   using Elem = float;
@@ -1033,9 +1036,9 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
 // among 16 exchanged by an XOR so that the stores of a row's pieces, which are 1 KB
 // or 256 bytes apart, fall into different banks.
 //
-// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions 323-354
-// (280-309 TFLOP/s of useful products, twice that of issued ones), 128 there 130, 2048
-// from position 0 209.  Two waves a SIMD hide about half of the LDS reads and the
+// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions 320-354
+// (280-312 TFLOP/s of useful products, twice that of issued ones), 128 there 114, 2048
+// from position 0 203.  Two waves a SIMD hide about half of the LDS reads and the
 // softmax; half of the waves half a step behind the others, to run one's
 // exponentials beside the other's products, took the registers past 256 and three
 // times as long (at hd 128, where nothing spills, 319 for 265).
