@@ -1207,21 +1207,45 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
       }
       const int p0 = p_beg + t * STEP;
       if (t >= 0 && p0 < my_end) {
-        const _Float16 *ks = tiles_s + (t & 1) * kTile, *vs = tiles_s + (2 + (t & 1)) * kTile;
+        // places of this lane's pieces, formed from these by an XOR where they are read:
+        // kept over the steps they would take 20 registers
+        int at_k = (t & 1) * kTile + (g * 16 + (c ^ g)) * 8;
+        int at_v = (2 + (t & 1)) * kTile + (g * 16 + c) * 8;
+        asm volatile("" : "+v"(at_k), "+v"(at_v));
         const uint32_t mask = mask_s[t & 3];
+        // operands are read a group of four ahead of the products, and not farther
+        h8 ahead[2][4];
+        const auto read_k = [&](int grp) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int kk = 2 * grp + (i >> 1);
+            ahead[grp & 1][i] = *reinterpret_cast<const h8 *>(
+                tiles_s + ((i & 1) * KK + kk) * 512 + (at_k ^ 32 * (kk & 3)));
+          }
+        };
+        const auto read_v = [&](int grp) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = 4 * grp + i;
+            ahead[grp & 1][i] = *reinterpret_cast<const h8 *>(tiles_s + d * 512 + (at_v ^ 8 * d));
+          }
+        };
         f32x4 sh[2], sl[2];
         sh[0] = sh[1] = sl[0] = sl[1] = f32x4{0, 0, 0, 0};
+        read_k(0);
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          if (kk % 2 == 0) __builtin_amdgcn_sched_barrier(0);  // (operands are not read far ahead)
-          const int o = (kk * 64 + g * 16 + (c ^ ((4 * kk + g) & 15))) * 8;
+        for (int grp = 0; grp < KK / 2; ++grp) {
+          if (grp + 1 < KK / 2) read_k(grp + 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const h8 k = *reinterpret_cast<const h8 *>(ks + s * KK * 512 + o);
-            sh[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[kk], sh[s], 0, 0, 0);
-            sl[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[kk], sl[s], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) {
+            const int kk = 2 * grp + (i >> 1), s = i & 1;
+            sh[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[grp & 1][i], qh[kk], sh[s], 0, 0, 0);
+            sl[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[grp & 1][i], ql[kk], sl[s], 0, 0, 0);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
+        read_v(0);
         float sc[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) sc[j] = (sl[j >> 2][j & 3] + sh[j >> 2][j & 3]) * fac;
@@ -1275,11 +1299,16 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
           pl[j] = static_cast<_Float16>(x - static_cast<float>(ph[j]));
         }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          if (d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-          const h8 v = *reinterpret_cast<const h8 *>(vs + (d * 64 + g * 16 + (c ^ (d & 15))) * 8);
-          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[d], 0, 0, 0);
-          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[d], 0, 0, 0);
+        for (int grp = 0; grp < DT / 4; ++grp) {
+          if (grp + 1 < DT / 4) read_v(grp + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = 4 * grp + i;
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[grp & 1][i], ph, acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[grp & 1][i], pl, acc[d], 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
         uint32_t apart = __builtin_amdgcn_readfirstlane(apart_s[t & 3]);
         while (__builtin_expect(apart != 0, false)) {
