@@ -1036,9 +1036,9 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
 // among 16 exchanged by an XOR so that the stores of a row's pieces, which are 1 KB
 // or 256 bytes apart, fall into different banks.
 //
-// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions 320-354
-// (280-312 TFLOP/s of useful products, twice that of issued ones), 128 there 114, 2048
-// from position 0 203.  Two waves a SIMD hide about half of the LDS reads and the
+// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions 311-330
+// (300-321 TFLOP/s of useful products, twice that of issued ones), 128 there 106, 2048
+// from position 0 177.  Two waves a SIMD hide about half of the LDS reads and the
 // softmax; half of the waves half a step behind the others, to run one's
 // exponentials beside the other's products, took the registers past 256 and three
 // times as long (at hd 128, where nothing spills, 319 for 265).
@@ -1214,6 +1214,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
         asm volatile("" : "+v"(at_k), "+v"(at_v));
         const uint32_t mask = mask_s[t & 3];
         // operands are read a group of four ahead of the products, and not farther
+        // (hd 128: 240 us for 258 with each group read beside its products)
         h8 ahead[2][4];
         const auto read_k = [&](int grp) {
 #pragma unroll
@@ -1280,15 +1281,18 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
           }
         }
         top = row_lanes(top, MaxOp{});
+        // What is kept moves only when a row's maximum has doubled its weights: they
+        // stand in f16 up to 2 kPUnit, and most new maxima are less above the last (512
+        // tokens at 8192 321 -> 312 us).
         const float now = fmaxf(m, top);
-        const float ref = now == -INFINITY ? 0.0f : now;
-        if (__any(now > m)) {
-          const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - ref);
+        if (__any(now > m + 1.0f)) {
+          const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
           l *= keep;
 #pragma unroll
           for (int d = 0; d < DT; ++d) acc[d] *= keep;
+          m = now;
         }
-        m = now;
+        const float ref = m == -INFINITY ? 0.0f : m;
         h8 ph, pl;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
