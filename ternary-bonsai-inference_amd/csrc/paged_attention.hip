@@ -417,7 +417,7 @@ struct EngineF16 {
 // c's row (dims 16 kk + 4 g ..), gets row c's scores at positions 4 g + i, and
 // multiplies them by 4 dims of those positions' values.  Decoders are bound by the
 // reads (64 at 8192: 6.2 TB/s, the matrix unit a quarter busy), many rows by that
-// instruction: 512 tokens at 8192 512 us, 94 of the 154 TFLOP/s of a large product.
+// instruction: 512 tokens at 8192 490 us, 99 of the 154 TFLOP/s of a large product.
 template <int HD, int RT>
 struct EngineF32 {
   using Elem = float;
@@ -880,14 +880,14 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
           for (int j = 1; j < E::kSlots; ++j) top = fmaxf(top, eng.sc[t][j]);
           top = row_lanes(top, MaxOp{});
           const float now = fmaxf(m[t], top);
-          // a row that has seen nothing above -inf is measured from 0
-          const float ref = now == -INFINITY ? 0.0f : now;
-          if (__any(now > m[t])) {
-            const float keep = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - ref);
+          if (__any(now > m[t] + 1.0f)) {  // (512 tokens over f32: 509 -> 490 us)
+            const float keep = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - now);
             l[t] *= keep;
             eng.scale_acc(t, keep);
+            m[t] = now;
           }
-          m[t] = now;
+          // a row that has seen nothing above -inf is measured from 0
+          const float ref = m[t] == -INFINITY ? 0.0f : m[t];
 #pragma unroll
           for (int j = 0; j < E::kSlots; ++j) {
             eng.sc[t][j] = __builtin_amdgcn_exp2f(eng.sc[t][j] - ref);
@@ -1036,8 +1036,8 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
 // among 16 exchanged by an XOR so that the stores of a row's pieces, which are 1 KB
 // or 256 bytes apart, fall into different banks.
 //
-// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions 311-330
-// (300-321 TFLOP/s of useful products, twice that of issued ones), 128 there 106, 2048
+// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions 280-330
+// (300-357 TFLOP/s of useful products, twice that of issued ones), 128 there 106, 2048
 // from position 0 177.  Two waves a SIMD hide about half of the LDS reads and the
 // softmax; half of the waves half a step behind the others, to run one's
 // exponentials beside the other's products, took the registers past 256 and three
@@ -1281,8 +1281,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
           }
         }
         top = row_lanes(top, MaxOp{});
-        // What is kept moves only when a row's maximum has doubled its weights: they
-        // stand in f16 up to 2 kPUnit, and most new maxima are less above the last (512
+        // As in attn_paged_kernel, what is kept moves only when a row's maximum has
+        // doubled its weights: they stand in f16 up to 2 kPUnit, and most new maxima are less above the last (512
         // tokens at 8192 321 -> 312 us).
         const float now = fmaxf(m, top);
         if (__any(now > m + 1.0f)) {
