@@ -44,7 +44,10 @@ extern "C" {
  *   page * page_stride + position * pos_stride + head * head_stride + dim
  * of k and of v (strides in elements, equal for both): a page may hold rows of
  * n_kv * hd as bh_kv_store's cache does, or lie head by head; K and V may share
- * one allocation.  page_size is any size from 1; n_pages * page_size < 2^31. */
+ * one allocation.  The dimensions nest, in any order: a larger stride is at least
+ * what all smaller ones reach, so that no two rows share memory (strides of
+ * dimensions of one entry don't count).  page_size is any size from 1; n_pages *
+ * page_size < 2^31. */
 typedef struct bh_paged_cache {
   void *k, *v;
   int kv_dtype; /* BH_KV_F32 or BH_KV_F16 */

@@ -554,9 +554,9 @@ def _call(fn, args, stream):
 
 def make_paged_cache(k, v) -> PagedCache:
     """The pool k, v [n_pages, page_size, n_kv, hd] of f32 or f16 (or 16-bit
-    integers holding f16 bits); any equal strides of the first three, so a
-    transposed [n_pages, n_kv, page_size, hd] or one of two halves of an
-    allocation will do."""
+    integers holding f16 bits); any equal strides of the first three whose rows
+    share no memory, so a transposed [n_pages, n_kv, page_size, hd] or one of
+    two halves of an allocation will do (the calls refuse others)."""
     if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
         raise ValueError("k and v must be [n_pages, page_size, n_kv, hd], alike in shape, "
                          "strides and type")

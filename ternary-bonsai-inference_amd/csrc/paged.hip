@@ -19,6 +19,7 @@
 // by side were slower (4.3, 6.0 and 15.9, 16.6 us): the searches are LDS reads.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "../../include/bonsai_hip_serve.h"
@@ -316,9 +317,17 @@ int check_paged_cache(const bh_paged_cache &c, const char *who) {
       !mul_size(c.n_kv - 1, c.head_stride, esz, &s2) || s0 > SIZE_MAX / 8 || s1 > SIZE_MAX / 8 ||
       s2 > SIZE_MAX / 8)
     return fail(BH_ERR_SHAPE, w + "the cache's strides overflow");
-  if ((c.n_pages > 1 && c.page_stride == 0) || (c.page_size > 1 && c.pos_stride < c.hd) ||
-      (c.n_kv > 1 && c.head_stride < c.hd))
-    return fail(BH_ERR_SHAPE, w + "the cache's strides let rows overlap");
+  // in the order of their strides, each dimension steps over all that lies within it
+  struct Dim {
+    size_t n, stride;
+  } dims[3] = {{c.n_pages, c.page_stride}, {c.page_size, c.pos_stride}, {c.n_kv, c.head_stride}};
+  std::sort(dims, dims + 3, [](const Dim &x, const Dim &y) { return x.stride < y.stride; });
+  size_t span = c.hd;
+  for (const Dim &d : dims) {
+    if (d.n == 1) continue;
+    if (d.stride < span) return fail(BH_ERR_SHAPE, w + "the cache's strides let rows overlap");
+    span += (d.n - 1) * d.stride;
+  }
   if (!c.k || !c.v) return fail(BH_ERR_ARG, w + "null cache");
   if ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & (esz - 1))
     return fail(BH_ERR_ARG, w + "misaligned cache");
