@@ -1636,7 +1636,8 @@ int prepare(const bh_attention_paged_args &p, PagedArgs *a) {
     return fail(BH_ERR_SHAPE, "attention_paged: hd " + std::to_string(c.hd) + " above " +
                                   std::to_string(kAnyMaxHd));
   size_t n;
-  if (p.n_head > 65535 || p.n_tok > kMostBlocks || p.n_req > 0x7ffffffeu ||
+  // (the threads that go through the requests step past the last by a round)
+  if (p.n_head > 65535 || p.n_tok > kMostBlocks || p.n_req > 0x7fff0000u ||
       p.n_tok * p.n_head > 0x7fffffffu || !mul_size(p.n_tok, p.n_head * c.hd, sizeof(float), &n) ||
       n > SIZE_MAX / 2)
     return fail(BH_ERR_SHAPE, "attention_paged: size overflow");
