@@ -144,8 +144,9 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PlanArgs a) {
       if (gone[k]) at = add_most(at, have[k]);
     }
     __syncthreads();
-    for (int p = tid; p < n_back; p += THREADS) {
-      const int r = find(start, a.n_req, top, p);
+    // (unsigned: n_back may be within a round of 2^31)
+    for (uint32_t p = tid; p < static_cast<uint32_t>(n_back); p += THREADS) {
+      const int r = find(start, a.n_req, top, static_cast<int>(p));
       a.free_pages[n_free + p] = a.table[static_cast<size_t>(r) * a.width + (p - start[r])];
     }
     __syncthreads();
