@@ -135,9 +135,10 @@ int bh_kv_store_paged(const bh_paged_cache *cache, const float *k, const float *
  * and gets zeros.  Tokens of no request are left as they were.
  *
  * q, out: [n_tok][n_head][hd] f32, out is not q; n_tok < 2^24, n_req at most 2^31 -
- * 65536.  Entries of q_start do not decrease (if they do, some tokens' results are
- * unspecified) and are clipped to 0 .. n_tok, kv_len to 0 .. table_width * page_size
- * (at most 2^31 - 65536).
+ * 65536.  Entries of q_start do not decrease (if they do, tokens' results are
+ * unspecified, and where requests ask for more than n_tok tokens in all, they may be
+ * left as they were) and are clipped to 0 .. n_tok, kv_len to 0 .. table_width *
+ * page_size (at most 2^31 - 65536).
  * A table entry outside 0 .. n_pages - 1 among a request's
  * ceil(kv_len / page_size) leaves its positions out, and is written to
  * *bad_page where that is not NULL (the caller presets it).

@@ -162,7 +162,7 @@ struct Cut {  // a tile, written by the worker of its first part
 struct Split {
   int *n_tiles;    // one word
   Cut *cut;        // [most_cut]
-  uint32_t most_cut;  // tiles of offsets that do not overlap; others may ask for more
+  uint32_t most_cut;  // tiles that a launch can have
   float *pm, *pl;  // [workers][2][R] running maximum (base 2) and sum
   float *pacc;     // [workers][2][R][hd]
   int workers;
@@ -591,21 +591,26 @@ struct Walk {
   // Every wave finds the run by itself: lane i adds up requests i per .. (i + 1)
   // per - 1, a scan over the lanes gives the total, and the lanes then go through
   // the one lane's requests that hold the run's beginning.
+  // Requests that have more tokens together than the call overlap: what they ask for
+  // may pass every count here and is bounded by nothing, so such a call does nothing.
   __device__ __forceinline__ void start(const PagedArgs &a, const Split &sp, int lane) {
     worker = blockIdx.x;
     const int per = (a.n_req + 63) / 64;
     int64_t mine = 0;
-    int mine_tiles = 0;
-    for (int i = lane * per; i < min((lane + 1) * per, a.n_req); ++i) {
+    int mine_tiles = 0, tokens = 0;  // (n_tok < 2^24: 64 lanes of n_tok + 1 stay below 2^31)
+    for (int i = lane * per; i < min((lane + 1) * per, a.n_req) && tokens <= a.n_tok; ++i) {
       work.load(a, sp, i);
       mine += work.cost(a);
       mine_tiles += work.tiles * a.n_kv;
+      tokens = min(tokens + work.n, a.n_tok + 1);
     }
     int64_t upto = mine;
     int upto_tiles = mine_tiles;
     upto = lane_scan(upto, SumOp{});
     upto_tiles = lane_scan(upto_tiles, SumOp{});
+    tokens = lane_scan(tokens, SumOp{});
     total = wave_uniform(__shfl(upto, 63));
+    if (__builtin_amdgcn_readlane(tokens, 63) > a.n_tok) total = 0, upto_tiles = 0;
     at = begin = wave_uniform(run_begin(total, sp.workers, worker));
     end = wave_uniform(run_begin(total, sp.workers, worker + 1));
     if (worker == 0 && threadIdx.x == 63) *sp.n_tiles = upto_tiles;
@@ -630,7 +635,7 @@ struct Walk {
         upto = mine;
         upto_tiles = mine_tiles;
         upto = lane_scan(upto, SumOp{});
-      upto_tiles = lane_scan(upto_tiles, SumOp{});
+        upto_tiles = lane_scan(upto_tiles, SumOp{});
         upto += base;
         upto_tiles += tile_base;
         const uint64_t past = __ballot(begin < upto);
