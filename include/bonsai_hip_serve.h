@@ -73,6 +73,10 @@ typedef struct bh_paged_cache {
  *           table not), are more than the stack holds with the released ones
  *           on it, or its new tokens counted so are more than n_tok:
  *           kv_len[i] = 0, no tokens, no pages, its table row as it was.
+ *           It holds its cached positions still: cached of the next step is
+ *           kv_len[i] where kv_len[i] > 0 or n_new[i] < 0, and as it was
+ *           otherwise.  (Refused are those with n_new[i] >= 0 and
+ *           kv_len[i] != cached[i] + n_new[i].)
  * otherwise its blocks from `have` on are popped from the stack into
  *           block_table[i], kv_len[i] = cached[i] + n_new[i].
  *
