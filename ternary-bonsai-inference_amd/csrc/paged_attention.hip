@@ -710,19 +710,21 @@ struct Walk {
   }
 };
 
-// WIDE: the waves of a block take rows of their own, 16 RT each, and go through all
-// positions of a piece side by side, so that K and V come to the CU once for 64
-// RT rows; for many rows.  Otherwise they share the rows and take every fourth
-// step of positions each, and join what they have at the piece's end.
-// (within a wave LDS operations are in order; this keeps the compiler to it)
+// Within a wave LDS operations are in order; this keeps the compiler to it.
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The waves of a block share its rows and take every fourth step of positions each;
+// what they have is joined at the piece's end.  WIDE, for many rows over an f32 cache:
+// the waves take rows of their own, 16 RT each, and go through all positions of a piece
+// side by side, so that three of the four loads of a K or V row are served by the
+// compute unit's own cache.  (Many rows over f16 have attn_paged_wide_kernel.)
 template <class E, bool WIDE>
 struct Shape {
+  static_assert(!WIDE || sizeof(typename E::Elem) == 4, "many rows over f16 have a kernel of their own");
   static constexpr int kWaveRows = 16 * E::kRt, R = kWaveRows * (WIDE ? kWaves : 1);
   static constexpr int kStride = E::kStep * (WIDE ? 1 : kWaves);  // from a wave's step to its next
   static constexpr int U = WIDE ? 128 : kStride;
@@ -957,7 +959,7 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
       float *mine_s = reinterpret_cast<float *>(lds + wave * E::kQBytes);
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const float by = !whole ? E::kAccUnit : m[t] == -INFINITY ? 0.0f : E::kAccUnit / l[t];
+        const float by = !whole ? 1.0f : m[t] == -INFINITY ? 0.0f : 1.0f / l[t];
         if (!whole && g == 0 && 16 * t + c < my_rows) {
           sp.pm[slot * R + row0 + 16 * t + c] = m[t];
           sp.pl[slot * R + row0 + 16 * t + c] = l[t];
@@ -988,46 +990,46 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
 #pragma unroll
       for (int t = 0; t < RT; ++t)
         if (g == 0) m_s[wave][16 * t + c] = m[t], l_s[wave][16 * t + c] = l[t];
-    float *join = reinterpret_cast<float *>(lds);
+      float *join = reinterpret_cast<float *>(lds);
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int half = 0; half < 16; half += kJoinRows) {
-        const int r0 = 16 * t + half;
-        if (r0 >= rows) continue;
-        __syncthreads();
-        if (c >= half && c < half + kJoinRows && 16 * t + c < rows)
-          eng.each_piece(t, lane, [&](int d, f32x4 o) {
-            *reinterpret_cast<f32x4 *>(join + (wave * kJoinRows + c - half) * kJoinStride + d) = o;
-          });
-        __syncthreads();
-        const int here = min(kJoinRows, rows - r0);
-        for (int i = tid; i < here * (HD / 4); i += kThreads) {
-          const int rr = i / (HD / 4), d = i % (HD / 4) * 4, row = r0 + rr;
-          float top = m_s[0][row];
+        for (int half = 0; half < 16; half += kJoinRows) {
+          const int r0 = 16 * t + half;
+          if (r0 >= rows) continue;
+          __syncthreads();
+          if (c >= half && c < half + kJoinRows && 16 * t + c < rows)
+            eng.each_piece(t, lane, [&](int d, f32x4 o) {
+              *reinterpret_cast<f32x4 *>(join + (wave * kJoinRows + c - half) * kJoinStride + d) = o;
+            });
+          __syncthreads();
+          const int here = min(kJoinRows, rows - r0);
+          for (int i = tid; i < here * (HD / 4); i += kThreads) {
+            const int rr = i / (HD / 4), d = i % (HD / 4) * 4, row = r0 + rr;
+            float top = m_s[0][row];
 #pragma unroll
-          for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_s[w][row]);
-          const float ref = top == -INFINITY ? 0.0f : top;
-          float sum = 0.0f;
-          f32x4 o = {0, 0, 0, 0};
+            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_s[w][row]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+            f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-          for (int w = 0; w < kWaves; ++w) {
-            const float keep = __builtin_amdgcn_exp2f(m_s[w][row] - ref);
-            sum += keep * l_s[w][row];
-            o += keep * *reinterpret_cast<const f32x4 *>(join + (w * kJoinRows + rr) * kJoinStride + d);
-          }
-          if (whole) {
-            const int tok = a.grp.div(tile * R + row);
-            const float inv = top == -INFINITY ? 0.0f : E::kAccUnit / sum;
-            float *dst = a.out + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
-                                  (tile * R + row - tok * a.group)) * HD + d;
-            *reinterpret_cast<f32x4 *>(dst) = o * inv;
-          } else {
-            *reinterpret_cast<f32x4 *>(sp.pacc + (slot * R + row) * HD + d) = o * E::kAccUnit;
-            if (d == 0) sp.pm[slot * R + row] = top, sp.pl[slot * R + row] = sum;
+            for (int w = 0; w < kWaves; ++w) {
+              const float keep = __builtin_amdgcn_exp2f(m_s[w][row] - ref);
+              sum += keep * l_s[w][row];
+              o += keep * *reinterpret_cast<const f32x4 *>(join + (w * kJoinRows + rr) * kJoinStride + d);
+            }
+            if (whole) {
+              const int tok = a.grp.div(tile * R + row);
+              const float inv = top == -INFINITY ? 0.0f : E::kAccUnit / sum;
+              float *dst = a.out + (static_cast<size_t>(q0 + tok) * a.n_head + head * a.group +
+                                    (tile * R + row - tok * a.group)) * HD + d;
+              *reinterpret_cast<f32x4 *>(dst) = o * inv;
+            } else {
+              *reinterpret_cast<f32x4 *>(sp.pacc + (slot * R + row) * HD + d) = o * E::kAccUnit;
+              if (d == 0) sp.pm[slot * R + row] = top, sp.pl[slot * R + row] = sum;
+            }
           }
         }
-      }
     }
   }
 }
