@@ -152,10 +152,11 @@ int bh_kv_store_paged(const bh_paged_cache *cache, const float *k, const float *
  * whatever it is.  Any hd up to 512 and any
  * n_head that n_kv divides; hd 64, 128 and 256 with strides and pointers of
  * whole 16 bytes run on the matrix cores.  Results agree with 64-bit arithmetic
- * to about 1e-6 of the output's magnitude and are the same bits from call to
- * call on one device.  Scores q.k / sqrtf(hd) stay below the largest f32.  What
- * is infinite or NaN among the values a query sees makes the dimensions it is in
- * not finite. */
+ * to about 1e-6 of sum w |v|, w being the weights, and are the same bits from call
+ * to call on one device.  Scores s are f32, which adds |s| 2^-22 of itself to a
+ * weight's error.  The partial sums of q.k, log2(e) q.k, and over an f32 cache the
+ * sum of the |v| that a query sees stay below the largest f32.  What is infinite or
+ * NaN among the values a query sees makes the dimensions it is in not finite. */
 typedef struct bh_attention_paged_args {
   bh_paged_cache cache;
   const float *q;
@@ -193,7 +194,8 @@ size_t bh_attention_paged_workspace(const bh_attention_paged_args *args);
  * not NULL (the caller presets it), the rest of its row is as any other's.
  * Either of logprob (then tokens too) and entropy may be NULL; with n_top = 0
  * top_ids and top_logprobs are.  n_top <= BH_MAX_TOP and <= vocab; inv_temp is
- * finite and above 0; vocab < 2^31. */
+ * finite and above 0; vocab < 2^31.  Finite logits of a row differ by less than the
+ * largest f32 (one further below the largest counts as -inf). */
 typedef struct bh_token_logprobs_args {
   const float *x;          /* [n_rows][row_stride]      */
   const uint32_t *tokens;  /* [n_rows] or NULL          */

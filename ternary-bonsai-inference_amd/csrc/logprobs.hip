@@ -19,9 +19,9 @@
 //
 // Long rows are split over as many blocks as fill the card; a second launch then
 // joins a row's parts.  Bound by reading the logits where there are many (2048 rows
-// of 248320 with 5 alternatives 345 us, 5.9 TB/s; 512 rows 102, with 20 116, with
-// none 94), by the chain load - exponentials - selection - second launch where
-// there are few (8 rows with 20 alternatives 15.6 us, with none 7.5).
+// of 248320 with 5 alternatives 342 us, 5.9 TB/s; 512 rows 101, with 20 107, with
+// none 93), by the chain load - exponentials - selection - second launch where
+// there are few (8 rows with 20 alternatives 15.2 us, with none 6.5).
 #include <hip/hip_runtime.h>
 
 #include <cmath>

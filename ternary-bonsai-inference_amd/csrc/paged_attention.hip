@@ -16,9 +16,12 @@
 //
 // Measured (24 / 4 heads of 256, us of the call, both launches): one token at 100 /
 // 5000 / 32768 f16 positions 12 / 15.9 / 30.6 (the last 4.4 TB/s), 64 requests at
-// 16384 715 (6.0 TB/s), 64 at 8192 f32 689 (6.2 TB/s); a copy reaches 5.1 TB/s
-// here.  Of one token's 12 us the wait for offsets, table, K and V one after the
-// other is most; K, V, q and the next table entry are asked for together.  Error against 64-bit arithmetic 2e-7 to 4e-7.
+// 16384 715 (6.0 TB/s), 64 at 8192 f32 689 (6.2 TB/s), 509 at 500 211 (4.9 TB/s), 1500
+// at 100 175 (3.5 TB/s); a copy reaches 5.1 TB/s here.  Of one token's 12 us the wait
+// for offsets, table, K and V one after the other is most; K, V, q and the next table
+// entry are asked for together.  The generic form, as it is: one token at 5000 1.9-3.0
+// ms, 64 at 4096 1.9-3.9 ms (hd 80 to 256), 512 tokens at 4096 6.9-11.5 ms.  Error
+// against 64-bit arithmetic 2e-7 to 4e-7.
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -236,7 +239,8 @@ struct Work {
 // v_perm a pair.  Row c's output and running state stay with the lanes of c.
 // With hd 256 a step is 16 positions: at 32 the accumulators and both tiles take
 // 192 of the 256 registers of two waves a SIMD and the rest spills (64 requests
-// at 16384 positions: 1222 us, 715 with 16).
+// at 16384 positions: 1222 us, 715 with 16).  Two row tiles of hd 128 take 16 too (24
+// caches of 3500, 24 rows: 80 us, 93 with 32).
 template <int HD, int RT>
 struct EngineF16 {
   using Elem = _Float16;
@@ -417,7 +421,9 @@ struct EngineF16 {
 // c's row (dims 16 kk + 4 g ..), gets row c's scores at positions 4 g + i, and
 // multiplies them by 4 dims of those positions' values.  Decoders are bound by the
 // reads (64 at 8192: 6.2 TB/s, the matrix unit a quarter busy), many rows by that
-// instruction: 512 tokens at 8192 490 us, 99 of the 154 TFLOP/s of a large product.
+// instruction and by each wave's wait for its own loads: 512 tokens at 4096 positions
+// (24 / 4 heads of 256, 48.3 GFLOP) 493 us, 98 of the 154 TFLOP/s of a large product;
+// at 8192 (99.9 GFLOP) 933 us.
 template <int HD, int RT>
 struct EngineF32 {
   using Elem = float;
@@ -1046,9 +1052,9 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
 // among 16 exchanged by an XOR so that the stores of a row's pieces, which are 1 KB
 // or 256 bytes apart, fall into different banks.
 //
-// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions 280-330
-// (300-357 TFLOP/s of useful products, twice that of issued ones), 128 there 106, 2048
-// from position 0 177.  Two waves a SIMD hide about half of the LDS reads and the
+// Measured (24 / 4 heads of 256, us of the call): 512 tokens at 8192 positions (99.9
+// GFLOP) 258-288 by the box (347-387 TFLOP/s of useful products, twice that of issued
+// ones), at 4096 (48.3) 152, 128 at 8192 103, 2048 from position 0 (51.6) 173-179.  Two waves a SIMD hide about half of the LDS reads and the
 // softmax; half of the waves half a step behind the others, to run one's
 // exponentials beside the other's products, took the registers past 256 and three
 // times as long (at hd 128, where nothing spills, 319 for 265).
@@ -1607,13 +1613,22 @@ bool on_matrix_cores(const bh_attention_paged_args &p) {
 }
 
 // The launches of a call, by the most rows a kv head that a request may have.
-constexpr int kWideOver = 32;  // rows from which a request goes to the wide form where there is one
+// Rows past which a request goes to the wide form where there is one.  A prompt of 512 at
+// 4096 beside 24 caches of 3500 (hd 256, us), line at 16 / 32 / 64 rows: with 18-30 rows
+// each 246-260 / 283-294 / as 32 over f16, 902 / 756-762 over f32; with 48 rows 247 /
+// 247 / 329 and 905 / 905 / 861.
+constexpr int kWideOver = 32;
 int forms_of(const bh_attention_paged_args &p, Form *f) {
   const size_t tokens = p.max_new == 0 || p.max_new > p.n_tok ? p.n_tok : p.max_new;
   const size_t rows = tokens * (p.n_head / p.cache.n_kv);
   constexpr int kAll = 0x7fffffff;
   const int two = p.cache.hd <= 128 ? 2 : 1;  // E::kBlocks of two row tiles
   const int wide = p.cache.kv_dtype == BH_KV_F16 ? 1 : two;
+  // 24 caches of 3500, us, hd 256 / 128 / 64 over f16: one row tile and two for up to 16
+  // rows 72, 76, 39 and 82, 76, 41; for 24 rows 120, 124, 75 and 87, 80, 42.  Narrow and
+  // wide at 48 rows 135, 129, 68 and 135, 178, 137; at 72 rows 176, 169, 92 and 143, 186,
+  // 139: the line is hd 256's.  Over f32 264, 256, 144 and 435, 404, 242 at 48; 353, 340,
+  // 197 and 442, 411, 245 at 72.
   if (rows <= 64) {
     const int rt = rows <= 16 ? 1 : 2;
     f[0] = Form{rt, false, 0, kAll, rt == 1 ? 2 : two};
