@@ -896,11 +896,13 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
           // What is kept moves only when a row's maximum has doubled its weights (512
           // tokens at 4096 over f32: 509 -> 490 us).  The difference of the two is exact where
           // they are near each other; m + 1 is not from 2^24 on, and may round up to m + 2.
-          if (__any(now - m[t] > 1.0f)) {
-            const float keep = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - now);
+          const bool grown = now - m[t] > 1.0f;
+          if (__any(grown)) {  // (the other rows stay as they are, bit for bit)
+            const float moved = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - now);
+            const float keep = grown ? moved : 1.0f;
             l[t] *= keep;
             eng.scale_acc(t, keep);
-            m[t] = now;
+            m[t] = grown ? now : m[t];
           }
           // a row that has seen nothing above -inf is measured from 0
           const float ref = m[t] == -INFINITY ? 0.0f : m[t];
@@ -1301,12 +1303,14 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
         // doubled its weights: they stand in f16 up to 2 kPUnit, and most new maxima are
         // less above the last (512 tokens at 8192 321 -> 312 us).
         const float now = fmaxf(m, top);
-        if (__any(now - m > 1.0f)) {
-          const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+        const bool grown = now - m > 1.0f;
+        if (__any(grown)) {
+          const float moved = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+          const float keep = grown ? moved : 1.0f;
           l *= keep;
 #pragma unroll
           for (int d = 0; d < DT; ++d) acc[d] *= keep;
-          m = now;
+          m = grown ? now : m;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
         h8 ph, pl;
