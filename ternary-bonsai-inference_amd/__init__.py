@@ -23,6 +23,7 @@ REPO_DIR = PKG_DIR.parent
 LIB_PATH = PKG_DIR / "lib" / "libbonsai_hip.so"
 HEADER_PATH = REPO_DIR / "include" / "bonsai_hip.h"
 SERVE_HEADER_PATH = REPO_DIR / "include" / "bonsai_hip_serve.h"
+BATCH_HEADER_PATH = REPO_DIR / "include" / "bonsai_hip_batch.h"
 
 BH_OK = 0
 BH_ERR_SHAPE = -1
@@ -203,6 +204,84 @@ _SERVE_SIGNATURES = {
     "bh_token_logprobs_workspace": (_c_size, [ctypes.POINTER(TokenLogprobsArgs)]),
 }
 
+
+class ConvRaggedArgs(ctypes.Structure):
+    """bh_conv_ragged_args (include/bonsai_hip_batch.h)."""
+
+    _fields_ = [
+        ("x", _vp), ("w", _vp), ("state", _vp), ("out", _vp), ("q_start", _vp),
+        ("src_slot", _vp), ("dst_slot", _vp), ("bad_slot", _vp),
+        ("n_tok", _c_size), ("n_req", _c_size), ("ch", _c_size), ("k", _c_size),
+        ("l2_dim", _c_size), ("head_dim", _c_size), ("n_slots", _c_size), ("x_stride", _c_size),
+        ("slot_stride", _c_size), ("max_new", _c_size), ("eps", _c_float),
+    ]
+
+
+class GdnRaggedArgs(ctypes.Structure):
+    """bh_gdn_ragged_args (include/bonsai_hip_batch.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("gate", _vp), ("beta", _vp), ("state", _vp),
+        ("attn", _vp), ("q_start", _vp), ("src_slot", _vp), ("dst_slot", _vp), ("bad_slot", _vp),
+        ("n_tok", _c_size), ("n_req", _c_size), ("h_k", _c_size), ("h_v", _c_size),
+        ("s", _c_size), ("n_slots", _c_size), ("q_stride", _c_size), ("k_stride", _c_size),
+        ("v_stride", _c_size), ("slot_stride", _c_size), ("max_new", _c_size),
+        ("workspace", _vp), ("workspace_bytes", _c_size),
+    ]
+
+
+class AttentionSharedArgs(ctypes.Structure):
+    """bh_attention_shared_args (include/bonsai_hip_batch.h)."""
+
+    _fields_ = [
+        ("paged", AttentionPagedArgs), ("group", _vp), ("group_start", _vp), ("shared_len", _vp),
+        ("n_group", _c_size), ("max_group_new", _c_size),
+    ]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """bh_beam_select_args (include/bonsai_hip_batch.h)."""
+
+    _fields_ = [
+        ("x", _vp), ("score", _vp), ("parent", _vp), ("token", _vp), ("score_out", _vp),
+        ("n_group", _c_size), ("width", _c_size), ("vocab", _c_size), ("row_stride", _c_size),
+        ("n_best", _c_size), ("inv_temp", _c_float), ("workspace", _vp),
+        ("workspace_bytes", _c_size),
+    ]
+
+
+class BeamReorderArgs(ctypes.Structure):
+    """bh_beam_reorder_args (include/bonsai_hip_batch.h)."""
+
+    _fields_ = [
+        ("parent", _vp), ("block_table", _vp), ("copy_from", _vp), ("src_slot", _vp),
+        ("dst_slot", _vp), ("spare_slot", _vp),
+        ("n_group", _c_size), ("width", _c_size), ("parent_stride", _c_size),
+        ("table_width", _c_size),
+    ]
+
+
+class KvCopyArgs(ctypes.Structure):
+    """bh_kv_copy_args (include/bonsai_hip_batch.h)."""
+
+    _fields_ = [
+        ("cache", PagedCache), ("block_table", _vp), ("copy_from", _vp), ("begin", _vp),
+        ("end", _vp), ("n_req", _c_size), ("table_width", _c_size),
+    ]
+
+
+_BATCH_SIGNATURES = {
+    "bh_conv1d_silu_ragged": (_c_int, [ctypes.POINTER(ConvRaggedArgs), _vp]),
+    "bh_gdn_ragged": (_c_int, [ctypes.POINTER(GdnRaggedArgs), _vp]),
+    "bh_gdn_ragged_workspace": (_c_size, [ctypes.POINTER(GdnRaggedArgs)]),
+    "bh_attention_shared": (_c_int, [ctypes.POINTER(AttentionSharedArgs), _vp]),
+    "bh_attention_shared_workspace": (_c_size, [ctypes.POINTER(AttentionSharedArgs)]),
+    "bh_beam_select": (_c_int, [ctypes.POINTER(BeamSelectArgs), _vp]),
+    "bh_beam_select_workspace": (_c_size, [ctypes.POINTER(BeamSelectArgs)]),
+    "bh_beam_reorder": (_c_int, [ctypes.POINTER(BeamReorderArgs), _vp]),
+    "bh_kv_copy_paged": (_c_int, [ctypes.POINTER(KvCopyArgs), _vp]),
+}
+
 _LIB = None
 
 
@@ -226,7 +305,7 @@ def lib() -> ctypes.CDLL:
     except ImportError:
         pass
     handle = ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_LOCAL)
-    for name, (res, args) in {**_SIGNATURES, **_SERVE_SIGNATURES}.items():
+    for name, (res, args) in {**_SIGNATURES, **_SERVE_SIGNATURES, **_BATCH_SIGNATURES}.items():
         fn = getattr(handle, name)
         fn.restype = res
         fn.argtypes = args
@@ -732,6 +811,252 @@ def token_logprobs(args: TokenLogprobsArgs, stream=None):
     """(logprob, entropy, top_ids, top_logprobs) of each row of logits."""
     _call(lib().bh_token_logprobs, args, stream)
     return args.results
+
+
+# ---------------------------------------------------------------------------
+# recurrent layers of many requests, and beam search (include/bonsai_hip_batch.h)
+# ---------------------------------------------------------------------------
+
+BH_MAX_BEAMS = 32
+
+
+def _rows_of(t, name: str, device, shape):
+    """t, checked: float32 rows of whole `shape[1:]` blocks, any stride apart; the stride."""
+    import torch
+    if t.dtype != torch.float32 or not t.is_cuda or t.get_device() != device.index:
+        raise ValueError(f"{name} must be a float32 tensor on {device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    inner = 1
+    for n, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n > 1 and stride != inner:
+            raise ValueError(f"what lies within a row of {name} must be contiguous")
+        inner *= n
+    if t.shape[0] > 1 and t.stride(0) < inner:
+        raise ValueError(f"rows of {name} must not overlap")
+    return t.stride(0) if t.shape[0] > 1 else inner
+
+
+def _step_of(q_start, src_slot, dst_slot, bad_slot, dev):
+    """Checks what names a ragged step's requests; their number."""
+    i32 = (_ids_dtypes()[0],)
+    n_req = src_slot.numel()
+    _dev_tensor(q_start, "q_start", i32, dev, (n_req + 1,))
+    _dev_tensor(src_slot, "src_slot", i32, dev, (n_req,))
+    _dev_tensor(dst_slot, "dst_slot", i32, dev, (n_req,))
+    if bad_slot is not None:
+        _dev_tensor(bad_slot, "bad_slot", i32, dev)
+    return n_req
+
+
+def make_conv_ragged_args(x, w, state, q_start, src_slot, dst_slot, out=None, l2_dim: int = 0,
+                          head_dim: int = 0, eps: float = EPS, max_new: int = 0,
+                          bad_slot=None) -> ConvRaggedArgs:
+    """Inputs x [n_tok, ch] f32 (rows any stride apart) of the requests whose tokens
+    begin at q_start int32 [n_req + 1], taps w [ch, k], the pool state
+    [n_slots, ch, k - 1] (slots any stride apart), slots int32 [n_req].  The result
+    is args.out_tensor (if out is None, zeros made on the current stream)."""
+    import torch
+    dev, f32 = x.device, (torch.float32,)
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError("x must be [n_tok, ch] and w [ch, k]")
+    n_tok, ch = x.shape
+    k = w.shape[1]
+    x_stride = _rows_of(x, "x", dev, x.shape)
+    _dev_tensor(w, "w", f32, dev, (ch, k))
+    if state is None and k > 1:
+        raise ValueError("state must be [n_slots, ch, k - 1]")
+    n_slots = 0 if state is None else state.shape[0]
+    slot_stride = 0 if state is None else _rows_of(state, "state", dev, (n_slots, ch, k - 1))
+    n_req = _step_of(q_start, src_slot, dst_slot, bad_slot, dev)
+    out = torch.zeros((n_tok, ch), dtype=torch.float32, device=dev) if out is None else out
+    _dev_tensor(out, "out", f32, dev, (n_tok, ch))
+    args = ConvRaggedArgs(_ptr(x), _ptr(w), _ptr(state), _ptr(out), _ptr(q_start), _ptr(src_slot),
+                          _ptr(dst_slot), _ptr(bad_slot), n_tok, n_req, ch, k, l2_dim, head_dim,
+                          n_slots, x_stride, slot_stride, max_new, eps)
+    args.out_tensor = out
+    return _hold(args, dev, x, w, state, out, q_start, src_slot, dst_slot, bad_slot)
+
+
+def conv1d_silu_ragged(args: ConvRaggedArgs, stream=None):
+    """conv1d_silu (and L2 norms) of many requests at once, states in slots; returns
+    the output tensor of the arguments."""
+    _call(lib().bh_conv1d_silu_ragged, args, stream)
+    return args.out_tensor
+
+
+def make_gdn_ragged_args(q, k, v, gate, beta, state, q_start, src_slot, dst_slot, attn=None,
+                         max_new: int = 0, bad_slot=None, workspace=None) -> GdnRaggedArgs:
+    """q, k [n_tok, h_k, s], v [n_tok, h_v, s] f32 (tokens any stride apart, so that
+    they may be parts of one row), gate, beta [n_tok, h_v], the pool state
+    [n_slots, h_v, s, s] (slots any stride apart), int32 q_start [n_req + 1] and slots
+    [n_req].  The result is args.attn_tensor (if attn is None, zeros made on the
+    current stream)."""
+    import torch
+    dev, f32 = q.device, (torch.float32,)
+    if q.dim() != 3 or v.dim() != 3 or state.dim() != 4:
+        raise ValueError("q, k, v must be [n_tok, heads, s] and state [n_slots, h_v, s, s]")
+    n_tok, h_k, s = q.shape
+    h_v, n_slots = v.shape[1], state.shape[0]
+    strides = [_rows_of(q, "q", dev, (n_tok, h_k, s)), _rows_of(k, "k", dev, (n_tok, h_k, s)),
+               _rows_of(v, "v", dev, (n_tok, h_v, s)),
+               _rows_of(state, "state", dev, (n_slots, h_v, s, s))]
+    _dev_tensor(gate, "gate", f32, dev, (n_tok, h_v))
+    _dev_tensor(beta, "beta", f32, dev, (n_tok, h_v))
+    n_req = _step_of(q_start, src_slot, dst_slot, bad_slot, dev)
+    attn = torch.zeros((n_tok, h_v, s), dtype=torch.float32, device=dev) if attn is None else attn
+    _dev_tensor(attn, "attn", f32, dev, (n_tok, h_v, s))
+    args = GdnRaggedArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(gate), _ptr(beta), _ptr(state),
+                         _ptr(attn), _ptr(q_start), _ptr(src_slot), _ptr(dst_slot),
+                         _ptr(bad_slot), n_tok, n_req, h_k, h_v, s, n_slots, *strides, max_new,
+                         None, 0)
+    if workspace is not None:
+        _dev_tensor(workspace, "workspace", (torch.uint8,), dev)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    args.attn_tensor = attn
+    return _hold(args, dev, q, k, v, gate, beta, state, attn, q_start, src_slot, dst_slot,
+                 bad_slot, workspace)
+
+
+def gdn_ragged_workspace(args: GdnRaggedArgs) -> int:
+    """Bytes of workspace of gdn_ragged(args) on the args' device."""
+    import torch
+    with torch.cuda.device(args.device):
+        return int(lib().bh_gdn_ragged_workspace(ctypes.byref(args)))
+
+
+def gdn_ragged(args: GdnRaggedArgs, stream=None):
+    """gdn_step of many requests at once, states in slots; returns the attn tensor of
+    the arguments."""
+    _call(lib().bh_gdn_ragged, args, stream)
+    return args.attn_tensor
+
+
+def make_attention_shared_args(cache: PagedCache, q, q_start, kv_len, block_table, group,
+                               group_start, shared_len, out=None, max_new: int = 0,
+                               max_group_new: int = 0, bad_page=None,
+                               workspace=None) -> AttentionSharedArgs:
+    """make_attention_paged_args, and the groups that share a prefix: group int32
+    [n_req], group_start int32 [n_group + 1], shared_len int32 [n_group]."""
+    paged = make_attention_paged_args(cache, q, q_start, kv_len, block_table, out, max_new,
+                                      bad_page, workspace)
+    i32, dev, n_group = (_ids_dtypes()[0],), paged.device, shared_len.numel()
+    _dev_tensor(group, "group", i32, dev, (paged.n_req,))
+    _dev_tensor(group_start, "group_start", i32, dev, (n_group + 1,))
+    _dev_tensor(shared_len, "shared_len", i32, dev, (n_group,))
+    args = AttentionSharedArgs(paged, _ptr(group), _ptr(group_start), _ptr(shared_len), n_group,
+                               max_group_new)
+    args.out_tensor = paged.out_tensor
+    return _hold(args, dev, paged.tensors, group, group_start, shared_len)
+
+
+def attention_shared_workspace(args: AttentionSharedArgs) -> int:
+    """Bytes of workspace of attention_shared(args) on the args' device."""
+    import torch
+    with torch.cuda.device(args.device):
+        return int(lib().bh_attention_shared_workspace(ctypes.byref(args)))
+
+
+def attention_shared(args: AttentionSharedArgs, stream=None):
+    """attention_paged of requests that share a prefix, which is read once for all of
+    a group; returns the output tensor of the arguments."""
+    _call(lib().bh_attention_shared, args, stream)
+    return args.out_tensor
+
+
+def make_beam_select_args(x, score, width: int, n_best: int, inv_temp: float = 1.0, *,
+                          parent=None, token=None, score_out=None,
+                          workspace=None) -> BeamSelectArgs:
+    """Logits x [n_group * width, vocab] f32 (rows any stride apart) and the beams'
+    scores f32 [n_group * width].  Outputs that are None are made; args.results holds
+    (parent, token, score_out), [n_group, n_best] each."""
+    import torch
+    dev, f32, ids = x.device, (torch.float32,), _ids_dtypes()
+    if x.dim() != 2 or width < 1 or x.shape[0] % width != 0:
+        raise ValueError("x must be [n_group * width, vocab]")
+    stride = _rows_of(x, "x", dev, x.shape)
+    _dev_tensor(score, "score", f32, dev, (x.shape[0],))
+    shape = (x.shape[0] // width, n_best)
+    parent = torch.empty(shape, dtype=torch.int32, device=dev) if parent is None \
+        else _dev_tensor(parent, "parent", ids[:1], dev, shape)
+    token = torch.empty(shape, dtype=torch.int32, device=dev) if token is None \
+        else _dev_tensor(token, "token", ids, dev, shape)
+    if score_out is None:
+        score_out = torch.empty(shape, dtype=torch.float32, device=dev)
+    elif score_out.data_ptr() != score.data_ptr():  # the scores in place are a vector
+        _dev_tensor(score_out, "score_out", f32, dev, shape)
+    elif score_out.numel() != shape[0] * n_best:
+        raise ValueError("score_out may be score only where n_best is width")
+    args = BeamSelectArgs(_ptr(x), _ptr(score), _ptr(parent), _ptr(token), _ptr(score_out),
+                          shape[0], width, x.shape[1], stride, n_best, inv_temp, None, 0)
+    if workspace is not None:
+        _dev_tensor(workspace, "workspace", (torch.uint8,), dev)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    args.results = (parent, token, score_out)
+    return _hold(args, dev, x, score, parent, token, score_out, workspace)
+
+
+def beam_select_workspace(args: BeamSelectArgs) -> int:
+    """Bytes of workspace of beam_select(args) on the args' device."""
+    import torch
+    with torch.cuda.device(args.device):
+        return int(lib().bh_beam_select_workspace(ctypes.byref(args)))
+
+
+def beam_select(args: BeamSelectArgs, stream=None):
+    """(parent, token, score) of each group's best continuations."""
+    _call(lib().bh_beam_select, args, stream)
+    return args.results
+
+
+def make_beam_reorder_args(parent, block_table, *, copy_from, src_slot=None, dst_slot=None,
+                           spare_slot=None) -> BeamReorderArgs:
+    """int32 tensors: parent [n_group, width] (rows any stride apart, as a slice of
+    beam_select's), block_table [n_group * width, table_width] and copy_from, src_slot,
+    dst_slot, spare_slot [n_group * width]."""
+    i32, dev = (_ids_dtypes()[0],), parent.device
+    if parent.dim() != 2 or block_table.dim() != 2:
+        raise ValueError("parent must be [n_group, width] and block_table a matrix")
+    n_group, width = parent.shape
+    stride = parent.stride(0) if n_group > 1 else width
+    if parent.dtype != i32[0] or not parent.is_cuda or (width > 1 and parent.stride(1) != 1) \
+            or stride < width:
+        raise ValueError("parent must be an int32 CUDA tensor of contiguous rows")
+    _dev_tensor(block_table, "block_table", i32, dev, (n_group * width, block_table.shape[1]))
+    for name, t in (("copy_from", copy_from), ("src_slot", src_slot), ("dst_slot", dst_slot),
+                    ("spare_slot", spare_slot)):
+        if t is not None:
+            _dev_tensor(t, name, i32, dev, (n_group * width,))
+    return _hold(BeamReorderArgs(_ptr(parent), _ptr(block_table), _ptr(copy_from),
+                                 _ptr(src_slot), _ptr(dst_slot), _ptr(spare_slot), n_group, width,
+                                 stride, block_table.shape[1]),
+                 dev, parent, block_table, copy_from, src_slot, dst_slot, spare_slot)
+
+
+def beam_reorder(args: BeamReorderArgs, stream=None) -> None:
+    """The beams' page tables and state slots in the order of the beams selected."""
+    _call(lib().bh_beam_reorder, args, stream)
+
+
+def make_kv_copy_args(cache: PagedCache, block_table, copy_from, begin, end) -> KvCopyArgs:
+    """int32 tensors: block_table [n_req, table_width], copy_from, begin (or None), end
+    [n_req]."""
+    i32, dev, n_req = (_ids_dtypes()[0],), cache.device, copy_from.numel()
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [n_req, table_width]")
+    _dev_tensor(block_table, "block_table", i32, dev, (n_req, block_table.shape[1]))
+    _dev_tensor(copy_from, "copy_from", i32, dev)
+    _dev_tensor(end, "end", i32, dev, (n_req,))
+    if begin is not None:
+        _dev_tensor(begin, "begin", i32, dev, (n_req,))
+    return _hold(KvCopyArgs(cache, _ptr(block_table), _ptr(copy_from), _ptr(begin), _ptr(end),
+                            n_req, block_table.shape[1]),
+                 dev, cache.tensors, block_table, copy_from, begin, end)
+
+
+def kv_copy_paged(args: KvCopyArgs, stream=None) -> None:
+    """The pages of one layer's cache of requests that go on from another's."""
+    _call(lib().bh_kv_copy_paged, args, stream)
 
 
 def env_info() -> dict:

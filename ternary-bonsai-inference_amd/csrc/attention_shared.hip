@@ -1,0 +1,242 @@
+// Attention of requests that share a prefix: the prefix's keys and values are read
+// once for the rows of all requests of a group.
+//
+// With o, m and l of a set of positions P the sums of a softmax over it (m the
+// largest score, l = sum e^(s - m), o = sum e^(s - m) v), those of two sets join as
+//   m' = max(m1, m2),  l' = e^(m1 - m') l1 + e^(m2 - m') l2,  o' likewise.
+// So a group's prefix is one more request of the walk (paged_attention.hpp), whose
+// tokens are those of all the group's requests and see all of it, and a request's own
+// walk begins where its prefix ends.  Both stand in one list that is cut into equal
+// runs, so that a long prefix and many short tails fill the card together; the join
+// takes each row's parts from its own tile and from its tile of the prefix.
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "../../include/bonsai_hip_batch.h"
+#include "common.hpp"
+#include "paged.hpp"
+#include "paged_attention.hpp"
+
+namespace bh {
+namespace {
+
+// The tiles of a group's prefix: which launch has them and where they begin there.
+struct Prefix {
+  int q0 = 0, n = 0, base = 0, tiles = 0;
+  uint32_t rows = 1, most = 0;  // of a tile; tiles of the launch
+  bool two = false;
+};
+
+// A row's tile of the prefix: its parts' first place and number (0: none), and the
+// row's number in it.
+struct At {
+  int slot = 0, parts = 0, row = 0;
+};
+
+template <int HD>
+__global__ __launch_bounds__(kThreads) void attn_shared_join_kernel(PagedArgs a, Join one, Join two) {
+  constexpr int kAt = kThreads / 16, kSlices = HD / 64, kAhead = 8;
+  __shared__ float part[kAt][64], sums[kAt], tops[kAt];
+  const bool of_two = blockIdx.x >= one.blocks;
+  const unsigned block = blockIdx.x - (of_two ? one.blocks : 0);
+  const Split sp = of_two ? two.sp : one.sp;
+  const int share = of_two ? two.share : one.share, R = of_two ? two.rows : one.rows;
+  const int tile = block / share, tid = threadIdx.x;
+  const SharedCut cut = static_cast<const SharedCut *>(sp.cut)[tile];
+  // (past n_tiles cut holds nothing; a prefix's tiles have no rows of their own)
+  if (tile >= *sp.n_tiles || cut.r < a.n_group) return;
+  int q0, n, len, g;
+  request(a, cut.r - a.n_group, &q0, &n, &len);
+  Prefix pre;
+  if (shared_of(a, cut.r - a.n_group, n, len, &g) > 0) {
+    group_tokens(a, g, &pre.q0, &pre.n);
+    const int64_t rows = static_cast<int64_t>(pre.n) * a.group;
+    pre.two = rows <= one.sp.over || rows > one.sp.most;
+    const Split &of = pre.two ? two.sp : one.sp;
+    pre.rows = pre.two ? two.rows : one.rows;
+    pre.tiles = static_cast<int>((rows + pre.rows - 1) / pre.rows);
+    pre.base = of.base[g];
+    pre.most = min(static_cast<uint32_t>(*of.n_tiles), of.most_cut);
+  }
+  const Split psp = pre.two ? two.sp : one.sp;
+  const auto prefix_of = [&](int row) {  // of the tile
+    At at;
+    if (pre.n == 0) return at;
+    const int q_row = cut.row0 + row, tok = a.grp.div(q_row), t = cut.q0 + tok - pre.q0;
+    if (t < 0 || t >= pre.n) return at;
+    const uint32_t p_row = static_cast<uint32_t>(t * a.group + (q_row - tok * a.group));
+    const uint32_t i = static_cast<uint32_t>(pre.base + cut.head * pre.tiles) + p_row / pre.rows;
+    if (i >= pre.most) return at;
+    const SharedCut &c = static_cast<const SharedCut *>(psp.cut)[i];
+    at.row = static_cast<int>(p_row % pre.rows);
+    at.slot = c.tile + c.first;
+    at.parts = c.last - c.first + 1;
+    return at;
+  };
+  const int own = cut.last - cut.first + 1, own_slot = cut.tile + cut.first;
+  // groups of 16 lanes that share a row, the same number for the block
+  const int most = own + max(prefix_of(0).parts, prefix_of(cut.rows - 1).parts);
+  int p = 1;
+  while (kAhead * p < most && p < kAt) p <<= 1;
+  const int group = tid >> 4, mine = group & (p - 1), d = (tid & 15) * 4;
+  const int items = cut.rows * kSlices, at_once = kAt / p;
+  for (int i0 = (block - tile * share) * at_once; i0 < items; i0 += share * at_once) {
+    const int item = i0 + group / p;
+    const bool live = item < items;
+    const int row = live ? item / kSlices : 0, dim = item % kSlices * 64 + d;
+    const At pr = prefix_of(row);
+    const int parts = own + pr.parts;
+    struct Place {
+      const float *m, *l, *o;
+    };
+    const auto at = [&](int x) {
+      const bool is_own = x < own;
+      const Split &of = is_own ? sp : psp;
+      const size_t o = is_own ? static_cast<size_t>(own_slot + x) * R + row
+                              : static_cast<size_t>(pr.slot + x - own) * pre.rows + pr.row;
+      return Place{of.pm + o, of.pl + o, of.pacc + o * HD + dim};
+    };
+    f32x4 ahead[kAhead];
+    float pm[kAhead], pl[kAhead];
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      // past the last part: the last again, at no weight
+      if (x * p >= most) break;
+      const Place w = at(min(mine + x * p, parts - 1));
+      ahead[x] = *reinterpret_cast<const f32x4 *>(w.o);
+      pm[x] = *w.m;
+      pl[x] = *w.l;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      if (x * p >= most) break;
+      top = fmaxf(top, pm[x]);
+    }
+    for (int x = mine + kAhead * p; x < parts; x += p) top = fmaxf(top, *at(x).m);
+    if (p > 1) {
+      if (d == 0) tops[group] = top;
+      __syncthreads();
+      for (int k = 0; k < p; ++k) top = fmaxf(top, tops[(group - mine) + k]);
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    f32x4 o = {0, 0, 0, 0};
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      if (x * p >= most) break;
+      if (mine + x * p >= parts) continue;
+      const float keep = __builtin_amdgcn_exp2f(pm[x] - ref);
+      sum += keep * pl[x];
+      o += keep * ahead[x];
+    }
+#pragma unroll 4
+    for (int x = mine + kAhead * p; x < parts; x += p) {
+      const Place w = at(x);
+      const float keep = __builtin_amdgcn_exp2f(*w.m - ref);
+      sum += keep * *w.l;
+      o += keep * *reinterpret_cast<const f32x4 *>(w.o);
+    }
+    if (p > 1) {
+      *reinterpret_cast<f32x4 *>(&part[group][d]) = o;
+      if (d == 0) sums[group] = sum;
+      __syncthreads();
+    }
+    if (mine == 0 && live) {
+      for (int k = 1; k < p; ++k) {
+        o += *reinterpret_cast<const f32x4 *>(&part[group + k][d]);
+        sum += sums[group + k];
+      }
+      const int q_row = cut.row0 + row, tok = a.grp.div(q_row);
+      *reinterpret_cast<f32x4 *>(
+          a.out + (static_cast<size_t>(cut.q0 + tok) * a.n_head + cut.head * a.group +
+                   (q_row - tok * a.group)) * HD + dim) = o * (top == -INFINITY ? 0.0f : 1.0f / sum);
+    }
+    if (p > 1) __syncthreads();  // for the next rows
+  }
+}
+
+int launch_shared_join(const PagedArgs &a, const Join &one, const Join &two, hipStream_t st) {
+  const unsigned blocks = one.blocks + two.blocks;
+  if (a.hd == 64) BH_LAUNCH(attn_shared_join_kernel<64>, blocks, kThreads, 0, st, a, one, two);
+  else if (a.hd == 128) BH_LAUNCH(attn_shared_join_kernel<128>, blocks, kThreads, 0, st, a, one, two);
+  else BH_LAUNCH(attn_shared_join_kernel<256>, blocks, kThreads, 0, st, a, one, two);
+  return BH_OK;
+}
+
+// As forms_of, the prefix of a group being a request of all the group's rows.
+int shared_forms(const bh_attention_shared_args &p, Form *f) {
+  bh_attention_paged_args q = p.paged;
+  const size_t own = q.max_new == 0 || q.max_new > q.n_tok ? q.n_tok : q.max_new;
+  const size_t all = p.max_group_new == 0 || p.max_group_new > q.n_tok ? q.n_tok : p.max_group_new;
+  q.max_new = all > own ? all : own;
+  q.n_req = 2;  // not one request's: both sorts are there
+  return forms_of(q, f);
+}
+
+int prepare_shared(const bh_attention_shared_args &p, PagedArgs *a) {
+  if (int e = prepare(p.paged, a, "attention_shared")) return e;
+  if (p.n_group > 0x7fff0000u || p.paged.n_req + p.n_group > 0x7fff0000u)
+    return fail(BH_ERR_SHAPE, "attention_shared: size overflow");
+  if (p.n_group != 0 && p.paged.n_tok != 0 && p.paged.n_req != 0 &&
+      (!p.group || !p.group_start || !p.shared_len))
+    return fail(BH_ERR_ARG, "attention_shared: null pointer");
+  a->group_of = p.group, a->group_start = p.group_start, a->shared_len = p.shared_len;
+  a->n_group = static_cast<int>(p.n_group);
+  return BH_OK;
+}
+
+}  // namespace
+}  // namespace bh
+
+using namespace bh;
+
+extern "C" size_t bh_attention_shared_workspace(const bh_attention_shared_args *args) {
+  PagedArgs a{};
+  if (!args || prepare_shared(*args, &a) != BH_OK) return 0;
+  if (a.n_group == 0 || !on_matrix_cores(args->paged))
+    return bh_attention_paged_workspace(&args->paged);
+  if (a.n_tok == 0 || a.n_req == 0) return 0;
+  Form f[2];
+  size_t need = 0;
+  for (int i = 0, n = shared_forms(*args, f); i < n; ++i) need += workspace_of<true>(a, f[i]);
+  return need;
+}
+
+extern "C" int bh_attention_shared(const bh_attention_shared_args *args, bh_stream stream) {
+  if (!args) return fail(BH_ERR_ARG, "attention_shared: null args");
+  const bh_attention_shared_args &p = *args;
+  PagedArgs a{};
+  if (int e = prepare_shared(p, &a)) return e;
+  if (a.n_tok == 0 || a.n_req == 0) return ok();
+  if (a.n_group == 0 || !on_matrix_cores(p.paged)) return bh_attention_paged(&p.paged, stream);
+  const bool f16 = p.paged.cache.kv_dtype == BH_KV_F16;
+  hipStream_t st = as_stream(stream);
+  Form f[2];
+  const int n = shared_forms(p, f);
+  size_t need = 0, tiles = 0;
+  for (int i = 0; i < n; ++i) {
+    need += workspace_of<true>(a, f[i]);
+    tiles += most_tiles<true>(a, f[i]);
+  }
+  if (tiles > kMostBlocks)  // (the join has more than a block a tile only of few)
+    return fail(BH_ERR_SHAPE, "attention_shared: more row tiles than a launch has blocks");
+  char *ws = static_cast<char *>(p.paged.workspace);
+  if (ws) {
+    if (!aligned16(ws) || p.paged.workspace_bytes < need)
+      return fail(BH_ERR_SHAPE, "attention_shared: workspace of " +
+                                    std::to_string(p.paged.workspace_bytes) + " bytes, " +
+                                    std::to_string(need) + " needed on a 16-byte boundary");
+  } else {
+    ws = static_cast<char *>(device_scratch(need, kScratchPaged, st));
+    if (!ws) return BH_ERR_HIP;
+  }
+  Join join[2] = {};
+  for (int i = 0; i < n; ++i) {
+    if (int e = launch_form<true>(a, f16, f[i], ws, st, &join[i])) return e;
+    ws += workspace_of<true>(a, f[i]);
+  }
+  if (int e = launch_shared_join(a, join[0], join[1], st)) return e;
+  return ok();
+}
