@@ -28,6 +28,7 @@ struct GdnArgs {
   size_t q_stride, k_stride, v_stride;
   int h_k, h_v, s;
   float scale;
+  int most;  // requests of more tokens are another launch's
   Ragged rag;
 };
 
@@ -43,7 +44,7 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_step_kernel(GdnArgs a) {
   const int sub = threadIdx.x % L, j = (rest - h * kTiles) * kRows + threadIdx.x / L * RPG;
   int t0, n, from, to;
   a.rag.tokens(r, &t0, &n);
-  if (n == 0) return;
+  if (n == 0 || n > a.most) return;
   a.rag.slots(r, &from, &to);
   const size_t row = (static_cast<size_t>(h) * S + j) * S + 4 * sub;
   f32x4 m[RPG][2];
@@ -166,6 +167,584 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_any_kernel(GdnArgs a) {
   }
 }
 
+// ---- prompts: chunks of 64 tokens on the matrix cores (s = 128) ----------------
+//
+// Over a chunk with decays a_t = e^gate_t, A_t = a_0 .. a_t, D_ts = A_t / A_s and a
+// state row m at its beginning, the tokens' steps unroll to
+//   delta = T (v - A (K m)),  T = (I + L)^-1 diag(beta),  L_ts = beta_t D_ts (k_t.k_s), s < t,
+//   attn = (A (Q m) + P delta) / sqrt(s),                 P_ts = D_ts (q_t.k_s), s <= t,
+//   m' = A_63 m + sum_s e_s delta_s k_s,                  e_s = A_63 / A_s,
+// where T, P, A and e are those of a (chunk, v-head), whatever the row.
+// gdn_chunk_prep_kernel forms them, all chunks at once; gdn_chunk_walk_kernel takes
+// 32 rows of a state through their chunks.
+//
+// Products are of f16 matrix instructions, each operand as hi + lo halves of 22 bits
+// (hi hi + hi lo + lo hi, a third of the f32 instruction's time) in units of a power
+// of two that brings the largest of what shares a unit to 2^14 .. 2^15: a token's row
+// of K and of Q, a row of T and of P; of the operands that carry state rows, a row j
+// and the 32 dims or the 16 tokens of one wave, whose products are summed apart.  An
+// operand's error is 2^-22 of the largest beside it, as that of a few f32 sums.
+//
+// Operands stand in memory as the instructions take them.  In 16x16x32 lane (lr =
+// lane % 16, lg = lane / 16) holds row lr and the 8 of the 32 summed over that are
+// 4 lg + i and 16 + 4 lg + i, i < 4; in 16x16x16 the 4 that are 4 lg + i.  Those are
+// the places that a result's lane holds of its column, so results become operands as
+// they stand.
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+constexpr int kCk = 64, kCkS = 128;
+constexpr int kCkMin = 128;           // tokens from which a request goes by chunks
+constexpr int kCkRows = 32;           // state rows of a walk
+constexpr int kFragK = kCk * kCkS * 4;           // bytes of K as halves; Q, K transposed
+constexpr int kHeadK = 3 * kFragK;               // of a (chunk, q/k head)
+constexpr int kFragT = 10 * 64 * 16;             // of T's and P's lower 16 x 16 tiles
+constexpr int kVecs = 5 * kCk + kCk;             // floats: A k, A q, T's, P's units, e k; A_63
+constexpr int kHeadV = 2 * kFragT + kVecs * 4;   // of a (chunk, v-head)
+constexpr float kGateFloor = -200.0f;            // e^x below this is 0 in f32
+constexpr int kPitch = 68;                       // floats of a row of a 64 x 64 matrix in LDS
+constexpr int kVWaves = 3;                       // v-heads prepared side by side
+
+struct GdnChunkArgs {
+  GdnArgs g;
+  char *ws;    // [slots][h_k kHeadK + h_v kHeadV]
+  int slots;   // of chunks
+  int n_long;  // requests of kCkMin tokens or more there can be
+  int xcd;     // the blocks of a q/k head on one die
+};
+
+// Where request r's chunks begin: n >= 128 tokens have ceil(n / 64) <= 3 n / 128.
+__device__ __forceinline__ int first_chunk(int begin) {
+  return static_cast<int>(static_cast<int64_t>(begin) * 3 / 128);
+}
+
+// The unit of values of which `most` is the largest: x up is its number of units.
+__device__ __forceinline__ void unit_of(float most, float *up, float *down) {
+  int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+  *up = *down = 1.0f;
+  if (ex > -127 && ex < 128) {
+    ex = max(ex, -100);
+    *up = __uint_as_float(static_cast<uint32_t>(141 - ex) << 23);
+    *down = __uint_as_float(static_cast<uint32_t>(113 + ex) << 23);
+  }
+}
+__device__ __forceinline__ float most_of(f32x4 x) {
+  return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+}
+// Over lanes lr, lr + 16, lr + 32, lr + 48.
+__device__ __forceinline__ float most_of_lanes(float x) {
+  float lo, hi;
+  lane_swap<16>(x, lo, hi);
+  x = fmaxf(lo, hi);
+  lane_swap<32>(x, lo, hi);
+  return fmaxf(lo, hi);
+}
+__device__ __forceinline__ void halves(f32x4 x, h4 *hi, h4 *lo) {
+  *hi = __builtin_convertvector(x, h4);
+  *lo = __builtin_convertvector(x - __builtin_convertvector(*hi, f32x4), h4);
+}
+__device__ __forceinline__ h8 both(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ h4 low(h8 a) { return __builtin_shufflevector(a, a, 0, 1, 2, 3); }
+__device__ __forceinline__ h4 high(h8 a) { return __builtin_shufflevector(a, a, 4, 5, 6, 7); }
+
+__device__ __forceinline__ f32x4 mma32(h8 ah, h8 al, h8 bh, h8 bl, f32x4 c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, c, 0, 0, 0);
+}
+// Operands hi | lo.
+__device__ __forceinline__ f32x4 mma16(h8 a, h8 b, f32x4 c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x16f16(high(a), low(b), c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x16f16(low(a), high(b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(low(a), low(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+// Orders the wave's LDS writes before its reads (the wave runs in step).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+constexpr int kTri[4] = {0, 1, 3, 6};  // tiles of a lower triangle before row i
+
+// What a wave forms for a v-head: `kq` holds Q K^T on and below the diagonal and K K^T,
+// transposed, above it; `l` is the wave's own matrix.  down: the units of K's and Q's rows.
+__device__ __forceinline__ void prep_head(const GdnArgs &a, int h, int t0, int nt, const float *kq,
+                                          float *l, double *G_s, float *w_s, float *b_s,
+                                          const float *k_down, const float *q_down, char *out) {
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  // decays: lane t = token t
+  float g = 0.0f, beta = 0.0f;
+  if (lane < nt) {
+    const size_t at = static_cast<size_t>(t0 + lane) * a.h_v + h;
+    g = a.gate[at], beta = a.beta[at];
+  }
+  g = g < kGateFloor ? kGateFloor : g;  // -inf too (a NaN stays)
+  double G = g;
+#pragma unroll
+  for (int d = 1; d < kCk; d <<= 1) {
+    const double o = __shfl_up(G, d, kCk);
+    if (lane >= d) G += o;
+  }
+  G_s[lane] = G;
+  b_s[lane] = beta;
+  const double last = __shfl(G, kCk - 1);
+  const double end = __shfl(G, lane | 15);  // of the lane's tile of 16 tokens
+  w_s[lane] = exp_hw(static_cast<float>(end - G));
+  const float decay = expf(static_cast<float>(G)), left = expf(static_cast<float>(last - G));
+  float *vec = reinterpret_cast<float *>(out + 2 * kFragT);
+  vec[lane] = decay * k_down[lane];
+  vec[kCk + lane] = decay * q_down[lane];
+  vec[4 * kCk + lane] = left * k_down[lane];
+  if (lane == kCk - 1) vec[5 * kCk] = decay;
+  wave_sync();
+  // P in its order, L into `l`: a tile's D_ts below the diagonal is e^(G_t - G_r)
+  // e^(G_r - G_s), r the last token of s's tile: neither factor passes 1
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 16 * i + lr;
+    const double Gt = G_s[t];
+    const float bt = b_s[t];
+    f32x4 p[4];
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+      const int s = 16 * j + 4 * lg;
+      const f32x4 q = *reinterpret_cast<const f32x4 *>(kq + t * kPitch + s);
+      f32x4 d, lv;
+      if (j < i) {
+        const float u = exp_hw(static_cast<float>(Gt - G_s[16 * j + 15]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = u * w_s[s + e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float arg = static_cast<float>(Gt - G_s[s + e]);
+          d[e] = s + e <= t ? exp_hw(arg < 0.0f ? arg : 0.0f) : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = j < i || s + e <= t, under = j < i || s + e < t;
+        p[j][e] = in ? d[e] * q[e] : 0.0f;
+        lv[e] = under ? bt * d[e] * kq[(s + e) * kPitch + t] : 0.0f;
+      }
+      most = fmaxf(most, most_of(p[j]));
+      *reinterpret_cast<f32x4 *>(l + t * kPitch + s) = lv;
+    }
+    float up, down;
+    unit_of(most_of_lanes(most), &up, &down);
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+      h4 hi, lo;
+      halves(p[j] * up, &hi, &lo);
+      *reinterpret_cast<h8 *>(out + kFragT + ((kTri[i] + j) * 64 + lane) * 16) = both(hi, lo);
+    }
+    if (lg == 0) vec[3 * kCk + t] = down;
+  }
+  wave_sync();
+  // (I + L)^-1: its diagonal blocks by substitution, lane (lr, lg) column lr of block lg
+  float x[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    f32x4 row[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (4 * c < r) row[c] = *reinterpret_cast<const f32x4 *>(l + (16 * lg + r) * kPitch + 16 * lg + 4 * c);
+    float v = r == lr ? 1.0f : 0.0f;
+#pragma unroll
+    for (int c = 0; c < r; ++c) v = fmaf(-row[c / 4][c % 4], x[c], v);
+    x[r] = v;
+  }
+  wave_sync();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) l[(16 * lg + r) * kPitch + 16 * lg + lr] = x[r];
+  wave_sync();
+  // the blocks below by their distance: T_ij = -T_ii sum_(j <= m < i) L_im T_mj.  The k
+  // index of step e in lane lg is 4 lg + e, which is what a result's lane holds.
+  f32x4 inv[4][4], diag[4];  // results' lanes: row 4 lg + e, column lr; rows of T_ii
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    diag[i] = *reinterpret_cast<const f32x4 *>(l + (16 * i + lr) * kPitch + 16 * i + 4 * lg);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) inv[i][i][e] = l[(16 * i + 4 * lg + e) * kPitch + 16 * i + lr];
+  }
+#pragma unroll
+  for (int dist = 1; dist < 4; ++dist)
+#pragma unroll
+    for (int j = 0; j + dist < 4; ++j) {
+      const int i = j + dist;
+      f32x4 sum = {0, 0, 0, 0}, t = {0, 0, 0, 0};
+#pragma unroll
+      for (int m = j; m < i; ++m) {
+        const f32x4 lm = *reinterpret_cast<const f32x4 *>(l + (16 * i + lr) * kPitch + 16 * m + 4 * lg);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = mma4(lm[e], inv[m][j][e], sum);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t = mma4(diag[i][e], sum[e], t);
+      inv[i][j] = -t;
+    }
+  wave_sync();
+  // T = (I + L)^-1 diag(beta), by rows through `l`
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j <= i; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        l[(16 * i + 4 * lg + e) * kPitch + 16 * j + lr] = inv[i][j][e] * b_s[16 * j + lr];
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f32x4 t[4];
+    float most = 0.0f, up, down;
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+      t[j] = *reinterpret_cast<const f32x4 *>(l + (16 * i + lr) * kPitch + 16 * j + 4 * lg);
+      most = fmaxf(most, most_of(t[j]));
+    }
+    unit_of(most_of_lanes(most), &up, &down);
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+      h4 hi, lo;
+      halves(t[j] * up, &hi, &lo);
+      *reinterpret_cast<h8 *>(out + ((kTri[i] + j) * 64 + lane) * 16) = both(hi, lo);
+    }
+    if (lg == 0) vec[2 * kCk + 16 * i + lr] = down;
+  }
+  wave_sync();
+}
+
+// Block (chunk, q/k head): wave w has the tokens 16 w .. 16 w + 15.
+__global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs c) {
+  constexpr int kMat = kCk * kPitch;
+  // K's halves; then the v-heads' matrices.  Behind them Q K^T and K K^T.
+  __shared__ __attribute__((aligned(16))) float lds[kVWaves * kMat + kMat];
+  static_assert(kVWaves * kMat * 4 >= kFragK, "K's halves fit");
+  __shared__ double G_s[kVWaves][kCk];
+  __shared__ float w_s[kVWaves][kCk], b_s[kVWaves][kCk], k_down[kCk], q_down[kCk];
+  const GdnArgs &a = c.g;
+  const int slot = blockIdx.x / a.h_k, kh = blockIdx.x - slot * a.h_k;
+  const int r = last_request(a.rag.n_req, [&](int i) {
+    return first_chunk(min(max(a.rag.q_start[i], 0), a.rag.n_tok)) <= slot;
+  });
+  if (r < 0) return;
+  int begin, n;
+  a.rag.tokens(r, &begin, &n);
+  const int at = (slot - first_chunk(begin)) * kCk;
+  if (n < kCkMin || at >= n) return;
+  const int t0 = begin + at, nt = min(kCk, n - at);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  char *of_slot = c.ws + static_cast<size_t>(slot) * (static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(a.h_v) * kHeadV);
+  char *out = of_slot + static_cast<size_t>(kh) * kHeadK;
+  float *kq = lds + kVWaves * kMat;
+  h8 *k_lds = reinterpret_cast<h8 *>(lds);
+
+  // K and Q of the wave's tokens as halves
+  h8 qh[4], ql[4], kh_[4], kl[4];
+  {
+    const int t = 16 * w + lr;
+    const bool in = t < nt;
+    const size_t row = static_cast<size_t>(t0 + (in ? t : 0));
+    const float *kp = a.k + row * a.k_stride + static_cast<size_t>(kh) * kCkS + 4 * lg;
+    const float *qp = a.q + row * a.q_stride + static_cast<size_t>(kh) * kCkS + 4 * lg;
+    f32x4 kv[8], qv[8];
+    float km = 0.0f, qm = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      kv[i] = in ? *reinterpret_cast<const f32x4 *>(kp + 16 * i) : f32x4{0, 0, 0, 0};
+      qv[i] = in ? *reinterpret_cast<const f32x4 *>(qp + 16 * i) : f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) km = fmaxf(km, most_of(kv[i])), qm = fmaxf(qm, most_of(qv[i]));
+    float ku, kd, qu, qd;
+    unit_of(most_of_lanes(km), &ku, &kd);
+    unit_of(most_of_lanes(qm), &qu, &qd);
+    if (lg == 0) k_down[t] = kd, q_down[t] = qd;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h4 h0, l0, h1, l1;
+      halves(kv[2 * i] * ku, &h0, &l0);
+      halves(kv[2 * i + 1] * ku, &h1, &l1);
+      kh_[i] = both(h0, h1), kl[i] = both(l0, l1);
+      halves(qv[2 * i] * qu, &h0, &l0);
+      halves(qv[2 * i + 1] * qu, &h1, &l1);
+      qh[i] = both(h0, h1), ql[i] = both(l0, l1);
+      const int f = (w * 4 + i) * 128 + lane;  // of 16 bytes: hi, and lo 64 places on
+      k_lds[f] = kh_[i], k_lds[f + 64] = kl[i];
+      h8 *ko = reinterpret_cast<h8 *>(out) + f, *qo = reinterpret_cast<h8 *>(out + kFragK) + f;
+      ko[0] = kh_[i], ko[64] = kl[i];
+      qo[0] = qh[i], qo[64] = ql[i];
+    }
+  }
+  __syncthreads();
+  // Q K^T and K K^T of the wave's tokens against those before: a row of one operand is a
+  // column of the other, in the same lanes
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j > w) continue;
+    f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const h8 bh = k_lds[(j * 4 + i) * 128 + lane], bl = k_lds[(j * 4 + i) * 128 + 64 + lane];
+      kk = mma32(kh_[i], kl[i], bh, bl, kk);
+      qk = mma32(qh[i], ql[i], bh, bl, qk);
+    }
+    const int s = 16 * j + lr;  // column
+    const float ds = k_down[s];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = 16 * w + 4 * lg + e;
+      if (s <= t) kq[t * kPitch + s] = qk[e] * q_down[t] * ds;
+      if (s < t) kq[s * kPitch + t] = kk[e] * k_down[t] * ds;
+    }
+  }
+  // K transposed: tile (d, t) of 16 dims and 16 tokens, lane's dim 16 d + lr
+  {
+    const _Float16 *halves_of = reinterpret_cast<const _Float16 *>(lds);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int d = 2 * w + (x >> 2), t = x & 3;  // wave w: dims 32 w .. 32 w + 31
+      const int dim = 16 * (d & 1) + lr;         // of 32
+      const int in = (dim >> 4) * 4 + (dim & 3), group = (dim >> 2) & 3;
+      h4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int f = ((t * 4 + (d >> 1)) * 128 + 4 * lg + e + 16 * group) * 8 + in;
+        hi[e] = halves_of[f], lo[e] = halves_of[f + 64 * 8];
+      }
+      *reinterpret_cast<h8 *>(out + 2 * kFragK + ((d * 4 + t) * 64 + lane) * 16) = both(hi, lo);
+    }
+  }
+  __syncthreads();
+  if (w >= kVWaves) return;  // (no barrier follows)
+  const int heads = (a.h_v - kh + a.h_k - 1) / a.h_k;  // v-heads kh + i h_k
+  for (int i = w; i < heads; i += kVWaves) {
+    const int h = kh + i * a.h_k;
+    prep_head(a, h, t0, nt, kq, lds + w * kMat, G_s[w], w_s[w], b_s[w], k_down, q_down,
+              of_slot + static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(h) * kHeadV);
+  }
+}
+
+// The nth request of kCkMin tokens or more; -1: there are not so many.
+__device__ __forceinline__ int nth_long(const Ragged &rag, int nth) {
+  const int lane = threadIdx.x & 63;
+  for (int i0 = 0; i0 < rag.n_req; i0 += 64) {
+    int begin, n = 0;
+    if (i0 + lane < rag.n_req) rag.tokens(i0 + lane, &begin, &n);
+    uint64_t is = __ballot(n >= kCkMin);
+    const int here = __popcll(is);
+    if (nth < here) {
+      for (; nth > 0; --nth) is &= is - 1;
+      return i0 + __builtin_ffsll(is) - 1;
+    }
+    nth -= here;
+  }
+  return -1;
+}
+
+// Block (request, v-head, 32 state rows).  Wave w has the tokens 16 w .. 16 w + 15 of
+// each product over them and the state's dims 32 w .. 32 w + 31.
+__global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs c) {
+  __shared__ __attribute__((aligned(16))) h8 m_s[4][2][2][64];    // state: dims, j tile, hi / lo
+  __shared__ __attribute__((aligned(16))) h8 r_s[4][2][64];       // right sides: tokens, j tile
+  __shared__ __attribute__((aligned(16))) h8 d_s[2][4][2][64];    // delta; delta e k
+  __shared__ float mu_s[4][2][16], ru_s[4][2][16], du_s[2][4][2][16];  // their units
+  __shared__ __attribute__((aligned(16))) float vec_s[2][kVecs];       // of two chunks in turn
+  const GdnArgs &a = c.g;
+  constexpr int kSlabs = kCkS / kCkRows;
+  const int per = a.h_v * kSlabs, nth = blockIdx.x / per;
+  int rest = blockIdx.x - nth * per, h, slab;
+  if (c.xcd) {  // block b runs on die b % 8: q/k heads x, x + 8, .. on die x
+    const int of_head = a.h_v / a.h_k * kSlabs, x = rest & 7, y = rest >> 3;
+    const int kh = y / of_head * 8 + x, z = y % of_head;
+    h = kh + z / kSlabs * a.h_k, slab = z % kSlabs;
+  } else {
+    h = rest / kSlabs, slab = rest % kSlabs;
+  }
+  const int r = nth_long(a.rag, nth);
+  if (r < 0) return;
+  int begin, n, from, to;
+  a.rag.tokens(r, &begin, &n);
+  a.rag.slots(r, &from, &to);
+  const int kh = h % a.h_k;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int lr = lane & 15, lg = lane >> 4;
+  const int chunks = (n + kCk - 1) / kCk;
+  const size_t slot_bytes = static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(a.h_v) * kHeadV;
+  const char *ws_k = c.ws + static_cast<size_t>(first_chunk(begin)) * slot_bytes + static_cast<size_t>(kh) * kHeadK;
+  const char *ws_v = c.ws + static_cast<size_t>(first_chunk(begin)) * slot_bytes +
+                     static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(h) * kHeadV;
+
+  // m[jt][d]: state row 16 jt + lr of the slab, dims 32 w + 16 d + 4 lg ..
+  f32x4 m[2][2];
+  const size_t row0 = (static_cast<size_t>(h) * kCkS + slab * kCkRows + lr) * kCkS + 32 * w + 4 * lg;
+#pragma unroll
+  for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+      m[jt][d] = from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + from * a.rag.slot_stride + row0 +
+                                                             16 * jt * kCkS + 16 * d)
+                           : f32x4{0, 0, 0, 0};
+  h8 kf[4][2], qf[4][2];
+  float vr[2][4];
+  const auto load_kq = [&](const char *p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        kf[i][x] = reinterpret_cast<const h8 *>(p)[(w * 4 + i) * 128 + 64 * x + lane];
+        qf[i][x] = reinterpret_cast<const h8 *>(p + kFragK)[(w * 4 + i) * 128 + 64 * x + lane];
+      }
+  };
+  const auto load_v = [&](int chunk) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = chunk * kCk + 16 * w + 4 * lg + e;
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt)
+        vr[jt][e] = t < n ? a.v[(begin + t) * a.v_stride + static_cast<size_t>(h) * kCkS + slab * kCkRows + 16 * jt + lr]
+                          : 0.0f;
+    }
+  };
+  load_kq(ws_k);
+  load_v(0);
+  for (int chunk = 0; chunk < chunks; ++chunk, ws_k += slot_bytes, ws_v += slot_bytes) {
+    // the state as an operand
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      float up, down;
+      unit_of(most_of_lanes(fmaxf(most_of(m[jt][0]), most_of(m[jt][1]))), &up, &down);
+      h4 h0, l0, h1, l1;
+      halves(m[jt][0] * up, &h0, &l0);
+      halves(m[jt][1] * up, &h1, &l1);
+      m_s[w][jt][0][lane] = both(h0, h1);
+      m_s[w][jt][1][lane] = both(l0, l1);
+      if (lg == 0) mu_s[w][jt][lr] = down;
+    }
+    h8 tf[4], pf[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j <= w) tf[j] = reinterpret_cast<const h8 *>(ws_v)[(w * (w + 1) / 2 + j) * 64 + lane];
+    float *vec = vec_s[chunk & 1];
+    if (threadIdx.x < kVecs / 4)
+      reinterpret_cast<f32x4 *>(vec)[threadIdx.x] =
+          reinterpret_cast<const f32x4 *>(ws_v + 2 * kFragT)[threadIdx.x];
+    const auto unit = [&](int i) {
+      return *reinterpret_cast<const f32x4 *>(vec + i * kCk + 16 * w + 4 * lg);
+    };
+    __syncthreads();
+    // K m and Q m
+    f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt) {
+        const h8 bh = m_s[i][jt][0][lane], bl = m_s[i][jt][1][lane];
+        const float by = mu_s[i][jt][lr];
+        const f32x4 zero = {0, 0, 0, 0};
+        x[jt] += by * mma32(kf[i][0], kf[i][1], bh, bl, zero);
+        y[jt] += by * mma32(qf[i][0], qf[i][1], bh, bl, zero);
+      }
+    const f32x4 ak = unit(0);
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      f32x4 rhs;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) rhs[e] = vr[jt][e] - ak[e] * x[jt][e];
+      float up, down;
+      unit_of(most_of_lanes(most_of(rhs)), &up, &down);
+      h4 hi, lo;
+      halves(rhs * up, &hi, &lo);
+      r_s[w][jt][lane] = both(hi, lo);
+      if (lg == 0) ru_s[w][jt][lr] = down;
+    }
+    // the next chunk's rows, this one's P and K for the update, on their way
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j <= w) pf[j] = reinterpret_cast<const h8 *>(ws_v + kFragT)[(w * (w + 1) / 2 + j) * 64 + lane];
+    h8 kt[2][4];
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        kt[d][t] = reinterpret_cast<const h8 *>(ws_k + 2 * kFragK)[((2 * w + d) * 4 + t) * 64 + lane];
+    if (chunk + 1 < chunks) {
+      load_kq(ws_k + slot_bytes);
+      load_v(chunk + 1);
+    }
+    __syncthreads();
+    // delta, and delta e with K's units
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      f32x4 d = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= w) {
+          const f32x4 zero = {0, 0, 0, 0};
+          d += ru_s[j][jt][lr] * mma16(tf[j], r_s[j][jt][lane], zero);
+        }
+      d *= unit(2);
+      const f32x4 de = d * unit(4);
+      float up, down;
+      h4 hi, lo;
+      unit_of(most_of_lanes(most_of(d)), &up, &down);
+      halves(d * up, &hi, &lo);
+      d_s[0][w][jt][lane] = both(hi, lo);
+      if (lg == 0) du_s[0][w][jt][lr] = down;
+      unit_of(most_of_lanes(most_of(de)), &up, &down);
+      halves(de * up, &hi, &lo);
+      d_s[1][w][jt][lane] = both(hi, lo);
+      if (lg == 0) du_s[1][w][jt][lr] = down;
+    }
+    __syncthreads();
+    // outputs
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= w) {
+          const f32x4 zero = {0, 0, 0, 0};
+          o += du_s[0][j][jt][lr] * mma16(pf[j], d_s[0][j][jt][lane], zero);
+        }
+      o = (unit(1) * y[jt] + unit(3) * o) * a.scale;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = chunk * kCk + 16 * w + 4 * lg + e;
+        if (t < n)
+          a.attn[(static_cast<size_t>(begin + t) * a.h_v + h) * kCkS + slab * kCkRows + 16 * jt + lr] = o[e];
+      }
+    }
+    // the new state
+    const float all = vec[5 * kCk];
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int d = 0; d < 2; ++d) m[jt][d] *= all;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt) {
+        const h8 b = d_s[1][t][jt][lane];
+        const float by = du_s[1][t][jt][lr];
+        const f32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < 2; ++d) m[jt][d] += by * mma16(kt[d][t], b, zero);
+      }
+  }
+  if (to < 0) return;
+#pragma unroll
+  for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+      *reinterpret_cast<f32x4 *>(a.state + to * a.rag.slot_stride + row0 + 16 * jt * kCkS + 16 * d) = m[jt][d];
+}
+
 // Blocks of a launch: a grid has fewer than 2^32 threads a dimension.
 constexpr size_t kMostBlocks = 0xffffff;
 
@@ -189,6 +768,10 @@ int check(const bh_gdn_ragged_args &p) {
       !mul_size(p.n_tok, p.v_stride, sizeof(float), &n) || p.n_slots > 0x7fffffffu ||
       !mul_size(p.n_slots, p.slot_stride, sizeof(float), &n))
     return fail(BH_ERR_SHAPE, "gdn_ragged: size overflow");
+  // (a chunk's block a q/k head; chunks are fewer than n_tok / 40 and one)
+  if (!mul_size(p.n_tok / 40 + 1, p.h_k, &n) || n > kMostBlocks ||
+      !mul_size(p.n_tok / 40 + 1, p.h_k * kHeadK + p.h_v * kHeadV, &n))
+    return fail(BH_ERR_SHAPE, "gdn_ragged: size overflow");
   if (p.n_req != 0 && p.n_tok != 0) {
     if (!p.q || !p.k || !p.v || !p.gate || !p.beta || !p.attn || !p.q_start || !p.src_slot ||
         !p.dst_slot || (p.n_slots != 0 && !p.state))
@@ -197,14 +780,28 @@ int check(const bh_gdn_ragged_args &p) {
   return BH_OK;
 }
 
+bool whole_rows(const bh_gdn_ragged_args &p) {
+  return (p.q_stride | p.k_stride | p.slot_stride) % 4 == 0 && aligned16(p.q) && aligned16(p.k) &&
+         aligned16(p.state);
+}
+
+// Slots of chunks of a call, 0: it has none.
+size_t chunk_slots(const bh_gdn_ragged_args &p) {
+  const size_t most = p.max_new == 0 || p.max_new > p.n_tok ? p.n_tok : p.max_new;
+  if (p.s != static_cast<size_t>(kCkS) || most < static_cast<size_t>(kCkMin) || !whole_rows(p)) return 0;
+  return p.n_tok * 3 / 128 + 1;
+}
+
+size_t slot_bytes(const bh_gdn_ragged_args &p) { return p.h_k * kHeadK + p.h_v * kHeadV; }
+
 }  // namespace
 }  // namespace bh
 
 using namespace bh;
 
 extern "C" size_t bh_gdn_ragged_workspace(const bh_gdn_ragged_args *args) {
-  if (!args || check(*args) != BH_OK) return 0;
-  return 0;
+  if (!args || check(*args) != BH_OK || args->n_req == 0 || args->n_tok == 0) return 0;
+  return chunk_slots(*args) * slot_bytes(*args);
 }
 
 extern "C" int bh_gdn_ragged(const bh_gdn_ragged_args *args, bh_stream stream) {
@@ -221,8 +818,28 @@ extern "C" int bh_gdn_ragged(const bh_gdn_ragged_args *args, bh_stream stream) {
   a.rag = Ragged{p.q_start, p.src_slot, p.dst_slot, p.bad_slot, static_cast<int>(p.n_tok),
                  static_cast<int>(p.n_req), static_cast<int>(p.n_slots), p.slot_stride};
   hipStream_t st = as_stream(stream);
-  const bool whole = (p.q_stride | p.k_stride | p.slot_stride) % 4 == 0 && aligned16(p.q) &&
-                     aligned16(p.k) && aligned16(p.state);
+  const bool whole = whole_rows(p);
+  a.most = 0x7fffffff;
+  if (const size_t slots = chunk_slots(p)) {
+    const size_t need = slots * slot_bytes(p);
+    char *ws = static_cast<char *>(p.workspace);
+    if (ws) {
+      if (!aligned16(ws) || p.workspace_bytes < need)
+        return fail(BH_ERR_SHAPE, "gdn_ragged: workspace of " + std::to_string(p.workspace_bytes) +
+                                      " bytes, " + std::to_string(need) +
+                                      " needed on a 16-byte boundary");
+    } else {
+      ws = static_cast<char *>(device_scratch(need, kScratchGdn, st));
+      if (!ws) return BH_ERR_HIP;
+    }
+    a.most = kCkMin - 1;
+    const size_t longs = p.n_tok / kCkMin < p.n_req ? p.n_tok / kCkMin : p.n_req;
+    GdnChunkArgs c{a, ws, static_cast<int>(slots), static_cast<int>(longs),
+                   p.h_k % 8 == 0 && p.h_v % p.h_k == 0};
+    BH_LAUNCH(gdn_chunk_prep_kernel, static_cast<unsigned>(slots * p.h_k), kBlock, 0, st, c);
+    BH_LAUNCH(gdn_chunk_walk_kernel, static_cast<unsigned>(longs * p.h_v * (kCkS / kCkRows)), kBlock,
+              0, st, c);
+  }
   const auto blocks = [&](size_t rows) { return static_cast<unsigned>(p.n_req * p.h_v * p.s / rows); };
   if (whole && p.s == 128) {
     if (blocks(64) >= 2 * device_cu_count())
