@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kBlock) void conv_ragged4_kernel(ConvArgs a, int pa
   });
   if (r < 0) return;
   int begin, n, from, to;
-  rag.tokens(r, &begin, &n);
+  rag.tokens_of(r, &begin, &n);
   const int64_t first = (run - (static_cast<int64_t>(begin / kRun) + r)) * kRun;
   if (first < 0 || first >= n) return;
   rag.slots(r, &from, &to);
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(kBlock) void conv_ragged_kernel(ConvArgs a, int par
   const int r = last_request(rag.n_req, [&](int i) { return rag.q_start[i] <= t; });
   if (r < 0) return;
   int begin, n, from, to;
-  rag.tokens(r, &begin, &n);
+  rag.tokens_of(r, &begin, &n);
   if (t < begin || t >= begin + n) return;
   rag.slots(r, &from, &to);
   if (c >= a.ch) return;
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(kBlock) void conv_ragged_l2_kernel(ConvArgs a) {
   const int r = last_request(a.rag.n_req, [&](int i) { return a.rag.q_start[i] <= t; });
   if (r < 0) return;
   int begin, n;
-  a.rag.tokens(r, &begin, &n);
+  a.rag.tokens_of(r, &begin, &n);
   if (t < begin || t >= begin + n) return;  // a row of no request
   float *y = a.out + static_cast<size_t>(t) * a.ch + static_cast<size_t>(g) * a.head_dim;
   double sum = 0.0;
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(kBlock) void conv_ragged_l2_kernel(ConvArgs a) {
 __global__ __launch_bounds__(kBlock) void conv_ragged_state_kernel(ConvArgs a, int parts) {
   const int r = blockIdx.x / parts, c = (blockIdx.x - r * parts) * kBlock + threadIdx.x;
   int begin, n, from, to;
-  a.rag.tokens(r, &begin, &n);
+  a.rag.tokens_of(r, &begin, &n);
   if (n == 0) return;
   a.rag.slots(r, &from, &to);
   if (to < 0 || c >= a.ch) return;

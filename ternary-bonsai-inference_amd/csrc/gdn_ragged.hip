@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_step_kernel(GdnArgs a) {
   const int h = rest / kTiles, kh = h % a.h_k;
   const int sub = threadIdx.x % L, j = (rest - h * kTiles) * kRows + threadIdx.x / L * RPG;
   int t0, n, from, to;
-  a.rag.tokens(r, &t0, &n);
+  a.rag.tokens_of(r, &t0, &n);
   if (n == 0 || n > a.most) return;
   a.rag.slots(r, &from, &to);
   const size_t row = (static_cast<size_t>(h) * S + j) * S + 4 * sub;
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_any_kernel(GdnArgs a) {
   const int r = blockIdx.x / blocks, lane = threadIdx.x & 63;
   const int row = (blockIdx.x - r * blocks) * 4 + (threadIdx.x >> 6);
   int t0, n, from, to;
-  a.rag.tokens(r, &t0, &n);
+  a.rag.tokens_of(r, &t0, &n);
   if (n == 0 || row >= rows) return;
   a.rag.slots(r, &from, &to);
   const int h = row / a.s, j = row - h * a.s, kh = h % a.h_k, s = a.s;
@@ -218,15 +218,16 @@ __device__ __forceinline__ int first_chunk(int begin) {
   return static_cast<int>(static_cast<int64_t>(begin) * 3 / 128);
 }
 
-// The unit of values of which `most` is the largest: x up is its number of units.
+// The unit of values of which `most` is the largest: x up is its number of units.  (Of
+// 0, an infinity or NaN the exponent is 0.)
 __device__ __forceinline__ void unit_of(float most, float *up, float *down) {
-  int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
-  *up = *down = 1.0f;
-  if (ex > -127 && ex < 128) {
-    ex = max(ex, -100);
-    *up = __uint_as_float(static_cast<uint32_t>(141 - ex) << 23);
-    *down = __uint_as_float(static_cast<uint32_t>(113 + ex) << 23);
-  }
+  const int ex = max(__builtin_amdgcn_frexp_expf(most), -100);
+  *up = __builtin_amdgcn_ldexpf(1.0f, 15 - ex);
+  *down = __builtin_amdgcn_ldexpf(1.0f, ex - 15);
+}
+// c + a b
+__device__ __forceinline__ f32x4 add_times(f32x4 c, float a, f32x4 b) {
+  return f32x4{fmaf(a, b.x, c.x), fmaf(a, b.y, c.y), fmaf(a, b.z, c.z), fmaf(a, b.w, c.w)};
 }
 __device__ __forceinline__ float most_of(f32x4 x) {
   return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
@@ -241,7 +242,7 @@ __device__ __forceinline__ float most_of_lanes(float x) {
 }
 __device__ __forceinline__ void halves(f32x4 x, h4 *hi, h4 *lo) {
   *hi = __builtin_convertvector(x, h4);
-  *lo = __builtin_convertvector(x - __builtin_convertvector(*hi, f32x4), h4);
+  *lo = __builtin_convertvector(add_times(x, -1.0f, __builtin_convertvector(*hi, f32x4)), h4);
 }
 __device__ __forceinline__ h8 both(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 __device__ __forceinline__ h4 low(h8 a) { return __builtin_shufflevector(a, a, 0, 1, 2, 3); }
@@ -267,6 +268,16 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+// Bytes of the workspace of a chunk from a base in scalars: a lane's place is 32 bits,
+// which saves the vector arithmetic of 64-bit addresses.
+struct Base {
+  __amdgpu_buffer_rsrc_t of;
+  __device__ explicit Base(const void *p)
+      : of(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, 0x7fffffff, 0x00027000)) {}
+  __device__ __forceinline__ h8 load(int lane_at, int at) const {
+    return __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(of, lane_at, at, 0));
+  }
+};
 constexpr int kTri[4] = {0, 1, 3, 6};  // tiles of a lower triangle before row i
 
 // What a wave forms for a v-head: `kq` holds Q K^T on and below the diagonal and K K^T,
@@ -433,7 +444,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
   });
   if (r < 0) return;
   int begin, n;
-  a.rag.tokens(r, &begin, &n);
+  a.rag.tokens_of(r, &begin, &n);
   const int at = (slot - first_chunk(begin)) * kCk;
   if (n < kCkMin || at >= n) return;
   const int t0 = begin + at, nt = min(kCk, n - at);
@@ -569,7 +580,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
   const int r = nth_long(a.rag, nth);
   if (r < 0) return;
   int begin, n, from, to;
-  a.rag.tokens(r, &begin, &n);
+  a.rag.tokens_of(r, &begin, &n);
   a.rag.slots(r, &from, &to);
   const int kh = h % a.h_k;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -592,28 +603,28 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
                            : f32x4{0, 0, 0, 0};
   h8 kf[4][2], qf[4][2];
   float vr[2][4];
-  const auto load_kq = [&](const char *p) {
+  const auto load_rows = [&](const Base &p, int at, h8(&f)[4][2]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        kf[i][x] = reinterpret_cast<const h8 *>(p)[(w * 4 + i) * 128 + 64 * x + lane];
-        qf[i][x] = reinterpret_cast<const h8 *>(p + kFragK)[(w * 4 + i) * 128 + 64 * x + lane];
-      }
+      for (int x = 0; x < 2; ++x)
+        f[i][x] = p.load(16 * lane, at + ((w * 4 + i) * 128 + 64 * x) * 16);
   };
-  const auto load_v = [&](int chunk) {
+  const size_t v_at = static_cast<size_t>(h) * kCkS + slab * kCkRows + lr;
+  const float *vp = a.v + static_cast<size_t>(begin + 16 * w + 4 * lg) * a.v_stride + v_at;
+  float *op = a.attn + static_cast<size_t>(begin + 16 * w + 4 * lg) * a.h_v * kCkS + v_at;
+  const auto load_v = [&](int left) {  // of the chunk at vp, of which `left` tokens are the request's
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int t = chunk * kCk + 16 * w + 4 * lg + e;
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int jt = 0; jt < 2; ++jt)
-        vr[jt][e] = t < n ? a.v[(begin + t) * a.v_stride + static_cast<size_t>(h) * kCkS + slab * kCkRows + 16 * jt + lr]
-                          : 0.0f;
-    }
+        vr[jt][e] = 16 * w + 4 * lg + e < left ? vp[e * a.v_stride + 16 * jt] : 0.0f;
   };
-  load_kq(ws_k);
-  load_v(0);
+  load_rows(Base(ws_k), 0, kf);
+  load_rows(Base(ws_k), kFragK, qf);
+  load_v(n);
   for (int chunk = 0; chunk < chunks; ++chunk, ws_k += slot_bytes, ws_v += slot_bytes) {
+    const int left = n - chunk * kCk;
     // the state as an operand
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt) {
@@ -626,10 +637,11 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
       m_s[w][jt][1][lane] = both(l0, l1);
       if (lg == 0) mu_s[w][jt][lr] = down;
     }
+    const Base of_k(ws_k), of_v(ws_v);
     h8 tf[4], pf[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j <= w) tf[j] = reinterpret_cast<const h8 *>(ws_v)[(w * (w + 1) / 2 + j) * 64 + lane];
+    for (int j = 0; j < 4; ++j)  // (0 above the diagonal: no branch parts the products)
+      tf[j] = j <= w ? of_v.load(16 * lane, (w * (w + 1) / 2 + j) * 1024) : h8{};
     float *vec = vec_s[chunk & 1];
     if (threadIdx.x < kVecs / 4)
       reinterpret_cast<f32x4 *>(vec)[threadIdx.x] =
@@ -638,24 +650,45 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
       return *reinterpret_cast<const f32x4 *>(vec + i * kCk + 16 * w + 4 * lg);
     };
     __syncthreads();
-    // K m and Q m
+    // K m and Q m, 32 dims at a time: operands are read while the ones before are
+    // multiplied, and not earlier (registers are short)
     f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    {
+      h8 b[2][2][2];
+      float by[2][2];
+      const auto read = [&](int d) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int jt = 0; jt < 2; ++jt) {
+          b[d & 1][jt][0] = m_s[d][jt][0][lane], b[d & 1][jt][1] = m_s[d][jt][1][lane];
+          by[d & 1][jt] = mu_s[d][jt][lr];
+        }
+      };
+      read(0);
 #pragma unroll
-      for (int jt = 0; jt < 2; ++jt) {
-        const h8 bh = m_s[i][jt][0][lane], bl = m_s[i][jt][1][lane];
-        const float by = mu_s[i][jt][lr];
+      for (int d = 0; d < 4; ++d) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (d + 1 < 4) read(d + 1);
         const f32x4 zero = {0, 0, 0, 0};
-        x[jt] += by * mma32(kf[i][0], kf[i][1], bh, bl, zero);
-        y[jt] += by * mma32(qf[i][0], qf[i][1], bh, bl, zero);
+        f32x4 p[2], q[2];
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt) {
+          p[jt] = mma32(kf[d][0], kf[d][1], b[d & 1][jt][0], b[d & 1][jt][1], zero);
+          q[jt] = mma32(qf[d][0], qf[d][1], b[d & 1][jt][0], b[d & 1][jt][1], zero);
+        }
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt) {
+          x[jt] = add_times(x[jt], by[d & 1][jt], p[jt]);
+          y[jt] = add_times(y[jt], by[d & 1][jt], q[jt]);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     const f32x4 ak = unit(0);
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt) {
       f32x4 rhs;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) rhs[e] = vr[jt][e] - ak[e] * x[jt][e];
+      for (int e = 0; e < 4; ++e) rhs[e] = fmaf(-ak[e], x[jt][e], vr[jt][e]);
       float up, down;
       unit_of(most_of_lanes(most_of(rhs)), &up, &down);
       h4 hi, lo;
@@ -663,19 +696,22 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
       r_s[w][jt][lane] = both(hi, lo);
       if (lg == 0) ru_s[w][jt][lr] = down;
     }
-    // the next chunk's rows, this one's P and K for the update, on their way
+    // P and K for the update, and the next chunk's rows, on their way
+    h8 kt[2][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (j <= w) pf[j] = reinterpret_cast<const h8 *>(ws_v + kFragT)[(w * (w + 1) / 2 + j) * 64 + lane];
-    h8 kt[2][4];
+      pf[j] = j <= w ? of_v.load(16 * lane, kFragT + (w * (w + 1) / 2 + j) * 1024) : h8{};
 #pragma unroll
     for (int d = 0; d < 2; ++d)
 #pragma unroll
       for (int t = 0; t < 4; ++t)
-        kt[d][t] = reinterpret_cast<const h8 *>(ws_k + 2 * kFragK)[((2 * w + d) * 4 + t) * 64 + lane];
+        kt[d][t] = of_k.load(16 * lane, 2 * kFragK + ((2 * w + d) * 4 + t) * 1024);
+    vp += kCk * a.v_stride;
     if (chunk + 1 < chunks) {
-      load_kq(ws_k + slot_bytes);
-      load_v(chunk + 1);
+      const Base next(ws_k + slot_bytes);
+      load_rows(next, 0, kf);
+      load_rows(next, kFragK, qf);
+      load_v(left - kCk);
     }
     __syncthreads();
     // delta, and delta e with K's units
@@ -683,11 +719,10 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
     for (int jt = 0; jt < 2; ++jt) {
       f32x4 d = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j <= w) {
-          const f32x4 zero = {0, 0, 0, 0};
-          d += ru_s[j][jt][lr] * mma16(tf[j], r_s[j][jt][lane], zero);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 zero = {0, 0, 0, 0};
+        d = add_times(d, ru_s[j][jt][lr], mma16(tf[j], r_s[j][jt][lane], zero));
+      }
       d *= unit(2);
       const f32x4 de = d * unit(4);
       float up, down;
@@ -707,19 +742,16 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
     for (int jt = 0; jt < 2; ++jt) {
       f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j <= w) {
-          const f32x4 zero = {0, 0, 0, 0};
-          o += du_s[0][j][jt][lr] * mma16(pf[j], d_s[0][j][jt][lane], zero);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 zero = {0, 0, 0, 0};
+        o = add_times(o, du_s[0][j][jt][lr], mma16(pf[j], d_s[0][j][jt][lane], zero));
+      }
       o = (unit(1) * y[jt] + unit(3) * o) * a.scale;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = chunk * kCk + 16 * w + 4 * lg + e;
-        if (t < n)
-          a.attn[(static_cast<size_t>(begin + t) * a.h_v + h) * kCkS + slab * kCkRows + 16 * jt + lr] = o[e];
-      }
+      for (int e = 0; e < 4; ++e)
+        if (16 * w + 4 * lg + e < left) op[e * (a.h_v * kCkS) + 16 * jt] = o[e];
     }
+    op += static_cast<size_t>(kCk) * a.h_v * kCkS;
     // the new state
     const float all = vec[5 * kCk];
 #pragma unroll
@@ -734,7 +766,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
         const float by = du_s[1][t][jt][lr];
         const f32x4 zero = {0, 0, 0, 0};
 #pragma unroll
-        for (int d = 0; d < 2; ++d) m[jt][d] += by * mma16(kt[d][t], b, zero);
+        for (int d = 0; d < 2; ++d) m[jt][d] = add_times(m[jt][d], by, mma16(kt[d][t], b, zero));
       }
   }
   if (to < 0) return;

@@ -23,9 +23,17 @@ struct Ragged {
     *begin = s;
     *n = max(e - s, 0);
   }
-  // Slots of request r, -1: none (below 0, or past the pool and then noted).
+  // The same of a request that is the wave's, in scalars: what follows from them is too.
+  __device__ __forceinline__ void tokens_of(int r, int *begin, int *n) const {
+    int s, count;
+    tokens(r, &s, &count);
+    *begin = __builtin_amdgcn_readfirstlane(s);
+    *n = __builtin_amdgcn_readfirstlane(count);
+  }
+  // Slots of the wave's request r, -1: none (below 0, or past the pool and then noted).
   __device__ __forceinline__ void slots(int r, int *from, int *to) const {
-    const int f = src[r], t = dst[r];
+    const int f = __builtin_amdgcn_readfirstlane(src[r]);
+    const int t = __builtin_amdgcn_readfirstlane(dst[r]);
     *from = f >= 0 && f < n_slots ? f : -1;
     *to = t >= 0 && t < n_slots ? t : -1;
     if (bad_slot && threadIdx.x == 0) {
