@@ -34,12 +34,12 @@ struct GdnArgs {
 
 // Rows of S floats in registers, S / 8 lanes a row and RPG rows a lane, for as many
 // tokens as the request has; the next token's inputs load under the present one.
-template <int S, int RPG>
-__global__ __launch_bounds__(kBlock) void gdn_ragged_step_kernel(GdnArgs a) {
-  constexpr int L = S / 8, kRows = kBlock / L * RPG, kTiles = S / kRows;
+template <int S, int RPG, int THREADS>
+__device__ __forceinline__ void step_rows(const GdnArgs &a, int block) {
+  constexpr int L = S / 8, kRows = THREADS / L * RPG, kTiles = S / kRows;
   static_assert(S % kRows == 0, "a block's rows are of one head");
   const int per = a.h_v * kTiles;
-  const int r = blockIdx.x / per, rest = blockIdx.x - r * per;
+  const int r = block / per, rest = block - r * per;
   const int h = rest / kTiles, kh = h % a.h_k;
   const int sub = threadIdx.x % L, j = (rest - h * kTiles) * kRows + threadIdx.x / L * RPG;
   int t0, n, from, to;
@@ -114,6 +114,11 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_step_kernel(GdnArgs a) {
       *reinterpret_cast<f32x4 *>(p + i * S + S / 2) = m[i][1];
     }
   }
+}
+
+template <int S, int RPG>
+__global__ __launch_bounds__(kBlock) void gdn_ragged_step_kernel(GdnArgs a) {
+  step_rows<S, RPG, kBlock>(a, blockIdx.x);
 }
 
 // Any s up to kAnyMaxS and any alignment: a wave a row, 16 of its floats a lane.
@@ -195,13 +200,13 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr int kCk = 64, kCkS = 128;
 constexpr int kCkMin = 128;           // tokens from which a request goes by chunks
-constexpr int kCkRows = 32;           // state rows of a walk
 constexpr int kFragK = kCk * kCkS * 4;           // bytes of K as halves; Q, K transposed
 constexpr int kHeadK = 3 * kFragK;               // of a (chunk, q/k head)
-constexpr int kFragT = 10 * 64 * 16;             // of T's and P's lower 16 x 16 tiles
+constexpr int kFragT = 12 * 64 * 16;             // of T's and P's 16 x 32 tiles to the diagonal
 constexpr int kVecs = 5 * kCk + kCk;             // floats: A k, A q, T's, P's units, e k; A_63
 constexpr int kHeadV = 2 * kFragT + kVecs * 4;   // of a (chunk, v-head)
 constexpr float kGateFloor = -200.0f;            // e^x below this is 0 in f32
+constexpr size_t kMostStride = 0x7fffff;         // floats: a chunk's v within 2^31 bytes
 constexpr int kPitch = 68;                       // floats of a row of a 64 x 64 matrix in LDS
 constexpr int kVWaves = 3;                       // v-heads prepared side by side
 
@@ -209,7 +214,7 @@ struct GdnChunkArgs {
   GdnArgs g;
   char *ws;    // [slots][h_k kHeadK + h_v kHeadV]
   int slots;   // of chunks
-  int n_long;  // requests of kCkMin tokens or more there can be
+  int walks;   // blocks of the walk
   int xcd;     // the blocks of a q/k head on one die
 };
 
@@ -240,24 +245,24 @@ __device__ __forceinline__ float most_of_lanes(float x) {
   lane_swap<32>(x, lo, hi);
   return fmaxf(lo, hi);
 }
-__device__ __forceinline__ void halves(f32x4 x, h4 *hi, h4 *lo) {
-  *hi = __builtin_convertvector(x, h4);
-  *lo = __builtin_convertvector(add_times(x, -1.0f, __builtin_convertvector(*hi, f32x4)), h4);
+// x up as hi + lo halves.
+__device__ __forceinline__ void halves(f32x4 x, float up, h4 *hi, h4 *lo) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const _Float16 h = static_cast<_Float16>(x[e] * up);
+    (*hi)[e] = h;
+    (*lo)[e] = static_cast<_Float16>(fmaf(x[e], up, -static_cast<float>(h)));
+  }
 }
 __device__ __forceinline__ h8 both(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
-__device__ __forceinline__ h4 low(h8 a) { return __builtin_shufflevector(a, a, 0, 1, 2, 3); }
-__device__ __forceinline__ h4 high(h8 a) { return __builtin_shufflevector(a, a, 4, 5, 6, 7); }
 
+__device__ __forceinline__ f32x4 mma(h8 a, h8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x4 mma32(h8 ah, h8 al, h8 bh, h8 bl, f32x4 c) {
   c = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, c, 0, 0, 0);
   c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, c, 0, 0, 0);
-}
-// Operands hi | lo.
-__device__ __forceinline__ f32x4 mma16(h8 a, h8 b, f32x4 c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x16f16(high(a), low(b), c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x16f16(low(a), high(b), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x16f16(low(a), low(b), c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -268,8 +273,8 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-// Bytes of the workspace of a chunk from a base in scalars: a lane's place is 32 bits,
-// which saves the vector arithmetic of 64-bit addresses.
+// What lies at a base in scalars: a lane's place and an offset that all lanes share are 32
+// bits each, which saves the vector arithmetic of 64-bit addresses.
 struct Base {
   __amdgpu_buffer_rsrc_t of;
   __device__ explicit Base(const void *p)
@@ -277,8 +282,28 @@ struct Base {
   __device__ __forceinline__ h8 load(int lane_at, int at) const {
     return __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(of, lane_at, at, 0));
   }
+  __device__ __forceinline__ float load1(int lane_at, int at) const {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(of, lane_at, at, 0));
+  }
+  __device__ __forceinline__ void store1(float x, int lane_at, int at) const {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), of, lane_at, at, 0);
+  }
 };
-constexpr int kTri[4] = {0, 1, 3, 6};  // tiles of a lower triangle before row i
+constexpr int kTri[4] = {0, 1, 2, 4};  // 16 x 32 tiles to the diagonal before row i
+// A row of up to four 16 x 16 tiles as operands of 32, hi and lo; 0 from tile n on.
+__device__ __forceinline__ void store_row(char *out, const f32x4 *x, int n, float up, int lane) {
+  h4 hi[4], lo[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    hi[j] = lo[j] = h4{0, 0, 0, 0};
+    if (j < n) halves(x[j], up, &hi[j], &lo[j]);
+  }
+#pragma unroll
+  for (int p = 0; 2 * p < n; ++p) {
+    h8 *o = reinterpret_cast<h8 *>(out) + p * 128 + lane;
+    o[0] = both(hi[2 * p], hi[2 * p + 1]), o[64] = both(lo[2 * p], lo[2 * p + 1]);
+  }
+}
 
 // What a wave forms for a v-head: `kq` holds Q K^T on and below the diagonal and K K^T,
 // transposed, above it; `l` is the wave's own matrix.  down: the units of K's and Q's rows.
@@ -347,12 +372,7 @@ __device__ __forceinline__ void prep_head(const GdnArgs &a, int h, int t0, int n
     }
     float up, down;
     unit_of(most_of_lanes(most), &up, &down);
-#pragma unroll
-    for (int j = 0; j <= i; ++j) {
-      h4 hi, lo;
-      halves(p[j] * up, &hi, &lo);
-      *reinterpret_cast<h8 *>(out + kFragT + ((kTri[i] + j) * 64 + lane) * 16) = both(hi, lo);
-    }
+    store_row(out + kFragT + kTri[i] * 2048, p, i + 1, up, lane);
     if (lg == 0) vec[3 * kCk + t] = down;
   }
   wave_sync();
@@ -418,12 +438,7 @@ __device__ __forceinline__ void prep_head(const GdnArgs &a, int h, int t0, int n
       most = fmaxf(most, most_of(t[j]));
     }
     unit_of(most_of_lanes(most), &up, &down);
-#pragma unroll
-    for (int j = 0; j <= i; ++j) {
-      h4 hi, lo;
-      halves(t[j] * up, &hi, &lo);
-      *reinterpret_cast<h8 *>(out + ((kTri[i] + j) * 64 + lane) * 16) = both(hi, lo);
-    }
+    store_row(out + kTri[i] * 2048, t, i + 1, up, lane);
     if (lg == 0) vec[2 * kCk + 16 * i + lr] = down;
   }
   wave_sync();
@@ -479,11 +494,11 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h4 h0, l0, h1, l1;
-      halves(kv[2 * i] * ku, &h0, &l0);
-      halves(kv[2 * i + 1] * ku, &h1, &l1);
+      halves(kv[2 * i], ku, &h0, &l0);
+      halves(kv[2 * i + 1], ku, &h1, &l1);
       kh_[i] = both(h0, h1), kl[i] = both(l0, l1);
-      halves(qv[2 * i] * qu, &h0, &l0);
-      halves(qv[2 * i + 1] * qu, &h1, &l1);
+      halves(qv[2 * i], qu, &h0, &l0);
+      halves(qv[2 * i + 1], qu, &h1, &l1);
       qh[i] = both(h0, h1), ql[i] = both(l0, l1);
       const int f = (w * 4 + i) * 128 + lane;  // of 16 bytes: hi, and lo 64 places on
       k_lds[f] = kh_[i], k_lds[f + 64] = kl[i];
@@ -514,21 +529,23 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
       if (s < t) kq[s * kPitch + t] = kk[e] * k_down[t] * ds;
     }
   }
-  // K transposed: tile (d, t) of 16 dims and 16 tokens, lane's dim 16 d + lr
+  // K transposed: tile (d, p) of 16 dims and 32 tokens, lane's dim 16 d + lr
   {
     const _Float16 *halves_of = reinterpret_cast<const _Float16 *>(lds);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const int d = 2 * w + (x >> 2), t = x & 3;  // wave w: dims 32 w .. 32 w + 31
+    for (int x = 0; x < 4; ++x) {
+      const int d = 2 * w + (x >> 1), p = x & 1;  // wave w: dims 32 w .. 32 w + 31
       const int dim = 16 * (d & 1) + lr;         // of 32
       const int in = (dim >> 4) * 4 + (dim & 3), group = (dim >> 2) & 3;
-      h4 hi, lo;
+      h8 hi, lo;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int f = ((t * 4 + (d >> 1)) * 128 + 4 * lg + e + 16 * group) * 8 + in;
+      for (int e = 0; e < 8; ++e) {
+        const int t = 2 * p + (e >> 2);
+        const int f = ((t * 4 + (d >> 1)) * 128 + 4 * lg + (e & 3) + 16 * group) * 8 + in;
         hi[e] = halves_of[f], lo[e] = halves_of[f + 64 * 8];
       }
-      *reinterpret_cast<h8 *>(out + 2 * kFragK + ((d * 4 + t) * 64 + lane) * 16) = both(hi, lo);
+      h8 *o = reinterpret_cast<h8 *>(out + 2 * kFragK) + (d * 2 + p) * 128 + lane;
+      o[0] = hi, o[64] = lo;
     }
   }
   __syncthreads();
@@ -558,16 +575,25 @@ __device__ __forceinline__ int nth_long(const Ragged &rag, int nth) {
   return -1;
 }
 
-// Block (request, v-head, 32 state rows).  Wave w has the tokens 16 w .. 16 w + 15 of
-// each product over them and the state's dims 32 w .. 32 w + 31.
-__global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs c) {
-  __shared__ __attribute__((aligned(16))) h8 m_s[4][2][2][64];    // state: dims, j tile, hi / lo
-  __shared__ __attribute__((aligned(16))) h8 r_s[4][2][64];       // right sides: tokens, j tile
-  __shared__ __attribute__((aligned(16))) h8 d_s[2][4][2][64];    // delta; delta e k
-  __shared__ float mu_s[4][2][16], ru_s[4][2][16], du_s[2][4][2][16];  // their units
-  __shared__ __attribute__((aligned(16))) float vec_s[2][kVecs];       // of two chunks in turn
+// Block (request, v-head, 16 WAVES state rows).  A wave has 16 rows to itself and takes
+// them through the chunks in registers: every result is the next product's operand as it
+// stands.  The operands that the waves share stand in LDS, K and Q apart from K
+// transposed, T and P, so that each part of the next chunk comes in while the other
+// is read: two barriers a chunk.
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(GdnChunkArgs c) {
+  constexpr int kThreads = 64 * WAVES, kRows = 16 * WAVES, kSlabs = kCkS / kRows;
+  constexpr int kA = 2 * kFragK / 16, kB = (kFragK + 2 * kFragT) / 16;
+  constexpr int kAs = kA / kThreads, kBk = kFragK / 16 / kThreads, kBt = 2 * kFragT / 16 / kThreads;
+  static_assert(kAs * kThreads == kA && (kBk + kBt) * kThreads == kB, "whole pieces a thread");
+  __shared__ __attribute__((aligned(16))) h8 kq_s[kA];           // K, Q
+  __shared__ __attribute__((aligned(16))) h8 u_s[kB];            // K transposed, T, P
+  __shared__ __attribute__((aligned(16))) float vec_s[2][kVecs];  // of two chunks in turn
   const GdnArgs &a = c.g;
-  constexpr int kSlabs = kCkS / kCkRows;
+  if (static_cast<int>(blockIdx.x) >= c.walks) {  // the requests of fewer tokens
+    step_rows<kCkS, 4, kThreads>(a, blockIdx.x - c.walks);
+    return;
+  }
   const int per = a.h_v * kSlabs, nth = blockIdx.x / per;
   int rest = blockIdx.x - nth * per, h, slab;
   if (c.xcd) {  // block b runs on die b % 8: q/k heads x, x + 8, .. on die x
@@ -591,190 +617,234 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_walk_kernel(GdnChunkArgs 
   const char *ws_v = c.ws + static_cast<size_t>(first_chunk(begin)) * slot_bytes +
                      static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(h) * kHeadV;
 
-  // m[jt][d]: state row 16 jt + lr of the slab, dims 32 w + 16 d + 4 lg ..
-  f32x4 m[2][2];
-  const size_t row0 = (static_cast<size_t>(h) * kCkS + slab * kCkRows + lr) * kCkS + 32 * w + 4 * lg;
+  // m[d]: state row lr of the wave's, dims 16 d + 4 lg ..
+  const int row_w = h * kCkS + slab * kRows + 16 * w;
+  const size_t m_at = (static_cast<size_t>(row_w) + lr) * kCkS + 4 * lg;
+  f32x4 m[8];
 #pragma unroll
-  for (int jt = 0; jt < 2; ++jt)
+  for (int d = 0; d < 8; ++d)
+    m[d] = from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + from * a.rag.slot_stride + m_at + 16 * d)
+                     : f32x4{0, 0, 0, 0};
+  h8 in_a[kAs], in_b[kBk + kBt];
+  f32x4 in_vec;
+  const auto load_a = [&](const char *p) {
+    const Base k(p);
 #pragma unroll
-    for (int d = 0; d < 2; ++d)
-      m[jt][d] = from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + from * a.rag.slot_stride + row0 +
-                                                             16 * jt * kCkS + 16 * d)
-                           : f32x4{0, 0, 0, 0};
-  h8 kf[4][2], qf[4][2];
-  float vr[2][4];
-  const auto load_rows = [&](const Base &p, int at, h8(&f)[4][2]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        f[i][x] = p.load(16 * lane, at + ((w * 4 + i) * 128 + 64 * x) * 16);
+    for (int i = 0; i < kAs; ++i) in_a[i] = k.load(16 * threadIdx.x, i * kThreads * 16);
   };
-  const size_t v_at = static_cast<size_t>(h) * kCkS + slab * kCkRows + lr;
-  const float *vp = a.v + static_cast<size_t>(begin + 16 * w + 4 * lg) * a.v_stride + v_at;
-  float *op = a.attn + static_cast<size_t>(begin + 16 * w + 4 * lg) * a.h_v * kCkS + v_at;
+  const auto store_a = [&] {
+#pragma unroll
+    for (int i = 0; i < kAs; ++i) kq_s[i * kThreads + threadIdx.x] = in_a[i];
+  };
+  const int vec_i = min(static_cast<int>(threadIdx.x), kVecs / 4 - 1);  // (the last ones the same)
+  const auto load_b = [&](const char *k, const char *v) {
+    const Base of_k(k), of_v(v);
+#pragma unroll
+    for (int i = 0; i < kBk; ++i) in_b[i] = of_k.load(16 * threadIdx.x, 2 * kFragK + i * kThreads * 16);
+#pragma unroll
+    for (int i = 0; i < kBt; ++i) in_b[kBk + i] = of_v.load(16 * threadIdx.x, i * kThreads * 16);
+    in_vec = __builtin_bit_cast(f32x4, of_v.load(16 * vec_i, 2 * kFragT));
+  };
+  const auto store_b = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < kBk + kBt; ++i) u_s[i * kThreads + threadIdx.x] = in_b[i];
+    reinterpret_cast<f32x4 *>(vec_s[chunk & 1])[vec_i] = in_vec;
+  };
+  // v and outputs: tokens 16 t + 4 lg + e
+  const int v_stride = 4 * static_cast<int>(a.v_stride), o_stride = 4 * a.h_v * kCkS;
+  const float *vp = a.v + static_cast<size_t>(begin) * a.v_stride + row_w;
+  float *op = a.attn + static_cast<size_t>(begin) * a.h_v * kCkS + row_w;
+  f32x4 v[4];
   const auto load_v = [&](int left) {  // of the chunk at vp, of which `left` tokens are the request's
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int jt = 0; jt < 2; ++jt)
-        vr[jt][e] = 16 * w + 4 * lg + e < left ? vp[e * a.v_stride + 16 * jt] : 0.0f;
-  };
-  load_rows(Base(ws_k), 0, kf);
-  load_rows(Base(ws_k), kFragK, qf);
-  load_v(n);
-  for (int chunk = 0; chunk < chunks; ++chunk, ws_k += slot_bytes, ws_v += slot_bytes) {
-    const int left = n - chunk * kCk;
-    // the state as an operand
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt) {
-      float up, down;
-      unit_of(most_of_lanes(fmaxf(most_of(m[jt][0]), most_of(m[jt][1]))), &up, &down);
-      h4 h0, l0, h1, l1;
-      halves(m[jt][0] * up, &h0, &l0);
-      halves(m[jt][1] * up, &h1, &l1);
-      m_s[w][jt][0][lane] = both(h0, h1);
-      m_s[w][jt][1][lane] = both(l0, l1);
-      if (lg == 0) mu_s[w][jt][lr] = down;
-    }
-    const Base of_k(ws_k), of_v(ws_v);
-    h8 tf[4], pf[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)  // (0 above the diagonal: no branch parts the products)
-      tf[j] = j <= w ? of_v.load(16 * lane, (w * (w + 1) / 2 + j) * 1024) : h8{};
-    float *vec = vec_s[chunk & 1];
-    if (threadIdx.x < kVecs / 4)
-      reinterpret_cast<f32x4 *>(vec)[threadIdx.x] =
-          reinterpret_cast<const f32x4 *>(ws_v + 2 * kFragT)[threadIdx.x];
-    const auto unit = [&](int i) {
-      return *reinterpret_cast<const f32x4 *>(vec + i * kCk + 16 * w + 4 * lg);
-    };
-    __syncthreads();
-    // K m and Q m, 32 dims at a time: operands are read while the ones before are
-    // multiplied, and not earlier (registers are short)
-    f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    {
-      h8 b[2][2][2];
-      float by[2][2];
-      const auto read = [&](int d) {
-#pragma unroll
-        for (int jt = 0; jt < 2; ++jt) {
-          b[d & 1][jt][0] = m_s[d][jt][0][lane], b[d & 1][jt][1] = m_s[d][jt][1][lane];
-          by[d & 1][jt] = mu_s[d][jt][lr];
-        }
-      };
-      read(0);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (d + 1 < 4) read(d + 1);
-        const f32x4 zero = {0, 0, 0, 0};
-        f32x4 p[2], q[2];
-#pragma unroll
-        for (int jt = 0; jt < 2; ++jt) {
-          p[jt] = mma32(kf[d][0], kf[d][1], b[d & 1][jt][0], b[d & 1][jt][1], zero);
-          q[jt] = mma32(qf[d][0], qf[d][1], b[d & 1][jt][0], b[d & 1][jt][1], zero);
-        }
-#pragma unroll
-        for (int jt = 0; jt < 2; ++jt) {
-          x[jt] = add_times(x[jt], by[d & 1][jt], p[jt]);
-          y[jt] = add_times(y[jt], by[d & 1][jt], q[jt]);
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    const f32x4 ak = unit(0);
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt) {
-      f32x4 rhs;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) rhs[e] = fmaf(-ak[e], x[jt][e], vr[jt][e]);
-      float up, down;
-      unit_of(most_of_lanes(most_of(rhs)), &up, &down);
-      h4 hi, lo;
-      halves(rhs * up, &hi, &lo);
-      r_s[w][jt][lane] = both(hi, lo);
-      if (lg == 0) ru_s[w][jt][lr] = down;
-    }
-    // P and K for the update, and the next chunk's rows, on their way
-    h8 kt[2][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      pf[j] = j <= w ? of_v.load(16 * lane, kFragT + (w * (w + 1) / 2 + j) * 1024) : h8{};
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
+    const Base of(vp);
+    if (left >= kCk) {
+      const int at = 4 * lg * v_stride + 4 * lr;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
-        kt[d][t] = of_k.load(16 * lane, 2 * kFragK + ((2 * w + d) * 4 + t) * 1024);
-    vp += kCk * a.v_stride;
-    if (chunk + 1 < chunks) {
-      const Base next(ws_k + slot_bytes);
-      load_rows(next, 0, kf);
-      load_rows(next, kFragK, qf);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[t][e] = of.load1(at, (16 * t + e) * v_stride);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 16 * t + 4 * lg + e;
+          const float x = of.load1(min(i, left - 1) * v_stride + 4 * lr, 0);
+          v[t][e] = i < left ? x : 0.0f;
+        }
+    }
+  };
+  // 32 or 64 of a lane's values as operands, in units of a power of two
+  const auto unit = [&](float most, float *up, float *down) { unit_of(most_of_lanes(most), up, down); };
+  const auto pair = [](f32x4 x, f32x4 y, float up, h8 *hi, h8 *lo) {
+    h4 h0, l0, h1, l1;
+    halves(x, up, &h0, &l0);
+    halves(y, up, &h1, &l1);
+    *hi = both(h0, h1), *lo = both(l0, l1);
+  };
+  const auto most4 = [](const f32x4 *x) {
+    return fmaxf(fmaxf(most_of(x[0]), most_of(x[1])), fmaxf(most_of(x[2]), most_of(x[3])));
+  };
+  const h8 *k_at = kq_s + lane, *u_at = u_s + lane;
+
+  load_a(ws_k);
+  load_b(ws_k, ws_v);
+  load_v(n);
+  store_a();
+  if (chunks > 1) load_a(ws_k + slot_bytes);
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    const int left = n - chunk * kCk;
+    const bool more = chunk + 1 < chunks;
+    const float *vec = vec_s[chunk & 1];
+    const auto of_token = [&](int i, int t) {
+      return *reinterpret_cast<const f32x4 *>(vec + i * kCk + 16 * t + 4 * lg);
+    };
+    float up, m_down;
+    h8 mh[4], ml[4];
+    unit(fmaxf(most4(m), most4(m + 4)), &up, &m_down);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pair(m[2 * i], m[2 * i + 1], up, &mh[i], &ml[i]);
+    __syncthreads();  // K and Q are there; K transposed, T and P of the chunk before are read
+    // K m, then Q m, 32 dims a step; operands are read a step ahead
+    h8 f[2][4][2];
+    const auto read = [&](int step) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          f[step & 1][t][p] = k_at[(step >> 2) * (kA / 2) + (t * 4 + (step & 3)) * 128 + 64 * p];
+    };
+    f32x4 x[4], y[4];
+    const auto times = [&](int step, f32x4 *z) {
+      const int i = step & 3;
+#pragma unroll
+      for (int p = 0; p < 3; ++p)  // lo hi, hi lo, hi hi
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          z[t] = mma(f[step & 1][t][p == 0], p == 1 ? ml[i] : mh[i], i == 0 && p == 0 ? f32x4{0, 0, 0, 0} : z[t]);
+    };
+    read(0);
+    store_b(chunk);
+    if (more) load_b(ws_k + slot_bytes, ws_v + slot_bytes);
+#pragma unroll
+    for (int step = 0; step < 8; ++step) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (step + 1 < 8) read(step + 1);
+      times(step, step < 4 ? x : y);
+    }
+    __syncthreads();  // K and Q are read; the others are there
+    h8 tf[6][2];
+#pragma unroll
+    for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[kFragK / 16 + i * 64];
+    // the right sides
+    f32x4 s[4];
+    h8 hi[2], lo[2];
+    float down;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f32x4 ak = of_token(0, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[t][e] = fmaf(-ak[e], x[t][e] * m_down, v[t][e]);
+    }
+    unit(most4(s), &up, &down);
+    pair(s[0], s[1], up, &hi[0], &lo[0]);
+    pair(s[2], s[3], up, &hi[1], &lo[1]);
+    if (more) {
+      store_a();
+      if (left > 2 * kCk) load_a(ws_k + 2 * slot_bytes);
+      vp += kCk * a.v_stride;
       load_v(left - kCk);
     }
-    __syncthreads();
+    // a row tile of T or P against the operand
+    const auto lower = [&](f32x4 *d) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+          for (int t = 2 * p; t < 4; ++t)
+            d[t] = mma(tf[kTri[t] + p][k == 0], k == 1 ? lo[p] : hi[p], p == 0 && k == 0 ? f32x4{0, 0, 0, 0} : d[t]);
+    };
     // delta, and delta e with K's units
+    f32x4 d[4];
+    lower(d);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int jt = 0; jt < 2; ++jt) {
-      f32x4 d = {0, 0, 0, 0};
+    for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[(kFragK + kFragT) / 16 + i * 64];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 zero = {0, 0, 0, 0};
-        d = add_times(d, ru_s[j][jt][lr], mma16(tf[j], r_s[j][jt][lane], zero));
-      }
-      d *= unit(2);
-      const f32x4 de = d * unit(4);
-      float up, down;
-      h4 hi, lo;
-      unit_of(most_of_lanes(most_of(d)), &up, &down);
-      halves(d * up, &hi, &lo);
-      d_s[0][w][jt][lane] = both(hi, lo);
-      if (lg == 0) du_s[0][w][jt][lr] = down;
-      unit_of(most_of_lanes(most_of(de)), &up, &down);
-      halves(de * up, &hi, &lo);
-      d_s[1][w][jt][lane] = both(hi, lo);
-      if (lg == 0) du_s[1][w][jt][lr] = down;
-    }
-    __syncthreads();
+    for (int t = 0; t < 4; ++t) d[t] = d[t] * (of_token(2, t) * down);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s[t] = d[t] * of_token(4, t);
+    unit(most4(d), &up, &down);
+    pair(d[0], d[1], up, &hi[0], &lo[0]);
+    pair(d[2], d[3], up, &hi[1], &lo[1]);
+    lower(d);
+    h8 eh[2], el[2];
+    float e_down;
+    unit(most4(s), &up, &e_down);
+    pair(s[0], s[1], up, &eh[0], &el[0]);
+    pair(s[2], s[3], up, &eh[1], &el[1]);
     // outputs
+    {
+      const Base of(op);
+      const int at = 4 * lg * o_stride + 4 * lr;
+      const float y_by = m_down * a.scale, d_by = down * a.scale;
 #pragma unroll
-    for (int jt = 0; jt < 2; ++jt) {
-      f32x4 o = {0, 0, 0, 0};
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 of_q = of_token(1, t) * y_by, of_p = of_token(3, t) * d_by;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 zero = {0, 0, 0, 0};
-        o = add_times(o, du_s[0][j][jt][lr], mma16(pf[j], d_s[0][j][jt][lane], zero));
+        for (int e = 0; e < 4; ++e) d[t][e] = fmaf(of_q[e], y[t][e], of_p[e] * d[t][e]);
       }
-      o = (unit(1) * y[jt] + unit(3) * o) * a.scale;
+      if (left >= kCk) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (16 * w + 4 * lg + e < left) op[e * (a.h_v * kCkS) + 16 * jt] = o[e];
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) of.store1(d[t][e], at, (16 * t + e) * o_stride);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * t + 4 * lg + e < left) of.store1(d[t][e], at, (16 * t + e) * o_stride);
+      }
     }
-    op += static_cast<size_t>(kCk) * a.h_v * kCkS;
-    // the new state
+    // the new state, half of its dims at a time
     const float all = vec[5 * kCk];
+    h8 kt[2][4][2];
+    const auto read_kt = [&](int step) {
 #pragma unroll
-    for (int jt = 0; jt < 2; ++jt)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int d = 0; d < 2; ++d) m[jt][d] *= all;
+        for (int k = 0; k < 2; ++k)
+          kt[step & 1][i][k] = u_at[(2 * (4 * (step >> 1) + i) + (step & 1)) * 128 + 64 * k];
+    };
+    f32x4 u[4];
+    read_kt(0);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int step = 0; step < 4; ++step) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (step + 1 < 4) read_kt(step + 1);
+      const int p = step & 1;
 #pragma unroll
-      for (int jt = 0; jt < 2; ++jt) {
-        const h8 b = d_s[1][t][jt][lane];
-        const float by = du_s[1][t][jt][lr];
-        const f32x4 zero = {0, 0, 0, 0};
+      for (int k = 0; k < 3; ++k)
 #pragma unroll
-        for (int d = 0; d < 2; ++d) m[jt][d] = add_times(m[jt][d], by, mma16(kt[d][t], b, zero));
-      }
+        for (int i = 0; i < 4; ++i)
+          u[i] = mma(kt[p][i][k == 0], k == 1 ? el[p] : eh[p], p == 0 && k == 0 ? f32x4{0, 0, 0, 0} : u[i]);
+      if (p == 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4 &to_m = m[4 * (step >> 1) + i];
+          to_m = add_times(to_m * all, e_down, u[i]);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    op += static_cast<size_t>(kCk) * a.h_v * kCkS;
+    ws_k += slot_bytes, ws_v += slot_bytes;
   }
   if (to < 0) return;
 #pragma unroll
-  for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-      *reinterpret_cast<f32x4 *>(a.state + to * a.rag.slot_stride + row0 + 16 * jt * kCkS + 16 * d) = m[jt][d];
+  for (int d = 0; d < 8; ++d)
+    *reinterpret_cast<f32x4 *>(a.state + to * a.rag.slot_stride + m_at + 16 * d) = m[d];
 }
 
 // Blocks of a launch: a grid has fewer than 2^32 threads a dimension.
@@ -820,7 +890,9 @@ bool whole_rows(const bh_gdn_ragged_args &p) {
 // Slots of chunks of a call, 0: it has none.
 size_t chunk_slots(const bh_gdn_ragged_args &p) {
   const size_t most = p.max_new == 0 || p.max_new > p.n_tok ? p.n_tok : p.max_new;
-  if (p.s != static_cast<size_t>(kCkS) || most < static_cast<size_t>(kCkMin) || !whole_rows(p)) return 0;
+  if (p.s != static_cast<size_t>(kCkS) || most < static_cast<size_t>(kCkMin) || !whole_rows(p) ||
+      p.v_stride > kMostStride)
+    return 0;
   return p.n_tok * 3 / 128 + 1;
 }
 
@@ -866,11 +938,15 @@ extern "C" int bh_gdn_ragged(const bh_gdn_ragged_args *args, bh_stream stream) {
     }
     a.most = kCkMin - 1;
     const size_t longs = p.n_tok / kCkMin < p.n_req ? p.n_tok / kCkMin : p.n_req;
-    GdnChunkArgs c{a, ws, static_cast<int>(slots), static_cast<int>(longs),
-                   p.h_k % 8 == 0 && p.h_v % p.h_k == 0};
+    GdnChunkArgs c{a, ws, static_cast<int>(slots), 0, p.h_k % 8 == 0 && p.h_v % p.h_k == 0};
     BH_LAUNCH(gdn_chunk_prep_kernel, static_cast<unsigned>(slots * p.h_k), kBlock, 0, st, c);
-    BH_LAUNCH(gdn_chunk_walk_kernel, static_cast<unsigned>(longs * p.h_v * (kCkS / kCkRows)), kBlock,
-              0, st, c);
+    const bool few = longs * p.h_v * 2 <= device_cu_count();
+    const size_t per = few ? 2 * p.h_v : p.h_v;
+    c.walks = static_cast<int>(longs * per);
+    const unsigned blocks = static_cast<unsigned>((longs + p.n_req) * per);
+    if (few) BH_LAUNCH(gdn_chunk_walk_kernel<4>, blocks, 256, 0, st, c);
+    else BH_LAUNCH(gdn_chunk_walk_kernel<8>, blocks, 512, 0, st, c);
+    return ok();
   }
   const auto blocks = [&](size_t rows) { return static_cast<unsigned>(p.n_req * p.h_v * p.s / rows); };
   if (whole && p.s == 128) {
