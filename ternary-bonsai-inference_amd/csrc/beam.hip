@@ -25,8 +25,10 @@ namespace bh {
 namespace {
 
 constexpr int kMostFirsts = 1024;  // parts of a group
-constexpr int kOwn = kMostFirsts / kLpThreads;
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;  // of a group's block
+constexpr int kOwn = kMostFirsts / kSelThreads;
 constexpr int kMostCand = 1024;    // candidates that are ranked at once
+constexpr int kAhead = 2;          // keys of a thread on their way
 
 struct BeamArgs {
   const float *score;
@@ -58,13 +60,16 @@ __device__ __forceinline__ T lane_xor(T x, int by) {
 }
 
 // One block a group.
-__global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
+__global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
   __shared__ double base_s[BH_MAX_BEAMS];  // score - ln S; NaN: no continuations
   __shared__ float m_s[BH_MAX_BEAMS];
-  __shared__ Cand cand[kMostCand];
-  __shared__ Cand best_s[kLpWaves];
-  __shared__ uint32_t bound_s[kLpWaves];
-  __shared__ int count_s, best_at[kLpWaves];
+  __shared__ __attribute__((aligned(16))) double score_s[kMostCand];  // of the candidates
+  __shared__ uint64_t key_s[kMostCand];
+  __shared__ uint8_t beam_s[kMostCand];
+  __shared__ Cand best_s[kSelWaves];
+  __shared__ uint32_t bound_s[kSelWaves];
+  __shared__ int count_s, n_live_s, best_at[kSelWaves];
+  __shared__ uint16_t live_s[kMostFirsts];  // parts whose first reaches the bound
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row0 = blockIdx.x * a.width, firsts = a.width * a.n_parts;
   const size_t part0 = static_cast<size_t>(row0) * a.n_parts;
@@ -72,11 +77,11 @@ __global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
   uint64_t first[kOwn];
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    const int p = tid + i * kLpThreads;
+    const int p = tid + i * kSelThreads;
     first[i] = p < firsts ? a.keys[(part0 + p) * a.n_best] : 0;
   }
-  if (tid == 0) count_s = 0;
-  for (int b = wave; b < a.width; b += kLpWaves) {
+  if (tid == 0) count_s = n_live_s = 0;
+  for (int b = wave; b < a.width; b += kSelWaves) {
     const Part *parts = a.parts + part0 + static_cast<size_t>(b) * a.n_parts;
     Part p[2] = {{0.0, 0.0, -INFINITY}, {0.0, 0.0, -INFINITY}};
     static_assert(kMaxParts == 128, "two parts a lane");
@@ -110,7 +115,7 @@ __global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    const int p = tid + i * kLpThreads;
+    const int p = tid + i * kSelThreads;
     if (p >= firsts) continue;
     const Cand c = of(p / a.n_parts, first[i]);
     const float f = static_cast<float>(c.score);
@@ -121,22 +126,32 @@ __global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
   __syncthreads();
   uint32_t bound = 0;
 #pragma unroll
-  for (int w = 0; w < kLpWaves; ++w) bound = bound_s[w] > bound ? bound_s[w] : bound;
+  for (int w = 0; w < kSelWaves; ++w) bound = bound_s[w] > bound ? bound_s[w] : bound;
   const auto reaches = [&](const Cand &c) {
     return c.score > -INFINITY && order_of(static_cast<float>(c.score)) >= bound;
   };
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    const int p = tid + i * kLpThreads;
-    if (p >= firsts) continue;
-    const int beam = p / a.n_parts;
-    const uint64_t *keys = a.keys + (part0 + p) * a.n_best;
-    Cand c = of(beam, first[i]);
-    for (int k = 0; reaches(c);) {
+    const int p = tid + i * kSelThreads;
+    if (p < firsts && reaches(of(p / a.n_parts, first[i]))) live_s[atomicAdd(&n_live_s, 1)] = p;
+  }
+  __syncthreads();
+  const int n_keys = n_live_s * a.n_best;
+  for (int i0 = tid; i0 < n_keys; i0 += kAhead * kSelThreads) {
+    uint64_t key[kAhead];
+    int of_part[kAhead];
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      const int i = min(i0 + x * kSelThreads, n_keys - 1), at = i / a.n_best;
+      of_part[x] = live_s[at];
+      key[x] = a.keys[(part0 + of_part[x]) * a.n_best + (i - at * a.n_best)];
+    }
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      const Cand c = of(of_part[x] / a.n_parts, key[x]);
+      if (i0 + x * kSelThreads >= n_keys || !reaches(c)) continue;
       const int at = atomicAdd(&count_s, 1);
-      if (at < kMostCand) cand[at] = c;
-      if (++k == a.n_best) break;
-      c = of(beam, keys[k]);
+      if (at < kMostCand) score_s[at] = c.score, key_s[at] = c.key, beam_s[at] = c.beam;
     }
   }
   __syncthreads();
@@ -153,13 +168,27 @@ __global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
     a.score_out[out + place] = -INFINITY;
   };
   if (count <= kMostCand) {
-    for (int i = tid; i < count; i += kLpThreads) {
-      const Cand c = cand[i];
-      int rank = 0;
-      for (int k = 0; k < count; ++k) rank += cand[k].before(c);
-      if (rank < a.n_best) put(rank, c);
+    // four lanes a candidate, each against every fourth
+    for (int i = count + tid; i < min((count + 31) & ~31, kMostCand); i += kSelThreads) score_s[i] = -INFINITY;
+    __syncthreads();
+    for (int i0 = 0; i0 < count; i0 += kSelThreads / 4) {
+      const int i = min(i0 + tid / 4, count - 1);
+      const Cand c{score_s[i], key_s[i], beam_s[i]};
+      int rank = 0, same = 0;
+      for (int k = tid & 3; k < count; k += 32) {
+#pragma unroll
+        for (int x = 0; x < 32; x += 4)
+          rank += score_s[k + x] > c.score, same += score_s[k + x] == c.score;
+      }
+      if (__any(lane_group_sum<4>(static_cast<float>(same)) > 1.0f)) {  // (its own is one)
+#pragma unroll 4
+        for (int k = tid & 3; k < count; k += 4)
+          rank += score_s[k] == c.score && Cand{score_s[k], key_s[k], beam_s[k]}.before(c);
+      }
+      rank = static_cast<int>(lane_group_sum<4>(static_cast<float>(rank)));
+      if ((tid & 3) == 0 && i0 + tid / 4 < count && rank < a.n_best) put(rank, c);
     }
-    for (int i = count + tid; i < a.n_best; i += kLpThreads) none(i);
+    for (int i = count + tid; i < a.n_best; i += kSelThreads) none(i);
     return;
   }
   // Too many equal ones: the parts' lists merged, one continuation a round.
@@ -167,7 +196,7 @@ __global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
   Cand head[kOwn];
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    const int p = tid + i * kLpThreads;
+    const int p = tid + i * kSelThreads;
     next[i] = 1;
     head[i] = p < firsts ? of(p / a.n_parts, first[i]) : Cand{-INFINITY, 0, a.width};
   }
@@ -176,7 +205,7 @@ __global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
     int at = tid;
 #pragma unroll
     for (int i = 1; i < kOwn; ++i)
-      if (head[i].before(best)) best = head[i], at = tid + i * kLpThreads;
+      if (head[i].before(best)) best = head[i], at = tid + i * kSelThreads;
 #pragma unroll
     for (int by = 32; by > 0; by >>= 1) {
       const Cand o{lane_xor(best.score, by),
@@ -190,7 +219,7 @@ __global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
     __syncthreads();
     best = best_s[0], at = best_at[0];
 #pragma unroll
-    for (int w = 1; w < kLpWaves; ++w)
+    for (int w = 1; w < kSelWaves; ++w)
       if (best_s[w].before(best)) best = best_s[w], at = best_at[w];
     if (tid == 0) {
       if (best.score > -INFINITY) put(place, best);
@@ -198,7 +227,7 @@ __global__ __launch_bounds__(kLpThreads) void beam_select_kernel(BeamArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int p = tid + i * kLpThreads;
+      const int p = tid + i * kSelThreads;
       if (p != at || p >= firsts) continue;
       head[i].score = -INFINITY;
       if (next[i] < a.n_best)
@@ -421,7 +450,7 @@ extern "C" int bh_beam_select(const bh_beam_select_args *args, bh_stream stream)
   a.score = p.score, a.parent = p.parent, a.token = p.token, a.score_out = p.score_out;
   a.width = static_cast<int>(p.width), a.n_best = l.n_top, a.n_parts = l.n_parts;
   a.inv_temp = l.inv_temp, a.k2 = l.k2, a.parts = l.parts, a.keys = l.keys;
-  BH_LAUNCH(beam_select_kernel, static_cast<unsigned>(p.n_group), kLpThreads, 0, st, a);
+  BH_LAUNCH(beam_select_kernel, static_cast<unsigned>(p.n_group), kSelThreads, 0, st, a);
   return ok();
 }
 
