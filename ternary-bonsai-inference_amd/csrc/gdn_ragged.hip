@@ -277,16 +277,17 @@ __device__ __forceinline__ void wave_sync() {
 // bits each, which saves the vector arithmetic of 64-bit addresses.
 struct Base {
   __amdgpu_buffer_rsrc_t of;
-  __device__ explicit Base(const void *p)
-      : of(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, 0x7fffffff, 0x00027000)) {}
+  // (what lies past `bytes` reads as 0 and is not written)
+  __device__ explicit Base(const void *p, int bytes = 0x7fffffff)
+      : of(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00027000)) {}
   __device__ __forceinline__ h8 load(int lane_at, int at) const {
     return __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(of, lane_at, at, 0));
   }
-  __device__ __forceinline__ float load1(int lane_at, int at) const {
-    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(of, lane_at, at, 0));
+  __device__ __forceinline__ float load1(int lane_at) const {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(of, lane_at, 0, 0));
   }
-  __device__ __forceinline__ void store1(float x, int lane_at, int at) const {
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), of, lane_at, at, 0);
+  __device__ __forceinline__ void store1(float x, int lane_at) const {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), of, lane_at, 0, 0);
   }
 };
 constexpr int kTri[4] = {0, 1, 2, 4};  // 16 x 32 tiles to the diagonal before row i
@@ -625,54 +626,25 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
   for (int d = 0; d < 8; ++d)
     m[d] = from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + from * a.rag.slot_stride + m_at + 16 * d)
                      : f32x4{0, 0, 0, 0};
+  // Pieces on their way to LDS: one is stored and the next chunk's loaded in its place.
   h8 in_a[kAs], in_b[kBk + kBt];
   f32x4 in_vec;
-  const auto load_a = [&](const char *p) {
-    const Base k(p);
-#pragma unroll
-    for (int i = 0; i < kAs; ++i) in_a[i] = k.load(16 * threadIdx.x, i * kThreads * 16);
-  };
-  const auto store_a = [&] {
-#pragma unroll
-    for (int i = 0; i < kAs; ++i) kq_s[i * kThreads + threadIdx.x] = in_a[i];
+  const int piece = 16 * threadIdx.x;
+  const auto load_a = [&](const Base &k, int i) { in_a[i] = k.load(piece, i * kThreads * 16); };
+  const auto load_b = [&](const Base &k, const Base &v, int i) {
+    in_b[i] = i < kBk ? k.load(piece, 2 * kFragK + i * kThreads * 16) : v.load(piece, (i - kBk) * kThreads * 16);
   };
   const int vec_i = min(static_cast<int>(threadIdx.x), kVecs / 4 - 1);  // (the last ones the same)
-  const auto load_b = [&](const char *k, const char *v) {
-    const Base of_k(k), of_v(v);
-#pragma unroll
-    for (int i = 0; i < kBk; ++i) in_b[i] = of_k.load(16 * threadIdx.x, 2 * kFragK + i * kThreads * 16);
-#pragma unroll
-    for (int i = 0; i < kBt; ++i) in_b[kBk + i] = of_v.load(16 * threadIdx.x, i * kThreads * 16);
-    in_vec = __builtin_bit_cast(f32x4, of_v.load(16 * vec_i, 2 * kFragT));
-  };
-  const auto store_b = [&](int chunk) {
-#pragma unroll
-    for (int i = 0; i < kBk + kBt; ++i) u_s[i * kThreads + threadIdx.x] = in_b[i];
-    reinterpret_cast<f32x4 *>(vec_s[chunk & 1])[vec_i] = in_vec;
-  };
+  const auto load_vec = [&](const Base &v) { in_vec = __builtin_bit_cast(f32x4, v.load(16 * vec_i, 2 * kFragT)); };
   // v and outputs: tokens 16 t + 4 lg + e
   const int v_stride = 4 * static_cast<int>(a.v_stride), o_stride = 4 * a.h_v * kCkS;
   const float *vp = a.v + static_cast<size_t>(begin) * a.v_stride + row_w;
   float *op = a.attn + static_cast<size_t>(begin) * a.h_v * kCkS + row_w;
+  const int v_at = 4 * lg * v_stride + 4 * lr, o_at = 4 * lg * o_stride + 4 * lr;
   f32x4 v[4];
-  const auto load_v = [&](int left) {  // of the chunk at vp, of which `left` tokens are the request's
-    const Base of(vp);
-    if (left >= kCk) {
-      const int at = 4 * lg * v_stride + 4 * lr;
+  const auto load_v = [&](const Base &of, int t) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[t][e] = of.load1(at, (16 * t + e) * v_stride);
-    } else {
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 16 * t + 4 * lg + e;
-          const float x = of.load1(min(i, left - 1) * v_stride + 4 * lr, 0);
-          v[t][e] = i < left ? x : 0.0f;
-        }
-    }
+    for (int e = 0; e < 4; ++e) v[t][e] = of.load1(v_at + (16 * t + e) * v_stride);
   };
   // 32 or 64 of a lane's values as operands, in units of a power of two
   const auto unit = [&](float most, float *up, float *down) { unit_of(most_of_lanes(most), up, down); };
@@ -687,17 +659,45 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
   };
   const h8 *k_at = kq_s + lane, *u_at = u_s + lane;
 
-  load_a(ws_k);
-  load_b(ws_k, ws_v);
-  load_v(n);
-  store_a();
-  if (chunks > 1) load_a(ws_k + slot_bytes);
+  {
+    const Base k(ws_k), of_v(ws_v), rows(vp, min(n, kCk) * v_stride);
+#pragma unroll
+    for (int i = 0; i < kAs; ++i) load_a(k, i);
+#pragma unroll
+    for (int i = 0; i < kBk + kBt; ++i) load_b(k, of_v, i);
+    load_vec(of_v);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) load_v(rows, t);
+    const Base k1(chunks > 1 ? ws_k + slot_bytes : ws_k);
+#pragma unroll
+    for (int i = 0; i < kAs; ++i) {
+      kq_s[i * kThreads + threadIdx.x] = in_a[i];
+      load_a(k1, i);
+    }
+  }
   for (int chunk = 0; chunk < chunks; ++chunk) {
     const int left = n - chunk * kCk;
-    const bool more = chunk + 1 < chunks;
+    // the chunks whose pieces load now (past the last: the last again, read by nobody)
+    const int ahead = min(chunks - 1 - chunk, 2);
+    const Base next_k(ws_k + min(ahead, 1) * slot_bytes), next_v(ws_v + min(ahead, 1) * slot_bytes);
+    const Base after_k(ws_k + ahead * slot_bytes);
     const float *vec = vec_s[chunk & 1];
     const auto of_token = [&](int i, int t) {
       return *reinterpret_cast<const f32x4 *>(vec + i * kCk + 16 * t + 4 * lg);
+    };
+    const auto stage_a = [&](int part, int parts) {
+#pragma unroll
+      for (int i = kAs * part / parts; i < kAs * (part + 1) / parts; ++i) {
+        kq_s[i * kThreads + threadIdx.x] = in_a[i];
+        load_a(after_k, i);
+      }
+    };
+    const auto stage_b = [&](int part, int parts) {
+#pragma unroll
+      for (int i = (kBk + kBt) * part / parts; i < (kBk + kBt) * (part + 1) / parts; ++i) {
+        u_s[i * kThreads + threadIdx.x] = in_b[i];
+        load_b(next_k, next_v, i);
+      }
     };
     float up, m_down;
     h8 mh[4], ml[4];
@@ -724,12 +724,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
           z[t] = mma(f[step & 1][t][p == 0], p == 1 ? ml[i] : mh[i], i == 0 && p == 0 ? f32x4{0, 0, 0, 0} : z[t]);
     };
     read(0);
-    store_b(chunk);
-    if (more) load_b(ws_k + slot_bytes, ws_v + slot_bytes);
+    reinterpret_cast<f32x4 *>(vec_s[chunk & 1])[vec_i] = in_vec;
+    load_vec(next_v);
 #pragma unroll
     for (int step = 0; step < 8; ++step) {
       __builtin_amdgcn_sched_barrier(0);
       if (step + 1 < 8) read(step + 1);
+      if (step < 7) stage_b(step, 7);
       times(step, step < 4 ? x : y);
     }
     __syncthreads();  // K and Q are read; the others are there
@@ -749,12 +750,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
     unit(most4(s), &up, &down);
     pair(s[0], s[1], up, &hi[0], &lo[0]);
     pair(s[2], s[3], up, &hi[1], &lo[1]);
-    if (more) {
-      store_a();
-      if (left > 2 * kCk) load_a(ws_k + 2 * slot_bytes);
-      vp += kCk * a.v_stride;
-      load_v(left - kCk);
-    }
+    __builtin_amdgcn_sched_barrier(0);
     // a row tile of T or P against the operand
     const auto lower = [&](f32x4 *d) {
 #pragma unroll
@@ -767,8 +763,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
     };
     // delta, and delta e with K's units
     f32x4 d[4];
+    vp += kCk * a.v_stride;
+    const Base rows(ahead ? vp : a.v, ahead ? min(left - kCk, kCk) * v_stride : 0);
+    stage_a(0, 8);
     lower(d);
+    load_v(rows, 0);
+    load_v(rows, 1);
     __builtin_amdgcn_sched_barrier(0);
+    stage_a(1, 8);
 #pragma unroll
     for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[(kFragK + kFragT) / 16 + i * 64];
 #pragma unroll
@@ -779,6 +781,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
     pair(d[0], d[1], up, &hi[0], &lo[0]);
     pair(d[2], d[3], up, &hi[1], &lo[1]);
     lower(d);
+    stage_a(2, 8);
+    load_v(rows, 2);
+    load_v(rows, 3);
     h8 eh[2], el[2];
     float e_down;
     unit(most4(s), &up, &e_down);
@@ -786,8 +791,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
     pair(s[2], s[3], up, &eh[1], &el[1]);
     // outputs
     {
-      const Base of(op);
-      const int at = 4 * lg * o_stride + 4 * lr;
       const float y_by = m_down * a.scale, d_by = down * a.scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -795,19 +798,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[t][e] = fmaf(of_q[e], y[t][e], of_p[e] * d[t][e]);
       }
-      if (left >= kCk) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) of.store1(d[t][e], at, (16 * t + e) * o_stride);
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (16 * t + 4 * lg + e < left) of.store1(d[t][e], at, (16 * t + e) * o_stride);
-      }
     }
+    stage_a(3, 8);
+    const Base to_rows(op, min(left, kCk) * o_stride);
     // the new state, half of its dims at a time
     const float all = vec[5 * kCk];
     h8 kt[2][4][2];
@@ -824,6 +817,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
     for (int step = 0; step < 4; ++step) {
       __builtin_amdgcn_sched_barrier(0);
       if (step + 1 < 4) read_kt(step + 1);
+      stage_a(4 + step, 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to_rows.store1(d[step][e], o_at + (16 * step + e) * o_stride);
       const int p = step & 1;
 #pragma unroll
       for (int k = 0; k < 3; ++k)
