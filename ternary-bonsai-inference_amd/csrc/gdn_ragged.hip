@@ -338,39 +338,53 @@ __device__ __forceinline__ void prep_head(const GdnArgs &a, int h, int t0, int n
   if (lane == kCk - 1) vec[5 * kCk] = decay;
   wave_sync();
   // P in its order, L into `l`: a tile's D_ts below the diagonal is e^(G_t - G_r)
-  // e^(G_r - G_s), r the last token of s's tile: neither factor passes 1
+  // e^(G_r - G_s), r the last token of s's tile: neither factor passes 1.  (All of LDS is
+  // read before the first is written: one wait instead of one a tile.)
+  f32x4 qk[4][4], kk[4][4];
+  double Gt[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = 16 * i + lr;
-    const double Gt = G_s[t];
+    Gt[i] = G_s[t];
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+      const int s = 16 * j + 4 * lg;
+      qk[i][j] = *reinterpret_cast<const f32x4 *>(kq + t * kPitch + s);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) kk[i][j][e] = kq[(s + e) * kPitch + t];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 16 * i + lr;
     const float bt = b_s[t];
-    f32x4 p[4];
+    f32x4 p[4], lv[4];
     float most = 0.0f;
 #pragma unroll
     for (int j = 0; j <= i; ++j) {
       const int s = 16 * j + 4 * lg;
-      const f32x4 q = *reinterpret_cast<const f32x4 *>(kq + t * kPitch + s);
-      f32x4 d, lv;
+      f32x4 d;
       if (j < i) {
-        const float u = exp_hw(static_cast<float>(Gt - G_s[16 * j + 15]));
+        const float u = exp_hw(static_cast<float>(Gt[i] - G_s[16 * j + 15]));
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[e] = u * w_s[s + e];
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float arg = static_cast<float>(Gt - G_s[s + e]);
+          const float arg = static_cast<float>(Gt[i] - G_s[s + e]);
           d[e] = s + e <= t ? exp_hw(arg < 0.0f ? arg : 0.0f) : 0.0f;
         }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool in = j < i || s + e <= t, under = j < i || s + e < t;
-        p[j][e] = in ? d[e] * q[e] : 0.0f;
-        lv[e] = under ? bt * d[e] * kq[(s + e) * kPitch + t] : 0.0f;
+        p[j][e] = in ? d[e] * qk[i][j][e] : 0.0f;
+        lv[j][e] = under ? bt * d[e] * kk[i][j][e] : 0.0f;
       }
       most = fmaxf(most, most_of(p[j]));
-      *reinterpret_cast<f32x4 *>(l + t * kPitch + s) = lv;
     }
+#pragma unroll
+    for (int j = 0; j <= i; ++j) *reinterpret_cast<f32x4 *>(l + t * kPitch + 16 * j + 4 * lg) = lv[j];
     float up, down;
     unit_of(most_of_lanes(most), &up, &down);
     store_row(out + kFragT + kTri[i] * 2048, p, i + 1, up, lane);
@@ -511,23 +525,31 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
   __syncthreads();
   // Q K^T and K K^T of the wave's tokens against those before: a row of one operand is a
   // column of the other, in the same lanes
+  h8 of_j[2][8];
+  const auto read = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) of_j[j & 1][i] = k_lds[(j * 4 + (i >> 1)) * 128 + 64 * (i & 1) + lane];
+  };
+  read(0);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (j > w) continue;
-    f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+    if (j > w) break;
+    if (j + 1 < 4) read(j + 1);
+    f32x4 kk[2], qk[2];  // two chains each
+#pragma unroll
+    for (int x = 0; x < 2; ++x) kk[x] = qk[x] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const h8 bh = k_lds[(j * 4 + i) * 128 + lane], bl = k_lds[(j * 4 + i) * 128 + 64 + lane];
-      kk = mma32(kh_[i], kl[i], bh, bl, kk);
-      qk = mma32(qh[i], ql[i], bh, bl, qk);
+      kk[i & 1] = mma32(kh_[i], kl[i], of_j[j & 1][2 * i], of_j[j & 1][2 * i + 1], kk[i & 1]);
+      qk[i & 1] = mma32(qh[i], ql[i], of_j[j & 1][2 * i], of_j[j & 1][2 * i + 1], qk[i & 1]);
     }
     const int s = 16 * j + lr;  // column
     const float ds = k_down[s];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int t = 16 * w + 4 * lg + e;
-      if (s <= t) kq[t * kPitch + s] = qk[e] * q_down[t] * ds;
-      if (s < t) kq[s * kPitch + t] = kk[e] * k_down[t] * ds;
+      if (s <= t) kq[t * kPitch + s] = (qk[0][e] + qk[1][e]) * q_down[t] * ds;
+      if (s < t) kq[s * kPitch + t] = (kk[0][e] + kk[1][e]) * k_down[t] * ds;
     }
   }
   // K transposed: tile (d, p) of 16 dims and 32 tokens, lane's dim 16 d + lr
