@@ -212,10 +212,13 @@ constexpr int kVWaves = 3;                       // v-heads prepared side by sid
 
 struct GdnChunkArgs {
   GdnArgs g;
-  char *ws;    // [slots][h_k kHeadK + h_v kHeadV]
-  int slots;   // of chunks
-  int walks;   // blocks of the walk
-  int xcd;     // the blocks of a q/k head on one die
+  char *ws;      // [slots][h_k kHeadK + h_v kHeadV]
+  int slots;     // of chunks
+  int walks;     // blocks of the walk
+  int xcd;       // the blocks of a q/k head on one die
+  int at_once;   // compute units / h_v
+  int longs;     // requests of kCkMin tokens or more there can be
+  int32_t *todo; // their number; they
 };
 
 // Where request r's chunks begin: n >= 128 tokens have ceil(n / 64) <= 3 n / 128.
@@ -459,6 +462,39 @@ __device__ __forceinline__ void prep_head(const GdnArgs &a, int h, int t0, int n
   wave_sync();
 }
 
+// The requests of kCkMin tokens or more, the longest first where a wave holds them all.
+// (At most `longs`: of offsets that decrease there may be more.)
+__device__ __forceinline__ void list_long(const Ragged &rag, int longs, int32_t *todo) {
+  const int lane = threadIdx.x & 63;
+  const auto tokens = [&](int r) {
+    int begin, n;
+    rag.tokens(r, &begin, &n);
+    return n;
+  };
+  int count = 0, own = -1;  // own: the lane-th of them
+  for (int i0 = 0; i0 < rag.n_req; i0 += 64) {
+    const uint64_t is = __ballot(i0 + lane < rag.n_req && tokens(min(i0 + lane, rag.n_req - 1)) >= kCkMin);
+    const int at = count + __popcll(is & ((uint64_t{1} << lane) - 1));
+    if ((is >> lane & 1) && at < longs) todo[1 + at] = i0 + lane;
+    uint64_t left = is;
+    for (int k = count; k <= lane && left != 0; ++k, left &= left - 1)
+      if (k == lane) own = i0 + __builtin_ffsll(left) - 1;
+    count += __popcll(is);
+  }
+  count = min(count, longs);
+  if (lane == 0) todo[0] = count;
+  if (count > 64) return;
+  if (lane >= count) own = -1;
+  const int n = own >= 0 ? tokens(own) : 0;
+  int rank = 0;
+  for (int k = 0; k < count; ++k) {
+    const int of = __builtin_amdgcn_readlane(n, k);
+    rank += of > n || (of == n && k < lane);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");  // behind the first writes
+  if (own >= 0) todo[1 + rank] = own;
+}
+
 // Block (chunk, q/k head): wave w has the tokens 16 w .. 16 w + 15.
 __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs c) {
   constexpr int kMat = kCk * kPitch;
@@ -469,6 +505,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
   __shared__ float w_s[kVWaves][kCk], b_s[kVWaves][kCk], k_down[kCk], q_down[kCk];
   const GdnArgs &a = c.g;
   const int slot = blockIdx.x / a.h_k, kh = blockIdx.x - slot * a.h_k;
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x < 64) list_long(a.rag, c.longs, c.todo);
   const int r = last_request(a.rag.n_req, [&](int i) {
     return first_chunk(min(max(a.rag.q_start[i], 0), a.rag.n_tok)) <= slot;
   });
@@ -581,83 +618,95 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
   }
 }
 
-// The nth request of kCkMin tokens or more; -1: there are not so many.
-__device__ __forceinline__ int nth_long(const Ragged &rag, int nth) {
-  const int lane = threadIdx.x & 63;
-  for (int i0 = 0; i0 < rag.n_req; i0 += 64) {
-    int begin, n = 0;
-    if (i0 + lane < rag.n_req) rag.tokens(i0 + lane, &begin, &n);
-    uint64_t is = __ballot(n >= kCkMin);
-    const int here = __popcll(is);
-    if (nth < here) {
-      for (; nth > 0; --nth) is &= is - 1;
-      return i0 + __builtin_ffsll(is) - 1;
+// The walk.  A wave has 16 state rows to itself and takes them through the chunks in
+// registers: every result is the next product's operand as it stands.  The operands that
+// the waves share stand in LDS, K and Q apart from K transposed, T and P, so that each
+// part of the next chunk comes in while the other is read: two barriers a chunk.
+
+// Operands of a chunk in LDS: K, Q; K transposed, T, P; their vectors, of two chunks in
+// turn.
+constexpr int kA = 2 * kFragK / 16, kB = (kFragK + 2 * kFragT) / 16;  // pieces of 16 bytes
+struct ChunkLds {
+  h8 kq[kA], u[kB];
+  float vec[2][kVecs];
+};
+struct WalkOf {
+  int begin, n, from, to;  // a request's tokens and slots
+  int h, row;              // v-head; a wave's first state row
+  const char *ws_k, *ws_v;
+  size_t slot_bytes;
+};
+
+// Pieces on their way to LDS: one is stored and the next chunk's loaded in its place.
+// THREADS threads do it, of which this is number tid.
+template <int THREADS>
+struct Stage {
+  static constexpr int kAs = kA / THREADS, kBk = kFragK / 16 / THREADS, kBt = 2 * kFragT / 16 / THREADS;
+  static_assert(kAs * THREADS == kA && (kBk + kBt) * THREADS == kB, "whole pieces a thread");
+  h8 in_a[kAs], in_b[kBk + kBt];
+  f32x4 in_vec;
+  int tid, vec_i;
+  __device__ __forceinline__ void load_a(const Base &k, int i) { in_a[i] = k.load(16 * tid, i * THREADS * 16); }
+  __device__ __forceinline__ void load_b(const Base &k, const Base &v, int i) {
+    in_b[i] = i < kBk ? k.load(16 * tid, 2 * kFragK + i * THREADS * 16) : v.load(16 * tid, (i - kBk) * THREADS * 16);
+  }
+  __device__ __forceinline__ void load_vec(const Base &v) {
+    in_vec = __builtin_bit_cast(f32x4, v.load(16 * vec_i, 2 * kFragT));
+  }
+  // The first chunk's, and the second's A on its way.
+  __device__ __forceinline__ void begin(ChunkLds &lds, const WalkOf &o, int chunks, int thread) {
+    tid = thread, vec_i = min(tid, kVecs / 4 - 1);  // (the last ones the same)
+    const Base k(o.ws_k), v(o.ws_v), k1(chunks > 1 ? o.ws_k + o.slot_bytes : o.ws_k);
+#pragma unroll
+    for (int i = 0; i < kAs; ++i) load_a(k, i);
+#pragma unroll
+    for (int i = 0; i < kBk + kBt; ++i) load_b(k, v, i);
+    load_vec(v);
+#pragma unroll
+    for (int i = 0; i < kAs; ++i) {
+      lds.kq[i * THREADS + tid] = in_a[i];
+      load_a(k1, i);
     }
-    nth -= here;
   }
-  return -1;
-}
+  // A part of the next chunk's A (and the one's after it on its way), of this chunk's B.
+  __device__ __forceinline__ void a(ChunkLds &lds, const Base &after_k, int part, int parts) {
+#pragma unroll
+    for (int i = kAs * part / parts; i < kAs * (part + 1) / parts; ++i) {
+      lds.kq[i * THREADS + tid] = in_a[i];
+      load_a(after_k, i);
+    }
+  }
+  __device__ __forceinline__ void b(ChunkLds &lds, const Base &next_k, const Base &next_v, int part, int parts) {
+#pragma unroll
+    for (int i = (kBk + kBt) * part / parts; i < (kBk + kBt) * (part + 1) / parts; ++i) {
+      lds.u[i * THREADS + tid] = in_b[i];
+      load_b(next_k, next_v, i);
+    }
+  }
+  __device__ __forceinline__ void vec(ChunkLds &lds, const Base &next_v, int chunk) {
+    reinterpret_cast<f32x4 *>(lds.vec[chunk & 1])[vec_i] = in_vec;
+    load_vec(next_v);
+  }
+};
 
-// Block (request, v-head, 16 WAVES state rows).  A wave has 16 rows to itself and takes
-// them through the chunks in registers: every result is the next product's operand as it
-// stands.  The operands that the waves share stand in LDS, K and Q apart from K
-// transposed, T and P, so that each part of the next chunk comes in while the other
-// is read: two barriers a chunk.
-template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(GdnChunkArgs c) {
-  constexpr int kThreads = 64 * WAVES, kRows = 16 * WAVES, kSlabs = kCkS / kRows;
-  constexpr int kA = 2 * kFragK / 16, kB = (kFragK + 2 * kFragT) / 16;
-  constexpr int kAs = kA / kThreads, kBk = kFragK / 16 / kThreads, kBt = 2 * kFragT / 16 / kThreads;
-  static_assert(kAs * kThreads == kA && (kBk + kBt) * kThreads == kB, "whole pieces a thread");
-  __shared__ __attribute__((aligned(16))) h8 kq_s[kA];           // K, Q
-  __shared__ __attribute__((aligned(16))) h8 u_s[kB];            // K transposed, T, P
-  __shared__ __attribute__((aligned(16))) float vec_s[2][kVecs];  // of two chunks in turn
-  const GdnArgs &a = c.g;
-  if (static_cast<int>(blockIdx.x) >= c.walks) {  // the requests of fewer tokens
-    step_rows<kCkS, 4, kThreads>(a, blockIdx.x - c.walks);
-    return;
-  }
-  const int per = a.h_v * kSlabs, nth = blockIdx.x / per;
-  int rest = blockIdx.x - nth * per, h, slab;
-  if (c.xcd) {  // block b runs on die b % 8: q/k heads x, x + 8, .. on die x
-    const int of_head = a.h_v / a.h_k * kSlabs, x = rest & 7, y = rest >> 3;
-    const int kh = y / of_head * 8 + x, z = y % of_head;
-    h = kh + z / kSlabs * a.h_k, slab = z % kSlabs;
-  } else {
-    h = rest / kSlabs, slab = rest % kSlabs;
-  }
-  const int r = nth_long(a.rag, nth);
-  if (r < 0) return;
-  int begin, n, from, to;
-  a.rag.tokens_of(r, &begin, &n);
-  a.rag.slots(r, &from, &to);
-  const int kh = h % a.h_k;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int lr = lane & 15, lg = lane >> 4;
+// A wave's 16 rows through the chunks.  SHARES: it stages its part of the operands too.
+template <bool SHARES>
+__device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const WalkOf &of) {
+  const int begin = of.begin, n = of.n;
+  const char *ws_k = of.ws_k, *ws_v = of.ws_v;
+  const size_t slot_bytes = of.slot_bytes;
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int chunks = (n + kCk - 1) / kCk;
-  const size_t slot_bytes = static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(a.h_v) * kHeadV;
-  const char *ws_k = c.ws + static_cast<size_t>(first_chunk(begin)) * slot_bytes + static_cast<size_t>(kh) * kHeadK;
-  const char *ws_v = c.ws + static_cast<size_t>(first_chunk(begin)) * slot_bytes +
-                     static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(h) * kHeadV;
-
+  Stage<512> stage;
+  if constexpr (SHARES) stage.begin(lds, of, chunks, threadIdx.x);
   // m[d]: state row lr of the wave's, dims 16 d + 4 lg ..
-  const int row_w = h * kCkS + slab * kRows + 16 * w;
+  const int row_w = of.h * kCkS + of.row;
   const size_t m_at = (static_cast<size_t>(row_w) + lr) * kCkS + 4 * lg;
   f32x4 m[8];
 #pragma unroll
   for (int d = 0; d < 8; ++d)
-    m[d] = from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + from * a.rag.slot_stride + m_at + 16 * d)
+    m[d] = of.from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + of.from * a.rag.slot_stride + m_at + 16 * d)
                      : f32x4{0, 0, 0, 0};
-  // Pieces on their way to LDS: one is stored and the next chunk's loaded in its place.
-  h8 in_a[kAs], in_b[kBk + kBt];
-  f32x4 in_vec;
-  const int piece = 16 * threadIdx.x;
-  const auto load_a = [&](const Base &k, int i) { in_a[i] = k.load(piece, i * kThreads * 16); };
-  const auto load_b = [&](const Base &k, const Base &v, int i) {
-    in_b[i] = i < kBk ? k.load(piece, 2 * kFragK + i * kThreads * 16) : v.load(piece, (i - kBk) * kThreads * 16);
-  };
-  const int vec_i = min(static_cast<int>(threadIdx.x), kVecs / 4 - 1);  // (the last ones the same)
-  const auto load_vec = [&](const Base &v) { in_vec = __builtin_bit_cast(f32x4, v.load(16 * vec_i, 2 * kFragT)); };
   // v and outputs: tokens 16 t + 4 lg + e
   const int v_stride = 4 * static_cast<int>(a.v_stride), o_stride = 4 * a.h_v * kCkS;
   const float *vp = a.v + static_cast<size_t>(begin) * a.v_stride + row_w;
@@ -679,23 +728,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
   const auto most4 = [](const f32x4 *x) {
     return fmaxf(fmaxf(most_of(x[0]), most_of(x[1])), fmaxf(most_of(x[2]), most_of(x[3])));
   };
-  const h8 *k_at = kq_s + lane, *u_at = u_s + lane;
-
+  const h8 *k_at = lds.kq + lane, *u_at = lds.u + lane;
   {
-    const Base k(ws_k), of_v(ws_v), rows(vp, min(n, kCk) * v_stride);
-#pragma unroll
-    for (int i = 0; i < kAs; ++i) load_a(k, i);
-#pragma unroll
-    for (int i = 0; i < kBk + kBt; ++i) load_b(k, of_v, i);
-    load_vec(of_v);
+    const Base rows(vp, min(n, kCk) * v_stride);
 #pragma unroll
     for (int t = 0; t < 4; ++t) load_v(rows, t);
-    const Base k1(chunks > 1 ? ws_k + slot_bytes : ws_k);
-#pragma unroll
-    for (int i = 0; i < kAs; ++i) {
-      kq_s[i * kThreads + threadIdx.x] = in_a[i];
-      load_a(k1, i);
-    }
   }
   for (int chunk = 0; chunk < chunks; ++chunk) {
     const int left = n - chunk * kCk;
@@ -703,23 +740,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
     const int ahead = min(chunks - 1 - chunk, 2);
     const Base next_k(ws_k + min(ahead, 1) * slot_bytes), next_v(ws_v + min(ahead, 1) * slot_bytes);
     const Base after_k(ws_k + ahead * slot_bytes);
-    const float *vec = vec_s[chunk & 1];
+    const float *vec = lds.vec[chunk & 1];
     const auto of_token = [&](int i, int t) {
       return *reinterpret_cast<const f32x4 *>(vec + i * kCk + 16 * t + 4 * lg);
     };
     const auto stage_a = [&](int part, int parts) {
-#pragma unroll
-      for (int i = kAs * part / parts; i < kAs * (part + 1) / parts; ++i) {
-        kq_s[i * kThreads + threadIdx.x] = in_a[i];
-        load_a(after_k, i);
-      }
+      if constexpr (SHARES) stage.a(lds, after_k, part, parts);
     };
     const auto stage_b = [&](int part, int parts) {
-#pragma unroll
-      for (int i = (kBk + kBt) * part / parts; i < (kBk + kBt) * (part + 1) / parts; ++i) {
-        u_s[i * kThreads + threadIdx.x] = in_b[i];
-        load_b(next_k, next_v, i);
-      }
+      if constexpr (SHARES) stage.b(lds, next_k, next_v, part, parts);
     };
     float up, m_down;
     h8 mh[4], ml[4];
@@ -746,8 +775,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
           z[t] = mma(f[step & 1][t][p == 0], p == 1 ? ml[i] : mh[i], i == 0 && p == 0 ? f32x4{0, 0, 0, 0} : z[t]);
     };
     read(0);
-    reinterpret_cast<f32x4 *>(vec_s[chunk & 1])[vec_i] = in_vec;
-    load_vec(next_v);
+    if constexpr (SHARES) stage.vec(lds, next_v, chunk);
 #pragma unroll
     for (int step = 0; step < 8; ++step) {
       __builtin_amdgcn_sched_barrier(0);
@@ -859,10 +887,75 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void gdn_chunk_walk_kernel(G
     op += static_cast<size_t>(kCk) * a.h_v * kCkS;
     ws_k += slot_bytes, ws_v += slot_bytes;
   }
-  if (to < 0) return;
+  if (of.to < 0) return;
 #pragma unroll
   for (int d = 0; d < 8; ++d)
-    *reinterpret_cast<f32x4 *>(a.state + to * a.rag.slot_stride + m_at + 16 * d) = m[d];
+    *reinterpret_cast<f32x4 *>(a.state + of.to * a.rag.slot_stride + m_at + 16 * d) = m[d];
+}
+
+// Blocks of the walk.  All rows of a (request, v-head) are a block's, 16 a wave; or, of the
+// longest requests, as far as blocks are fewer than compute units, half of them, and the
+// other four waves stage the operands.  What bounds a block is its waves' reads of them
+// from LDS (120 KB a wave and chunk), so half the rows are through sooner: 4.7 us a chunk
+// for 7.2.
+__global__ __launch_bounds__(512, 2) void gdn_chunk_walk_kernel(GdnChunkArgs c) {
+  __shared__ __attribute__((aligned(16))) ChunkLds lds;
+  const GdnArgs &a = c.g;
+  if (static_cast<int>(blockIdx.x) >= c.walks) {  // the requests of fewer tokens
+    step_rows<kCkS, 4, 512>(a, blockIdx.x - c.walks);
+    return;
+  }
+  const int count = __builtin_amdgcn_readfirstlane(c.todo[0]);
+  // requests in halves
+  const int halves = count > 64 ? 0 : min(count, max(c.at_once - count, 0));
+  int nth = blockIdx.x / (2 * a.h_v), rest = blockIdx.x - nth * 2 * a.h_v;
+  const bool half = nth < halves;
+  if (!half) {
+    rest = blockIdx.x - 2 * halves * a.h_v;
+    nth = rest / a.h_v;
+    rest -= nth * a.h_v;
+    nth += halves;
+  }
+  if (nth >= count) return;
+  const int r = __builtin_amdgcn_readfirstlane(c.todo[1 + nth]), slabs = half ? 2 : 1;
+  WalkOf of;
+  int slab;
+  if (c.xcd) {  // block b runs on die b % 8: q/k heads x, x + 8, .. on die x
+    const int of_head = a.h_v / a.h_k * slabs, x = rest & 7, y = rest >> 3;
+    const int kh = y / of_head * 8 + x, z = y % of_head;
+    of.h = kh + z / slabs * a.h_k, slab = z % slabs;
+  } else {
+    of.h = rest / slabs, slab = rest % slabs;
+  }
+  a.rag.tokens_of(r, &of.begin, &of.n);
+  a.rag.slots(r, &of.from, &of.to);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  of.slot_bytes = static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(a.h_v) * kHeadV;
+  of.ws_k = c.ws + static_cast<size_t>(first_chunk(of.begin)) * of.slot_bytes +
+            static_cast<size_t>(of.h % a.h_k) * kHeadK;
+  of.ws_v = c.ws + static_cast<size_t>(first_chunk(of.begin)) * of.slot_bytes +
+            static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(of.h) * kHeadV;
+  of.row = slab * (kCkS / 2) + 16 * (half ? w & 3 : w);
+  if (!half) {
+    walk_rows<true>(a, lds, of);
+  } else if (w < 4) {
+    walk_rows<false>(a, lds, of);
+  } else {  // the barriers are walk_rows'
+    const int chunks = (of.n + kCk - 1) / kCk;
+    Stage<256> stage;
+    stage.begin(lds, of, chunks, threadIdx.x - 256);
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+      const int ahead = min(chunks - 1 - chunk, 2);
+      const Base next_k(of.ws_k + min(ahead, 1) * of.slot_bytes), next_v(of.ws_v + min(ahead, 1) * of.slot_bytes);
+      const Base after_k(of.ws_k + ahead * of.slot_bytes);
+      __syncthreads();
+      stage.vec(lds, next_v, chunk);
+      stage.b(lds, next_k, next_v, 0, 1);
+      __syncthreads();
+      stage.a(lds, after_k, 0, 1);
+      of.ws_k += of.slot_bytes, of.ws_v += of.slot_bytes;
+    }
+  }
 }
 
 // Blocks of a launch: a grid has fewer than 2^32 threads a dimension.
@@ -916,6 +1009,17 @@ size_t chunk_slots(const bh_gdn_ragged_args &p) {
 
 size_t slot_bytes(const bh_gdn_ragged_args &p) { return p.h_k * kHeadK + p.h_v * kHeadV; }
 
+// Requests of kCkMin tokens or more that there can be.
+size_t most_long(const bh_gdn_ragged_args &p) {
+  return p.n_tok / kCkMin < p.n_req ? p.n_tok / kCkMin : p.n_req;
+}
+
+// The chunks' operands, and the list of the requests that go by chunks.
+size_t workspace_of(const bh_gdn_ragged_args &p) {
+  const size_t slots = chunk_slots(p);
+  return slots == 0 ? 0 : slots * slot_bytes(p) + (1 + most_long(p)) * sizeof(int32_t);
+}
+
 }  // namespace
 }  // namespace bh
 
@@ -923,7 +1027,7 @@ using namespace bh;
 
 extern "C" size_t bh_gdn_ragged_workspace(const bh_gdn_ragged_args *args) {
   if (!args || check(*args) != BH_OK || args->n_req == 0 || args->n_tok == 0) return 0;
-  return chunk_slots(*args) * slot_bytes(*args);
+  return workspace_of(*args);
 }
 
 extern "C" int bh_gdn_ragged(const bh_gdn_ragged_args *args, bh_stream stream) {
@@ -943,7 +1047,7 @@ extern "C" int bh_gdn_ragged(const bh_gdn_ragged_args *args, bh_stream stream) {
   const bool whole = whole_rows(p);
   a.most = 0x7fffffff;
   if (const size_t slots = chunk_slots(p)) {
-    const size_t need = slots * slot_bytes(p);
+    const size_t need = workspace_of(p);
     char *ws = static_cast<char *>(p.workspace);
     if (ws) {
       if (!aligned16(ws) || p.workspace_bytes < need)
@@ -955,15 +1059,15 @@ extern "C" int bh_gdn_ragged(const bh_gdn_ragged_args *args, bh_stream stream) {
       if (!ws) return BH_ERR_HIP;
     }
     a.most = kCkMin - 1;
-    const size_t longs = p.n_tok / kCkMin < p.n_req ? p.n_tok / kCkMin : p.n_req;
-    GdnChunkArgs c{a, ws, static_cast<int>(slots), 0, p.h_k % 8 == 0 && p.h_v % p.h_k == 0};
+    const size_t longs = most_long(p);
+    const size_t at_once = device_cu_count() / p.h_v;
+    size_t walks = 2 * longs;  // of h_v blocks
+    if (walks > at_once) walks = longs > at_once ? longs : at_once;
+    GdnChunkArgs c{a, ws, static_cast<int>(slots), static_cast<int>(walks * p.h_v),
+                   p.h_k % 8 == 0 && p.h_v % p.h_k == 0, static_cast<int>(at_once), static_cast<int>(longs),
+                   reinterpret_cast<int32_t *>(ws + slots * slot_bytes(p))};
     BH_LAUNCH(gdn_chunk_prep_kernel, static_cast<unsigned>(slots * p.h_k), kBlock, 0, st, c);
-    const bool few = longs * p.h_v * 2 <= device_cu_count();
-    const size_t per = few ? 2 * p.h_v : p.h_v;
-    c.walks = static_cast<int>(longs * per);
-    const unsigned blocks = static_cast<unsigned>((longs + p.n_req) * per);
-    if (few) BH_LAUNCH(gdn_chunk_walk_kernel<4>, blocks, 256, 0, st, c);
-    else BH_LAUNCH(gdn_chunk_walk_kernel<8>, blocks, 512, 0, st, c);
+    BH_LAUNCH(gdn_chunk_walk_kernel, static_cast<unsigned>((walks + p.n_req) * p.h_v), 512, 0, st, c);
     return ok();
   }
   const auto blocks = [&](size_t rows) { return static_cast<unsigned>(p.n_req * p.h_v * p.s / rows); };
