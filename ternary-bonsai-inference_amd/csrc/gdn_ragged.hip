@@ -199,7 +199,10 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr int kCk = 64, kCkS = 128;
-constexpr int kCkMin = 128;           // tokens from which a request goes by chunks
+// Tokens from which a request goes by chunks.  One request of 32 / 48 / 64 / 127 tokens, us:
+// 24.3, 24.7, 25.1, 29.2, token by token 17.2, 24.3, 30.8, 63.3; 64 of 32 259 for 317.
+constexpr int kCkMin = 48;
+constexpr int kCkPlace = 32;          // a chunk's place in the workspace every so many tokens
 constexpr int kFragK = kCk * kCkS * 4;           // bytes of K as halves; Q, K transposed
 constexpr int kHeadK = 3 * kFragK;               // of a (chunk, q/k head)
 constexpr int kFragT = 12 * 64 * 16;             // of T's and P's 16 x 32 tiles to the diagonal
@@ -221,10 +224,10 @@ struct GdnChunkArgs {
   int32_t *todo; // their number; they
 };
 
-// Where request r's chunks begin: n >= 128 tokens have ceil(n / 64) <= 3 n / 128.
-__device__ __forceinline__ int first_chunk(int begin) {
-  return static_cast<int>(static_cast<int64_t>(begin) * 3 / 128);
-}
+// Where the chunks of a request begin whose first token is `begin`: from 32 tokens on n
+// have ceil(n / 64) <= floor(n / 32), and a floor of a sum is no less than the floors'.
+static_assert(kCkMin >= kCkPlace, "");
+__device__ __forceinline__ int first_chunk(int begin) { return begin / kCkPlace; }
 
 // The unit of values of which `most` is the largest: x up is its number of units.  (Of
 // 0, an infinity or NaN the exponent is 0.)
@@ -981,9 +984,9 @@ int check(const bh_gdn_ragged_args &p) {
       !mul_size(p.n_tok, p.v_stride, sizeof(float), &n) || p.n_slots > 0x7fffffffu ||
       !mul_size(p.n_slots, p.slot_stride, sizeof(float), &n))
     return fail(BH_ERR_SHAPE, "gdn_ragged: size overflow");
-  // (a chunk's block a q/k head; chunks are fewer than n_tok / 40 and one)
-  if (!mul_size(p.n_tok / 40 + 1, p.h_k, &n) || n > kMostBlocks ||
-      !mul_size(p.n_tok / 40 + 1, p.h_k * kHeadK + p.h_v * kHeadV, &n))
+  // (a chunk's block a q/k head; a place every kCkPlace tokens)
+  if (!mul_size(p.n_tok / kCkPlace + 1, p.h_k, &n) || n > kMostBlocks ||
+      !mul_size(p.n_tok / kCkPlace + 1, p.h_k * kHeadK + p.h_v * kHeadV, &n))
     return fail(BH_ERR_SHAPE, "gdn_ragged: size overflow");
   if (p.n_req != 0 && p.n_tok != 0) {
     if (!p.q || !p.k || !p.v || !p.gate || !p.beta || !p.attn || !p.q_start || !p.src_slot ||
@@ -1004,7 +1007,7 @@ size_t chunk_slots(const bh_gdn_ragged_args &p) {
   if (p.s != static_cast<size_t>(kCkS) || most < static_cast<size_t>(kCkMin) || !whole_rows(p) ||
       p.v_stride > kMostStride)
     return 0;
-  return p.n_tok * 3 / 128 + 1;
+  return p.n_tok / kCkPlace + 1;
 }
 
 size_t slot_bytes(const bh_gdn_ragged_args &p) { return p.h_k * kHeadK + p.h_v * kHeadV; }
