@@ -46,17 +46,14 @@ __global__ __launch_bounds__(kThreads) void attn_shared_join_kernel(PagedArgs a,
   const SharedCut cut = static_cast<const SharedCut *>(sp.cut)[tile];
   // (past n_tiles cut holds nothing; a prefix's tiles have no rows of their own)
   if (tile >= *sp.n_tiles || cut.r < a.n_group) return;
-  int q0, n, len, g;
-  request(a, cut.r - a.n_group, &q0, &n, &len);
   Prefix pre;
-  if (shared_of(a, cut.r - a.n_group, n, len, &g) > 0) {
-    group_tokens(a, g, &pre.q0, &pre.n);
+  if (cut.group >= 0) {
+    const PrefixOf of_group = a.prefix[cut.group];
+    pre.q0 = of_group.q0, pre.n = of_group.n, pre.base = of_group.base, pre.two = of_group.launch != 0;
     const int64_t rows = static_cast<int64_t>(pre.n) * a.group;
-    pre.two = rows <= one.sp.over || rows > one.sp.most;
     const Split &of = pre.two ? two.sp : one.sp;
     pre.rows = pre.two ? two.rows : one.rows;
     pre.tiles = static_cast<int>((rows + pre.rows - 1) / pre.rows);
-    pre.base = of.base[g];
     pre.most = min(static_cast<uint32_t>(*of.n_tiles), of.most_cut);
   }
   const Split psp = pre.two ? two.sp : one.sp;
@@ -175,6 +172,8 @@ int shared_forms(const bh_attention_shared_args &p, Form *f) {
   return forms_of(q, f);
 }
 
+size_t prefix_bytes(const PagedArgs &a) { return align256(a.n_group * sizeof(PrefixOf)); }
+
 int prepare_shared(const bh_attention_shared_args &p, PagedArgs *a) {
   if (int e = prepare(p.paged, a, "attention_shared")) return e;
   if (p.n_group > 0x7fff0000u || p.paged.n_req + p.n_group > 0x7fff0000u)
@@ -201,7 +200,7 @@ extern "C" size_t bh_attention_shared_workspace(const bh_attention_shared_args *
   Form f[2];
   size_t need = 0;
   for (int i = 0, n = shared_forms(*args, f); i < n; ++i) need += workspace_of<true>(a, f[i]);
-  return need;
+  return need + prefix_bytes(a);
 }
 
 extern "C" int bh_attention_shared(const bh_attention_shared_args *args, bh_stream stream) {
@@ -215,7 +214,7 @@ extern "C" int bh_attention_shared(const bh_attention_shared_args *args, bh_stre
   hipStream_t st = as_stream(stream);
   Form f[2];
   const int n = shared_forms(p, f);
-  size_t need = 0, tiles = 0;
+  size_t need = prefix_bytes(a), tiles = 0;
   for (int i = 0; i < n; ++i) {
     need += workspace_of<true>(a, f[i]);
     tiles += most_tiles<true>(a, f[i]);
@@ -233,7 +232,10 @@ extern "C" int bh_attention_shared(const bh_attention_shared_args *args, bh_stre
     if (!ws) return BH_ERR_HIP;
   }
   Join join[2] = {};
+  a.prefix = reinterpret_cast<PrefixOf *>(ws);
+  ws += prefix_bytes(a);
   for (int i = 0; i < n; ++i) {
+    a.launch = i;
     if (int e = launch_form<true>(a, f16, f[i], ws, st, &join[i])) return e;
     ws += workspace_of<true>(a, f[i]);
   }

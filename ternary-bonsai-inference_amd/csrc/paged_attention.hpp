@@ -29,6 +29,14 @@ struct PagedArgs {
   // of requests that share a prefix
   const int32_t *group_of, *group_start, *shared_len;
   int n_group;
+  struct PrefixOf *prefix;  // [n_group]
+  int launch;               // which of the call's
+};
+
+// Where the tiles of a group's prefix are: their launch and their first place in it, and
+// the group's tokens.
+struct PrefixOf {
+  int launch, base, q0, n;
 };
 
 __device__ __forceinline__ float cache_at(const float *p) { return *p; }
@@ -78,6 +86,7 @@ struct Cut {  // a tile, written by the worker of its first part
 };
 struct SharedCut : Cut {
   int r, tile;  // request, place among the launch's tiles in the line's order
+  int group;    // whose prefix its rows see, -1: none
 };
 template <bool SHARED>
 using CutOf = std::conditional_t<SHARED, SharedCut, Cut>;
@@ -89,7 +98,6 @@ struct Split {
   float *pacc;     // [workers][2][R][hd]
   int workers;
   int over, most;  // requests of more than `over` and up to `most` rows a kv head
-  int *base;       // SHARED: [n_group] where the tiles of a group's prefix begin
 };
 
 // x / d; by the 32-bit divide, a tenth of the 64-bit one, where that does.
@@ -131,10 +139,10 @@ __device__ __forceinline__ int group_tokens(const PagedArgs &a, int g, int *q0, 
 // Of SHARED work: its first position; its row of the table, below 0: ~row, and a
 // group's prefix.
 struct Part_of {
-  int first, row;
+  int first, row, group;  // group: whose prefix ends at `first`, -1: none
 };
 struct All_of {
-  static constexpr int first = 0, row = 0;
+  static constexpr int first = 0, row = 0, group = -1;
 };
 template <bool SHARED>
 using Extent = std::conditional_t<SHARED, Part_of, All_of>;
@@ -144,6 +152,7 @@ template <int R, int U, bool SHARED>
 struct Work : Extent<SHARED> {
   using Extent<SHARED>::first;
   using Extent<SHARED>::row;
+  using Extent<SHARED>::group;
   int q0, n, len;  // first token, tokens (0: not this launch's), positions
   int tiles, pair, mid;  // units of a pair of tiles; of the one in the middle, or 0
   int64_t head;          // units of a kv head
@@ -159,7 +168,7 @@ struct Work : Extent<SHARED> {
   }
   __device__ __forceinline__ void load(const PagedArgs &a, const Split &sp, int r) {
     if constexpr (SHARED) {
-      first = 0;
+      first = 0, group = -1;
       if (r < a.n_group) {
         row = ~group_tokens(a, r, &q0, &n);
         len = min(max(a.shared_len[r], 0), a.max_len);
@@ -168,6 +177,7 @@ struct Work : Extent<SHARED> {
         int g;
         request(a, row, &q0, &n, &len);
         first = shared_of(a, row, n, len, &g);
+        if (first > 0) group = g;
       }
     } else {
       request(a, r, &q0, &n, &len);
@@ -189,7 +199,8 @@ struct Work : Extent<SHARED> {
     len = __builtin_amdgcn_readlane(len, l), tiles = __builtin_amdgcn_readlane(tiles, l);
     pair = __builtin_amdgcn_readlane(pair, l), mid = __builtin_amdgcn_readlane(mid, l);
     if constexpr (SHARED)
-      first = __builtin_amdgcn_readlane(first, l), row = __builtin_amdgcn_readlane(row, l);
+      first = __builtin_amdgcn_readlane(first, l), row = __builtin_amdgcn_readlane(row, l),
+      group = __builtin_amdgcn_readlane(group, l);
     head = static_cast<int64_t>(tiles / 2) * pair + mid;
   }
 };
@@ -679,8 +690,8 @@ struct Walk {
         const uint32_t i = static_cast<uint32_t>(tile_base + head * work.tiles + nth);
         p->slot = uni(static_cast<int>(min(i, sp.most_cut - 1)) + worker);
         p->whole = false;
-        p->first = uni(work.first), p->row = uni(work.row);
-        work.first = p->first, work.row = p->row;
+        p->first = uni(work.first), p->row = uni(work.row), p->group = uni(work.group);
+        work.first = p->first, work.row = p->row, work.group = p->group;
       }
       at = wave_uniform(at), base = wave_uniform(base), tile_base = uni(tile_base), r = p->r;
       work.q0 = p->q0, work.n = p->n, work.len = p->len, work.tiles = uni(work.tiles);
@@ -700,8 +711,9 @@ struct Walk {
       const uint32_t i = static_cast<uint32_t>(tile_base + p.head * work.tiles + p.tile);
       if constexpr (SHARED) {
         if (i < sp.most_cut)
-          static_cast<SharedCut *>(sp.cut)[i] = SharedCut{cut, p.r, p.slot - worker};
-        if (p.r < a.n_group && p.head == 0 && p.tile == 0) sp.base[p.r] = tile_base;
+          static_cast<SharedCut *>(sp.cut)[i] = SharedCut{cut, p.r, p.slot - worker, p.group};
+        if (p.r < a.n_group && p.head == 0 && p.tile == 0)
+          a.prefix[p.r] = PrefixOf{a.launch, tile_base, p.q0, p.n};
       } else {
         if (i < sp.most_cut) sp.cut[i] = cut;
       }
@@ -1534,12 +1546,12 @@ size_t part_rows(const PagedArgs &a, const Form &f) {
   return (f.workers() * size_t{2} + (SHARED ? most_tiles<SHARED>(a, f) - f.workers() : 0)) * f.rows();
 }
 
-// Workspace: tile count, tiles, maxima, sums, accumulators, the groups' first tiles.
+// Workspace: tile count, tiles, maxima, sums, accumulators.
 template <bool SHARED>
 size_t workspace_of(const PagedArgs &a, const Form &f) {
   const size_t parts = part_rows<SHARED>(a, f);
   return 256 + align256(most_tiles<SHARED>(a, f) * sizeof(CutOf<SHARED>)) + 2 * align256(parts * 4) +
-         align256(parts * a.hd * 4) + (SHARED ? align256(a.n_group * size_t{4}) : 0);
+         align256(parts * a.hd * 4);
 }
 
 // Where a launch's parts lie in its workspace.
@@ -1558,7 +1570,6 @@ Split split_of(const PagedArgs &a, const Form &f, char *ws) {
   sp.pl = reinterpret_cast<float *>(ws);
   ws += align256(parts * 4);
   sp.pacc = reinterpret_cast<float *>(ws);
-  if (SHARED) sp.base = reinterpret_cast<int *>(ws + align256(parts * a.hd * 4));
   return sp;
 }
 
