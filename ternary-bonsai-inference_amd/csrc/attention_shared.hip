@@ -162,13 +162,51 @@ int launch_shared_join(const PagedArgs &a, const Join &one, const Join &two, hip
   return BH_OK;
 }
 
-// As forms_of, the prefix of a group being a request of all the group's rows.
+// As forms_of, the prefix of a group being a request of all the group's rows; but the
+// tiles of a prefix read the same pages, which then come from the last level cache, so
+// that small tiles, whose steps are shorter, cost less than there, and one launch saves
+// more than the wide form's larger tiles while the work is small.  What counts is the work
+// as far as the host knows it: rows of the call times positions of the table, in millions.
+// Measured, us of the call, in order: as in forms_of, one row tile, two; "rows" of a group.
+//   up to 64 rows.  hd 256, f16: 0.2 38, 30, 38; 1.2 110, 79, 108; 2.4 205, 146, 205
+//     f32: 0.4 47, 47, 47; 1.0 (60 rows) 105, 117, 105; 2.4 (48 rows: three tiles for
+//     four) 259, 246, 257
+//     hd 128, f16: 0.13 27, 24, 27; 0.5 (24 rows) 43, 46, 43; 1.0 (48 rows) 74, 66, 73
+//     f32: 0.13 31, 29, 31; 0.28 40, 42, 40; 1.1 91, 122, 90
+//     hd 64, f16: 0.3 17, 16, 17; 1.0 25, 23, 25; 3.1 31, 42, 31; f32: 0.3 19, 16, 18; 1.6 33, 39, 32
+//   more.  hd 256, f16: 0.4 46, 29, 38; 0.7 58, 54, 75; 0.8 53, 61, 67; 1.5 74, 102, 137
+//     f32: 0.4 87, 57, 57; 1.3 149, 129, 119; 1.7 151, 175, 156
+//     hd 128, f16: 0.5 51, 44, 50; 0.8 52, 58, 57; f32: 0.25 52, 27, 28; 0.5 72, 71, 66; 2.4 119, 131, 114
+//     hd 64, f16: 1.1 33, 22, 25; 2.1 36, 33, 28; 4.7 42, 35, 29; f32: 0.6 38, 21, 24; 1.3 40, 35, 32;
+//     4.7 53, 47, 45
 int shared_forms(const bh_attention_shared_args &p, Form *f) {
   bh_attention_paged_args q = p.paged;
   const size_t own = q.max_new == 0 || q.max_new > q.n_tok ? q.n_tok : q.max_new;
   const size_t all = p.max_group_new == 0 || p.max_group_new > q.n_tok ? q.n_tok : p.max_group_new;
   q.max_new = all > own ? all : own;
   q.n_req = 2;  // not one request's: both sorts are there
+  const size_t group = q.n_head / q.cache.n_kv, rows = q.max_new * group;
+  const double work = 1e-6 * static_cast<double>(q.n_tok * group) *
+                      static_cast<double>(q.table_width * q.cache.page_size);
+  // up to which one tile is taken: up to 64 rows, of more; two tiles of more
+  struct Line {
+    double few, one, two;
+  };
+  const bool f16 = q.cache.kv_dtype == BH_KV_F16;
+  const Line line = q.cache.hd == 256   ? (f16 ? Line{1e30, 0.75, 0} : Line{0.45, 1.3, 0})
+                    : q.cache.hd == 128 ? (f16 ? Line{0.45, 0.75, 0} : Line{0.13, 0.25, 2.5})
+                                        : (f16 ? Line{1.1, 1.5, 5} : Line{0.8, 1.0, 5});
+  // (an odd number of tiles of 16 rows leaves half of the last two empty)
+  const bool odd = (rows + 15) / 16 % 2 == 1 && rows <= 64 && f16 != (q.cache.hd == 256) && q.cache.hd != 64;
+  constexpr int kAll = 0x7fffffff;
+  if (odd || work <= (rows <= 64 ? line.few : line.one)) {
+    f[0] = Form{1, false, 0, kAll, 2};
+    return 1;
+  }
+  if (rows > 64 && work <= line.two) {
+    f[0] = Form{2, false, 0, kAll, 2};
+    return 1;
+  }
   return forms_of(q, f);
 }
 
