@@ -323,7 +323,7 @@ struct CopyArgs {
   FastDiv page, row, head;                      // row, head: pieces of T
 };
 
-constexpr int kCopyItems = 4;  // pieces a thread has on their way at once
+constexpr int kCopyItems = 2;  // pieces a thread has on their way at once
 
 // Block (request, share): the request's pieces of sizeof(T) bytes, position by
 // position, kCopyItems a thread at a time.
@@ -506,8 +506,11 @@ int launch_copy(const bh_kv_copy_args &p, hipStream_t st) {
   a.page = FastDiv(static_cast<uint32_t>(c.page_size));
   a.row = FastDiv(static_cast<uint32_t>(a.elems));
   a.head = FastDiv(static_cast<uint32_t>(a.hd));
-  // about eight blocks a compute unit, as many as the table's longest could need
-  size_t blocks = 8 * device_cu_count() / p.n_req;
+  // 64 blocks a compute unit, of which those of requests without a copy are gone at once, or
+  // as many as the table's longest could need: blocks that go round twice wait twice.  54 of
+  // 128 beams, 255 positions each (117 MB): 8 a unit, 4 pieces a thread 32.2 us; 16 26.3, 32
+  // 23.2; 64 and 2 pieces 20.3, 128 and 1 21.2.
+  size_t blocks = 64 * device_cu_count() / p.n_req;
   const size_t most = (static_cast<size_t>(a.max_len) * a.elems + 256 * kCopyItems - 1) / (256 * kCopyItems);
   if (blocks > most) blocks = most;
   if (blocks < 1) blocks = 1;
