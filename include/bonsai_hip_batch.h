@@ -190,9 +190,9 @@ size_t bh_beam_select_workspace(const bh_beam_select_args *args);
  *
  * States (all three slot arrays or none): src_slot = dst_slot of the parent (its
  * own without one), which is what the parent's last step wrote, and dst_slot and
- * spare_slot change places.  Before the first step dst_slot holds the slots
- * of the beams' states; the 2 * n_group * width slots of dst_slot and spare_slot
- * are distinct.
+ * spare_slot change places.  Before the first selection the beams' states are in
+ * dst_slot, or, where a step goes before it, in src_slot, of which spare_slot is a
+ * copy; the 2 * n_group * width slots of dst_slot and spare_slot are distinct.
  *
  * No scratch.  parent must not be one of the outputs. */
 typedef struct bh_beam_reorder_args {
