@@ -181,20 +181,23 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_any_kernel(GdnArgs a) {
 //   m' = A_63 m + sum_s e_s delta_s k_s,                  e_s = A_63 / A_s,
 // where T, P, A and e are those of a (chunk, v-head), whatever the row.
 // gdn_chunk_prep_kernel forms them, all chunks at once; gdn_chunk_walk_kernel takes
-// 32 rows of a state through their chunks.
+// the rows of a state through their chunks.
 //
-// Products are of f16 matrix instructions, each operand as hi + lo halves of 22 bits
-// (hi hi + hi lo + lo hi, a third of the f32 instruction's time) in units of a power
-// of two that brings the largest of what shares a unit to 2^14 .. 2^15: a token's row
-// of K and of Q, a row of T and of P; of the operands that carry state rows, a row j
-// and the 32 dims or the 16 tokens of one wave, whose products are summed apart.  An
-// operand's error is 2^-22 of the largest beside it, as that of a few f32 sums.
+// Products are of f16 matrix instructions, each operand as hi + lo halves (hi hi + hi lo +
+// lo hi, a third of the f32 instruction's time) in units of a power of two that brings
+// the largest of what shares a unit to 2^14 .. 2^15: a token's row of K and of Q, a row of T
+// and of P, a state row, its 64 right sides and deltas.  The halves keep 22 bits of each
+// value down to 2^-17 of the largest, and 2^-40 of that one below: both round, by half a step
+// of 11 bits each, or of f16's last place.
 //
 // Operands stand in memory as the instructions take them.  In 16x16x32 lane (lr =
 // lane % 16, lg = lane / 16) holds row lr and the 8 of the 32 summed over that are
-// 4 lg + i and 16 + 4 lg + i, i < 4; in 16x16x16 the 4 that are 4 lg + i.  Those are
-// the places that a result's lane holds of its column, so results become operands as
-// they stand.
+// 4 lg + i and 16 + 4 lg + i, i < 4.  Those are the places that a result's lane holds of
+// its column, so results become operands as they stand.
+//
+// A product over tokens that are not before a row's has weights of 0 there, which a value
+// that is not finite would make NaN: where a delta is not finite, a wave takes its rows through
+// the request again, token by token, before it leaves their state.  So do gates above 0.
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
@@ -336,7 +339,10 @@ __device__ __forceinline__ void prep_head(const GdnArgs &a, int h, int t0, int n
   const double last = __shfl(G, kCk - 1);
   const double end = __shfl(G, lane | 15);  // of the lane's tile of 16 tokens
   w_s[lane] = exp_hw(static_cast<float>(end - G));
-  const float decay = expf(static_cast<float>(G)), left = expf(static_cast<float>(last - G));
+  // (A state that grows would share its units with one far larger: such a chunk's decays are
+  // NaN, and its request goes token by token.)
+  const bool grows = __any(g > 0.0f);
+  const float decay = grows ? NAN : expf(static_cast<float>(G)), left = expf(static_cast<float>(last - G));
   float *vec = reinterpret_cast<float *>(out + 2 * kFragT);
   vec[lane] = decay * k_down[lane];
   vec[kCk + lane] = decay * q_down[lane];
@@ -344,8 +350,8 @@ __device__ __forceinline__ void prep_head(const GdnArgs &a, int h, int t0, int n
   if (lane == kCk - 1) vec[5 * kCk] = decay;
   wave_sync();
   // P in its order, L into `l`: a tile's D_ts below the diagonal is e^(G_t - G_r)
-  // e^(G_r - G_s), r the last token of s's tile: neither factor passes 1.  (All of LDS is
-  // read before the first is written: one wait instead of one a tile.)
+  // e^(G_r - G_s), r the last token of s's tile: of decays neither factor passes 1.  (All of
+  // LDS is read before the first is written: one wait instead of one a tile.)
   f32x4 qk[4][4], kk[4][4];
   double Gt[4];
 #pragma unroll
@@ -378,7 +384,7 @@ __device__ __forceinline__ void prep_head(const GdnArgs &a, int h, int t0, int n
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float arg = static_cast<float>(Gt[i] - G_s[s + e]);
-          d[e] = s + e <= t ? exp_hw(arg < 0.0f ? arg : 0.0f) : 0.0f;
+          d[e] = s + e <= t ? exp_hw(arg) : 0.0f;
         }
       }
 #pragma unroll
@@ -692,6 +698,43 @@ struct Stage {
   }
 };
 
+// Sum over lanes lr, lr + 16, lr + 32, lr + 48.
+__device__ __forceinline__ float sum_of_lanes(float x) {
+  float lo, hi;
+  lane_swap<16>(x, lo, hi);
+  x = lo + hi;
+  lane_swap<32>(x, lo, hi);
+  return lo + hi;
+}
+
+// A request's tokens one by one; m as walk_rows has it.
+__device__ __forceinline__ void walk_tokens(const GdnArgs &a, const WalkOf &of, f32x4 (&m)[8]) {
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  for (int t = of.begin; t < of.begin + of.n; ++t) {
+    const size_t at = static_cast<size_t>(of.h % a.h_k) * kCkS + 4 * lg;
+    const float *kp = a.k + t * a.k_stride + at, *qp = a.q + t * a.q_stride + at;
+    const size_t row = static_cast<size_t>(of.h) * kCkS + of.row + lr, head = static_cast<size_t>(t) * a.h_v + of.h;
+    const float eg = expf(a.gate[head]);
+    float dk = 0.0f, dq = 0.0f, kq = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const f32x4 k = *reinterpret_cast<const f32x4 *>(kp + 16 * d), q = *reinterpret_cast<const f32x4 *>(qp + 16 * d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        dk = fmaf(m[d][e], k[e], dk), dq = fmaf(m[d][e], q[e], dq), kq = fmaf(k[e], q[e], kq);
+    }
+    dk = sum_of_lanes(dk), dq = sum_of_lanes(dq), kq = sum_of_lanes(kq);
+    const float delta = fmaf(-eg, dk, a.v[t * a.v_stride + row]) * a.beta[head];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const f32x4 k = *reinterpret_cast<const f32x4 *>(kp + 16 * d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m[d][e] = fmaf(k[e], delta, eg * m[d][e]);
+    }
+    if (lg == 0) a.attn[static_cast<size_t>(t) * a.h_v * kCkS + row] = fmaf(eg, dq, delta * kq) * a.scale;
+  }
+}
+
 // A wave's 16 rows through the chunks.  SHARES: it stages its part of the operands too.
 template <bool SHARES>
 __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const WalkOf &of) {
@@ -706,10 +749,13 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
   const int row_w = of.h * kCkS + of.row;
   const size_t m_at = (static_cast<size_t>(row_w) + lr) * kCkS + 4 * lg;
   f32x4 m[8];
+  const auto load_m = [&] {
 #pragma unroll
-  for (int d = 0; d < 8; ++d)
-    m[d] = of.from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + of.from * a.rag.slot_stride + m_at + 16 * d)
-                     : f32x4{0, 0, 0, 0};
+    for (int d = 0; d < 8; ++d)
+      m[d] = of.from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + of.from * a.rag.slot_stride + m_at + 16 * d)
+                          : f32x4{0, 0, 0, 0};
+  };
+  load_m();
   // v and outputs: tokens 16 t + 4 lg + e
   const int v_stride = 4 * static_cast<int>(a.v_stride), o_stride = 4 * a.h_v * kCkS;
   const float *vp = a.v + static_cast<size_t>(begin) * a.v_stride + row_w;
@@ -737,6 +783,7 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
 #pragma unroll
     for (int t = 0; t < 4; ++t) load_v(rows, t);
   }
+  bool odd = false;  // a delta was not finite
   for (int chunk = 0; chunk < chunks; ++chunk) {
     const int left = n - chunk * kCk;
     // the chunks whose pieces load now (past the last: the last again, read by nobody)
@@ -823,6 +870,8 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
     load_v(rows, 0);
     load_v(rows, 1);
     __builtin_amdgcn_sched_barrier(0);
+    const f32x4 all_d = (d[0] + d[1]) + (d[2] + d[3]);
+    odd = odd || __any(!(fabsf((all_d.x + all_d.y) + (all_d.z + all_d.w)) < INFINITY));
     stage_a(1, 8);
 #pragma unroll
     for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[(kFragK + kFragT) / 16 + i * 64];
@@ -889,6 +938,10 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
     __builtin_amdgcn_sched_barrier(0);
     op += static_cast<size_t>(kCk) * a.h_v * kCkS;
     ws_k += slot_bytes, ws_v += slot_bytes;
+  }
+  if (__builtin_expect(odd, false)) {
+    load_m();
+    walk_tokens(a, of, m);
   }
   if (of.to < 0) return;
 #pragma unroll

@@ -121,3 +121,51 @@ def test_captured_and_replayed_with_other_lengths(bh, dev):
         bh.gdn_ragged(make(other, other_attn))
         torch.cuda.synchronize()
         assert torch.equal(attn, other_attn) and torch.equal(pool, other), new
+
+
+@pytest.mark.parametrize("what", ["v", "k", "q", "gate", "beta", "inf v", "inf k", "state"])
+def test_a_value_that_is_not_finite_reaches_no_earlier_token(bh, dev, what):
+    """As the recurrence has it: outputs of the tokens before are as without it, those
+    after are not finite where the formula's are not."""
+    import batchdata as bd
+    from test_gdn_ragged_gpu import _views
+    from conftest import rel_err
+    c = _case([3, 200, 70], 2, 4, 128)
+    at = 3 + 100  # in the second chunk of the second request
+    bad = np.inf if what.startswith("inf") else np.nan
+    for name in ("rows", "gate", "beta", "pool"):
+        c[name] = c[name].copy()
+    if what.endswith("v"):
+        c["rows"][at, 4 * 128 + 128 + 9] = bad  # v-head 1, row 9
+    elif what.endswith("k"):
+        c["rows"][at, 2 * 128 + 17] = bad
+    elif what == "q":
+        c["rows"][at, 17] = bad
+    elif what == "state":
+        c["pool"][c["src"][1], 5 * 128 + 3] = bad  # v-head 0, row 5
+    else:
+        c[what][at, 1] = bad
+    q, k, v = _views(c)
+    with np.errstate(all="ignore"):
+        want, state = bd.gdn(q, k, v, c["gate"], c["beta"], c["pool"].reshape(-1, 4, 128, 128),
+                             c["start"], c["src"], c["dst"], np.full(v.shape, -7.0))
+    for kw in ({}, dict(max_new=1)):  # by chunks and token by token
+        attn, pool, _ = _run(bh, dev, c, **kw)
+        for got, ref in ((attn, want), (pool.reshape(state.shape)[c["dst"]], state[c["dst"]])):
+            fine = np.isfinite(ref)  # (q reaches no state)
+            assert fine.any() and (what == "q" or not fine.all()), what
+            assert np.array_equal(np.isfinite(got), fine), what
+            assert rel_err(got[fine], ref[fine]) < 1e-5, what
+
+
+@pytest.mark.parametrize("gate", [0.02, 0.5, 3.0])
+def test_states_that_grow(bh, dev, gate):
+    """Gates above 0, to where a state passes what f32 holds."""
+    c = _case([130, 1, 60], 1, 2, 128, decay=gate)
+    if gate < 3:
+        c["beta"] *= 0.1
+        _check(bh, dev, c, tol=1e-5)
+    else:
+        with np.errstate(all="ignore"):
+            attn, pool, _ = _run(bh, dev, c)
+        assert np.isfinite(attn[:20]).all() and not np.isfinite(attn[129]).any()
