@@ -172,7 +172,7 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_any_kernel(GdnArgs a) {
   }
 }
 
-// ---- prompts: chunks of 64 tokens on the matrix cores (s = 128) ----------------
+// ---- prompts: chunks of 64 tokens on the matrix cores (s = 64, 128) ------------
 //
 // Over a chunk with decays a_t = e^gate_t, A_t = a_0 .. a_t, D_ts = A_t / A_s and a
 // state row m at its beginning, the tokens' steps unroll to
@@ -201,13 +201,15 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_any_kernel(GdnArgs a) {
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
-constexpr int kCk = 64, kCkS = 128;
+constexpr int kCk = 64;
 // Tokens from which a request goes by chunks.  One request of 32 / 48 / 64 / 127 tokens, us:
 // 24.3, 24.7, 25.1, 29.2, token by token 17.2, 24.3, 30.8, 63.3; 64 of 32 259 for 317.
 constexpr int kCkMin = 48;
 constexpr int kCkPlace = 32;          // a chunk's place in the workspace every so many tokens
-constexpr int kFragK = kCk * kCkS * 4;           // bytes of K as halves; Q, K transposed
-constexpr int kHeadK = 3 * kFragK;               // of a (chunk, q/k head)
+template <int S>
+constexpr int kFragK = kCk * S * 4;              // bytes of K as halves; Q, K transposed
+template <int S>
+constexpr int kHeadK = 3 * kFragK<S>;            // of a (chunk, q/k head)
 constexpr int kFragT = 12 * 64 * 16;             // of T's and P's 16 x 32 tiles to the diagonal
 constexpr int kVecs = 5 * kCk + kCk;             // floats: A k, A q, T's, P's units, e k; A_63
 constexpr int kHeadV = 2 * kFragT + kVecs * 4;   // of a (chunk, v-head)
@@ -505,11 +507,12 @@ __device__ __forceinline__ void list_long(const Ragged &rag, int longs, int32_t 
 }
 
 // Block (chunk, q/k head): wave w has the tokens 16 w .. 16 w + 15.
+template <int S>
 __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs c) {
-  constexpr int kMat = kCk * kPitch;
+  constexpr int kMat = kCk * kPitch, N = S / 32;  // N: of 32 dims
   // K's halves; then the v-heads' matrices.  Behind them Q K^T and K K^T.
   __shared__ __attribute__((aligned(16))) float lds[kVWaves * kMat + kMat];
-  static_assert(kVWaves * kMat * 4 >= kFragK, "K's halves fit");
+  static_assert(kVWaves * kMat * 4 >= kFragK<S>, "K's halves fit");
   __shared__ double G_s[kVWaves][kCk];
   __shared__ float w_s[kVWaves][kCk], b_s[kVWaves][kCk], k_down[kCk], q_down[kCk];
   const GdnArgs &a = c.g;
@@ -526,34 +529,34 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
   const int t0 = begin + at, nt = min(kCk, n - at);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int lr = lane & 15, lg = lane >> 4;
-  char *of_slot = c.ws + static_cast<size_t>(slot) * (static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(a.h_v) * kHeadV);
-  char *out = of_slot + static_cast<size_t>(kh) * kHeadK;
+  char *of_slot = c.ws + static_cast<size_t>(slot) * (static_cast<size_t>(a.h_k) * kHeadK<S> + static_cast<size_t>(a.h_v) * kHeadV);
+  char *out = of_slot + static_cast<size_t>(kh) * kHeadK<S>;
   float *kq = lds + kVWaves * kMat;
   h8 *k_lds = reinterpret_cast<h8 *>(lds);
 
   // K and Q of the wave's tokens as halves
-  h8 qh[4], ql[4], kh_[4], kl[4];
+  h8 qh[N], ql[N], kh_[N], kl[N];
   {
     const int t = 16 * w + lr;
     const bool in = t < nt;
     const size_t row = static_cast<size_t>(t0 + (in ? t : 0));
-    const float *kp = a.k + row * a.k_stride + static_cast<size_t>(kh) * kCkS + 4 * lg;
-    const float *qp = a.q + row * a.q_stride + static_cast<size_t>(kh) * kCkS + 4 * lg;
-    f32x4 kv[8], qv[8];
+    const float *kp = a.k + row * a.k_stride + static_cast<size_t>(kh) * S + 4 * lg;
+    const float *qp = a.q + row * a.q_stride + static_cast<size_t>(kh) * S + 4 * lg;
+    f32x4 kv[2 * N], qv[2 * N];
     float km = 0.0f, qm = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 2 * N; ++i) {
       kv[i] = in ? *reinterpret_cast<const f32x4 *>(kp + 16 * i) : f32x4{0, 0, 0, 0};
       qv[i] = in ? *reinterpret_cast<const f32x4 *>(qp + 16 * i) : f32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) km = fmaxf(km, most_of(kv[i])), qm = fmaxf(qm, most_of(qv[i]));
+    for (int i = 0; i < 2 * N; ++i) km = fmaxf(km, most_of(kv[i])), qm = fmaxf(qm, most_of(qv[i]));
     float ku, kd, qu, qd;
     unit_of(most_of_lanes(km), &ku, &kd);
     unit_of(most_of_lanes(qm), &qu, &qd);
     if (lg == 0) k_down[t] = kd, q_down[t] = qd;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
       h4 h0, l0, h1, l1;
       halves(kv[2 * i], ku, &h0, &l0);
       halves(kv[2 * i + 1], ku, &h1, &l1);
@@ -561,9 +564,9 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
       halves(qv[2 * i], qu, &h0, &l0);
       halves(qv[2 * i + 1], qu, &h1, &l1);
       qh[i] = both(h0, h1), ql[i] = both(l0, l1);
-      const int f = (w * 4 + i) * 128 + lane;  // of 16 bytes: hi, and lo 64 places on
+      const int f = (w * N + i) * 128 + lane;  // of 16 bytes: hi, and lo 64 places on
       k_lds[f] = kh_[i], k_lds[f + 64] = kl[i];
-      h8 *ko = reinterpret_cast<h8 *>(out) + f, *qo = reinterpret_cast<h8 *>(out + kFragK) + f;
+      h8 *ko = reinterpret_cast<h8 *>(out) + f, *qo = reinterpret_cast<h8 *>(out + kFragK<S>) + f;
       ko[0] = kh_[i], ko[64] = kl[i];
       qo[0] = qh[i], qo[64] = ql[i];
     }
@@ -571,10 +574,10 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
   __syncthreads();
   // Q K^T and K K^T of the wave's tokens against those before: a row of one operand is a
   // column of the other, in the same lanes
-  h8 of_j[2][8];
+  h8 of_j[2][2 * N];
   const auto read = [&](int j) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) of_j[j & 1][i] = k_lds[(j * 4 + (i >> 1)) * 128 + 64 * (i & 1) + lane];
+    for (int i = 0; i < 2 * N; ++i) of_j[j & 1][i] = k_lds[(j * N + (i >> 1)) * 128 + 64 * (i & 1) + lane];
   };
   read(0);
 #pragma unroll
@@ -585,7 +588,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
 #pragma unroll
     for (int x = 0; x < 2; ++x) kk[x] = qk[x] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
       kk[i & 1] = mma32(kh_[i], kl[i], of_j[j & 1][2 * i], of_j[j & 1][2 * i + 1], kk[i & 1]);
       qk[i & 1] = mma32(qh[i], ql[i], of_j[j & 1][2 * i], of_j[j & 1][2 * i + 1], qk[i & 1]);
     }
@@ -602,18 +605,18 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
   {
     const _Float16 *halves_of = reinterpret_cast<const _Float16 *>(lds);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int d = 2 * w + (x >> 1), p = x & 1;  // wave w: dims 32 w .. 32 w + 31
+    for (int x = 0; x < N; ++x) {
+      const int d = N / 2 * w + (x >> 1), p = x & 1;  // wave w: dims 8 N w .. 8 N (w + 1) - 1
       const int dim = 16 * (d & 1) + lr;         // of 32
       const int in = (dim >> 4) * 4 + (dim & 3), group = (dim >> 2) & 3;
       h8 hi, lo;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int t = 2 * p + (e >> 2);
-        const int f = ((t * 4 + (d >> 1)) * 128 + 4 * lg + (e & 3) + 16 * group) * 8 + in;
+        const int f = ((t * N + (d >> 1)) * 128 + 4 * lg + (e & 3) + 16 * group) * 8 + in;
         hi[e] = halves_of[f], lo[e] = halves_of[f + 64 * 8];
       }
-      h8 *o = reinterpret_cast<h8 *>(out + 2 * kFragK) + (d * 2 + p) * 128 + lane;
+      h8 *o = reinterpret_cast<h8 *>(out + 2 * kFragK<S>) + (d * 2 + p) * 128 + lane;
       o[0] = hi, o[64] = lo;
     }
   }
@@ -623,7 +626,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
   for (int i = w; i < heads; i += kVWaves) {
     const int h = kh + i * a.h_k;
     prep_head(a, h, t0, nt, kq, lds + w * kMat, G_s[w], w_s[w], b_s[w], k_down, q_down,
-              of_slot + static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(h) * kHeadV);
+              of_slot + static_cast<size_t>(a.h_k) * kHeadK<S> + static_cast<size_t>(h) * kHeadV);
   }
 }
 
@@ -634,9 +637,13 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
 
 // Operands of a chunk in LDS: K, Q; K transposed, T, P; their vectors, of two chunks in
 // turn.
-constexpr int kA = 2 * kFragK / 16, kB = (kFragK + 2 * kFragT) / 16;  // pieces of 16 bytes
+template <int S>
+constexpr int kA = 2 * kFragK<S> / 16;  // pieces of 16 bytes
+template <int S>
+constexpr int kB = (kFragK<S> + 2 * kFragT) / 16;
+template <int S>
 struct ChunkLds {
-  h8 kq[kA], u[kB];
+  h8 kq[kA<S>], u[kB<S>];
   float vec[2][kVecs];
 };
 struct WalkOf {
@@ -648,22 +655,22 @@ struct WalkOf {
 
 // Pieces on their way to LDS: one is stored and the next chunk's loaded in its place.
 // THREADS threads do it, of which this is number tid.
-template <int THREADS>
+template <int S, int THREADS>
 struct Stage {
-  static constexpr int kAs = kA / THREADS, kBk = kFragK / 16 / THREADS, kBt = 2 * kFragT / 16 / THREADS;
-  static_assert(kAs * THREADS == kA && (kBk + kBt) * THREADS == kB, "whole pieces a thread");
+  static constexpr int kAs = kA<S> / THREADS, kBk = kFragK<S> / 16 / THREADS, kBt = 2 * kFragT / 16 / THREADS;
+  static_assert(kAs * THREADS == kA<S> && (kBk + kBt) * THREADS == kB<S>, "whole pieces a thread");
   h8 in_a[kAs], in_b[kBk + kBt];
   f32x4 in_vec;
   int tid, vec_i;
   __device__ __forceinline__ void load_a(const Base &k, int i) { in_a[i] = k.load(16 * tid, i * THREADS * 16); }
   __device__ __forceinline__ void load_b(const Base &k, const Base &v, int i) {
-    in_b[i] = i < kBk ? k.load(16 * tid, 2 * kFragK + i * THREADS * 16) : v.load(16 * tid, (i - kBk) * THREADS * 16);
+    in_b[i] = i < kBk ? k.load(16 * tid, 2 * kFragK<S> + i * THREADS * 16) : v.load(16 * tid, (i - kBk) * THREADS * 16);
   }
   __device__ __forceinline__ void load_vec(const Base &v) {
     in_vec = __builtin_bit_cast(f32x4, v.load(16 * vec_i, 2 * kFragT));
   }
   // The first chunk's, and the second's A on its way.
-  __device__ __forceinline__ void begin(ChunkLds &lds, const WalkOf &o, int chunks, int thread) {
+  __device__ __forceinline__ void begin(ChunkLds<S> &lds, const WalkOf &o, int chunks, int thread) {
     tid = thread, vec_i = min(tid, kVecs / 4 - 1);  // (the last ones the same)
     const Base k(o.ws_k), v(o.ws_v), k1(chunks > 1 ? o.ws_k + o.slot_bytes : o.ws_k);
 #pragma unroll
@@ -678,21 +685,21 @@ struct Stage {
     }
   }
   // A part of the next chunk's A (and the one's after it on its way), of this chunk's B.
-  __device__ __forceinline__ void a(ChunkLds &lds, const Base &after_k, int part, int parts) {
+  __device__ __forceinline__ void a(ChunkLds<S> &lds, const Base &after_k, int part, int parts) {
 #pragma unroll
     for (int i = kAs * part / parts; i < kAs * (part + 1) / parts; ++i) {
       lds.kq[i * THREADS + tid] = in_a[i];
       load_a(after_k, i);
     }
   }
-  __device__ __forceinline__ void b(ChunkLds &lds, const Base &next_k, const Base &next_v, int part, int parts) {
+  __device__ __forceinline__ void b(ChunkLds<S> &lds, const Base &next_k, const Base &next_v, int part, int parts) {
 #pragma unroll
     for (int i = (kBk + kBt) * part / parts; i < (kBk + kBt) * (part + 1) / parts; ++i) {
       lds.u[i * THREADS + tid] = in_b[i];
       load_b(next_k, next_v, i);
     }
   }
-  __device__ __forceinline__ void vec(ChunkLds &lds, const Base &next_v, int chunk) {
+  __device__ __forceinline__ void vec(ChunkLds<S> &lds, const Base &next_v, int chunk) {
     reinterpret_cast<f32x4 *>(lds.vec[chunk & 1])[vec_i] = in_vec;
     load_vec(next_v);
   }
@@ -708,16 +715,17 @@ __device__ __forceinline__ float sum_of_lanes(float x) {
 }
 
 // A request's tokens one by one; m as walk_rows has it.
-__device__ __forceinline__ void walk_tokens(const GdnArgs &a, const WalkOf &of, f32x4 (&m)[8]) {
+template <int S>
+__device__ __forceinline__ void walk_tokens(const GdnArgs &a, const WalkOf &of, f32x4 (&m)[S / 16]) {
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   for (int t = of.begin; t < of.begin + of.n; ++t) {
-    const size_t at = static_cast<size_t>(of.h % a.h_k) * kCkS + 4 * lg;
+    const size_t at = static_cast<size_t>(of.h % a.h_k) * S + 4 * lg;
     const float *kp = a.k + t * a.k_stride + at, *qp = a.q + t * a.q_stride + at;
-    const size_t row = static_cast<size_t>(of.h) * kCkS + of.row + lr, head = static_cast<size_t>(t) * a.h_v + of.h;
+    const size_t row = static_cast<size_t>(of.h) * S + of.row + lr, head = static_cast<size_t>(t) * a.h_v + of.h;
     const float eg = expf(a.gate[head]);
     float dk = 0.0f, dq = 0.0f, kq = 0.0f;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
+    for (int d = 0; d < S / 16; ++d) {
       const f32x4 k = *reinterpret_cast<const f32x4 *>(kp + 16 * d), q = *reinterpret_cast<const f32x4 *>(qp + 16 * d);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -726,40 +734,41 @@ __device__ __forceinline__ void walk_tokens(const GdnArgs &a, const WalkOf &of, 
     dk = sum_of_lanes(dk), dq = sum_of_lanes(dq), kq = sum_of_lanes(kq);
     const float delta = fmaf(-eg, dk, a.v[t * a.v_stride + row]) * a.beta[head];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
+    for (int d = 0; d < S / 16; ++d) {
       const f32x4 k = *reinterpret_cast<const f32x4 *>(kp + 16 * d);
 #pragma unroll
       for (int e = 0; e < 4; ++e) m[d][e] = fmaf(k[e], delta, eg * m[d][e]);
     }
-    if (lg == 0) a.attn[static_cast<size_t>(t) * a.h_v * kCkS + row] = fmaf(eg, dq, delta * kq) * a.scale;
+    if (lg == 0) a.attn[static_cast<size_t>(t) * a.h_v * S + row] = fmaf(eg, dq, delta * kq) * a.scale;
   }
 }
 
 // A wave's 16 rows through the chunks.  SHARES: it stages its part of the operands too.
-template <bool SHARES>
-__device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const WalkOf &of) {
+template <int S, bool SHARES>
+__device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds<S> &lds, const WalkOf &of) {
   const int begin = of.begin, n = of.n;
   const char *ws_k = of.ws_k, *ws_v = of.ws_v;
   const size_t slot_bytes = of.slot_bytes;
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  constexpr int N = S / 32;  // of 32 dims
   const int chunks = (n + kCk - 1) / kCk;
-  Stage<512> stage;
+  Stage<S, 512> stage;
   if constexpr (SHARES) stage.begin(lds, of, chunks, threadIdx.x);
   // m[d]: state row lr of the wave's, dims 16 d + 4 lg ..
-  const int row_w = of.h * kCkS + of.row;
-  const size_t m_at = (static_cast<size_t>(row_w) + lr) * kCkS + 4 * lg;
-  f32x4 m[8];
+  const int row_w = of.h * S + of.row;
+  const size_t m_at = (static_cast<size_t>(row_w) + lr) * S + 4 * lg;
+  f32x4 m[2 * N];
   const auto load_m = [&] {
 #pragma unroll
-    for (int d = 0; d < 8; ++d)
+    for (int d = 0; d < S / 16; ++d)
       m[d] = of.from >= 0 ? *reinterpret_cast<const f32x4 *>(a.state + of.from * a.rag.slot_stride + m_at + 16 * d)
                           : f32x4{0, 0, 0, 0};
   };
   load_m();
   // v and outputs: tokens 16 t + 4 lg + e
-  const int v_stride = 4 * static_cast<int>(a.v_stride), o_stride = 4 * a.h_v * kCkS;
+  const int v_stride = 4 * static_cast<int>(a.v_stride), o_stride = 4 * a.h_v * S;
   const float *vp = a.v + static_cast<size_t>(begin) * a.v_stride + row_w;
-  float *op = a.attn + static_cast<size_t>(begin) * a.h_v * kCkS + row_w;
+  float *op = a.attn + static_cast<size_t>(begin) * a.h_v * S + row_w;
   const int v_at = 4 * lg * v_stride + 4 * lr, o_at = 4 * lg * o_stride + 4 * lr;
   f32x4 v[4];
   const auto load_v = [&](const Base &of, int t) {
@@ -801,10 +810,10 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
       if constexpr (SHARES) stage.b(lds, next_k, next_v, part, parts);
     };
     float up, m_down;
-    h8 mh[4], ml[4];
-    unit(fmaxf(most4(m), most4(m + 4)), &up, &m_down);
+    h8 mh[N], ml[N];
+    unit(fmaxf(most4(m), most4(m + 2 * N - 4)), &up, &m_down);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pair(m[2 * i], m[2 * i + 1], up, &mh[i], &ml[i]);
+    for (int i = 0; i < N; ++i) pair(m[2 * i], m[2 * i + 1], up, &mh[i], &ml[i]);
     __syncthreads();  // K and Q are there; K transposed, T and P of the chunk before are read
     // K m, then Q m, 32 dims a step; operands are read a step ahead
     h8 f[2][4][2];
@@ -813,11 +822,11 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int p = 0; p < 2; ++p)
-          f[step & 1][t][p] = k_at[(step >> 2) * (kA / 2) + (t * 4 + (step & 3)) * 128 + 64 * p];
+          f[step & 1][t][p] = k_at[step / N * (kA<S> / 2) + (t * N + step % N) * 128 + 64 * p];
     };
     f32x4 x[4], y[4];
     const auto times = [&](int step, f32x4 *z) {
-      const int i = step & 3;
+      const int i = step % N;
 #pragma unroll
       for (int p = 0; p < 3; ++p)  // lo hi, hi lo, hi hi
 #pragma unroll
@@ -827,16 +836,16 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
     read(0);
     if constexpr (SHARES) stage.vec(lds, next_v, chunk);
 #pragma unroll
-    for (int step = 0; step < 8; ++step) {
+    for (int step = 0; step < 2 * N; ++step) {
       __builtin_amdgcn_sched_barrier(0);
-      if (step + 1 < 8) read(step + 1);
-      if (step < 7) stage_b(step, 7);
-      times(step, step < 4 ? x : y);
+      if (step + 1 < 2 * N) read(step + 1);
+      if (step + 1 < 2 * N) stage_b(step, 2 * N - 1);
+      times(step, step < N ? x : y);
     }
     __syncthreads();  // K and Q are read; the others are there
     h8 tf[6][2];
 #pragma unroll
-    for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[kFragK / 16 + i * 64];
+    for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[kFragK<S> / 16 + i * 64];
     // the right sides
     f32x4 s[4];
     h8 hi[2], lo[2];
@@ -874,7 +883,7 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
     odd = odd || __any(!(fabsf((all_d.x + all_d.y) + (all_d.z + all_d.w)) < INFINITY));
     stage_a(1, 8);
 #pragma unroll
-    for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[(kFragK + kFragT) / 16 + i * 64];
+    for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[(kFragK<S> + kFragT) / 16 + i * 64];
 #pragma unroll
     for (int t = 0; t < 4; ++t) d[t] = d[t] * (of_token(2, t) * down);
 #pragma unroll
@@ -903,7 +912,7 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
     }
     stage_a(3, 8);
     const Base to_rows(op, min(left, kCk) * o_stride);
-    // the new state, half of its dims at a time
+    // the new state, 64 of its dims at a time
     const float all = vec[5 * kCk];
     h8 kt[2][4][2];
     const auto read_kt = [&](int step) {
@@ -916,12 +925,14 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
     f32x4 u[4];
     read_kt(0);
 #pragma unroll
-    for (int step = 0; step < 4; ++step) {
+    for (int step = 0; step < N; ++step) {
       __builtin_amdgcn_sched_barrier(0);
-      if (step + 1 < 4) read_kt(step + 1);
-      stage_a(4 + step, 8);
+      if (step + 1 < N) read_kt(step + 1);
+      stage_a(N + step, 2 * N);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) to_rows.store1(d[step][e], o_at + (16 * step + e) * o_stride);
+      for (int t = 4 * step / N; t < 4 * (step + 1) / N; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to_rows.store1(d[t][e], o_at + (16 * t + e) * o_stride);
       const int p = step & 1;
 #pragma unroll
       for (int k = 0; k < 3; ++k)
@@ -936,34 +947,35 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds &lds, const
         }
     }
     __builtin_amdgcn_sched_barrier(0);
-    op += static_cast<size_t>(kCk) * a.h_v * kCkS;
+    op += static_cast<size_t>(kCk) * a.h_v * S;
     ws_k += slot_bytes, ws_v += slot_bytes;
   }
   if (__builtin_expect(odd, false)) {
     load_m();
-    walk_tokens(a, of, m);
+    walk_tokens<S>(a, of, m);
   }
   if (of.to < 0) return;
 #pragma unroll
-  for (int d = 0; d < 8; ++d)
+  for (int d = 0; d < S / 16; ++d)
     *reinterpret_cast<f32x4 *>(a.state + of.to * a.rag.slot_stride + m_at + 16 * d) = m[d];
 }
 
 // Blocks of the walk.  All rows of a (request, v-head) are a block's, 16 a wave; or, of the
 // longest requests, as far as blocks are fewer than compute units, half of them, and the
-// other four waves stage the operands.  What bounds a block is its waves' reads of them
-// from LDS (120 KB a wave and chunk), so half the rows are through sooner: 4.7 us a chunk
+// other four waves stage the operands (as they do for heads of 64).  What bounds a block is its waves' reads of them
+// from LDS (120 KB a wave and chunk), so half the rows are through sooner: 4.0 us a chunk
 // for 7.2.
+template <int S>
 __global__ __launch_bounds__(512, 2) void gdn_chunk_walk_kernel(GdnChunkArgs c) {
-  __shared__ __attribute__((aligned(16))) ChunkLds lds;
+  __shared__ __attribute__((aligned(16))) ChunkLds<S> lds;
   const GdnArgs &a = c.g;
   if (static_cast<int>(blockIdx.x) >= c.walks) {  // the requests of fewer tokens
-    step_rows<kCkS, 4, 512>(a, blockIdx.x - c.walks);
+    step_rows<S, S == 128 ? 4 : 1, 512>(a, blockIdx.x - c.walks);
     return;
   }
   const int count = __builtin_amdgcn_readfirstlane(c.todo[0]);
   // requests in halves
-  const int halves = count > 64 ? 0 : min(count, max(c.at_once - count, 0));
+  const int halves = S == 64 || count > 64 ? 0 : min(count, max(c.at_once - count, 0));
   int nth = blockIdx.x / (2 * a.h_v), rest = blockIdx.x - nth * 2 * a.h_v;
   const bool half = nth < halves;
   if (!half) {
@@ -986,19 +998,20 @@ __global__ __launch_bounds__(512, 2) void gdn_chunk_walk_kernel(GdnChunkArgs c) 
   a.rag.tokens_of(r, &of.begin, &of.n);
   a.rag.slots(r, &of.from, &of.to);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  of.slot_bytes = static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(a.h_v) * kHeadV;
+  of.slot_bytes = static_cast<size_t>(a.h_k) * kHeadK<S> + static_cast<size_t>(a.h_v) * kHeadV;
   of.ws_k = c.ws + static_cast<size_t>(first_chunk(of.begin)) * of.slot_bytes +
-            static_cast<size_t>(of.h % a.h_k) * kHeadK;
+            static_cast<size_t>(of.h % a.h_k) * kHeadK<S>;
   of.ws_v = c.ws + static_cast<size_t>(first_chunk(of.begin)) * of.slot_bytes +
-            static_cast<size_t>(a.h_k) * kHeadK + static_cast<size_t>(of.h) * kHeadV;
-  of.row = slab * (kCkS / 2) + 16 * (half ? w & 3 : w);
-  if (!half) {
-    walk_rows<true>(a, lds, of);
-  } else if (w < 4) {
-    walk_rows<false>(a, lds, of);
+            static_cast<size_t>(a.h_k) * kHeadK<S> + static_cast<size_t>(of.h) * kHeadV;
+  const int walkers = S / 16 / slabs;  // waves
+  of.row = 16 * (slab * walkers + w % walkers);
+  if (S == 128 && walkers == 8) {
+    walk_rows<S, S == 128>(a, lds, of);
+  } else if (w < walkers) {
+    walk_rows<S, false>(a, lds, of);
   } else {  // the barriers are walk_rows'
     const int chunks = (of.n + kCk - 1) / kCk;
-    Stage<256> stage;
+    Stage<S, 256> stage;
     stage.begin(lds, of, chunks, threadIdx.x - 256);
     for (int chunk = 0; chunk < chunks; ++chunk) {
       const int ahead = min(chunks - 1 - chunk, 2);
@@ -1016,6 +1029,11 @@ __global__ __launch_bounds__(512, 2) void gdn_chunk_walk_kernel(GdnChunkArgs c) 
 
 // Blocks of a launch: a grid has fewer than 2^32 threads a dimension.
 constexpr size_t kMostBlocks = 0xffffff;
+
+// Bytes of a chunk in the workspace.
+size_t slot_bytes(const bh_gdn_ragged_args &p) {
+  return p.h_k * (p.s == 64 ? kHeadK<64> : kHeadK<128>) + p.h_v * kHeadV;
+}
 
 int check(const bh_gdn_ragged_args &p) {
   if (p.h_k == 0 || p.h_v == 0 || p.s == 0)
@@ -1039,7 +1057,7 @@ int check(const bh_gdn_ragged_args &p) {
     return fail(BH_ERR_SHAPE, "gdn_ragged: size overflow");
   // (a chunk's block a q/k head; a place every kCkPlace tokens)
   if (!mul_size(p.n_tok / kCkPlace + 1, p.h_k, &n) || n > kMostBlocks ||
-      !mul_size(p.n_tok / kCkPlace + 1, p.h_k * kHeadK + p.h_v * kHeadV, &n))
+      !mul_size(p.n_tok / kCkPlace + 1, slot_bytes(p), &n))
     return fail(BH_ERR_SHAPE, "gdn_ragged: size overflow");
   if (p.n_req != 0 && p.n_tok != 0) {
     if (!p.q || !p.k || !p.v || !p.gate || !p.beta || !p.attn || !p.q_start || !p.src_slot ||
@@ -1057,13 +1075,11 @@ bool whole_rows(const bh_gdn_ragged_args &p) {
 // Slots of chunks of a call, 0: it has none.
 size_t chunk_slots(const bh_gdn_ragged_args &p) {
   const size_t most = p.max_new == 0 || p.max_new > p.n_tok ? p.n_tok : p.max_new;
-  if (p.s != static_cast<size_t>(kCkS) || most < static_cast<size_t>(kCkMin) || !whole_rows(p) ||
+  if ((p.s != 64 && p.s != 128) || most < static_cast<size_t>(kCkMin) || !whole_rows(p) ||
       p.v_stride > kMostStride)
     return 0;
   return p.n_tok / kCkPlace + 1;
 }
-
-size_t slot_bytes(const bh_gdn_ragged_args &p) { return p.h_k * kHeadK + p.h_v * kHeadV; }
 
 // Requests of kCkMin tokens or more that there can be.
 size_t most_long(const bh_gdn_ragged_args &p) {
@@ -1122,8 +1138,14 @@ extern "C" int bh_gdn_ragged(const bh_gdn_ragged_args *args, bh_stream stream) {
     GdnChunkArgs c{a, ws, static_cast<int>(slots), static_cast<int>(walks * p.h_v),
                    p.h_k % 8 == 0 && p.h_v % p.h_k == 0, static_cast<int>(at_once), static_cast<int>(longs),
                    reinterpret_cast<int32_t *>(ws + slots * slot_bytes(p))};
-    BH_LAUNCH(gdn_chunk_prep_kernel, static_cast<unsigned>(slots * p.h_k), kBlock, 0, st, c);
-    BH_LAUNCH(gdn_chunk_walk_kernel, static_cast<unsigned>((walks + p.n_req) * p.h_v), 512, 0, st, c);
+    const unsigned preps = static_cast<unsigned>(slots * p.h_k), blocks = static_cast<unsigned>((walks + p.n_req) * p.h_v);
+    if (p.s == 128) {
+      BH_LAUNCH(gdn_chunk_prep_kernel<128>, preps, kBlock, 0, st, c);
+      BH_LAUNCH(gdn_chunk_walk_kernel<128>, blocks, 512, 0, st, c);
+    } else {
+      BH_LAUNCH(gdn_chunk_prep_kernel<64>, preps, kBlock, 0, st, c);
+      BH_LAUNCH(gdn_chunk_walk_kernel<64>, blocks, 512, 0, st, c);
+    }
     return ok();
   }
   const auto blocks = [&](size_t rows) { return static_cast<unsigned>(p.n_req * p.h_v * p.s / rows); };

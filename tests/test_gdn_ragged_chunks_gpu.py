@@ -169,3 +169,16 @@ def test_states_that_grow(bh, dev, gate):
         with np.errstate(all="ignore"):
             attn, pool, _ = _run(bh, dev, c)
         assert np.isfinite(attn[:20]).all() and not np.isfinite(attn[129]).any()
+
+
+@pytest.mark.parametrize("new", [[47], [48, 1], [63, 64, 65], [130, 0, 3, 257], [50] * 70])
+@pytest.mark.parametrize("h_k,h_v", [(1, 3), (8, 16), (3, 2)])
+def test_heads_of_64(bh, dev, new, h_k, h_v):
+    print(new[:4], h_k, h_v, flush=True)
+    _check(bh, dev, _case(new, h_k, h_v, 64, fresh=[0]))
+    _check(bh, dev, _case(new, h_k, h_v, 64, seed=1, inplace=True, slot_pad=4), max_new=max(new))
+
+
+@pytest.mark.parametrize("decay", [0.0, -30.0, -np.inf, -0.3])
+def test_heads_of_64_with_hard_decays(bh, dev, decay):
+    _check(bh, dev, _case([200, 1, 140], 1, 2, 64, decay=decay, alike=0.9, beta_one=True))
