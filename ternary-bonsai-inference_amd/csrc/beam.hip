@@ -10,7 +10,9 @@
 // reach it matter: a few more than n_best, whose ranks, counted against one another,
 // are their places.  Scores are compared in f64, so that rounding puts no two beams
 // out of order: a step of f32 at a score of -100 is 8e-6.
-// Bound by reading the logits.
+// Bound by reading the logits: 256 rows of 248320 in 32 groups, best 16: 56.4 us, 4.5 TB/s,
+// and 10.7 for the groups (30 with 256 threads that went through their lists one key after
+// the other); 4 rows 8.0 and 4.6.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

@@ -7,7 +7,8 @@
 //   delta = (v - e^gate d_k) beta,  m' = e^gate m + delta k,
 //   m'.q = e^gate d_q + delta (k.q),
 // so that both dots come from the old row at once.  Decoding reads and writes the
-// states, 2 x 4 h_v s^2 bytes a request, and is bound by that.
+// states, 2 x 4 h_v s^2 bytes a request, and is bound by that: 48 heads of 128, 64 requests
+// 81.7 us, 4.96 TB/s; 8 10.2; one 3.7.
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -507,6 +508,9 @@ __device__ __forceinline__ void list_long(const Ragged &rag, int longs, int32_t 
 }
 
 // Block (chunk, q/k head): wave w has the tokens 16 w .. 16 w + 15.
+// Bound by the chain of small products and LDS trips that a wave takes a v-head through,
+// 16 us for a chunk, two blocks a compute unit by LDS: 46 chunks of 16 / 48 heads 44 us, of
+// which writing 127 MB is 26.
 template <int S>
 __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs c) {
   constexpr int kMat = kCk * kPitch, N = S / 32;  // N: of 32 dims
@@ -634,6 +638,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
 // registers: every result is the next product's operand as it stands.  The operands that
 // the waves share stand in LDS, K and Q apart from K transposed, T and P, so that each
 // part of the next chunk comes in while the other is read: two barriers a chunk.
+// Three prompts of 1536 tokens, 16 / 48 heads of 128: 176 us, one 98.
 
 // Operands of a chunk in LDS: K, Q; K transposed, T, P; their vectors, of two chunks in
 // turn.
