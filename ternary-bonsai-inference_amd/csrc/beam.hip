@@ -6,12 +6,12 @@
 // part of a row, m, S and the part's n_best largest logits in order; the n_best best
 // of a group are among these, as a row's continuations are in the order of its
 // logits.  One block a group then forms the rows' ln S, and with them the score of
-// each part's first logit.  Where n_best parts' firsts reach a bound, only keys that
-// reach it matter: a few more than n_best, whose ranks, counted against one another,
-// are their places.  Scores are compared in f64, so that rounding puts no two beams
+// each part's logits.  Where n_best of them reach a bound, only keys that reach it
+// matter: a few more than n_best, whose ranks, counted against one another, are
+// their places.  Scores are compared in f64, so that rounding puts no two beams
 // out of order: a step of f32 at a score of -100 is 8e-6.
 // Bound by reading the logits: 256 rows of 248320 in 32 groups, best 16: 56.4 us, 4.5 TB/s,
-// and 10.7 for the groups (30 with 256 threads that went through their lists one key after
+// and 8.0 for the groups (30 with 256 threads that went through their lists one key after
 // the other); 4 rows 8.0 and 4.6.
 #include <hip/hip_runtime.h>
 
@@ -28,7 +28,7 @@ namespace {
 
 constexpr int kMostFirsts = 1024;  // parts of a group
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;  // of a group's block
-constexpr int kOwn = kMostFirsts / kSelThreads;
+constexpr int kDepths = 3;  // keys 1, 4, 16 of a part
 constexpr int kMostCand = 1024;    // candidates that are ranked at once
 constexpr int kAhead = 2;          // keys of a thread on their way
 
@@ -76,12 +76,13 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
   const int row0 = blockIdx.x * a.width, firsts = a.width * a.n_parts;
   const size_t part0 = static_cast<size_t>(row0) * a.n_parts;
 
-  uint64_t first[kOwn];
+  static_assert(kMostFirsts == kSelThreads, "a part a thread");
+  uint64_t of_part[kDepths];  // its keys 1, 4, 16
 #pragma unroll
-  for (int i = 0; i < kOwn; ++i) {
-    const int p = tid + i * kSelThreads;
-    first[i] = p < firsts ? a.keys[(part0 + p) * a.n_best] : 0;
-  }
+  for (int i = 0; i < kDepths; ++i)
+    of_part[i] = tid < firsts && 1 << 2 * i <= a.n_best
+                     ? a.keys[(part0 + tid) * a.n_best + (1 << 2 * i) - 1] : 0;
+  const uint64_t first = of_part[0];
   if (tid == 0) count_s = n_live_s = 0;
   for (int b = wave; b < a.width; b += kSelWaves) {
     const Part *parts = a.parts + part0 + static_cast<size_t>(b) * a.n_parts;
@@ -112,18 +113,19 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
     return Cand{score, key, beam};
   };
 
-  // the bound: of each wave's firsts, so many lanes' best reach one of 16 bits; the
-  // highest of the waves'
-  float top = -INFINITY;
+  // The bound: where n_best / q parts' q-th keys reach one of 16 bits, n_best keys do.  The
+  // highest of the waves' and of those of q = 1, 4 and 16 (where one beam has most of the
+  // best, the first keys alone leave hundreds: 11 groups of 16 beams, best 26 59 us, so 10.2;
+  // up to 8 they leave few enough: one of 4 4.6, so 5.3).
+  uint32_t lanes_bound = 0;
 #pragma unroll
-  for (int i = 0; i < kOwn; ++i) {
-    const int p = tid + i * kSelThreads;
-    if (p >= firsts) continue;
-    const Cand c = of(p / a.n_parts, first[i]);
-    const float f = static_cast<float>(c.score);
-    top = f > top ? f : top;
+  for (int i = 0; i < kDepths; ++i) {
+    if (1 << 2 * i > a.n_best || (i > 0 && a.n_best <= 8)) break;
+    float top = -INFINITY;
+    if (tid < firsts) top = static_cast<float>(of(tid / a.n_parts, of_part[i]).score);
+    const uint32_t at = bound_of_lanes(order_of(top), (a.n_best + (1 << 2 * i) - 1) >> 2 * i);
+    lanes_bound = at > lanes_bound ? at : lanes_bound;
   }
-  const uint32_t lanes_bound = bound_of_lanes(order_of(top), a.n_best);
   if (lane == 0) bound_s[wave] = lanes_bound;
   __syncthreads();
   uint32_t bound = 0;
@@ -132,11 +134,7 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
   const auto reaches = [&](const Cand &c) {
     return c.score > -INFINITY && order_of(static_cast<float>(c.score)) >= bound;
   };
-#pragma unroll
-  for (int i = 0; i < kOwn; ++i) {
-    const int p = tid + i * kSelThreads;
-    if (p < firsts && reaches(of(p / a.n_parts, first[i]))) live_s[atomicAdd(&n_live_s, 1)] = p;
-  }
+  if (tid < firsts && reaches(of(tid / a.n_parts, first))) live_s[atomicAdd(&n_live_s, 1)] = tid;
   __syncthreads();
   const int n_keys = n_live_s * a.n_best;
   for (int i0 = tid; i0 < n_keys; i0 += kAhead * kSelThreads) {
@@ -194,20 +192,11 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
     return;
   }
   // Too many equal ones: the parts' lists merged, one continuation a round.
-  int next[kOwn];
-  Cand head[kOwn];
-#pragma unroll
-  for (int i = 0; i < kOwn; ++i) {
-    const int p = tid + i * kSelThreads;
-    next[i] = 1;
-    head[i] = p < firsts ? of(p / a.n_parts, first[i]) : Cand{-INFINITY, 0, a.width};
-  }
+  int next = 1;
+  Cand head = tid < firsts ? of(tid / a.n_parts, first) : Cand{-INFINITY, 0, a.width};
   for (int place = 0; place < a.n_best; ++place) {
-    Cand best = head[0];
+    Cand best = head;
     int at = tid;
-#pragma unroll
-    for (int i = 1; i < kOwn; ++i)
-      if (head[i].before(best)) best = head[i], at = tid + i * kSelThreads;
 #pragma unroll
     for (int by = 32; by > 0; by >>= 1) {
       const Cand o{lane_xor(best.score, by),
@@ -227,13 +216,9 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
       if (best.score > -INFINITY) put(place, best);
       else none(place);
     }
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      const int p = tid + i * kSelThreads;
-      if (p != at || p >= firsts) continue;
-      head[i].score = -INFINITY;
-      if (next[i] < a.n_best)
-        head[i] = of(p / a.n_parts, a.keys[(part0 + p) * a.n_best + next[i]++]);
+    if (tid == at && tid < firsts) {
+      head.score = -INFINITY;
+      if (next < a.n_best) head = of(tid / a.n_parts, a.keys[(part0 + tid) * a.n_best + next++]);
     }
   }
 }
