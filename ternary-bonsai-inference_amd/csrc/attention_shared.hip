@@ -181,6 +181,21 @@ int launch_shared_join(const PagedArgs &a, const Join &one, const Join &two, hip
 //     hd 128, f16: 0.5 51, 44, 50; 0.8 52, 58, 57; f32: 0.25 52, 27, 28; 0.5 72, 71, 66; 2.4 119, 131, 114
 //     hd 64, f16: 1.1 33, 22, 25; 2.1 36, 33, 28; 4.7 42, 35, 29; f32: 0.6 38, 21, 24; 1.3 40, 35, 32;
 //     4.7 53, 47, 45
+//
+// A tile has whole runs (Walk::run) where few requests and groups have few units a worker:
+// us of the call without and with, f16 hd 256 at 6 units a worker 60 and 46, at 7 71 and 63;
+// hd 128 at 7 54 and 39; hd 64 at 4 28 and 26; f32 102 and 84, 53 and 49, 39 and 33.
+// Where runs are longer, or tiles many, the walk's further registers only cost, up to 4 per
+// cent: the host leaves out what can be told from the table, the rows and the requests.
+bool whole_runs_pay(const bh_attention_paged_args &q, size_t n_group, const Form &f) {
+  const size_t n = q.n_req + n_group, most = f.workers() / kRunPads;
+  if (n > 64 || n * q.cache.n_kv > most) return false;
+  const size_t tiles = q.n_tok * (q.n_head / q.cache.n_kv) / f.rows() + n_group;
+  const int unit = q.cache.kv_dtype == BH_KV_F16 && q.cache.hd <= 128 ? 128 : 64;  // Shape::U
+  return static_cast<double>(tiles * q.cache.n_kv) * static_cast<double>(q.table_width * q.cache.page_size) <=
+         1.25 * kRunUnits * unit * f.workers();
+}
+
 int shared_forms(const bh_attention_shared_args &p, Form *f) {
   bh_attention_paged_args q = p.paged;
   const size_t own = q.max_new == 0 || q.max_new > q.n_tok ? q.n_tok : q.max_new;
@@ -203,13 +218,17 @@ int shared_forms(const bh_attention_shared_args &p, Form *f) {
   constexpr int kAll = 0x7fffffff;
   if (odd || work <= (rows <= 64 ? line.few : line.one)) {
     f[0] = Form{1, false, 0, kAll, 2};
+    f[0].runs = whole_runs_pay(p.paged, p.n_group, f[0]);
     return 1;
   }
   if (rows > 64 && work <= line.two) {
     f[0] = Form{2, false, 0, kAll, 2};
+    f[0].runs = whole_runs_pay(p.paged, p.n_group, f[0]);
     return 1;
   }
-  return forms_of(q, f);
+  const int n = forms_of(q, f);
+  if (n == 1 && !f[0].wide) f[0].runs = whole_runs_pay(p.paged, p.n_group, f[0]);
+  return n;
 }
 
 size_t prefix_bytes(const PagedArgs &a) { return align256(a.n_group * sizeof(PrefixOf)); }

@@ -60,6 +60,9 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kPUnit = 16384.0f;  // probabilities in f16 stand in units of 2^-14
 constexpr float kNoScore = -3.402823466e38f;  // the maximum of scores that are all -inf
+// RUNS: units a worker below which a tile has whole runs, and how many workers the tiles'
+// further units leave for one of them.
+constexpr int kRunUnits = 8, kRunPads = 4;
 constexpr int kJoinRows = 8;        // rows of a tile that the waves join at a time
 
 // Where a call's work lies.  A request with n tokens has T = ceil(n group / R) row
@@ -77,6 +80,8 @@ constexpr int kJoinRows = 8;        // rows of a tile that the waves join at a t
 // the call's request r from where its group's prefix ends.  A row is in a tile of
 // each, so no tile is done when its parts are: all leave them, a tile's part at its
 // worker's number behind the tile's (along the line either grows from part to part).
+// While runs are short, a run that goes on in a second tile, with its q, its table and its
+// join, takes half as long again as the others: each tile then has whole runs.
 struct Cut {  // a tile, written by the worker of its first part
   int rows;         // 0: it has one part, and its rows are done
   int first, last;  // workers of its parts
@@ -108,6 +113,11 @@ __device__ __forceinline__ int64_t divide(int64_t x, int64_t d) {
 __device__ __forceinline__ int64_t run_begin(int64_t total, int workers, int w) {
   const int64_t base = divide(total, workers), rest = total - base * workers;
   return w * base + (w < rest ? w : rest);
+}
+
+// `units` rounded up to runs (0: as they are).
+__device__ __forceinline__ int whole_runs(int units, int run) {
+  return run == 0 ? units : static_cast<int>(static_cast<uint32_t>(units + run - 1) / static_cast<uint32_t>(run)) * run;
 }
 
 // The worker whose run holds unit u.
@@ -193,6 +203,14 @@ struct Work : Extent<SHARED> {
     head = static_cast<int64_t>(tiles / 2) * pair + mid;
   }
   __device__ __forceinline__ int64_t cost(const PagedArgs &a) const { return head * a.n_kv; }
+  // Each tile in whole runs: its units from a multiple of `run` on.  A pair then takes up to
+  // 3 (run - 1) units more.
+  __device__ __forceinline__ int pads() const { return tiles / 2 * 3 + (tiles & 1); }
+  __device__ __forceinline__ void pad(int run) {
+    pair = whole_runs(pair + 2 * (run - 1), run);
+    if (mid != 0) mid = whole_runs(mid, run);
+    head = static_cast<int64_t>(tiles / 2) * pair + mid;
+  }
   // From lane `l`.
   __device__ __forceinline__ void take(int l) {
     q0 = __builtin_amdgcn_readlane(q0, l), n = __builtin_amdgcn_readlane(n, l);
@@ -569,10 +587,12 @@ struct PieceOf {
 template <bool SHARED>
 struct Piece : PieceOf, Extent<SHARED> {};
 
-template <int R, int U, bool SHARED>
+// RUNS, of SHARED: each tile in whole runs, where the call's sizes are such that it pays.
+template <int R, int U, bool SHARED, bool RUNS>
 struct Walk {
   int64_t total, end, at, base, begin;
   int tile_base, r, worker;
+  int run;  // RUNS: units of a run that is one tile's; 0: runs are cut anywhere
   Work<R, U, SHARED> work;
 
   // Every wave finds the run by itself: lane i adds up requests i per .. (i + 1)
@@ -601,13 +621,38 @@ struct Walk {
     upto_tiles = lane_scan(upto_tiles, SumOp{});
     tokens = lane_scan(tokens, SumOp{});
     total = wave_uniform(__shfl(upto, 63));
+    if constexpr (RUNS) {
+      run = 0;
+      // of n tiles and t units runs of (t - n) / (workers - n) units at most are enough
+      if (per == 1 && total < kRunUnits * sp.workers) {
+        const int pads = __builtin_amdgcn_readlane(lane_scan(lane < n_req ? work.pads() * a.n_kv : 0, SumOp{}), 63);
+        if (pads > 0 && pads <= sp.workers / kRunPads) {
+          run = max((static_cast<int>(total) - pads + sp.workers - pads - 1) / (sp.workers - pads), 1);
+          // (a run that is longer by more than a second tile costs pays nothing)
+          if (2 * run > 3 * ((static_cast<int>(total) + sp.workers - 1) / sp.workers)) run = 0;
+        }
+        if (run != 0) {
+          if (lane < n_req) {
+            work.pad(run);
+            mine = work.cost(a);
+          }
+          upto = lane_scan(mine, SumOp{});
+          total = wave_uniform(__shfl(upto, 63));
+        }
+      }
+    }
     if (__builtin_amdgcn_readlane(tokens, 63) > a.n_tok) total = 0, upto_tiles = 0;
     if constexpr (SHARED) {
       prefix_tokens = lane_scan(prefix_tokens, SumOp{});
       if (__builtin_amdgcn_readlane(prefix_tokens, 63) > a.n_tok) total = 0, upto_tiles = 0;
     }
-    at = begin = wave_uniform(run_begin(total, sp.workers, worker));
-    end = wave_uniform(run_begin(total, sp.workers, worker + 1));
+    if (RUNS && run != 0) {
+      at = begin = min<int64_t>(static_cast<int64_t>(worker) * run, total);
+      end = worker == sp.workers - 1 ? total : min<int64_t>(begin + run, total);
+    } else {
+      at = begin = wave_uniform(run_begin(total, sp.workers, worker));
+      end = wave_uniform(run_begin(total, sp.workers, worker + 1));
+    }
     if (worker == 0 && threadIdx.x == 63) *sp.n_tiles = upto_tiles;
     base = 0, tile_base = 0, r = 0;
     if (begin >= end) {
@@ -657,6 +702,7 @@ struct Walk {
         base += work.cost(a);
         tile_base += work.tiles * a.n_kv;
         work.load(a, sp, ++r);
+        if (RUNS && run != 0) work.pad(run);
         continue;
       }
       const int head = static_cast<int>(divide(at - base, work.head));
@@ -667,16 +713,20 @@ struct Walk {
       if (pair < work.tiles / 2) {  // the longer tile first, then its partner
         tile = work.tiles - 1 - pair;
         units = work.units(a, tile);
-        if (unit >= units) {
-          unit -= units;
+        if (unit >= runs_of(units)) {
+          unit -= runs_of(units);
           tile = pair;
-          const int before = units;
+          const int before = runs_of(units);
           units = work.units(a, tile);
           if (unit >= units) {  // the rest of the pair's space is empty
             at += work.pair - before - unit;
             continue;
           }
         }
+      }
+      if (RUNS && unit >= units) {  // the rest of the tile's last run
+        at += runs_of(units) - unit;
+        continue;
       }
       const int unit_end = static_cast<int>(min<int64_t>(units, unit + (end - at)));
       // all of it is the wave's, and stays in scalars
@@ -701,13 +751,18 @@ struct Walk {
     }
     return false;
   }
+  // Units of a tile's part of the line.
+  __device__ __forceinline__ int runs_of(int units) const { return RUNS ? whole_runs(units, run) : units; }
   static __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
   // The worker of a tile's first part says where its parts are; then past the piece.
   __device__ __forceinline__ void pass(const PagedArgs &a, const Split &sp, const Piece<SHARED> &p) {
     if (p.unit == 0 && threadIdx.x == 0) {
       Cut cut{p.whole ? 0 : p.rows, worker, worker, at == begin ? 0 : 1, p.tile * R, p.q0, p.head};
-      if (!p.whole) cut.last = worker_of(total, sp.workers, at + p.units - 1);
+      if (!p.whole)
+        cut.last = RUNS && run != 0
+                       ? min(static_cast<int>(divide(at + p.units - 1, run)), sp.workers - 1)
+                       : worker_of(total, sp.workers, at + p.units - 1);
       const uint32_t i = static_cast<uint32_t>(tile_base + p.head * work.tiles + p.tile);
       if constexpr (SHARED) {
         if (i < sp.most_cut)
@@ -742,7 +797,7 @@ struct Shape {
   static constexpr int U = WIDE ? 128 : kStride;
 };
 
-template <class E, bool WIDE, bool SHARED>
+template <class E, bool WIDE, bool SHARED, bool RUNS>
 __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedArgs a, Split sp) {
   using Elem = typename E::Elem;
   using S = Shape<E, WIDE>;
@@ -758,7 +813,7 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
 
-  Walk<R, U, SHARED> walk;
+  Walk<R, U, SHARED, RUNS> walk;
   walk.start(a, sp, lane);
   Piece<SHARED> piece;
   while (walk.next(a, sp, &piece)) {
@@ -1088,7 +1143,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
 
-  Walk<R, U, SHARED> walk;
+  Walk<R, U, SHARED, false> walk;
   walk.start(a, sp, lane);
   Piece<SHARED> piece;
   while (walk.next(a, sp, &piece)) {
@@ -1515,6 +1570,7 @@ struct Form {
   bool wide;
   int over, most;  // the requests it takes, by rows a kv head
   int blocks;      // a compute unit
+  bool runs = false;
 
   int rows() const { return 16 * rt * (wide ? kWaves : 1); }
   int workers() const { return static_cast<int>(device_cu_count()) * blocks; }
@@ -1597,10 +1653,10 @@ Join join_of(const PagedArgs &a, const Form &f, const Split &sp, int unit) {
   return BH_OK;
 }
 
-template <class E, bool WIDE, bool SHARED>
+template <class E, bool WIDE, bool SHARED, bool RUNS = false>
 int launch(const PagedArgs &a, const Form &f, char *ws, hipStream_t st, Join *join) {
   const Split sp = split_of<SHARED>(a, f, ws);
-  BH_LAUNCH((attn_paged_kernel<E, WIDE, SHARED>), static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
+  BH_LAUNCH((attn_paged_kernel<E, WIDE, SHARED, RUNS>), static_cast<unsigned>(sp.workers), kThreads, 0, st, a, sp);
   *join = join_of<SHARED>(a, f, sp, Shape<E, WIDE>::U);
   return BH_OK;
 }
@@ -1613,16 +1669,16 @@ int launch_wide(const PagedArgs &a, const Form &f, char *ws, hipStream_t st, Joi
   return BH_OK;
 }
 
-template <int RT, bool SHARED>
+template <int RT, bool SHARED, bool RUNS = false>
 int launch_rt(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream_t st, Join *join) {
   if (f16) {
-    if (a.hd == 64) return launch<EngineF16<64, RT>, false, SHARED>(a, f, ws, st, join);
-    if (a.hd == 128) return launch<EngineF16<128, RT>, false, SHARED>(a, f, ws, st, join);
-    return launch<EngineF16<256, RT>, false, SHARED>(a, f, ws, st, join);
+    if (a.hd == 64) return launch<EngineF16<64, RT>, false, SHARED, RUNS>(a, f, ws, st, join);
+    if (a.hd == 128) return launch<EngineF16<128, RT>, false, SHARED, RUNS>(a, f, ws, st, join);
+    return launch<EngineF16<256, RT>, false, SHARED, RUNS>(a, f, ws, st, join);
   }
-  if (a.hd == 64) return launch<EngineF32<64, RT>, false, SHARED>(a, f, ws, st, join);
-  if (a.hd == 128) return launch<EngineF32<128, RT>, false, SHARED>(a, f, ws, st, join);
-  return launch<EngineF32<256, RT>, false, SHARED>(a, f, ws, st, join);
+  if (a.hd == 64) return launch<EngineF32<64, RT>, false, SHARED, RUNS>(a, f, ws, st, join);
+  if (a.hd == 128) return launch<EngineF32<128, RT>, false, SHARED, RUNS>(a, f, ws, st, join);
+  return launch<EngineF32<256, RT>, false, SHARED, RUNS>(a, f, ws, st, join);
 }
 
 template <bool SHARED>
@@ -1636,6 +1692,10 @@ int launch_form(const PagedArgs &a, bool f16, const Form &f, char *ws, hipStream
     if (a.hd == 64) return launch<EngineF32<64, 2>, true, SHARED>(a, f, ws, st, join);
     if (a.hd == 128) return launch<EngineF32<128, 2>, true, SHARED>(a, f, ws, st, join);
     return launch<EngineF32<256, 2>, true, SHARED>(a, f, ws, st, join);
+  }
+  if constexpr (SHARED) {
+    if (f.runs && f.rt == 1) return launch_rt<1, SHARED, true>(a, f16, f, ws, st, join);
+    if (f.runs) return launch_rt<2, SHARED, true>(a, f16, f, ws, st, join);
   }
   if (f.rt == 1) return launch_rt<1, SHARED>(a, f16, f, ws, st, join);
   return launch_rt<2, SHARED>(a, f16, f, ws, st, join);

@@ -74,3 +74,44 @@ def test_garbage_offsets_stay_in_bounds(bh, dev, columns):
         c[key] = np.array(val, np.int32)
         print(columns, key, val, flush=True)
         assert _run(bh, dev, c).shape == base["q"].shape
+
+
+# Groups of long prefixes and few rows, where a tile's parts are whole runs of several units
+# (with 256 compute units 2 to 7), short, odd, and none of a request's own among them.  The
+# tolerance holds at these lengths too: of n positions with scores of unit variance the
+# output and the part of the scores' errors that a mean leaves both go with 1 / sqrt(n).
+LONG = [
+    [(16384, [(100, 1)] * 7)],
+    [(9001, [(30, 1)] * 10), (5003, [(333, 3)] * 4), (0, [(70, 1)])],
+    [(30017, [(1, 1)] * 3)],
+    [(12000, [(65, 1), (640, 2), (3, 1)]), (7999, [(1, 1), (63, 9)]), (33, [(700, 1)])],
+]
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("n_head,n_kv,hd,page", [(8, 2, 64, 16), (6, 2, 128, 7), (12, 2, 256, 16)])
+@pytest.mark.parametrize("nth", range(len(LONG)))
+def test_long_prefixes_of_few_rows(bh, dev, nth, n_head, n_kv, hd, page, f16):
+    groups = LONG[nth]
+    c = _case(groups, page=page, n_head=n_head, n_kv=n_kv, hd=hd, f16=f16)
+    print(nth, hd, f16, flush=True)
+    got = _check(bh, dev, c)
+    new = [n for _, reqs in groups for _, n in reqs]
+    most = max(sum(n for _, n in reqs) for _, reqs in groups)
+    again = _check(bh, dev, c, max_new=max(new), max_group_new=most)
+    assert np.array_equal(again, _run(bh, dev, c, max_new=max(new), max_group_new=most))
+    assert np.array_equal(got, _run(bh, dev, c))
+
+
+def test_long_prefix_under_garbage_offsets(bh, dev):
+    base = _case([(9001, [(30, 1)] * 3), (4100, [(70, 5), (9, 2)])], n_head=8, n_kv=2, hd=128,
+                 spare_tokens=0)
+    n = len(base["q"])
+    for key, val in (("q_start", [0, 3, 2, 3, 2 ** 30, n]), ("q_start", [n, 8, 6, 4, 2, 1]),
+                     ("group_start", [3, 1, 5]), ("group_start", [-9, 2 ** 30, 1]),
+                     ("group", [0, 1, 0, 1, 0]), ("shared", [2 ** 31 - 1, 2 ** 31 - 1]),
+                     ("kv_len", [2 ** 31 - 1, -4, 0, 1, 2]), ("kv_len", [9031, 0, 9031, 4170, 4109])):
+        c = dict(base)
+        c[key] = np.array(val, np.int32)
+        print(key, val, flush=True)
+        assert _run(bh, dev, c).shape == base["q"].shape
