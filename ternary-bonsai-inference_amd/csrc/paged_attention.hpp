@@ -127,25 +127,6 @@ __device__ __forceinline__ int worker_of(int64_t total, int workers, int64_t u) 
   return static_cast<int>(u < big ? divide(u, base + 1) : rest + divide(u - big, base));
 }
 
-// The group of request r, and the positions that it shares with it: 0 where it is by
-// itself.  (n, len: its tokens and length.)
-__device__ __forceinline__ int shared_of(const PagedArgs &a, int r, int n, int len, int *group) {
-  const int g = a.group_of[r];
-  *group = g;
-  if (g < 0 || g >= a.n_group || r < a.group_start[g] || r >= a.group_start[g + 1]) return 0;
-  const int shared = min(max(a.shared_len[g], 0), a.max_len);
-  return len - n < shared ? 0 : shared;
-}
-// Clipped tokens of group g; its first request.
-__device__ __forceinline__ int group_tokens(const PagedArgs &a, int g, int *q0, int *n) {
-  const int from = min(max(a.group_start[g], 0), a.n_req);
-  const int to = min(max(a.group_start[g + 1], from), a.n_req);
-  const int s = min(max(a.q_start[from], 0), a.n_tok), e = min(max(a.q_start[to], 0), a.n_tok);
-  *q0 = s;
-  *n = max(e - s, 0);
-  return from;
-}
-
 // Of SHARED work: its first position; its row of the table, below 0: ~row, and a
 // group's prefix.
 struct Part_of {
@@ -178,17 +159,25 @@ struct Work : Extent<SHARED> {
   }
   __device__ __forceinline__ void load(const PagedArgs &a, const Split &sp, int r) {
     if constexpr (SHARED) {
+      // A group's tokens are its requests'; a request has a prefix where its group names
+      // it too and the prefix ends before its tokens.  What either kind reads goes side by
+      // side: two loads after one another, not five.
+      const bool prefix = r < a.n_group;
+      const int own = prefix ? 0 : r - a.n_group;
+      const int32_t *const bounds = prefix ? a.group_start + r : a.q_start + own;
+      const int from = bounds[0], to = bounds[1], g = a.group_of[own];
+      const int have = *(prefix ? a.shared_len + r : a.kv_len + own);
+      const bool grouped = !prefix && g >= 0 && g < a.n_group;
+      const int r0 = min(max(from, 0), a.n_req), r1 = min(max(to, r0), a.n_req);
+      const int32_t *const start = prefix ? a.q_start + r0 : a.group_start + (grouped ? g : 0);
+      const int s = start[0], e = start[prefix ? r1 - r0 : 1], of_group = a.shared_len[grouped ? g : 0];
       first = 0, group = -1;
-      if (r < a.n_group) {
-        row = ~group_tokens(a, r, &q0, &n);
-        len = min(max(a.shared_len[r], 0), a.max_len);
-      } else {
-        row = r - a.n_group;
-        int g;
-        request(a, row, &q0, &n, &len);
-        first = shared_of(a, row, n, len, &g);
-        if (first > 0) group = g;
-      }
+      row = prefix ? ~r0 : own;
+      q0 = min(max(prefix ? s : from, 0), a.n_tok);
+      n = max(min(max(prefix ? e : to, 0), a.n_tok) - q0, 0);
+      len = min(max(have, 0), a.max_len);
+      const int shared = min(max(of_group, 0), a.max_len);
+      if (grouped && own >= s && own < e && len - n >= shared && shared > 0) first = shared, group = g;
     } else {
       request(a, r, &q0, &n, &len);
     }
