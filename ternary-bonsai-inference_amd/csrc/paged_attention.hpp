@@ -115,9 +115,9 @@ __device__ __forceinline__ int64_t run_begin(int64_t total, int workers, int w) 
   return w * base + (w < rest ? w : rest);
 }
 
-// `units` rounded up to runs (0: as they are).
+// `units` rounded up to runs.
 __device__ __forceinline__ int whole_runs(int units, int run) {
-  return run == 0 ? units : static_cast<int>(static_cast<uint32_t>(units + run - 1) / static_cast<uint32_t>(run)) * run;
+  return static_cast<int>(static_cast<uint32_t>(units + run - 1) / static_cast<uint32_t>(run)) * run;
 }
 
 // The worker whose run holds unit u.
@@ -138,8 +138,9 @@ struct All_of {
 template <bool SHARED>
 using Extent = std::conditional_t<SHARED, Part_of, All_of>;
 
-// A request's tiles and units.
-template <int R, int U, bool SHARED>
+// A request's tiles and units.  COST: a tile's further units, for what it takes before and
+// behind its steps.
+template <int R, int U, bool SHARED, int COST>
 struct Work : Extent<SHARED> {
   using Extent<SHARED>::first;
   using Extent<SHARED>::row;
@@ -188,7 +189,8 @@ struct Work : Extent<SHARED> {
     // two tiles with as many positions in all, but for a token of rounding, have as
     // many units but for one
     if (tiles > 1) pair = units(a, 0) + units(a, tiles - 1, true) + 1;
-    if (tiles & 1) mid = units(a, tiles / 2);
+    if (tiles & 1) mid = units(a, tiles / 2) + COST;
+    pair += 2 * COST;
     head = static_cast<int64_t>(tiles / 2) * pair + mid;
   }
   __device__ __forceinline__ int64_t cost(const PagedArgs &a) const { return head * a.n_kv; }
@@ -196,8 +198,8 @@ struct Work : Extent<SHARED> {
   // 3 (run - 1) units more.
   __device__ __forceinline__ int pads() const { return tiles / 2 * 3 + (tiles & 1); }
   __device__ __forceinline__ void pad(int run) {
-    pair = whole_runs(pair + 2 * (run - 1), run);
-    if (mid != 0) mid = whole_runs(mid, run);
+    pair = whole_runs(pair - 2 * COST + 2 * (run - 1), run);
+    if (mid != 0) mid = whole_runs(mid - COST, run);
     head = static_cast<int64_t>(tiles / 2) * pair + mid;
   }
   // From lane `l`.
@@ -577,12 +579,12 @@ template <bool SHARED>
 struct Piece : PieceOf, Extent<SHARED> {};
 
 // RUNS, of SHARED: each tile in whole runs, where the call's sizes are such that it pays.
-template <int R, int U, bool SHARED, bool RUNS>
+template <int R, int U, bool SHARED, bool RUNS, int COST>
 struct Walk {
   int64_t total, end, at, base, begin;
   int tile_base, r, worker;
   int run;  // RUNS: units of a run that is one tile's; 0: runs are cut anywhere
-  Work<R, U, SHARED> work;
+  Work<R, U, SHARED, COST> work;
 
   // Every wave finds the run by itself: lane i adds up requests i per .. (i + 1)
   // per - 1, a scan over the lanes gives the total, and the lanes then go through
@@ -613,12 +615,14 @@ struct Walk {
     if constexpr (RUNS) {
       run = 0;
       // of n tiles and t units runs of (t - n) / (workers - n) units at most are enough
-      if (per == 1 && total < kRunUnits * sp.workers) {
+      const int units = static_cast<int>(min<int64_t>(
+          total - static_cast<int64_t>(COST) * __builtin_amdgcn_readlane(upto_tiles, 63), 1 << 30));
+      if (per == 1 && units < kRunUnits * sp.workers) {
         const int pads = __builtin_amdgcn_readlane(lane_scan(lane < n_req ? work.pads() * a.n_kv : 0, SumOp{}), 63);
         if (pads > 0 && pads <= sp.workers / kRunPads) {
-          run = max((static_cast<int>(total) - pads + sp.workers - pads - 1) / (sp.workers - pads), 1);
+          run = max((units - pads + sp.workers - pads - 1) / (sp.workers - pads), 1);
           // (a run that is longer by more than a second tile costs pays nothing)
-          if (2 * run > 3 * ((static_cast<int>(total) + sp.workers - 1) / sp.workers)) run = 0;
+          if (2 * run > 3 * ((units + sp.workers - 1) / sp.workers)) run = 0;
         }
         if (run != 0) {
           if (lane < n_req) {
@@ -713,7 +717,7 @@ struct Walk {
           }
         }
       }
-      if (RUNS && unit >= units) {  // the rest of the tile's last run
+      if ((RUNS || COST != 0) && unit >= units) {  // the rest of the tile's part of the line
         at += runs_of(units) - unit;
         continue;
       }
@@ -741,7 +745,9 @@ struct Walk {
     return false;
   }
   // Units of a tile's part of the line.
-  __device__ __forceinline__ int runs_of(int units) const { return RUNS ? whole_runs(units, run) : units; }
+  __device__ __forceinline__ int runs_of(int units) const {
+    return RUNS && run != 0 ? whole_runs(units, run) : units + COST;
+  }
   static __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
   // The worker of a tile's first part says where its parts are; then past the piece.
@@ -786,6 +792,12 @@ struct Shape {
   static constexpr int U = WIDE ? 128 : kStride;
 };
 
+// Of SHARED, whose line holds tiles of hundreds of units and tiles of one or two: without a
+// tile's cost the workers of the small ones, nine or so each, are the last to end.  In units,
+// which over f16 take half as long.
+template <class E>
+constexpr int kTileCost = sizeof(typename E::Elem) == 2 ? 2 : 1;
+
 template <class E, bool WIDE, bool SHARED, bool RUNS>
 __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedArgs a, Split sp) {
   using Elem = typename E::Elem;
@@ -802,7 +814,7 @@ __global__ __launch_bounds__(kThreads, E::kBlocks) void attn_paged_kernel(PagedA
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
 
-  Walk<R, U, SHARED, RUNS> walk;
+  Walk<R, U, SHARED, RUNS, SHARED && !WIDE ? kTileCost<E> : 0> walk;
   walk.start(a, sp, lane);
   Piece<SHARED> piece;
   while (walk.next(a, sp, &piece)) {
@@ -1132,7 +1144,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_paged_wide_kernel(PagedA
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
 
-  Walk<R, U, SHARED, false> walk;
+  Walk<R, U, SHARED, false, 0> walk;
   walk.start(a, sp, lane);
   Piece<SHARED> piece;
   while (walk.next(a, sp, &piece)) {
