@@ -170,17 +170,18 @@ int launch_shared_join(const PagedArgs &a, const Join &one, const Join &two, hip
 // more than the wide form's larger tiles while the work is small.  What counts is the work
 // as far as the host knows it: rows of the call times positions of the table, in millions.
 // Measured, us of the call, in order: as in forms_of, one row tile, two; "rows" of a group.
-//   up to 64 rows.  hd 256, f16: 0.2 38, 30, 38; 1.2 110, 79, 108; 2.4 205, 146, 205
-//     f32: 0.4 47, 47, 47; 1.0 (60 rows) 105, 117, 105; 2.4 (48 rows: three tiles for
-//     four) 259, 246, 257
-//     hd 128, f16: 0.13 27, 24, 27; 0.5 (24 rows) 43, 46, 43; 1.0 (48 rows) 74, 66, 73
-//     f32: 0.13 31, 29, 31; 0.28 40, 42, 40; 1.1 91, 122, 90
-//     hd 64, f16: 0.3 17, 16, 17; 1.0 25, 23, 25; 3.1 31, 42, 31; f32: 0.3 19, 16, 18; 1.6 33, 39, 32
-//   more.  hd 256, f16: 0.4 46, 29, 38; 0.7 58, 54, 75; 0.8 53, 61, 67; 1.5 74, 102, 137
-//     f32: 0.4 87, 57, 57; 1.3 149, 129, 119; 1.7 151, 175, 156
-//     hd 128, f16: 0.5 51, 44, 50; 0.8 52, 58, 57; f32: 0.25 52, 27, 28; 0.5 72, 71, 66; 2.4 119, 131, 114
-//     hd 64, f16: 1.1 33, 22, 25; 2.1 36, 33, 28; 4.7 42, 35, 29; f32: 0.6 38, 21, 24; 1.3 40, 35, 32;
-//     4.7 53, 47, 45
+//   up to 64 rows.  hd 256, f16: 0.2 32, 26, 32; 0.8 50, 46, 51; 1.0 54, 57, 54; 2.0 72, 86, 74
+//     f32: 0.5 73, 65, 70; 0.6 82, 83, 82; 1.0 81, 98, 84
+//     hd 128, f16: 0.07 24, 21, 21; 0.3 34, 34, 33; 0.4 32, 38, 31; 1.1 44, 56, 45
+//     f32: 0.05 25, 22, 25; 0.13 28, 29, 29; 0.5 50, 55, 50
+//     hd 64, f16: 0.3 18, 16, 18; 1.1 21, 21, 21; 8.5 41, 49, 41; f32: 0.3 20, 18, 19; 1.9 38, 36, 38;
+//     3.2 38, 47, 38
+//   more.  hd 256, f16: 0.4 46, 26, 31; 0.8 71, 47, 56; 1.3 66, 62, 58; 2.5 64, 68, 58; 3.1 106, 128, 116
+//     f32: 0.4 86, 38, 39; 0.8 96, 81, 73; 2.1 171, 153, 134; 6.4 321, 492, 322
+//     hd 128, f16: 0.3 47, 32, 34; 0.8 52, 44, 41; 3.3 114, 138, 93; 4.3 102, 176, 106
+//     f32: 0.3 74, 47, 52; 0.8 80, 83, 65; 4.3 228, 342, 207
+//     hd 64, f16: 1.1 31, 21, 23; 2.8 44, 29, 30; 4.1 50, 34, 31; 8.5 59, 52, 44
+//     f32: 1.1 40, 25, 27; 2.1 45, 35, 34; 8.5 88, 104, 77
 //
 // A tile has whole runs (Walk::run) where few requests and groups have few units a worker:
 // us of the call without and with, f16 hd 256 at 6 units a worker 60 and 46, at 7 71 and 63;
@@ -210,19 +211,17 @@ int shared_forms(const bh_attention_shared_args &p, Form *f) {
     double few, one, two;
   };
   const bool f16 = q.cache.kv_dtype == BH_KV_F16;
-  const Line line = q.cache.hd == 256   ? (f16 ? Line{1e30, 0.75, 0} : Line{0.45, 1.3, 0})
-                    : q.cache.hd == 128 ? (f16 ? Line{0.45, 0.75, 0} : Line{0.13, 0.25, 2.5})
-                                        : (f16 ? Line{1.1, 1.5, 5} : Line{0.8, 1.0, 5});
-  // (an odd number of tiles of 16 rows leaves half of the last two empty)
-  const bool odd = (rows + 15) / 16 % 2 == 1 && rows <= 64 && f16 != (q.cache.hd == 256) && q.cache.hd != 64;
+  const Line line = q.cache.hd == 256   ? (f16 ? Line{0.9, 1.0, 2.6} : Line{0.55, 0.6, 6})
+                    : q.cache.hd == 128 ? (f16 ? Line{0.3, 0.5, 4.2} : Line{0.13, 0.5, 5})
+                                        : (f16 ? Line{1.1, 3, 16} : Line{2, 2, 12});
   constexpr int kAll = 0x7fffffff;
-  if (odd || work <= (rows <= 64 ? line.few : line.one)) {
+  if (work <= (rows <= 64 ? line.few : line.one)) {
     f[0] = Form{1, false, 0, kAll, 2};
     f[0].runs = whole_runs_pay(p.paged, p.n_group, f[0]);
     return 1;
   }
   if (rows > 64 && work <= line.two) {
-    f[0] = Form{2, false, 0, kAll, 2};
+    f[0] = Form{2, false, 0, kAll, q.cache.hd == 256 ? 1 : 2};  // (E::kBlocks)
     f[0].runs = whole_runs_pay(p.paged, p.n_group, f[0]);
     return 1;
   }

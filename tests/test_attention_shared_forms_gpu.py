@@ -84,6 +84,7 @@ LONG = [
     [(16384, [(100, 1)] * 7)],
     [(9001, [(30, 1)] * 10), (5003, [(333, 3)] * 4), (0, [(70, 1)])],
     [(30017, [(1, 1)] * 3)],
+    [(9001, [(30, 1)] * 24)],
     [(12000, [(65, 1), (640, 2), (3, 1)]), (7999, [(1, 1), (63, 9)]), (33, [(700, 1)])],
 ]
 
