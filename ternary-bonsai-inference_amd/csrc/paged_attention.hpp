@@ -34,7 +34,8 @@ struct PagedArgs {
 };
 
 // Where the tiles of a group's prefix are: their launch and their first place in it, and
-// the group's tokens.
+// the group's tokens.  Every call writes every group's: of a group without tiles `n` is 0,
+// which only offsets that decrease can leave a request with tokens in.
 struct PrefixOf {
   int launch, base, q0, n;
 };
@@ -598,11 +599,14 @@ struct Walk {
     int64_t mine = 0;
     int mine_tiles = 0, tokens = 0;  // (n_tok < 2^24: 64 lanes of n_tok + 1 stay below 2^31)
     int prefix_tokens = 0;           // a group's tokens count once more
+    // the records of groups without tiles here (a later launch has them, or none)
+    const bool records = SHARED && a.launch == 0 && worker == 0 && threadIdx.x < 64;
     for (int i = lane * per; i < min((lane + 1) * per, n_req) && tokens <= a.n_tok &&
                              (!SHARED || prefix_tokens <= a.n_tok); ++i) {
       work.load(a, sp, i);
       mine += work.cost(a);
       mine_tiles += work.tiles * a.n_kv;
+      if (SHARED && records && work.row < 0 && work.n == 0) a.prefix[i] = PrefixOf{0, 0, 0, 0};
       if (SHARED && work.row < 0) prefix_tokens = min(prefix_tokens + work.n, a.n_tok + 1);
       else tokens = min(tokens + work.n, a.n_tok + 1);
     }
@@ -638,6 +642,8 @@ struct Walk {
     if constexpr (SHARED) {
       prefix_tokens = lane_scan(prefix_tokens, SumOp{});
       if (__builtin_amdgcn_readlane(prefix_tokens, 63) > a.n_tok) total = 0, upto_tiles = 0;
+      if (records && total == 0)
+        for (int i = lane; i < a.n_group; i += 64) a.prefix[i] = PrefixOf{0, 0, 0, 0};
     }
     if (RUNS && run != 0) {
       at = begin = min<int64_t>(static_cast<int64_t>(worker) * run, total);
