@@ -34,7 +34,9 @@
  * the PQ2_0 products (bh_pq2_matvec_range, bh_pq2_matmul_n) with more than 4
  * tokens or on shapes outside the integer path, and bh_gdn_step on batches
  * of 128 or more tokens at s = 128, which use per-device scratch buffers:
- * each must not run concurrently with itself on one device.
+ * each must not run concurrently with itself on one device, nor
+ * bh_attention with bh_attention_planar, or one PQ2_0 product with the other,
+ * which share a buffer.
  *
  * Scratch and HIP graphs: a scratch buffer grows (allocates) the first time
  * a call needs more than it holds.  The buffer it replaces is kept until the

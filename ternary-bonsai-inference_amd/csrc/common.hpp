@@ -43,9 +43,9 @@ inline int pow2ceil(size_t v) {
   return p;
 }
 
-// Per-device scratch owned by the library, one buffer per client so
-// different entry points never share one.  Calls of the same client on one
-// device must not overlap in time.  A buffer grows on demand (at least
+// Per-device scratch owned by the library, one buffer per client: an entry
+// point, or a few that the headers name together.  Calls of the same client on
+// one device must not overlap in time; those of different ones may.  A buffer grows on demand (at least
 // twofold) and the buffer it replaces is kept until the process ends, so a
 // graph captured earlier keeps valid addresses.  Growth while `stream` is
 // capturing is refused (it would allocate inside the capture).  A caller may
@@ -61,7 +61,8 @@ constexpr int kScratchGdn = 4;        // gated delta-net chunks: prepared matric
 constexpr int kScratchKvSplit = 5;    // attention: f32 cache split into f16 hi / lo
 constexpr int kScratchPaged = 6;      // paged attention: partial results of split requests
 constexpr int kScratchLogprobs = 7;   // log probabilities: chunk sums and candidates
-constexpr int kScratchSlots = 8;
+constexpr int kScratchGdnRagged = 8;  // the same of many requests at once
+constexpr int kScratchSlots = 9;
 void *device_scratch(size_t bytes, int slot, hipStream_t stream, size_t least = 0);
 // Current size of this device's buffer for `slot` (0 before the first use).
 size_t scratch_bytes(int slot);

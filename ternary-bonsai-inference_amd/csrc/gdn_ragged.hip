@@ -1132,7 +1132,7 @@ extern "C" int bh_gdn_ragged(const bh_gdn_ragged_args *args, bh_stream stream) {
                                       " bytes, " + std::to_string(need) +
                                       " needed on a 16-byte boundary");
     } else {
-      ws = static_cast<char *>(device_scratch(need, kScratchGdn, st));
+      ws = static_cast<char *>(device_scratch(need, kScratchGdnRagged, st));
       if (!ws) return BH_ERR_HIP;
     }
     a.most = kCkMin - 1;
