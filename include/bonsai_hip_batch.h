@@ -194,7 +194,7 @@ size_t bh_beam_select_workspace(const bh_beam_select_args *args);
  * dst_slot, or, where a step goes before it, in src_slot, of which spare_slot is a
  * copy; the 2 * n_group * width slots of dst_slot and spare_slot are distinct.
  *
- * No scratch.  parent must not be one of the outputs. */
+ * No scratch.  The groups' rows of parent share no memory with an output (refused). */
 typedef struct bh_beam_reorder_args {
   const int32_t *parent; /* [n_group][parent_stride], of which `width`  */
   int32_t *block_table;  /* [n_group * width][table_width]              */

@@ -387,6 +387,16 @@ int check(const bh_beam_select_args &p) {
   return BH_OK;
 }
 
+// Whether one of the groups' rows of `parent` shares memory with n words at `out`.
+bool parents_meet(const bh_beam_reorder_args &p, const int32_t *out, size_t n) {
+  const int64_t row = 4 * static_cast<int64_t>(p.width), stride = 4 * static_cast<int64_t>(p.parent_stride);
+  const int64_t begin = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out) - reinterpret_cast<uintptr_t>(p.parent));
+  const int64_t end = begin + 4 * static_cast<int64_t>(n);
+  if (end <= 0) return false;
+  const int64_t g = begin < row ? 0 : (begin - row) / stride + 1;  // the first that ends behind `begin`
+  return g < static_cast<int64_t>(p.n_group) && g * stride < end;
+}
+
 size_t parts_of(const bh_beam_select_args &p) {
   const size_t parts = parts_of_rows(p.n_group * p.width, p.vocab);
   const size_t most = kMostFirsts / p.width;  // (a group's parts have a thread each to look at them)
@@ -465,7 +475,11 @@ extern "C" int bh_beam_reorder(const bh_beam_reorder_args *args, bh_stream strea
   if (p.src_slot && (p.src_slot == p.dst_slot || p.src_slot == p.spare_slot ||
                      p.dst_slot == p.spare_slot))
     return fail(BH_ERR_ARG, "beam_reorder: src_slot, dst_slot and spare_slot must differ");
-  if (p.parent == p.copy_from || p.parent == p.block_table || p.parent == p.src_slot)
+  // (a group's blocks all read its parents while one of them writes)
+  const size_t beams = p.n_group * p.width;
+  if (parents_meet(p, p.block_table, beams * p.table_width) || parents_meet(p, p.copy_from, beams) ||
+      (p.src_slot && (parents_meet(p, p.src_slot, beams) || parents_meet(p, p.dst_slot, beams) ||
+                      parents_meet(p, p.spare_slot, beams))))
     return fail(BH_ERR_ARG, "beam_reorder: parent must not be an output");
   ReorderArgs a{p.parent, p.block_table, p.copy_from, p.src_slot, p.dst_slot, p.spare_slot,
                 static_cast<int>(p.width), static_cast<int>(p.parent_stride),
