@@ -983,10 +983,12 @@ def make_beam_select_args(x, score, width: int, n_best: int, inv_temp: float = 1
         else _dev_tensor(token, "token", ids, dev, shape)
     if score_out is None:
         score_out = torch.empty(shape, dtype=torch.float32, device=dev)
-    elif score_out.data_ptr() != score.data_ptr():  # the scores in place are a vector
+    elif score_out.data_ptr() != score.data_ptr():
         _dev_tensor(score_out, "score_out", f32, dev, shape)
-    elif score_out.numel() != shape[0] * n_best:
-        raise ValueError("score_out may be score only where n_best is width")
+    else:  # the scores in place, of any shape (a vector)
+        _dev_tensor(score_out, "score_out", f32, dev)
+        if score_out.numel() != shape[0] * n_best:
+            raise ValueError("score_out may be score only where n_best is width")
     args = BeamSelectArgs(_ptr(x), _ptr(score), _ptr(parent), _ptr(token), _ptr(score_out),
                           shape[0], width, x.shape[1], stride, n_best, inv_temp, None, 0)
     if workspace is not None:
