@@ -61,8 +61,9 @@ extern "C" {
  * and out_t = y_t, but for the first l2_dim channels (a multiple of head_dim; 0:
  * none), of which each group of head_dim is scaled by 1 / max(|group|, eps).  The
  * slot written holds the last k - 1 inputs, [ch][k - 1], oldest first.  out:
- * [n_tok][ch], not x; w: [ch][k], 1 <= k <= 64; k = 1 has no state (state NULL).
- * max_new is a hint as in bh_gdn_ragged.  No scratch. */
+ * [n_tok][ch], not x; w: [ch][k], 1 <= k <= 64; k = 1 has no state (state NULL), and
+ * no slot is bad then.  max_new is as in bh_gdn_ragged; no form depends on it here.  No
+ * scratch. */
 typedef struct bh_conv_ragged_args {
   const float *x, *w;
   float *state; /* [n_slots][ch][k - 1] */

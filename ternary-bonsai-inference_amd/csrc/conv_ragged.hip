@@ -238,9 +238,10 @@ extern "C" int bh_conv1d_silu_ragged(const bh_conv_ragged_args *args, bh_stream 
   a.l2_dim = static_cast<int>(p.l2_dim), a.head_dim = static_cast<int>(p.head_dim);
   a.groups = p.l2_dim == 0 ? 0 : static_cast<int>(p.l2_dim / p.head_dim);
   a.eps = p.eps;
-  a.rag = Ragged{p.q_start, p.src_slot, p.dst_slot, p.bad_slot, static_cast<int>(p.n_tok),
-                 static_cast<int>(p.n_req), static_cast<int>(p.k > 1 ? p.n_slots : 0),
-                 p.slot_stride};
+  // (one tap: no state, so that no slot of it is bad)
+  a.rag = Ragged{p.q_start, p.src_slot, p.dst_slot, p.k > 1 ? p.bad_slot : nullptr,
+                 static_cast<int>(p.n_tok), static_cast<int>(p.n_req),
+                 static_cast<int>(p.k > 1 ? p.n_slots : 0), p.slot_stride};
   hipStream_t st = as_stream(stream);
   // lanes of a group: a power of two up to a wave's, whole groups a lane's four channels
   const size_t lanes = p.l2_dim == 0 ? 1 : p.head_dim / 4;
