@@ -86,7 +86,10 @@ int bh_conv1d_silu_ragged(const bh_conv_ragged_args *args, bh_stream stream);
  * q_stride, k_stride, v_stride floats apart (so that they may be parts of one row,
  * as the conv leaves them); gate, beta: [n_tok][h_v]; attn: [n_tok][h_v][s].
  * max_new: no request has more tokens than this (0: n_tok); it steers how the work
- * is laid out, and a wrong one costs time only. */
+ * is laid out, and a wrong one costs time only.
+ * Prompts of s = 64 and 128 go by chunks of 64 tokens whose operands keep 22 bits: an
+ * output is off by a few 2^-22 of |M[j]| |q| / sqrt(s), the largest of 16 rows j, whatever
+ * values other tokens hold. */
 typedef struct bh_gdn_ragged_args {
   const float *q, *k, *v, *gate, *beta;
   float *state; /* [n_slots][h_v][s][s] */
