@@ -8,7 +8,7 @@
  *   bh_conv1d_silu_ragged  a recurrent layer's causal conv + SiLU + L2 norms
  *   bh_gdn_ragged          its gated delta rule, one token or a prompt a request
  *   bh_attention_shared    bh_attention_paged of requests that share a prefix,
- *                          the prefix read once for all of them
+ *                          the prefix not read by each of them
  *   bh_beam_select         the best continuations of a group's beams
  *   bh_beam_reorder        page tables and state slots put in the new beams' order
  *   bh_kv_copy_paged       the pages of beams that went on more than once (a layer)
@@ -88,8 +88,8 @@ int bh_conv1d_silu_ragged(const bh_conv_ragged_args *args, bh_stream stream);
  * max_new: no request has more tokens than this (0: n_tok); it steers how the work
  * is laid out, and a wrong one costs time only.
  * Prompts of s = 64 and 128 go by chunks of 64 tokens whose operands keep 22 bits: an
- * output is off by a few 2^-22 of |M[j]| |q| / sqrt(s), the largest of 16 rows j, whatever
- * values other tokens hold. */
+ * output is off by a few 2^-22 of |M[j]| |q| / sqrt(s), the largest of 16 rows j and of what
+ * M has been in the chunk, as it has decayed by then; values of later tokens do not enter. */
 typedef struct bh_gdn_ragged_args {
   const float *q, *k, *v, *gate, *beta;
   float *state; /* [n_slots][h_v][s][s] */
@@ -115,7 +115,8 @@ size_t bh_gdn_ragged_workspace(const bh_gdn_ragged_args *args);
 /* bh_attention_paged where groups of requests have the same keys and values at
  * their first positions, as the beams of one prompt and the users of one system
  * prompt do: results are those of bh_attention_paged on `paged` (to rounding), and
- * the first shared_len[g] positions are read once for all rows of group g.
+ * the first shared_len[g] positions are read once a tile of 16 to 128 (token, head)
+ * rows of all requests of group g.
  *
  * Group g is the requests group_start[g] .. group_start[g + 1] - 1, and group[i]
  * is request i's (a request of group[i] outside 0 .. n_group - 1, or that does not
@@ -156,7 +157,8 @@ size_t bh_attention_shared_workspace(const bh_attention_shared_args *args);
  * and those of a group's beams are ordered by it, largest first, of equal ones the
  * lower row first, then the lower token.  (Compared in f64, before the score is
  * rounded to f32, and a row's own by their logits, of which -0 equals 0; rows of the
- * same bits have the same log Z.)  The n_best first go to parent (row r), token and
+ * same bits have the same log Z.  log Z is within 4e-6, commonly 1e-7: continuations of
+ * two beams of other bits that are nearer than that may change places.)  The n_best first go to parent (row r), token and
  * score_out, [n_group][n_best].
  * A beam whose score is not finite (-inf: it has ended, or not begun) and a row
  * with a NaN or +inf among its logits or with nothing above -inf have no

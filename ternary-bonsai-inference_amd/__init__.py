@@ -958,8 +958,8 @@ def attention_shared_workspace(args: AttentionSharedArgs) -> int:
 
 
 def attention_shared(args: AttentionSharedArgs, stream=None):
-    """attention_paged of requests that share a prefix, which is read once for all of
-    a group; returns the output tensor of the arguments."""
+    """attention_paged of requests that share a prefix, which is read once a tile of
+    rows of a group; returns the output tensor of the arguments."""
     _call(lib().bh_attention_shared, args, stream)
     return args.out_tensor
 

@@ -1,5 +1,5 @@
 // Attention of requests that share a prefix: the prefix's keys and values are read
-// once for the rows of all requests of a group.
+// once a tile of 16 to 128 rows of all requests of a group, not once a request.
 //
 // With o, m and l of a set of positions P the sums of a softmax over it (m the
 // largest score, l = sum e^(s - m), o = sum e^(s - m) v), those of two sets join as
@@ -9,8 +9,9 @@
 // walk begins where its prefix ends.  Both stand in one list that is cut into equal
 // runs, so that a long prefix and many short tails fill the card together; the join
 // takes each row's parts from its own tile and from its tile of the prefix.
-// 8 requests behind 4096 positions (24 / 4 heads of 256, f16): 23.0 us and 7.8 of the join,
-// bh_attention_paged reads 8 times as much; 64 behind 8192, tails to 2000: 67, 52 and 16.
+// 8 requests behind 4096 positions (24 / 4 heads of 256, f16): 18.1 us and 7.0 of the join, the
+// prefix read by three tiles, from memory once; bh_attention_paged reads 8 times as much; 64
+// behind 8192, tails to 2000: 66, 44 and 16.
 #include <hip/hip_runtime.h>
 
 #include <string>

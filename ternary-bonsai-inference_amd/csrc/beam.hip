@@ -8,11 +8,13 @@
 // logits.  One block a group then forms the rows' ln S, and with them the score of
 // each part's logits.  Where n_best of them reach a bound, only keys that reach it
 // matter: a few more than n_best, whose ranks, counted against one another, are
-// their places.  Scores are compared in f64, so that rounding puts no two beams
-// out of order: a step of f32 at a score of -100 is 8e-6.
-// Bound by reading the logits: 256 rows of 248320 in 32 groups, best 16: 56.4 us, 4.5 TB/s,
-// and 8.0 for the groups (30 with 256 threads that went through their lists one key after
-// the other); 4 rows 8.0 and 4.6.
+// their places.  Scores are compared in f64: a step of f32 at a score of -100 is 8e-6, and
+// what rounds before is ln S, which is the same for a beam's own continuations.  Its
+// exponentials are f32's, of arguments z log2(e) that round three times: |z| 3 2^-24, and
+// terms that matter have z down to -20: within 4e-6, commonly 1e-7.
+// Bound by reading the logits: 256 rows of 248320 in 32 groups, best 16: 57.0 us, 4.5 TB/s,
+// and 8.2 for the groups (30 with 256 threads that went through their lists one key after
+// the other); 4 rows 8.8 and 4.6.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -261,7 +263,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a, int pa
       with_children |= uint64_t{1} << of;
       if (of == p) heir = b;
     }
-    const uint64_t all = a.width == 64 ? ~uint64_t{0} : (uint64_t{1} << a.width) - 1;
+    const uint64_t all = (uint64_t{1} << a.width) - 1;
     const bool takes = lane < a.width && (p < 0 || heir != lane);
     const uint64_t takers = __ballot(takes);
     int from = p;

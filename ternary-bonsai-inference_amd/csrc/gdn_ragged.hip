@@ -175,7 +175,8 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_any_kernel(GdnArgs a) {
 
 // ---- prompts: chunks of 64 tokens on the matrix cores (s = 64, 128) ------------
 //
-// Over a chunk with decays a_t = e^gate_t, A_t = a_0 .. a_t, D_ts = A_t / A_s and a
+// (The compact WY form of the product of the tokens' steps, which is published for such
+// recurrences.)  Over a chunk with decays a_t = e^gate_t, A_t = a_0 .. a_t, D_ts = A_t / A_s and a
 // state row m at its beginning, the tokens' steps unroll to
 //   delta = T (v - A (K m)),  T = (I + L)^-1 diag(beta),  L_ts = beta_t D_ts (k_t.k_s), s < t,
 //   attn = (A (Q m) + P delta) / sqrt(s),                 P_ts = D_ts (q_t.k_s), s <= t,
@@ -197,7 +198,8 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_any_kernel(GdnArgs a) {
 // its column, so results become operands as they stand.
 //
 // What that floor may cost: over the dims of a state row it is small beside |m| |k| and |m| |q|,
-// as any sum's rounding.  Over the tokens of a chunk it is not: a value far larger than the
+// as any sum's rounding (m the largest that it has been in the chunk: what a later token takes
+// back of it leaves its rounding behind).  Over the tokens of a chunk it is not: a value far larger than the
 // others would leave its error in the outputs of tokens before it, or in the state when it has
 // decayed.  So the wave that has the rows looks whether each token's outputs reach 2^-18 of
 // P's row times the largest delta (or T's largest row times the largest right side), and the
@@ -213,7 +215,8 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr int kCk = 64;
 // Tokens from which a request goes by chunks.  One request of 32 / 48 / 64 / 127 tokens, us:
-// 24.3, 24.7, 25.1, 29.2, token by token 17.2, 24.3, 30.8, 63.3; 64 of 32 259 for 317.
+// 24.3, 24.7, 25.1, 29.2, token by token 17.2, 24.3, 30.8, 63.3; 64 of 32 259 for 317.  (Before
+// the look at a chunk's outputs, which adds 0.3.)
 constexpr int kCkMin = 48;
 constexpr int kCkPlace = 32;          // a chunk's place in the workspace every so many tokens
 template <int S>
@@ -534,8 +537,8 @@ __device__ __forceinline__ void list_long(const Ragged &rag, int longs, int32_t 
 
 // Block (chunk, q/k head): wave w has the tokens 16 w .. 16 w + 15.
 // Bound by the chain of small products and LDS trips that a wave takes a v-head through,
-// 16 us for a chunk, two blocks a compute unit by LDS: 46 chunks of 16 / 48 heads 44 us, of
-// which writing 127 MB is 26.
+// 16 us for a chunk, two blocks a compute unit by LDS: 47 chunks of 16 / 48 heads 48 us on
+// inputs of the call before, 56 on others, of which writing 134 MB is 27.
 template <int S>
 __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs c) {
   constexpr int kMat = kCk * kPitch, N = S / 32;  // N: of 32 dims
@@ -664,7 +667,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
 // registers: every result is the next product's operand as it stands.  The operands that
 // the waves share stand in LDS, K and Q apart from K transposed, T and P, so that each
 // part of the next chunk comes in while the other is read: two barriers a chunk.
-// Three prompts of 1536 tokens, 16 / 48 heads of 128: 176 us, one 98.
+// Three prompts of 1536 tokens, 16 / 48 heads of 128: 185 us, one 102.
 
 // Operands of a chunk in LDS: K, Q; K transposed, T, P; their vectors, of two chunks in
 // turn.
@@ -1015,8 +1018,8 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds<S> &lds, co
 // Blocks of the walk.  All rows of a (request, v-head) are a block's, 16 a wave; or, of the
 // longest requests, as far as blocks are fewer than compute units, half of them, and the
 // other four waves stage the operands (as they do for heads of 64).  What bounds a block is its waves' reads of them
-// from LDS (120 KB a wave and chunk), so half the rows are through sooner: 4.0 us a chunk
-// for 7.2.
+// from LDS (120 KB a wave and chunk), so half the rows are through sooner: 4.2 us a chunk
+// for 7.7.
 template <int S>
 __global__ __launch_bounds__(512, 2) void gdn_chunk_walk_kernel(GdnChunkArgs c) {
   __shared__ __attribute__((aligned(16))) ChunkLds<S> lds;
