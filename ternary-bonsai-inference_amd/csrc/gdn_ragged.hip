@@ -197,19 +197,19 @@ __global__ __launch_bounds__(kBlock) void gdn_ragged_any_kernel(GdnArgs a) {
 // 4 lg + i and 16 + 4 lg + i, i < 4.  Those are the places that a result's lane holds of
 // its column, so results become operands as they stand.
 //
-// What that floor may cost: over the dims of a state row it is small beside |m| |k| and |m| |q|,
-// as any sum's rounding (m the largest that it has been in the chunk: what a later token takes
-// back of it leaves its rounding behind).  Over the tokens of a chunk it is not: a value far larger than the
-// others would leave its error in the outputs of tokens before it, or in the state when it has
-// decayed.  So the wave that has the rows looks whether each token's outputs reach 2^-18 of
-// P's row times the largest delta (or T's largest row times the largest right side), and the
-// chunk's part of the state the same; a chunk of which one does not it takes its rows through
-// token by token.  64 products of two operands off by 2^-39 of their largest are then off by
-// 4e-6 of the result at random.  (The look costs 3 per cent: a prompt of 1500 121.5 us for
-// 116.5, three of 783 to 1172 beside 21 decoders 153.5 for 150.  A chunk token by token 55 us,
-// all of them 1430.)  A product over tokens that are not before a row's has weights
-// of 0 there, which a value that is not finite would make NaN: where a delta is not finite the
-// chunk goes token by token too, and where gates are above 0.
+// What that floor may cost: over the dims of a state row it is small beside |m| |k| and
+// |m| |q|, as any sum's rounding (m the largest that it has been in the chunk: what a later
+// token takes back of it leaves its rounding behind).  Over the tokens of a chunk it is not: a
+// value far larger than the others would leave its error in the outputs of tokens before it, or
+// in the state when it has decayed.  So the wave that has the rows looks whether each token's
+// outputs reach 2^-18 of P's row times the largest delta (or T's largest row times the largest
+// right side), and the chunk's part of the state the same; a chunk of which one does not it
+// takes its rows through token by token.  64 products of two operands off by 2^-39 of their
+// largest are then off by 4e-6 of the result at random.  (The look costs 1 to 4 per cent: a
+// prompt of 1500 120.8 us for 116.5, three of 783 to 1172 beside 21 decoders 152.3 for 150.  A
+// chunk token by token 55 us, all of them 1430.)  A product over tokens that are not before a
+// row's has weights of 0 there, which a value that is not finite would make NaN: where an output
+// is NaN the chunk goes token by token too, and where gates are above 0.
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
@@ -667,7 +667,7 @@ __global__ __launch_bounds__(kBlock, 2) void gdn_chunk_prep_kernel(GdnChunkArgs 
 // registers: every result is the next product's operand as it stands.  The operands that
 // the waves share stand in LDS, K and Q apart from K transposed, T and P, so that each
 // part of the next chunk comes in while the other is read: two barriers a chunk.
-// Three prompts of 1536 tokens, 16 / 48 heads of 128: 185 us, one 102.
+// Three prompts of 1536 tokens, 16 / 48 heads of 128: 183 us, one 100.
 
 // Operands of a chunk in LDS: K, Q; K transposed, T, P; their vectors, of two chunks in
 // turn.
@@ -917,8 +917,6 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds<S> &lds, co
     for (int i = 0; i < 12; ++i) tf[i >> 1][i & 1] = u_at[(kFragK<S> + kFragT) / 16 + i * 64];
 #pragma unroll
     for (int t = 0; t < 4; ++t) d[t] = d[t] * (of_token(2, t) * down);
-    const f32x4 sum_d = (d[0] + d[1]) + (d[2] + d[3]);
-    const float all_d = fabsf((sum_d.x + sum_d.y) + (sum_d.z + sum_d.w));
 #pragma unroll
     for (int t = 0; t < 4; ++t) s[t] = d[t] * of_token(4, t);
     const float most_d = most_of_lanes(most4(d));
@@ -938,6 +936,7 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds<S> &lds, co
     pair(s[0], s[1], up, &eh[0], &el[0]);
     pair(s[2], s[3], up, &eh[1], &el[1]);
     // outputs, and how far the row's are at least above kLeast of what their operands could give
+    // (NaN where one is: a delta that is not finite makes its own output so)
     const float least = most_ds * (a.scale * (kUnits * kLeast));
     const auto above = [&](int t, int e, f32x4 p_unit) { return fmaf(-p_unit[e], least, fabsf(d[t][e])); };
     float lowest = INFINITY;
@@ -950,12 +949,13 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds<S> &lds, co
         for (int e = 0; e < 4; ++e) d[t][e] = fmaf(of_q[e], y[t][e], of_p[e] * d[t][e]);
 #pragma unroll
         for (int e = 0; e < 4; e += 2)
-          lowest = fminf(fminf(above(t, e, p_unit), above(t, e + 1, p_unit)), lowest);
+          lowest = __builtin_elementwise_minimum(
+              __builtin_elementwise_minimum(above(t, e, p_unit), above(t, e + 1, p_unit)), lowest);
       }
     }
     // One row whose outputs all are clears its 16 lanes' tokens; else each token needs one.
     const uint64_t clear = __ballot(lowest >= 0.0f);
-    const uint64_t fine = __ballot(all_d < INFINITY && most_s * (of_chunk.z * (kUnits * kLeast)) <= most_e);
+    const uint64_t fine = __ballot(lowest == lowest && most_s * (of_chunk.z * (kUnits * kLeast)) <= most_e);
     bool odd = fine != ~uint64_t{0};
     if (__builtin_expect(((clear - kOnes) & ~clear & kOnes << 15) != 0, false)) {
       uint32_t below = 0;  // a bit a token
@@ -1019,7 +1019,7 @@ __device__ __forceinline__ void walk_rows(const GdnArgs &a, ChunkLds<S> &lds, co
 // longest requests, as far as blocks are fewer than compute units, half of them, and the
 // other four waves stage the operands (as they do for heads of 64).  What bounds a block is its waves' reads of them
 // from LDS (120 KB a wave and chunk), so half the rows are through sooner: 4.2 us a chunk
-// for 7.7.
+// for 7.6.
 template <int S>
 __global__ __launch_bounds__(512, 2) void gdn_chunk_walk_kernel(GdnChunkArgs c) {
   __shared__ __attribute__((aligned(16))) ChunkLds<S> lds;
